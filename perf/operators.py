@@ -371,10 +371,10 @@ def run(state):
     kind = case["kind"]
     if kind == "rotary":
         if own:
-            import ascendflow_amd.sparse_attention  # noqa: F401  (registers the torch ops)
+            from ascendflow_amd.sparse_attention import apply_rotary
 
-            y = torch.ops.ascendflow_amd.apply_rotary(state["x"], state["positions"], state["frequencies"], case["layout"],
-                                                      state["offset"], state["magnitude"])
+            y = apply_rotary(state["x"], state["positions"], state["frequencies"], layout=case["layout"],
+                             offset=state["offset"], magnitude=state["magnitude"])
             return (y, torch.autograd.grad(y, state["x"], state["grad"])[0]) if case["gradient"] else y
         if case["gradient"]:
             return _run_rotary(state, state["x"].detach()), _run_rotary(state, state["grad"], inverse=True)
