@@ -48,6 +48,10 @@ EXPORTS = (
     "workspace_size_attention_target",
     "workspace_size_attention_target_split",
     "workspace_size_simple_attention",
+    "launch_apply_rotary",
+    "launch_append_paged_kv",
+    "launch_latent_attention",
+    "launch_latent_attention_expanded",
     "launch_cache_flush",
     "launch_clock_probe",
     "ascendflow_amd_version",
@@ -89,6 +93,42 @@ class FaParams(ct.Structure):
         ("scale", ct.c_float),
         ("reserved", ct.c_int32),
     ]
+
+
+class RotaryParams(ct.Structure):
+    _fields_ = (
+        [(n, ct.c_int32) for n in ("dtype", "layout", "inverse", "position_bytes", "H", "D", "R", "offset")]
+        + [(n, ct.c_int64) for n in ("B", "S", "x_stride_b", "x_stride_s", "x_stride_h", "out_stride_b", "out_stride_s",
+                                     "out_stride_h", "position_stride_b")]
+        + [("magnitude", ct.c_float), ("reserved", ct.c_int32)]
+    )
+
+
+class AppendPagedKvParams(ct.Structure):
+    _fields_ = (
+        [(n, ct.c_int32) for n in ("dtype", "layout", "T", "B", "W", "PAGE", "BLOCKS", "HKV", "DK", "DV", "R", "offset")]
+        + [(n, ct.c_int64) for n in ("k_stride_t", "k_stride_h", "rope_stride_t", "rope_stride_h", "v_stride_t",
+                                     "v_stride_h")]
+        + [("magnitude", ct.c_float), ("reserved", ct.c_int32)]
+    )
+
+
+class LatentParams(ct.Structure):
+    _fields_ = (
+        [(n, ct.c_int32) for n in ("dtype", "causal", "T", "B", "H", "L", "R", "PAGE", "W", "BLOCKS")]
+        + [(n, ct.c_int64) for n in ("q_stride_t", "q_stride_h", "q_rope_stride_t", "q_rope_stride_h", "out_stride_t",
+                                     "out_stride_h")]
+        + [("scale", ct.c_float), ("reserved", ct.c_int32)]
+    )
+
+
+class LatentExpandedParams(ct.Structure):
+    _fields_ = (
+        [(n, ct.c_int32) for n in ("dtype", "causal", "Tq", "Tk", "B", "H", "D", "R")]
+        + [(n, ct.c_int64) for n in ("q_stride_t", "q_stride_h", "k_stride_t", "k_stride_h", "k_rope_stride_t",
+                                     "v_stride_t", "v_stride_h", "out_stride_t", "out_stride_h")]
+        + [("scale", ct.c_float), ("reserved", ct.c_int32)]
+    )
 
 
 _P = ct.c_void_p
@@ -138,6 +178,10 @@ _SIGNATURES = {
         [ct.POINTER(ct.c_uint64), ct.c_int64, ct.c_int64],
         ct.c_int,
     ),
+    "launch_apply_rotary": ([_P] * 5 + [ct.POINTER(RotaryParams)], ct.c_int),
+    "launch_append_paged_kv": ([_P] * 10 + [ct.POINTER(AppendPagedKvParams)], ct.c_int),
+    "launch_latent_attention": ([_P] * 9 + [ct.POINTER(LatentParams)], ct.c_int),
+    "launch_latent_attention_expanded": ([_P] * 9 + [ct.POINTER(LatentExpandedParams)], ct.c_int),
     "launch_cache_flush": ([_P, _P, ct.c_uint64], ct.c_int),
     "launch_clock_probe": ([_P, _P, ct.c_int32], ct.c_int),
     "ascendflow_amd_version": ([], ct.c_char_p),

@@ -127,3 +127,59 @@ def raw_stream(device_index) -> int:
 
 def stream_handle(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def check_rows(name, tensor, shape, dtype, device=None):
+    """``check_tensor`` for a tensor of any strides whose last dimension is contiguous."""
+    require(isinstance(tensor, torch.Tensor), f"{name} must be a torch.Tensor")
+    require(tuple(tensor.shape) == tuple(shape), f"{name} shape {tuple(tensor.shape)} != {tuple(shape)}")
+    require(tensor.dtype == dtype, f"{name} dtype {tensor.dtype} != {dtype}")
+    require(tensor.shape[-1] <= 1 or tensor.stride(-1) == 1, f"{name} must have contiguous rows")
+    require(tensor.is_cuda, f"{name} must live on a ROCm device")
+    if device is not None:
+        require(tensor.device == device, f"{name} is on {tensor.device}, expected {device}")
+
+
+def live_strides(tensor):
+    """Strides of a tensor, 0 for a dimension of at most one entry (whose stride means nothing)."""
+    return tuple(st if n > 1 else 0 for n, st in zip(tensor.shape, tensor.stride()))
+
+
+def check_distinct_rows(name, tensor):
+    """A written tensor names every element once: its dimensions, from the
+    smallest stride up, do not reach into one another."""
+    reach = 1
+    for stride, size in sorted((st, n) for n, st in zip(tensor.shape, tensor.stride()) if n > 1):
+        require(stride >= reach, f"{name} has elements that overlap")
+        reach = stride * (size - 1) + reach
+
+
+def memory_span(tensor):
+    """First byte and the byte past the last of a tensor of any (non-negative) strides."""
+    start = tensor.data_ptr()
+    if tensor.numel() == 0:
+        return start, start
+    last = sum((n - 1) * st for n, st in zip(tensor.shape, tensor.stride()))
+    return start, start + (last + 1) * tensor.element_size()
+
+
+def check_apart(named):
+    """``check_disjoint`` for tensors of any strides: (name, tensor, written) each,
+    None tensors left out. Memory is compared from first to last byte, so two
+    views that interleave in one buffer count as overlapping."""
+    spans = [(name, *memory_span(t), write) for name, t, write in named if t is not None and t.numel()]
+    for i, (a, a0, a1, aw) in enumerate(spans):
+        if not aw:
+            continue
+        for j, (b, b0, b1, _) in enumerate(spans):
+            if j != i and a0 < b1 and b0 < a1:
+                first, second = (a, b) if i < j else (b, a)
+                raise ValueError(f"external tensors {first} and {second} overlap")
+
+
+def launch_on(device_index, launch, *args):
+    """``launch(current stream of the device, *args)`` with that device current."""
+    if torch._C._cuda_getDevice() == device_index:
+        return launch(raw_stream(device_index), *args)
+    with torch.cuda.device(device_index):
+        return launch(raw_stream(device_index), *args)

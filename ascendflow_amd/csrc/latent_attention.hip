@@ -1,0 +1,749 @@
+// Attention whose keys and values come from one latent vector a token, for
+// gfx950: the absorbed form over a paged cache and the expanded form over
+// contiguous keys and values.
+//
+// Absorbed (latent_attention): a cache row is [c | k_rope], c of L columns, one
+// row for all heads. With the key projection absorbed into the query,
+//   s = scale (q . c + q_rope . k_rope),  o = softmax(s) c,
+// so a row is read once and serves as key and as value. The rows of a request's
+// (token, head) pairs are packed token by token into tiles of 16 * NW rows; each
+// wave owns 16 of them, whose Q (L + R columns) and O (L columns, float32) stay
+// in registers. Cache rows stream in chunks of 32 through an LDS ring filled by
+// the load-to-LDS path, XOR-swizzled on the global side, and every wave reads
+// every row twice: S^T[keys, rows] = K Q^T with ds_read_b128, O^T[columns, rows]
+// += V^T P^T with the transposing ds_read_b64_tr_b16. P stays in the wave's
+// registers (the accumulator layout of S^T is the operand layout of P^T, up to
+// an order of keys that both sides share), so a chunk costs one barrier.
+//
+// Online softmax in float32, exp2 domain: the running maximum m is raised only
+// when a row's maximum exceeds it by more than LAT_TAU (log2 units), so that O
+// is rescaled rarely; P <= 2^LAT_TAU is rounded to the storage type (a matrix
+// operand has to be), and O is divided by the sum of the rounded P, so that the
+// weights that were applied add up to one; the log-sum-exp takes the sum before
+// rounding.
+#include <algorithm>
+
+#include "common.h"
+#include "../../include/ascendflow_amd.h"
+
+namespace afa {
+
+constexpr float LAT_LOG2E = 1.4426950408889634f, LAT_LN2 = 0.6931471805599453f;
+constexpr float LAT_TAU = 8.0f;
+constexpr int LAT_KEYS = 32;  // cache rows per chunk
+
+struct LatentArgs {
+  const void* q;
+  const void* q_rope;
+  const void* cache;
+  const int32_t* table;
+  const int32_t* cu;
+  const int32_t* used;
+  void* out;
+  float* lse;  // [T][H] or NULL
+  int64_t q_t, q_h, qr_t, qr_h, o_t, o_h;
+  int32_t T, B, H, W, page_shift, blocks, causal;
+  float scale;
+};
+
+// New tokens of request b: cu[b] .. cu[b + 1], held inside [0, T).
+__device__ __forceinline__ void request_tokens(const int32_t* cu, int b, int T, int& start, int& count) {
+  start = min(max(cu[b], 0), T);
+  count = max(min(cu[b + 1], T) - start, 0);
+}
+
+// The request and the tile inside it of tile `index` in the order of requests
+// (tiles_of(tokens) each); false, for the whole workgroup, if there are fewer.
+template <int THREADS, typename F>
+__device__ __forceinline__ bool find_tile(const int32_t* cu, int B, int T, uint32_t index, F&& tiles_of, int& request,
+                                          uint32_t& tile, uint32_t& tiles) {
+  __shared__ uint32_t wave_total[THREADS / 64];
+  __shared__ uint32_t found[3];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  uint32_t before = 0;
+  for (int base = 0; base < B; base += THREADS) {
+    const int b = base + tid;
+    int start = 0, count = 0;
+    if (b < B) request_tokens(cu, b, T, start, count);
+    const uint32_t mine = b < B ? tiles_of(count) : 0u;
+    const uint32_t upto = (uint32_t)wave_inclusive_scan((int)mine);
+    if (lane == 63) wave_total[wave] = upto;
+    __syncthreads();
+    uint32_t first = before, all = before;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      if (w < wave) first += wave_total[w];
+      all += wave_total[w];
+    }
+    const uint32_t begin = first + upto - mine;
+    if (index >= begin && index < begin + mine) {
+      found[0] = (uint32_t)b;
+      found[1] = index - begin;
+      found[2] = mine;
+    }
+    __syncthreads();
+    if (index < all) {
+      request = __builtin_amdgcn_readfirstlane((int)found[0]);
+      tile = (uint32_t)__builtin_amdgcn_readfirstlane((int)found[1]);
+      tiles = (uint32_t)__builtin_amdgcn_readfirstlane((int)found[2]);
+      return true;
+    }
+    before = all;
+  }
+  return false;
+}
+
+template <int DT, int L, int R, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(LatentArgs a) {
+  typedef typename B16<DT>::scalar scalar;
+  typedef typename B16<DT>::x8 x8;
+  typedef typename B16<DT>::x4 x4;
+  static_assert(L % 128 == 0 && L <= 512 && (R == 0 || R == 64) && (NW == 4 || NW == 8), "supported rows");
+  constexpr int ROWS = 16 * NW;
+  constexpr int LROW = 2 * L;                  // bytes of a latent row in LDS
+  constexpr int GROW = 2 * (L + R);            // bytes of a cache row
+  constexpr int ROPE_AT = LAT_KEYS * LROW;     // the rotary parts follow the latents
+  constexpr int SLOT = LAT_KEYS * GROW;
+  constexpr int NS = NW == 8 ? 4 : 2;          // ring slots: one workgroup per CU, or two
+  constexpr int RW = LAT_KEYS / NW;            // rows that one wave loads
+  constexpr int LR = 512 / L, LOADS_L = RW / LR, LOADS = LOADS_L + (R ? 1 : 0);
+  constexpr int KSTEPS = L / 32, RSTEPS = R / 32, VTILES = L / 16;
+  __shared__ __attribute__((aligned(256))) uint8_t ring[NS][SLOT];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int g = lane >> 4, i16 = lane & 15;
+
+  int request;
+  uint32_t tile, tiles;
+  const int H = a.H;
+  if (!find_tile<NW * 64>(a.cu, a.B, a.T, blockIdx.x,
+                          [&](int n) { return ((uint32_t)n * (uint32_t)H + ROWS - 1) / ROWS; }, request, tile, tiles))
+    return;
+  if (a.causal) tile = tiles - 1 - tile;  // the longest first
+  int start, count;
+  request_tokens(a.cu, request, a.T, start, count);
+  const int used = (int)min((int64_t)max(a.used[request], 0), (int64_t)a.W << a.page_shift);
+  const int rows = count * H;
+
+  // This lane's (token, head) row, and the keys it sees: [0, limit).
+  const int row = (int)tile * ROWS + wave * 16 + i16;
+  const bool valid = row < rows;
+  const int token = valid ? row / H : 0, head = valid ? row - token * H : 0;
+  auto visible = [&](int t) { return a.causal ? min(max(used - count + t + 1, 0), used) : used; };
+  const int limit = valid ? visible(token) : 0;
+  const int kv_end = visible((min((int)(tile + 1) * ROWS, rows) - 1) / H);
+  const int clean_end = visible((int)tile * ROWS / H);  // no row of the tile hides a key below
+  const int chunks = (kv_end + LAT_KEYS - 1) / LAT_KEYS;
+
+  // ---- cache rows to LDS -----------------------------------------------------
+  const uint32_t ring_base = lds_address(ring[0]);
+  // In the constant address space, so that the uniform reads are scalar loads,
+  // which leave the vector load counter to the ring.
+  typedef const __attribute__((address_space(4))) int32_t* const_ints;
+  const const_ints pages = (const_ints)(uintptr_t)(a.table + (int64_t)request * a.W);
+  const int page_mask = (1 << a.page_shift) - 1;
+  // Page of the 16-row group that holds `key`; -1 past the end.
+  auto page_of = [&](int key) { return key < kv_end ? pages[key >> a.page_shift] : -1; };
+  auto inside = [&](int page) { return (uint32_t)page < (uint32_t)a.blocks; };
+  int next[2];         // pages of the two 16-row groups of the next chunk to load
+  uint32_t good = 0;   // two bits per chunk loaded, the latest lowest: its groups' pages lie in the cache
+  int partial = 0;     // chunks until every one in flight has all its loads
+  auto look_up = [&](int chunk) {
+    next[0] = page_of(chunk * LAT_KEYS);
+    next[1] = page_of(chunk * LAT_KEYS + 16);
+  };
+  auto fetch = [&](int chunk) {
+    const bool ok0 = inside(next[0]), ok1 = inside(next[1]);
+    good = (good << 2) | (ok0 ? 1u : 0u) | (ok1 ? 2u : 0u);
+    const int first = wave * RW;  // of the chunk's rows
+    const int key = chunk * LAT_KEYS + first;
+    const bool upper = first >= 16;
+    const int page = upper ? next[1] : next[0];
+    const int have = (upper ? ok1 : ok0) ? min(max(kv_end - key, 0), RW) : 0;
+    const char* from = (const char*)a.cache + ((int64_t)page * (page_mask + 1) + (key & page_mask)) * GROW;
+    const uint32_t slot = ring_base + (uint32_t)(chunk % NS) * SLOT;
+    const uint32_t to = opaque_uniform(slot + (uint32_t)(first * LROW));
+    const uint32_t to_rope = opaque_uniform(slot + (uint32_t)(ROPE_AT + first * 2 * R));
+    if (partial > 0) --partial;
+    if (have < RW) partial = NS;
+#pragma unroll
+    for (int p = 0; p < LOADS_L; ++p) {
+      const int r = p * LR + lane / (L / 8);
+      const uint32_t off = (uint32_t)(r * GROW + (((lane % (L / 8)) ^ ((first + r) & 15)) << 4));
+      if (r < have)
+        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                         :: "s"(to + (uint32_t)p * 1024u), "v"(off), "s"(from) : "memory");
+      else  // rows past the end or without a page: zeros, which no weight can turn into anything else
+        *(AFA_LDS u32x4*)(uintptr_t)(to + (uint32_t)(p * 1024 + lane * 16)) = u32x4{0u, 0u, 0u, 0u};
+    }
+    if constexpr (R != 0) {
+      const int r = lane >> 3;
+      const uint32_t off = (uint32_t)(r * GROW + LROW + (((lane & 7) ^ (((first + r) >> 1) & 7)) << 4));
+      if (r < have)
+        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                         :: "s"(to_rope), "v"(off), "s"(from) : "memory");
+      else if (r < RW)
+        *(AFA_LDS u32x4*)(uintptr_t)(to_rope + (uint32_t)lane * 16u) = u32x4{0u, 0u, 0u, 0u};
+    }
+    look_up(chunk + 1);
+  };
+
+  // ---- Q fragments: B operand, columns 32 j + 8 g .. + 7 of row i16 -----------
+  x8 qf[KSTEPS + RSTEPS];
+  {
+    const scalar* q = (const scalar*)a.q + (int64_t)(start + token) * a.q_t + (int64_t)head * a.q_h + 8 * g;
+#pragma unroll
+    for (int j = 0; j < KSTEPS; ++j)
+      qf[j] = valid ? *(const x8*)(q + 32 * j) : __builtin_bit_cast(x8, u32x4{0u, 0u, 0u, 0u});
+    if constexpr (R != 0) {
+      const scalar* qr = (const scalar*)a.q_rope + (int64_t)(start + token) * a.qr_t + (int64_t)head * a.qr_h + 8 * g;
+#pragma unroll
+      for (int j = 0; j < RSTEPS; ++j)
+        qf[KSTEPS + j] = valid ? *(const x8*)(qr + 32 * j) : __builtin_bit_cast(x8, u32x4{0u, 0u, 0u, 0u});
+    }
+  }
+
+  // ---- fragment addresses (relative to a slot; XOR picks the 64- or 32-byte group) --
+  const int ra = sigma(i16), rt = sigma(4 * g + (i16 >> 2));
+  const uint32_t qk_at = (uint32_t)(ra * LROW + ((g ^ (ra & 15)) << 4));
+  const uint32_t qr_at = (uint32_t)(ROPE_AT + ra * 2 * R + ((g ^ ((ra >> 1) & 7)) << 4));
+  const uint32_t tr_at = (uint32_t)(rt * LROW + ((((i16 & 3) >> 1) ^ (rt & 15)) << 4) + (i16 & 1) * 8);
+
+  f32x4 o[VTILES];
+#pragma unroll
+  for (int t = 0; t < VTILES; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -1e30f;  // finite: a chunk that hides all its keys gives p = 0, never NaN
+  float l_run = 0.f, l_rounded = 0.f;
+  const float scale_log2 = a.scale * LAT_LOG2E;
+
+  look_up(0);
+#pragma unroll
+  for (int c = 0; c < NS - 1; ++c)
+    if (c < chunks) fetch(c);
+
+  for (int c = 0; c < chunks; ++c) {
+    // Chunk c has landed once at most the loads of the NS - 2 younger chunks are
+    // in flight; where one of those has fewer loads, or is missing, all must have.
+    if (partial == 0 && c + NS - 2 < chunks)
+      wait_vmcnt<(NS - 2) * LOADS>();
+    else
+      wait_vmcnt<0>();
+    block_barrier();  // every wave's part of chunk c is there, and chunk c - 1 is read
+    const int loaded = min(c + NS - 1, chunks);  // chunks fetched so far
+    const uint32_t bits = (good >> (2 * (loaded - 1 - c))) & 3u;
+    if (c + NS - 1 < chunks) fetch(c + NS - 1);
+    const uint32_t slot = ring_base + (uint32_t)(c % NS) * SLOT;
+
+    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    {
+      constexpr int FRAGS = 2 * (KSTEPS + RSTEPS), LOOK = 6;
+      const uint32_t base = opaque(slot + qk_at), rope = opaque(slot + qr_at);
+      x8 kf[FRAGS];
+      auto load = [&](int f) {  // (step j, key tile t)
+        const int j = f / 2, t = f % 2;
+        kf[f] = j < KSTEPS ? *(const AFA_LDS x8*)(lds_at<uint8_t>(base ^ (uint32_t)((j & 3) << 6)) + (j >> 2) * 256 + t * 16 * LROW)
+                           : *(const AFA_LDS x8*)(lds_at<uint8_t>(rope ^ (uint32_t)((j - KSTEPS) << 6)) + t * 16 * 2 * R);
+      };
+#pragma unroll
+      for (int f = 0; f < LOOK; ++f) load(f);
+#pragma unroll
+      for (int f = 0; f < FRAGS; ++f) {
+        if (f + LOOK < FRAGS) load(f + LOOK);
+        s[f % 2] = B16<DT>::mfma(kf[f], qf[f / 2], s[f % 2]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    const int key0 = c * LAT_KEYS;
+    if (key0 + LAT_KEYS > clean_end || bits != 3u) {  // uniform
+      const int lim = limit - key0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[t][i] = 16 * t + sigma(4 * g + i) < lim && ((bits >> t) & 1u) ? s[t][i] : -INFINITY;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
+    const float m_new = fmaxf(m_run, max_over_lane_groups(top) * scale_log2);
+    if (__ballot(m_new > m_run + LAT_TAU) != 0ull) {
+      const float alpha = fast_exp2(m_run - m_new);
+      l_run *= alpha;
+      l_rounded *= alpha;
+#pragma unroll
+      for (int t = 0; t < VTILES; ++t) o[t] *= alpha;
+      m_run = m_new;
+    }
+    x8 pf;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = fast_exp2(__builtin_fmaf(s[t][i], scale_log2, -m_run));
+        const scalar r = (scalar)p;
+        l_run += p;
+        l_rounded += (float)r;
+        pf[4 * t + i] = r;
+      }
+    {
+      constexpr int LOOK = 3;
+      const uint32_t base = opaque(slot + tr_at);
+      x4 lo[VTILES], hi[VTILES];
+      auto load = [&](int t) {
+        const AFA_LDS uint8_t* p = lds_at<uint8_t>(base ^ (uint32_t)((t & 7) << 5)) + (t >> 3) * 256;
+        lo[t] = B16<DT>::read_tr((const AFA_LDS void*)p);
+        hi[t] = B16<DT>::read_tr((const AFA_LDS void*)(p + 16 * LROW));
+      };
+#pragma unroll
+      for (int t = 0; t < LOOK; ++t) load(t);
+#pragma unroll
+      for (int t = 0; t < VTILES; ++t) {
+        if (t + LOOK < VTILES) load(t + LOOK);
+        const x8 vf = {lo[t][0], lo[t][1], lo[t][2], lo[t][3], hi[t][0], hi[t][1], hi[t][2], hi[t][3]};
+        o[t] = B16<DT>::mfma(vf, pf, o[t]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  const float total = sum_over_lane_groups(l_run), applied = sum_over_lane_groups(l_rounded);
+  if (!valid) return;
+  const float inv = applied > 0.f ? 1.0f / applied : 0.f;
+  scalar* out = (scalar*)a.out + (int64_t)(start + token) * a.o_t + (int64_t)head * a.o_h + 4 * g;
+#pragma unroll
+  for (int t = 0; t < VTILES; ++t) {
+    x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[t][i] * inv);
+    *(x4*)(out + 16 * t) = v;
+  }
+  if (a.lse && g == 0)
+    a.lse[(int64_t)(start + token) * H + head] = total > 0.f ? (m_run + __log2f(total)) * LAT_LN2 : -INFINITY;
+}
+
+// Expanded form (latent_attention_expanded), for prompts: keys [k_nope | k_rope]
+// of 128 + 64 columns, k_nope and the values of each head, k_rope of all heads,
+//   s = scale (q_nope . k_nope[h] + q_rope . k_rope),  o = softmax(s) v[h].
+// 2 (128 + 64 + 128) flops a pair instead of the absorbed 2 (2 L + 64), for keys
+// and values that the caller expands once per prompt. The two parts of a key are
+// read from where they lie, so no concatenated, per-head copy of k_rope is made.
+// One workgroup per (request, head, 256 query rows): 8 waves of two 16-row tiles
+// with Q resident; 64-key chunks of k_nope, k_rope and v stream through a
+// three-slot LDS ring two chunks ahead. QK of chunk c + 1 is issued ahead of the
+// softmax of chunk c, whose exponentials run in the shadow of the matrix
+// instructions of QK (c + 1) and PV (c).
+struct ExpandedArgs {
+  const void* q;
+  const void* k;
+  const void* k_rope;
+  const void* v;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  void* out;
+  float* lse;  // [Tq][H] or NULL
+  int64_t q_t, q_h, k_t, k_h, kr_t, v_t, v_h, o_t, o_h;
+  int32_t Tq, Tk, B, H, causal;
+  float scale;
+};
+
+template <int DT>
+__global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
+  typedef typename B16<DT>::scalar scalar;
+  typedef typename B16<DT>::x8 x8;
+  typedef typename B16<DT>::x4 x4;
+  constexpr int NW = 8, QT = 2, BQ = NW * QT * 16, KC = 64, KT = KC / 16, NS = 3;
+  constexpr int D = 128, R = 64, ROW_BYTES = 2 * D, ROPE_BYTES = 2 * R;
+  constexpr int ROPE_AT = KC * ROW_BYTES, V_AT = ROPE_AT + KC * ROPE_BYTES, SLOT = V_AT + KC * ROW_BYTES;
+  constexpr int KSTEPS = D / 32, STEPS = KSTEPS + R / 32;
+  constexpr int LOADS = 5;  // wave loads per chunk: two of k_nope, two of v (4 rows each), one of k_rope (8 rows)
+  __shared__ __attribute__((aligned(256))) uint8_t ring[NS][SLOT];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int g = lane >> 4, i16 = lane & 15;
+  const int head = (int)(blockIdx.x % (uint32_t)a.H);
+  int request;
+  uint32_t tile, tiles;
+  if (!find_tile<512>(a.cu_q, a.B, a.Tq, blockIdx.x / (uint32_t)a.H,
+                      [&](int n) { return ((uint32_t)n + BQ - 1) / BQ; }, request, tile, tiles))
+    return;
+  if (a.causal) tile = tiles - 1 - tile;  // the longest first
+  int q_start, nq, k_start, nk;
+  request_tokens(a.cu_q, request, a.Tq, q_start, nq);
+  request_tokens(a.cu_k, request, a.Tk, k_start, nk);
+  const int q0 = (int)tile * BQ;
+
+  const scalar* Q = (const scalar*)a.q + (int64_t)q_start * a.q_t + (int64_t)head * a.q_h;
+  const char* K = (const char*)a.k + 2 * ((int64_t)k_start * a.k_t + (int64_t)head * a.k_h);
+  const char* KR = (const char*)a.k_rope + 2 * (int64_t)k_start * a.kr_t;
+  const char* V = (const char*)a.v + 2 * ((int64_t)k_start * a.v_t + (int64_t)head * a.v_h);
+
+  // Query i sees keys [0, nk - nq + i + 1) (causal, aligned at the end) or all.
+  auto visible = [&](int i) { return a.causal ? min(max(nk - nq + i + 1, 0), nk) : nk; };
+  int limit[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) limit[qt] = visible(min(q0 + (wave * QT + qt) * 16 + i16, nq - 1));
+  const int kv_end = visible(min(q0 + BQ, nq) - 1);
+  const int clean_end = visible(q0);
+  const int chunks = (kv_end + KC - 1) / KC, clean_chunks = clean_end / KC;
+
+  x8 qf[QT][STEPS];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int row = q0 + (wave * QT + qt) * 16 + i16;
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j)
+      qf[qt][j] = row < nq ? *(const x8*)(Q + row * a.q_t + 32 * j + 8 * g) : __builtin_bit_cast(x8, u32x4{0u, 0u, 0u, 0u});
+  }
+
+  const uint32_t ring_base = lds_address(ring[0]);
+  auto slot_of = [&](int chunk) { return opaque_uniform(ring_base + (uint32_t)(chunk % NS) * SLOT); };
+  // Rows past the last key read the last key instead (masked later). 32-bit row
+  // offsets: the host holds 64 rows of any stride below 2^31 bytes.
+  const uint32_t k_row = (uint32_t)(2 * a.k_t), v_row = (uint32_t)(2 * a.v_t), r_row = (uint32_t)(2 * a.kr_t);
+  auto fetch = [&](int chunk) {
+    const int key0 = chunk * KC;
+    const char* kbase = K + (int64_t)key0 * (2 * a.k_t);
+    const char* vbase = V + (int64_t)key0 * (2 * a.v_t);
+    const char* rbase = KR + (int64_t)key0 * (2 * a.kr_t);
+    const int last = nk - 1 - key0;
+    const uint32_t slot = slot_of(chunk);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int r = (wave * 2 + p) * 4 + (lane >> 4);
+      const uint32_t rr = (uint32_t)min(r, last), unit = (uint32_t)(((lane & 15) ^ (r & 15)) << 4);
+      const uint32_t to = slot + (uint32_t)((wave * 2 + p) * 4 * ROW_BYTES);
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                       :: "s"(to), "v"(rr * k_row + unit), "s"(kbase) : "memory");
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                       :: "s"(to + (uint32_t)V_AT), "v"(rr * v_row + unit), "s"(vbase) : "memory");
+    }
+    const int r = wave * 8 + (lane >> 3);
+    const uint32_t off = (uint32_t)min(r, last) * r_row + (uint32_t)(((lane & 7) ^ ((r >> 1) & 7)) << 4);
+    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :: "s"(slot + (uint32_t)(ROPE_AT + wave * 8 * ROPE_BYTES)), "v"(off), "s"(rbase) : "memory");
+  };
+
+  const int ra = sigma(i16), rt = sigma(4 * g + (i16 >> 2));
+  const uint32_t qk_at = (uint32_t)(ra * ROW_BYTES + ((g ^ (ra & 15)) << 4));
+  const uint32_t qr_at = (uint32_t)(ROPE_AT + ra * ROPE_BYTES + ((g ^ ((ra >> 1) & 7)) << 4));
+  const uint32_t tr_at = (uint32_t)(V_AT + rt * ROW_BYTES + ((((i16 & 3) >> 1) ^ (rt & 15)) << 4) + (i16 & 1) * 8);
+
+  f32x4 o[QT][D / 16];
+  float m_run[QT], l_run[QT], l_rounded[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m_run[qt] = -1e30f;
+    l_run[qt] = l_rounded[qt] = 0.f;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float scale_log2 = a.scale * LAT_LOG2E;
+
+  constexpr int QK_FRAGS = STEPS * KT, LOOK = 6;
+  auto qk_chunk = [&](int chunk, f32x4 (&s)[KT][QT], auto&& between) {
+    const uint32_t slot = slot_of(chunk);
+    const uint32_t base = opaque(slot + qk_at), rope = opaque(slot + qr_at);
+    x8 kf[QK_FRAGS];
+    auto load = [&](int f) {  // (step j, key tile t)
+      const int j = f / KT, t = f % KT;
+      kf[f] = j < KSTEPS ? *(const AFA_LDS x8*)(lds_at<uint8_t>(base ^ (uint32_t)(j << 6)) + t * 16 * ROW_BYTES)
+                         : *(const AFA_LDS x8*)(lds_at<uint8_t>(rope ^ (uint32_t)((j - KSTEPS) << 6)) + t * 16 * ROPE_BYTES);
+    };
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) s[t][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int f = 0; f < LOOK; ++f) load(f);
+#pragma unroll
+    for (int f = 0; f < QK_FRAGS; ++f) {
+      if (f + LOOK < QK_FRAGS) load(f + LOOK);
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) s[f % KT][qt] = B16<DT>::mfma(kf[f], qf[qt][f / KT], s[f % KT][qt]);
+      between(f);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr int PV_FRAGS = (KC / 32) * (D / 16);
+  auto pv_chunk = [&](int chunk, x8 (&pf)[QT][KC / 32], auto&& between) {
+    const uint32_t base = opaque(slot_of(chunk) + tr_at);
+    constexpr int VLOOK = 3;
+    x4 lo[PV_FRAGS], hi[PV_FRAGS];
+    auto load = [&](int f) {  // (32 keys ks, column tile t)
+      const int ks = f / (D / 16), t = f % (D / 16);
+      const AFA_LDS uint8_t* p = lds_at<uint8_t>(base ^ (uint32_t)(t << 5)) + ks * 32 * ROW_BYTES;
+      lo[f] = B16<DT>::read_tr((const AFA_LDS void*)p);
+      hi[f] = B16<DT>::read_tr((const AFA_LDS void*)(p + 16 * ROW_BYTES));
+    };
+#pragma unroll
+    for (int f = 0; f < VLOOK; ++f) load(f);
+#pragma unroll
+    for (int f = 0; f < PV_FRAGS; ++f) {
+      if (f + VLOOK < PV_FRAGS) load(f + VLOOK);
+      const int ks = f / (D / 16), t = f % (D / 16);
+      const x8 vf = {lo[f][0], lo[f][1], lo[f][2], lo[f][3], hi[f][0], hi[f][1], hi[f][2], hi[f][3]};
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) o[qt][t] = B16<DT>::mfma(vf, pf[qt][ks], o[qt][t]);
+      between(f);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto mask = [&](int chunk, f32x4 (&s)[KT][QT]) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int lim = limit[qt] - chunk * KC;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][qt][i] = 16 * t + sigma(4 * g + i) < lim ? s[t][qt][i] : -INFINITY;
+    }
+  };
+
+  constexpr int HALF = QT * 8, QK_EXP0 = QT + 2, PV_EXP_STEPS = PV_FRAGS / 2 - 1;
+  f32x4 s_a[KT][QT], s_b[KT][QT];
+  if (chunks > 0) {
+    fetch(0);
+    if (chunks > 1) {
+      fetch(1);
+      wait_vmcnt<LOADS>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    block_barrier();
+    qk_chunk(0, s_a, [](int) {});
+  }
+  auto iteration = [&](int c, f32x4 (&cur)[KT][QT], f32x4 (&nxt)[KT][QT]) {
+    // Chunk c + 1 has landed, and every wave is past QK (c) and PV (c - 1).
+    wait_vmcnt<0>();
+    block_barrier();
+    if (c + 2 < chunks) fetch(c + 2);
+    if (c >= clean_chunks) mask(c, cur);
+    x8 pf[QT][KC / 32];
+    float top[QT], m_new[QT], psum[QT], rsum[QT];
+    auto exp_element = [&](int e) {  // (half, qt, key tile of the half, i)
+      const int h = e / HALF, qt = (e / 8) % QT, t = 2 * h + (e / 4) % 2, i = e % 4;
+      const float p = fast_exp2(__builtin_fmaf(cur[t][qt][i], scale_log2, -m_run[qt]));
+      const scalar r = (scalar)p;
+      psum[qt] += p;
+      rsum[qt] += (float)r;
+      pf[qt][h][(t & 1) * 4 + i] = r;
+    };
+    auto qk_between = [&](int f) {
+      if (f == QK_FRAGS / 2 - 1) __builtin_amdgcn_s_setprio(2);
+      if (f < QT) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m = fmaxf(m, cur[t][f][i]);
+        top[f] = m;
+      } else if (f == QT) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          m_new[qt] = fmaxf(m_run[qt], max_over_lane_groups(top[qt]) * scale_log2);
+          psum[qt] = rsum[qt] = 0.f;
+        }
+      } else if (f == QT + 1) {
+        bool grow = false;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) grow |= m_new[qt] > m_run[qt] + LAT_TAU;
+        if (__ballot(grow) != 0ull) {
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            const float alpha = fast_exp2(m_run[qt] - m_new[qt]);
+            l_run[qt] *= alpha;
+            l_rounded[qt] *= alpha;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) o[qt][t] *= alpha;
+            m_run[qt] = m_new[qt];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < HALF; ++e)
+          if (QK_EXP0 + e * (QK_FRAGS - QK_EXP0) / HALF == f) exp_element(e);
+      }
+    };
+    auto pv_between = [&](int f) {
+      if (f == PV_FRAGS / 2 - 1) __builtin_amdgcn_s_setprio(0);
+      if (f < PV_EXP_STEPS) {
+#pragma unroll
+        for (int e = 0; e < HALF; ++e)
+          if (e * PV_EXP_STEPS / HALF == f) exp_element(HALF + e);
+      } else if (f == PV_EXP_STEPS + 1) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          l_run[qt] += psum[qt];
+          l_rounded[qt] += rsum[qt];
+        }
+      }
+    };
+    // Wave priority steps down with the wave's progress through a chunk: of the
+    // two waves of a SIMD the one behind wins. The last chunk also runs a QK,
+    // over a slot that no load is in flight into; nobody reads those scores.
+    __builtin_amdgcn_s_setprio(3);
+    qk_chunk(c + 1, nxt, qk_between);
+    __builtin_amdgcn_s_setprio(1);
+    pv_chunk(c, pf, pv_between);
+  };
+  for (int c = 0; c < chunks; c += 2) {
+    iteration(c, s_a, s_b);
+    if (c + 1 < chunks) iteration(c + 1, s_b, s_a);
+  }
+
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int row = q0 + (wave * QT + qt) * 16 + i16;
+    const float total = sum_over_lane_groups(l_run[qt]), applied = sum_over_lane_groups(l_rounded[qt]);
+    const float inv = applied > 0.f ? 1.0f / applied : 0.f;
+    if (row < nq) {
+      scalar* out = (scalar*)a.out + (int64_t)(q_start + row) * a.o_t + (int64_t)head * a.o_h + 4 * g;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) {
+        x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[qt][t][i] * inv);
+        *(x4*)(out + 16 * t) = v;
+      }
+      if (a.lse && g == 0)
+        a.lse[(int64_t)(q_start + row) * a.H + head] = total > 0.f ? (m_run[qt] + __log2f(total)) * LAT_LN2 : -INFINITY;
+    }
+  }
+}
+
+namespace {
+
+bool rows_fit(const void* p, int64_t a, int64_t b) { return ((uintptr_t)p & 15) == 0 && (a | b) % 8 == 0; }
+
+int check_latent(const LatentParams* p) {
+  if (!p) return AFA_E_NULL;
+  if (p->dtype != AFA_DTYPE_BF16 && p->dtype != AFA_DTYPE_F16) return AFA_E_DTYPE;
+  if (p->T < 0 || p->B <= 0 || p->H <= 0 || p->W <= 0 || p->BLOCKS <= 0) return AFA_E_SHAPE;
+  if ((p->L != 128 && p->L != 256 && p->L != 512) || (p->R != 0 && p->R != 64)) return AFA_E_SHAPE;
+  if (p->PAGE < 16 || p->PAGE > (1 << 20) || (p->PAGE & (p->PAGE - 1))) return AFA_E_SHAPE;
+  // Packed rows, tiles and positions are 32-bit numbers.
+  if ((int64_t)p->T * p->H > 0x7fffff00ll || (int64_t)p->W * p->PAGE > 0x7fffff00ll || p->B > 0x3fffffff) return AFA_E_SHAPE;
+  if (!(p->scale > 0.0f)) return AFA_E_SHAPE;
+  return AFA_OK;
+}
+
+// Waves (of 16 rows each) of a tile: 8 where a request has more than 64 rows on average, else 4.
+int latent_waves(const LatentParams* p) { return ((int64_t)p->T + p->B - 1) / p->B * p->H > 64 ? 8 : 4; }
+
+template <int DT, int L, int R>
+int launch_latent(const LatentArgs& a, int waves, hipStream_t s) {
+  const int64_t tiles = (int64_t)a.T * a.H / (16 * waves) + a.B;  // at least as many as there are
+  if (tiles > 0x7fffffffll) return AFA_E_SHAPE;
+  if (waves == 8)
+    hipLaunchKernelGGL((latent_kernel<DT, L, R, 8>), dim3((unsigned)tiles), dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL((latent_kernel<DT, L, R, 4>), dim3((unsigned)tiles), dim3(256), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+template <int DT>
+int dispatch_latent(const LatentArgs& a, const LatentParams* p, hipStream_t s) {
+  const int waves = latent_waves(p);
+  if (p->R == 64) {
+    if (p->L == 512) return launch_latent<DT, 512, 64>(a, waves, s);
+    if (p->L == 256) return launch_latent<DT, 256, 64>(a, waves, s);
+    return launch_latent<DT, 128, 64>(a, waves, s);
+  }
+  if (p->L == 512) return launch_latent<DT, 512, 0>(a, waves, s);
+  if (p->L == 256) return launch_latent<DT, 256, 0>(a, waves, s);
+  return launch_latent<DT, 128, 0>(a, waves, s);
+}
+
+}  // namespace
+}  // namespace afa
+
+extern "C" int launch_latent_attention(void* stream, const void* q, const void* q_rope, const void* kv_cache,
+                                       const int32_t* block_table, const int32_t* cu_seqlens_q, const int32_t* seqused_kv,
+                                       void* out, float* softmax_lse, const LatentParams* p) {
+  using namespace afa;
+  const int status = check_latent(p);
+  if (status) return status;
+  if (!q || !kv_cache || !block_table || !cu_seqlens_q || !seqused_kv || !out || (p->R && !q_rope)) return AFA_E_NULL;
+  if (p->T == 0) return AFA_OK;
+  if (!rows_fit(q, p->q_stride_t, p->q_stride_h) || !rows_fit(out, p->out_stride_t, p->out_stride_h) ||
+      (p->R && !rows_fit(q_rope, p->q_rope_stride_t, p->q_rope_stride_h)) || !rows_fit(kv_cache, 0, 0))
+    return AFA_E_SHAPE;
+  LatentArgs a;
+  a.q = q;
+  a.q_rope = q_rope;
+  a.cache = kv_cache;
+  a.table = block_table;
+  a.cu = cu_seqlens_q;
+  a.used = seqused_kv;
+  a.out = out;
+  a.lse = softmax_lse;
+  a.q_t = p->q_stride_t;
+  a.q_h = p->q_stride_h;
+  a.qr_t = p->q_rope_stride_t;
+  a.qr_h = p->q_rope_stride_h;
+  a.o_t = p->out_stride_t;
+  a.o_h = p->out_stride_h;
+  a.T = p->T;
+  a.B = p->B;
+  a.H = p->H;
+  a.W = p->W;
+  a.page_shift = __builtin_ctz((unsigned)p->PAGE);
+  a.blocks = p->BLOCKS;
+  a.causal = p->causal ? 1 : 0;
+  a.scale = p->scale;
+  return p->dtype == AFA_DTYPE_F16 ? dispatch_latent<DT_F16>(a, p, (hipStream_t)stream)
+                                   : dispatch_latent<DT_BF16>(a, p, (hipStream_t)stream);
+}
+
+extern "C" int launch_latent_attention_expanded(void* stream, const void* q, const void* k_nope, const void* k_rope,
+                                                const void* v, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                                void* out, float* softmax_lse, const LatentExpandedParams* p) {
+  using namespace afa;
+  if (!p || !q || !cu_seqlens_q || !cu_seqlens_k || !out) return AFA_E_NULL;
+  if (p->dtype != AFA_DTYPE_BF16 && p->dtype != AFA_DTYPE_F16) return AFA_E_DTYPE;
+  if (p->Tq < 0 || p->Tk < 0 || p->B <= 0 || p->H <= 0 || p->Tq > 0x7fffff00 || p->Tk > 0x7fffff00) return AFA_E_SHAPE;
+  if (p->D != 128 || p->R != 64 || !(p->scale > 0.0f)) return AFA_E_SHAPE;
+  if (p->Tk > 0 && (!k_nope || !k_rope || !v)) return AFA_E_NULL;
+  if (!rows_fit(q, p->q_stride_t, p->q_stride_h) || !rows_fit(out, p->out_stride_t, p->out_stride_h) ||
+      !rows_fit(k_nope, p->k_stride_t, p->k_stride_h) || !rows_fit(k_rope, p->k_rope_stride_t, 0) ||
+      !rows_fit(v, p->v_stride_t, p->v_stride_h))
+    return AFA_E_SHAPE;
+  for (int64_t stride : {p->k_stride_t, p->k_rope_stride_t, p->v_stride_t})
+    if (stride < 0 || stride >= (1ll << 23)) return AFA_E_SHAPE;  // 64 rows span less than 2^31 bytes
+  if (p->Tq == 0) return AFA_OK;
+  const int64_t blocks = ((int64_t)p->Tq / 256 + p->B) * p->H;
+  if (blocks > 0x7fffffffll) return AFA_E_SHAPE;
+  ExpandedArgs a;
+  a.q = q;
+  a.k = k_nope;
+  a.k_rope = k_rope;
+  a.v = v;
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.out = out;
+  a.lse = softmax_lse;
+  a.q_t = p->q_stride_t;
+  a.q_h = p->q_stride_h;
+  a.k_t = p->k_stride_t;
+  a.k_h = p->k_stride_h;
+  a.kr_t = p->k_rope_stride_t;
+  a.v_t = p->v_stride_t;
+  a.v_h = p->v_stride_h;
+  a.o_t = p->out_stride_t;
+  a.o_h = p->out_stride_h;
+  a.Tq = p->Tq;
+  a.Tk = p->Tk;
+  a.B = p->B;
+  a.H = p->H;
+  a.causal = p->causal ? 1 : 0;
+  a.scale = p->scale;
+  if (p->dtype == AFA_DTYPE_F16)
+    hipLaunchKernelGGL(expanded_kernel<DT_F16>, dim3((unsigned)blocks), dim3(512), 0, (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL(expanded_kernel<DT_BF16>, dim3((unsigned)blocks), dim3(512), 0, (hipStream_t)stream, a);
+  return (int)hipGetLastError();
+}

@@ -1,0 +1,118 @@
+"""Latent attention of prompts, expanded form.
+
+Keys and values of every head are expanded from the latents by the caller (one
+matrix product), and each head's keys share one rotary part:
+``s_j = SCALE (q[:128] . k_nope[j, h] + q[128:] . k_rope[j])``,
+``out = softmax(s) v[:, h]``. 640 flops a (query, key, head) instead of the
+absorbed form's 2176 at a latent of 512
+(``ascendflow_amd.sparse_attention.latent_attention``). The two parts of a key
+are read from where they lie: no per-head copy of ``k_rope`` is made.
+"""
+
+from __future__ import annotations
+
+import ctypes as ct
+
+import torch
+
+from .. import _native
+from .._tensors import (DTYPES, check_apart, check_distinct_rows, check_rows, check_tensor, kept_by_value, launch_on,
+                        live_strides, require)
+
+_STORAGE = {dt: name for name, dt in DTYPES.items()}
+D, R = 128, 64  # columns of k_nope and v, and of k_rope
+
+
+@kept_by_value
+def _params(dtype, Tq, Tk, B, H, qt, qh, kt, kh, rt, vt, vh, ot, oh, SCALE, causal):
+    """Launcher parameters of a call of checked sizes (not changed afterwards)."""
+    require(B > 0 and H > 0, "positive request and head counts")
+    require(SCALE > 0, "positive attention scale")
+    return ct.pointer(_native.LatentExpandedParams(
+        dtype=_native.AFA_DTYPE[dtype], causal=int(causal), Tq=Tq, Tk=Tk, B=B, H=H, D=D, R=R, q_stride_t=qt,
+        q_stride_h=qh, k_stride_t=kt, k_stride_h=kh, k_rope_stride_t=rt, v_stride_t=vt, v_stride_h=vh, out_stride_t=ot,
+        out_stride_h=oh, scale=SCALE, reserved=0))
+
+
+def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, *, SCALE, CAUSAL=True, out=None,
+                              softmax_lse=None):
+    """Returns ``out`` [Tq, H, 128]: attention of ragged requests over their own keys.
+
+    ``q`` [Tq, H, 192] (128 columns against ``k_nope``, 64 rotated ones against
+    ``k_rope``), ``k_nope`` and ``v`` [Tk, H, 128], ``k_rope`` [Tk, 64]: bf16 or
+    f16, any strides of tokens and heads (views of one projection), rows on 16
+    bytes. ``cu_seqlens_q`` and ``cu_seqlens_k`` int32 [B + 1]. With ``CAUSAL``
+    query i of a request's nq sees keys up to nk - nq + i (the queries are the
+    last of the context), without all of them. ``softmax_lse`` (optional float32
+    [Tq, H]) receives ln(sum_j exp(s_j)).
+
+    A query that sees no key gets zeros and -inf; queries at or past
+    ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``).
+    Keys and values that some query of a request sees have to be finite.
+    """
+    require(isinstance(q, torch.Tensor) and q.dim() == 3, f"q must be [Tq, H, {D + R}]")
+    b16 = q.dtype
+    require(b16 in _STORAGE, f"q dtype {b16} is not supported; expected bf16 or f16")
+    Tq, H = q.shape[:2]
+    require(isinstance(k_rope, torch.Tensor) and k_rope.dim() == 2, f"k_rope must be [Tk, {R}]")
+    Tk = k_rope.shape[0]
+    check_rows("q", q, (Tq, H, D + R), b16)
+    device = q.device
+    check_rows("k_nope", k_nope, (Tk, H, D), b16, device)
+    check_rows("k_rope", k_rope, (Tk, R), b16, device)
+    check_rows("v", v, (Tk, H, D), b16, device)
+    require(isinstance(cu_seqlens_q, torch.Tensor) and cu_seqlens_q.dim() == 1, "cu_seqlens_q must be int32 [B + 1]")
+    B = cu_seqlens_q.numel() - 1
+    check_tensor("cu_seqlens_q", cu_seqlens_q, (B + 1,), torch.int32, device)
+    check_tensor("cu_seqlens_k", cu_seqlens_k, (B + 1,), torch.int32, device)
+    inputs = [("q", q, False), ("k_nope", k_nope, False), ("k_rope", k_rope, False), ("v", v, False),
+              ("cu_seqlens_q", cu_seqlens_q, False), ("cu_seqlens_k", cu_seqlens_k, False)]
+    if out is None:
+        out = torch.empty((Tq, H, D), dtype=b16, device=device)
+    else:
+        check_rows("out", out, (Tq, H, D), b16, device)
+        check_distinct_rows("out", out)
+        check_apart(inputs + [("out", out, True)])
+    if softmax_lse is not None:
+        check_tensor("softmax_lse", softmax_lse, (Tq, H), torch.float32, device)
+        check_apart(inputs + [("out", out, False), ("softmax_lse", softmax_lse, True)])
+    strides = []
+    for name, t in (("q", q), ("k_nope", k_nope), ("k_rope", k_rope), ("v", v), ("out", out)):
+        mine = live_strides(t)[:-1]
+        require(all(s % 8 == 0 for s in mine) and t.data_ptr() % 16 == 0, f"{name} rows must lie on 16-byte boundaries")
+        if name in ("k_nope", "k_rope", "v"):
+            require(mine[0] < 2**23, f"{name} tokens may lie at most 2^23 - 1 elements apart")
+        strides += mine
+    params = _params(_STORAGE[b16], Tq, Tk, B, H, *strides, float(SCALE), bool(CAUSAL))
+    if Tq:
+        status = launch_on(q.get_device(), _native.library().launch_latent_attention_expanded, q.data_ptr(),
+                           k_nope.data_ptr(), k_rope.data_ptr(), v.data_ptr(), cu_seqlens_q.data_ptr(),
+                           cu_seqlens_k.data_ptr(), out.data_ptr(),
+                           None if softmax_lse is None else softmax_lse.data_ptr(), params)
+        if status:
+            _native.check(status, "launch_latent_attention_expanded")
+    return out
+
+
+@torch.library.custom_op("ascendflow_amd::latent_attention_expanded", mutates_args=())
+def latent_attention_expanded_op(
+    q: torch.Tensor,
+    k_nope: torch.Tensor,
+    k_rope: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: torch.Tensor,
+    softmax_scale: float,
+    causal: bool = True,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Framework-facing form of ``latent_attention_expanded``: returns (out, softmax_lse float32 [Tq, H])."""
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    out = latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, SCALE=softmax_scale, CAUSAL=causal,
+                                    softmax_lse=lse)
+    return out, lse
+
+
+@latent_attention_expanded_op.register_fake
+def _(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, causal=True):
+    return (torch.empty((*q.shape[:2], D), dtype=q.dtype, device=q.device),
+            q.new_empty(q.shape[:2], dtype=torch.float32))

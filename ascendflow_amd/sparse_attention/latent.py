@@ -1,0 +1,136 @@
+"""Latent attention over a paged cache, absorbed form.
+
+The dense counterpart of ``sparse_mla`` over the same kind of cache: every
+token of the context is attended, no row is selected. A cache row holds the
+latent c of a token, which is key and value of all heads, and behind it the
+rotary key that all heads share (or nothing, where the rotation lies inside c as
+in ``ori_kv``). With the key projection absorbed into the query,
+``s_j = SCALE (q . c_j + q_rope . k_rope_j)`` and ``out = softmax(s) c``; the
+value projection is applied to ``out`` by the caller. One call serves single-token
+decode, verification of several tokens a request, and chunks of prompts
+(whole prompts are cheaper in the expanded form,
+``ascendflow_amd.flash_attention.latent_attention_expanded``).
+"""
+
+from __future__ import annotations
+
+import ctypes as ct
+from typing import Optional
+
+import torch
+
+from .. import _native
+from .._tensors import (DTYPES, check_apart, check_distinct_rows, check_rows, check_tensor, kept_by_value, launch_on,
+                        live_strides, require)
+
+_STORAGE = {dt: name for name, dt in DTYPES.items()}
+
+
+def row_strides(name, tensor):
+    """(token, head) strides of a tensor whose rows the kernels read in 16-byte pieces."""
+    t, h = live_strides(tensor)[:2]
+    require(t % 8 == 0 and h % 8 == 0 and tensor.data_ptr() % 16 == 0, f"{name} rows must lie on 16-byte boundaries")
+    return t, h
+
+
+@kept_by_value
+def _params(dtype, T, B, H, L, R, PAGE, W, BLOCKS, qt, qh, rt, rh, ot, oh, SCALE, causal):
+    """Launcher parameters of a call of checked sizes (not changed afterwards)."""
+    require(H > 0 and B > 0 and W > 0 and BLOCKS > 0, "heads, requests and pages must not be empty")
+    require(L in (128, 256, 512), "the latent width (columns of q) must be 128, 256 or 512")
+    require(R in (0, 64), "the rotary width must be 64, or 0 without q_rope")
+    require(PAGE >= 16 and PAGE & (PAGE - 1) == 0, "PAGE must be a power of two from 16 on")
+    require(SCALE > 0, "positive attention scale")
+    return ct.pointer(_native.LatentParams(
+        dtype=_native.AFA_DTYPE[dtype], causal=int(causal), T=T, B=B, H=H, L=L, R=R, PAGE=PAGE, W=W, BLOCKS=BLOCKS,
+        q_stride_t=qt, q_stride_h=qh, q_rope_stride_t=rt, q_rope_stride_h=rh, out_stride_t=ot, out_stride_h=oh,
+        scale=SCALE, reserved=0))
+
+
+def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCALE, q_rope=None, CAUSAL=True, out=None,
+                     softmax_lse=None):
+    """Returns ``out`` [T, H, L]: dense attention of every token over its request's cache rows.
+
+    ``q`` [T, H, L] (L 128, 256 or 512) and ``q_rope`` [T, H, 64], or None:
+    bf16 or f16, any strides of tokens and heads, rows on 16 bytes. ``kv_cache``
+    [BLOCKS, PAGE, 1, L + R], contiguous, R the width of ``q_rope`` or 0, PAGE a
+    power of two from 16 on. ``block_table`` int32 [B, W], ``cu_seqlens_q`` int32
+    [B + 1], ``seqused_kv`` int32 [B]: rows of each request, the new tokens'
+    included (``append_paged_kv`` writes them). With ``CAUSAL`` token j of a
+    request's n sees rows up to ``seqused_kv[b] - n + j``, without all of them.
+    ``softmax_lse`` (optional float32 [T, H]) receives ln(sum_j exp(s_j)).
+
+    A token that sees no row gets zeros and -inf; tokens at or past
+    ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``).
+    Rows behind ``seqused_kv`` are never read and pages outside the cache hold no
+    keys, but the rows that some token of a request sees have to be finite.
+    """
+    require(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [T, H, L]")
+    b16 = q.dtype
+    require(b16 in _STORAGE, f"q dtype {b16} is not supported; expected bf16 or f16")
+    T, H, L = q.shape
+    R = 0
+    if q_rope is not None:
+        require(isinstance(q_rope, torch.Tensor) and q_rope.dim() == 3, "q_rope must be [T, H, R]")
+        R = q_rope.shape[2]
+    require(isinstance(kv_cache, torch.Tensor) and kv_cache.dim() == 4, "kv_cache must be [BLOCKS, PAGE, 1, L + R]")
+    BLOCKS, PAGE = kv_cache.shape[:2]
+    require(isinstance(block_table, torch.Tensor) and block_table.dim() == 2, "block_table must be int32 [B, W]")
+    B, W = block_table.shape
+    i32 = torch.int32
+    check_rows("q", q, q.shape, b16)
+    device = q.device
+    check_tensor("kv_cache", kv_cache, (BLOCKS, PAGE, 1, L + R), b16, device)
+    check_tensor("block_table", block_table, (B, W), i32, device)
+    check_tensor("cu_seqlens_q", cu_seqlens_q, (B + 1,), i32, device)
+    check_tensor("seqused_kv", seqused_kv, (B,), i32, device)
+    if q_rope is not None:
+        check_rows("q_rope", q_rope, (T, H, R), b16, device)
+    if softmax_lse is not None:
+        check_tensor("softmax_lse", softmax_lse, (T, H), torch.float32, device)
+    if out is None:
+        out = torch.empty((T, H, L), dtype=b16, device=device)
+    else:
+        check_rows("out", out, (T, H, L), b16, device)
+        check_distinct_rows("out", out)
+        check_apart([("q", q, False), ("q_rope", q_rope, False), ("kv_cache", kv_cache, False),
+                     ("block_table", block_table, False), ("cu_seqlens_q", cu_seqlens_q, False),
+                     ("seqused_kv", seqused_kv, False), ("out", out, True)])
+    if softmax_lse is not None:
+        check_apart([("q", q, False), ("q_rope", q_rope, False), ("kv_cache", kv_cache, False),
+                     ("block_table", block_table, False), ("cu_seqlens_q", cu_seqlens_q, False),
+                     ("seqused_kv", seqused_kv, False), ("out", out, False), ("softmax_lse", softmax_lse, True)])
+    params = _params(_STORAGE[b16], T, B, H, L, R, PAGE, W, BLOCKS, *row_strides("q", q),
+                     *((0, 0) if q_rope is None else row_strides("q_rope", q_rope)), *row_strides("out", out),
+                     float(SCALE), bool(CAUSAL))
+    if T:
+        status = launch_on(q.get_device(), _native.library().launch_latent_attention, q.data_ptr(),
+                           None if q_rope is None else q_rope.data_ptr(), kv_cache.data_ptr(), block_table.data_ptr(),
+                           cu_seqlens_q.data_ptr(), seqused_kv.data_ptr(), out.data_ptr(),
+                           None if softmax_lse is None else softmax_lse.data_ptr(), params)
+        if status:
+            _native.check(status, "launch_latent_attention")
+    return out
+
+
+@torch.library.custom_op("ascendflow_amd::latent_attention", mutates_args=())
+def latent_attention_op(
+    q: torch.Tensor,
+    q_rope: Optional[torch.Tensor],
+    kv_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    seqused_kv: torch.Tensor,
+    softmax_scale: float,
+    causal: bool = True,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Framework-facing form of ``latent_attention``: returns (out [T, H, L], softmax_lse float32 [T, H])."""
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    out = latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, SCALE=softmax_scale, q_rope=q_rope,
+                           CAUSAL=causal, softmax_lse=lse)
+    return out, lse
+
+
+@latent_attention_op.register_fake
+def _(q, q_rope, kv_cache, block_table, cu_seqlens_q, seqused_kv, softmax_scale, causal=True):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device), q.new_empty(q.shape[:2], dtype=torch.float32)

@@ -1,0 +1,213 @@
+"""Rotary positions of queries, keys and attention outputs.
+
+The attention operators take query and cache rows already rotated.
+``apply_rotary`` turns the pairs of a part of each head by ``position *
+frequency``, in either pair layout, in place or into a new tensor; ``inverse=True`` turns them back, which an attention
+whose values carry the rotation (``sparse_mla`` with the rotated columns inside
+D) needs on its output. ``rotary_frequencies`` gives the frequencies, scaled for
+long contexts or not.
+
+The result carries its gradient (the inverse rotation of the incoming one), and
+the call is registered as the torch custom op ``ascendflow_amd::apply_rotary``
+with a shape-only fake and the same gradient.
+"""
+
+from __future__ import annotations
+
+import ctypes as ct
+import math
+
+import torch
+
+from .. import _native
+from .._tensors import DTYPES, check_apart, check_distinct_rows, check_rows, kept_by_value, launch_on, live_strides, require
+
+LAYOUTS = {"half": 0, "interleaved": 1}
+_STORAGE = {dt: name for name, dt in DTYPES.items()}
+
+
+def rotary_frequencies(R, base=10000.0, *, scaling=None, factor=1.0, original_length=4096, beta_fast=32.0, beta_slow=1.0,
+                       device="cuda"):
+    """Float64 [R / 2]: radians per position of each pair, ``base ** (-2 i / R)``.
+
+    ``scaling`` stretches a model trained at ``original_length`` tokens to
+    ``factor`` times that: ``"linear"`` divides every frequency by ``factor``,
+    ``"ntk"`` raises the base so that the lowest frequency is divided by it, and
+    ``"yarn"`` keeps the pairs that turn at least ``beta_fast`` times within
+    ``original_length``, divides those that turn at most ``beta_slow`` times and
+    blends the others between (with ``rotary_magnitude(factor)`` as magnitude).
+    """
+    require(isinstance(R, int) and R >= 2 and R % 2 == 0, "R must be a positive even number")
+    require(scaling in (None, "linear", "ntk", "yarn"), 'scaling must be None, "linear", "ntk" or "yarn"')
+    require(base > 1.0 and factor >= 1.0 and original_length > 0, "base > 1, factor >= 1, original_length > 0")
+    if scaling == "ntk" and R > 2:
+        base = base * factor ** (R / (R - 2))
+    frequencies = base ** (-torch.arange(0, R, 2, dtype=torch.float64) / R)
+    if scaling == "linear":
+        frequencies = frequencies / factor
+    elif scaling == "yarn":
+        require(beta_fast > beta_slow > 0, "beta_fast > beta_slow > 0")
+        # Pair index at which a frequency turns `turns` times within the original length.
+        low, high = (R * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+                     for turns in (beta_fast, beta_slow))
+        low, high = max(0, math.floor(low)), min(R - 1, math.ceil(high))
+        ramp = ((torch.arange(R // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+        frequencies = frequencies / factor * ramp + frequencies * (1 - ramp)
+    return frequencies.to(device)
+
+
+def rotary_magnitude(factor, coefficient=1.0):
+    """Magnitude that goes with ``"yarn"`` frequencies: 0.1 coefficient ln(factor) + 1."""
+    return 0.1 * coefficient * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+
+
+@kept_by_value
+def _params(dtype, layout, inverse, position_bytes, H, D, R, offset, B, S, xb, xs, xh, ob, os, oh, position_stride, magnitude):
+    """Launcher parameters of a call of checked sizes (not changed afterwards)."""
+    require(layout in LAYOUTS, 'layout must be "half" or "interleaved"')
+    require(R >= 2 and 0 <= offset <= D - R, f"the rotated columns {offset} to {offset + R} must lie inside the head ({D})")
+    require(math.isfinite(magnitude), "magnitude must be finite")
+    return ct.pointer(_native.RotaryParams(
+        dtype=_native.AFA_DTYPE[dtype], layout=LAYOUTS[layout], inverse=int(inverse), position_bytes=position_bytes,
+        H=H, D=D, R=R, offset=offset, B=B, S=S, x_stride_b=xb, x_stride_s=xs, x_stride_h=xh, out_stride_b=ob,
+        out_stride_s=os, out_stride_h=oh, position_stride_b=position_stride, magnitude=magnitude, reserved=0))
+
+
+def _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out):
+    require(isinstance(x, torch.Tensor) and x.dim() in (3, 4), "x must be [T, H, D] or [B, H, S, D]")
+    require(x.dtype in _STORAGE, f"x dtype {x.dtype} is not supported; expected bf16 or f16")
+    if x.dim() == 3:
+        (S, H, D), B = x.shape, 1
+    else:
+        B, H, S, D = x.shape
+    require(H > 0 and D > 0, "x must have heads and columns")
+    require(isinstance(positions, torch.Tensor) and positions.dtype in (torch.int32, torch.int64),
+            "positions must be an int32 or int64 tensor")
+    require(tuple(positions.shape) == (S,) or (x.dim() == 4 and tuple(positions.shape) == (B, S)),
+            f"positions shape {tuple(positions.shape)} does not fit x {tuple(x.shape)}")
+    require(isinstance(frequencies, torch.Tensor) and frequencies.dim() == 1 and frequencies.numel() > 0,
+            "frequencies must be a float64 [R / 2] tensor")
+    check_rows("x", x, x.shape, x.dtype)
+    device = x.device
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    elif out is not x:
+        check_rows("out", out, x.shape, x.dtype, device)
+    check_rows("positions", positions, positions.shape, positions.dtype, device)
+    check_rows("frequencies", frequencies, frequencies.shape, torch.float64, device)
+    in_place = out is x or (out.data_ptr() == x.data_ptr() and out.stride() == x.stride())
+    check_distinct_rows("out", out)
+    check_apart([("x", None if in_place else x, False), ("positions", positions, False),
+                 ("frequencies", frequencies, False), ("out", out, True)])
+    xs, os = live_strides(x), live_strides(out)
+    if x.dim() == 3:
+        xs, os = (0, xs[0], xs[1]), (0, os[0], os[1])
+    else:
+        xs, os = (xs[0], xs[2], xs[1]), (os[0], os[2], os[1])
+    params = _params(_STORAGE[x.dtype], layout, bool(inverse), positions.element_size(), H, D, 2 * frequencies.numel(),
+                     offset, B, S, *xs, *os, live_strides(positions)[0] if positions.dim() == 2 else 0, float(magnitude))
+    if x.numel():
+        status = launch_on(x.get_device(), _native.library().launch_apply_rotary, x.data_ptr(), positions.data_ptr(),
+                           frequencies.data_ptr(), out.data_ptr(), params)
+        if status:
+            _native.check(status, "launch_apply_rotary")
+    return out
+
+
+_EAGER = "ascendflow_amd_eager_graph"
+
+
+def _watch_leaf(ctx):
+    """Marks the node that takes the gradient of a leaf as part of an eager graph, or, under capture, refuses it if marked.
+
+    That node remembers the stream it was made on for as long as some graph holds
+    it. A backward pass captured into a HIP graph would record an event on that
+    other stream, which breaks the capture and ends the process."""
+    node = ctx.next_functions[0][0] if ctx.next_functions else None
+    if node is None or node.next_functions:  # x is no leaf
+        return
+    if not torch.cuda.is_current_stream_capturing():
+        node.metadata[_EAGER] = True
+    elif node.metadata.get(_EAGER):
+        raise RuntimeError("a gradient cannot be captured while a graph recorded eagerly from the same tensor lives: "
+                           "drop its results before the capture")
+
+
+class _Rotary(torch.autograd.Function):
+    """The rotation as a differentiable map of x: its gradient is the inverse rotation, magnitude kept."""
+
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, layout, offset, magnitude, inverse):
+        _watch_leaf(ctx)
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = layout, offset, magnitude, inverse
+        return _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, None)
+
+    @staticmethod
+    def backward(ctx, grad):
+        layout, offset, magnitude, inverse = ctx.how
+        return _Rotary.apply(_dense_rows(grad), *ctx.saved_tensors, layout, offset, magnitude, not inverse), *[None] * 6
+
+
+def _dense_rows(grad):
+    """A gradient with contiguous rows (a sum's arrives expanded from one element)."""
+    return grad if grad.shape[-1] <= 1 or grad.stride(-1) == 1 else grad.contiguous()
+
+
+def apply_rotary(x, positions, frequencies, *, layout="half", offset=0, magnitude=1.0, inverse=False, out=None):
+    """Returns ``x`` with the R = 2 len(frequencies) columns from ``offset`` on of every head rotated.
+
+    ``x`` is [T, H, D] with ``positions`` [T], or [B, H, S, D] with ``positions``
+    [S] or [B, S]; bf16 or f16, any strides of tokens and heads, contiguous
+    columns. ``frequencies``: float64 [R / 2], radians per position. Pair i is
+    columns (i, i + R / 2) of the part with ``layout="half"``, (2 i, 2 i + 1) with
+    ``"interleaved"``. The rotated pairs are multiplied by ``magnitude``;
+    ``inverse`` turns them by the negative angle. Positions may be any integers
+    of their type, negative ones included; angles are formed in float64.
+
+    Without ``out`` the result is a new contiguous tensor and carries its
+    gradient with respect to ``x`` (a captured backward pass of a leaf needs the
+    leaf's eager graphs gone, and is refused otherwise); with ``out`` (``x`` itself for a rotation in
+    place, otherwise memory apart from it) it is written there, without one.
+    Raises ``ValueError`` for shapes, types, devices or overlaps that do not fit.
+    """
+    if out is not None or not (torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad):
+        require(out is None or not (torch.is_grad_enabled() and (x.requires_grad or out.requires_grad)),
+                "out cannot be given where a gradient is recorded")
+        return _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out)
+    return _Rotary.apply(x, positions, frequencies, layout, offset, float(magnitude), bool(inverse))
+
+
+@torch.library.custom_op("ascendflow_amd::apply_rotary", mutates_args=())
+def apply_rotary_op(
+    x: torch.Tensor,
+    positions: torch.Tensor,
+    frequencies: torch.Tensor,
+    layout: str = "half",
+    offset: int = 0,
+    magnitude: float = 1.0,
+    inverse: bool = False,
+) -> torch.Tensor:
+    """Framework-facing form of ``apply_rotary``: returns a new contiguous tensor."""
+    return _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, None)
+
+
+@apply_rotary_op.register_fake
+def _(x, positions, frequencies, layout="half", offset=0, magnitude=1.0, inverse=False):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _op_context(ctx, inputs, output):
+    _, positions, frequencies, *how = inputs
+    _watch_leaf(ctx)
+    ctx.save_for_backward(positions, frequencies)
+    ctx.how = how
+
+
+def _op_gradient(ctx, grad):
+    layout, offset, magnitude, inverse = ctx.how
+    turned = apply_rotary_op(_dense_rows(grad), *ctx.saved_tensors, layout, offset, magnitude, not inverse)
+    return turned, None, None, None, None, None, None
+
+
+apply_rotary_op.register_autograd(_op_gradient, setup_context=_op_context)

@@ -302,6 +302,105 @@ int launch_sparse_topk_indices_split(void* stream, const float* scores, const in
  * filter pass, 3 the streaming passes. For tests and profiles. */
 int form_sparse_topk_indices(int64_t form[3], const SparseTopkParams* params, int with_workspace);
 
+/* Rotary positions. Pairs (u, v) of the R columns from `offset` on of every row
+ * turn by the angle position * frequencies[i] (radians, float64 [R / 2]):
+ *   u' = magnitude (u cos - v sin), v' = magnitude (u sin + v cos);
+ * pair i is columns (i, i + R / 2) with layout 0 (halves) or (2 i, 2 i + 1) with
+ * layout 1 (interleaved). inverse turns by the negative angle with the same
+ * magnitude: the transposed map, which is the gradient. x and out [B][S][H][D]
+ * with strides in elements, columns contiguous; the other columns are copied,
+ * or, where out is x (equal strides), not touched. positions int32 or int64
+ * (position_bytes 4 or 8) [S], position_stride_b elements apart for each b.
+ * 16-byte accesses where R % 16, offset, D and the strides allow them. */
+typedef struct RotaryParams {
+  int32_t dtype;
+  int32_t layout;          /* 0 halves, 1 interleaved */
+  int32_t inverse;
+  int32_t position_bytes;  /* 4 or 8 */
+  int32_t H, D, R, offset;
+  int64_t B, S;
+  int64_t x_stride_b, x_stride_s, x_stride_h;
+  int64_t out_stride_b, out_stride_s, out_stride_h;
+  int64_t position_stride_b;
+  float magnitude;
+  int32_t reserved;
+} RotaryParams;
+
+int launch_apply_rotary(void* stream, const void* x, const void* positions, const double* frequencies, void* out,
+                        const RotaryParams* params);
+
+/* Append of new tokens to a paged cache, the rotation applied on the way. Token
+ * t of request b (cu_seqlens_q[b] <= t < cu_seqlens_q[b + 1]) goes to position
+ * p = seqused_kv[b] - cu_seqlens_q[b + 1] + t (seqused_kv counts the new tokens,
+ * as seqused_ori_kv does), row p % PAGE of page block_table[b][p / PAGE] of
+ * k_cache [BLOCKS][PAGE][HKV][DK]. Its columns offset .. offset + R - 1 are
+ * rotated by p as in launch_apply_rotary (R = 0: none); with `rope` [T][HKV][R]
+ * they come from there, are the row's last (offset = DK - R), and k [T][HKV]
+ * holds the DK - R others. v [T][HKV][DV] is copied to v_cache
+ * [BLOCKS][PAGE][HKV][DV] (DV = 0: none). Strides in elements, columns
+ * contiguous. Tokens at or past cu_seqlens_q[B], positions below 0 or beyond W
+ * pages, and pages outside [0, BLOCKS) write nothing. No two new tokens may
+ * name the same cache row. */
+typedef struct AppendPagedKvParams {
+  int32_t dtype;
+  int32_t layout;
+  int32_t T, B, W, PAGE, BLOCKS;
+  int32_t HKV, DK, DV, R, offset;
+  int64_t k_stride_t, k_stride_h, rope_stride_t, rope_stride_h, v_stride_t, v_stride_h;
+  float magnitude;
+  int32_t reserved;
+} AppendPagedKvParams;
+
+int launch_append_paged_kv(void* stream, const void* k, const void* rope, const void* v, const int32_t* block_table,
+                           const int32_t* cu_seqlens_q, const int32_t* seqused_kv, const double* frequencies,
+                           void* k_cache, void* v_cache, const AppendPagedKvParams* params);
+
+/* Latent attention, absorbed form, over a paged cache of rows [c | k_rope] of
+ * L + R columns, kv_cache [BLOCKS][PAGE][L + R]: for token t, head h of request b
+ *   s_j = scale (q[t][h] . c_j + q_rope[t][h] . k_rope_j),  out[t][h] = softmax(s) c,
+ * over the rows j < seqused_kv[b], and, causal, j <= seqused_kv[b] - n + i for
+ * the i-th of the request's n tokens. L 128, 256 or 512, R 0 or 64, PAGE a power
+ * of two from 16 on. q and out [T][H][L], q_rope [T][H][R] with strides in
+ * elements (multiples of 8; rows contiguous and on 16 bytes). Rows behind
+ * seqused_kv are not read; pages outside [0, BLOCKS) hold no keys; a token that
+ * sees no key gets zeros; tokens at or past cu_seqlens_q[B] are left as they
+ * were. softmax_lse f32 [T][H] or NULL: ln(sum_j e^(s_j)), -inf without a key.
+ * Values of a row that some token of the request sees have to be finite. */
+typedef struct LatentParams {
+  int32_t dtype;
+  int32_t causal;
+  int32_t T, B, H, L, R;
+  int32_t PAGE, W, BLOCKS;
+  int64_t q_stride_t, q_stride_h, q_rope_stride_t, q_rope_stride_h, out_stride_t, out_stride_h;
+  float scale;
+  int32_t reserved;
+} LatentParams;
+
+int launch_latent_attention(void* stream, const void* q, const void* q_rope, const void* kv_cache,
+                            const int32_t* block_table, const int32_t* cu_seqlens_q, const int32_t* seqused_kv,
+                            void* out, float* softmax_lse, const LatentParams* params);
+
+/* Latent attention, expanded form, ragged requests: for query i of the nq and
+ * key j of the nk of request b, head h
+ *   s_j = scale (q[i][h][0:D] . k_nope[j][h] + q[i][h][D:D+R] . k_rope[j]),  out[i][h] = softmax(s) v[:, h],
+ * causal: j <= nk - nq + i. D 128, R 64. q [Tq][H][D + R], k_nope and v
+ * [Tk][H][D], k_rope [Tk][R], out [Tq][H][D], strides in elements (multiples of
+ * 8, rows contiguous and on 16 bytes, token strides of keys and values below
+ * 2^23). softmax_lse as above, f32 [Tq][H] or NULL. */
+typedef struct LatentExpandedParams {
+  int32_t dtype;
+  int32_t causal;
+  int32_t Tq, Tk, B, H, D, R;
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, k_rope_stride_t, v_stride_t, v_stride_h, out_stride_t,
+      out_stride_h;
+  float scale;
+  int32_t reserved;
+} LatentExpandedParams;
+
+int launch_latent_attention_expanded(void* stream, const void* q, const void* k_nope, const void* k_rope, const void* v,
+                                     const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, void* out,
+                                     float* softmax_lse, const LatentExpandedParams* params);
+
 /* Measurement helpers (no reference kernel; the reference sweeps a >= 4x L2
  * buffer before each timed launch, benchmarks/cache.py:13-92 and
  * benchmarks/cache_sweep.py:15-32). Reads `bytes` of `buffer` through the
