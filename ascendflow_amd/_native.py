@@ -51,6 +51,8 @@ EXPORTS = (
     "launch_apply_rotary",
     "launch_append_paged_kv",
     "launch_latent_attention",
+    "workspace_size_latent_attention",
+    "form_latent_attention",
     "launch_latent_attention_expanded",
     "launch_cache_flush",
     "launch_clock_probe",
@@ -180,7 +182,9 @@ _SIGNATURES = {
     ),
     "launch_apply_rotary": ([_P] * 5 + [ct.POINTER(RotaryParams)], ct.c_int),
     "launch_append_paged_kv": ([_P] * 10 + [ct.POINTER(AppendPagedKvParams)], ct.c_int),
-    "launch_latent_attention": ([_P] * 9 + [ct.POINTER(LatentParams)], ct.c_int),
+    "launch_latent_attention": ([_P] * 10 + [ct.c_uint64, ct.POINTER(LatentParams)], ct.c_int),
+    "workspace_size_latent_attention": ([ct.POINTER(ct.c_uint64), ct.POINTER(LatentParams)], ct.c_int),
+    "form_latent_attention": ([ct.POINTER(ct.c_int64), ct.POINTER(LatentParams)], ct.c_int),
     "launch_latent_attention_expanded": ([_P] * 9 + [ct.POINTER(LatentExpandedParams)], ct.c_int),
     "launch_cache_flush": ([_P, _P, ct.c_uint64], ct.c_int),
     "launch_clock_probe": ([_P, _P, ct.c_int32], ct.c_int),

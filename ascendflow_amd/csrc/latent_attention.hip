@@ -44,7 +44,32 @@ struct LatentArgs {
   int64_t q_t, q_h, qr_t, qr_h, o_t, o_h;
   int32_t T, B, H, W, page_shift, blocks, causal;
   float scale;
+  // Split form (below): workgroups, and its workspace.
+  int32_t workers;
+  float* partial_o;         // [2 * workers][rows of a tile][L], not normalised
+  float* partial_ml;        // [2 * workers][rows of a tile][4]: running maximum (log2), sum, sum of rounded weights
+  struct LatentRecord* records;  // [tiles]
+  uint32_t* tile_count;
 };
+
+// A tile of the split form as its merge needs it: its first row is row `row` of
+// the packed rows of the request that starts at token `start`; workgroups
+// first .. last hold parts of it (first == last: the tile is whole and written).
+struct LatentRecord {
+  int32_t start, row, rows;
+  int32_t first, last;
+};
+
+// Split form: the chunks of all tiles, in order, are one sequence that the
+// workgroups share evenly, so that few or unequal requests fill the GPU and end
+// together. A tile counts its chunks (those of its request's last token) and
+// LAT_START chunks for its start and end. A workgroup takes at most one tile's
+// end, whole tiles and one tile's beginning; parts go to the workspace (slot
+// 2 w the end, 2 w + 1 the beginning) as float32 and latent_merge_kernel
+// combines them in order. Everything is computed on the device from
+// cu_seqlens_q and seqused_kv, alike in every workgroup.
+constexpr uint32_t LAT_START = 2;
+constexpr uint32_t LAT_LEAST = 4;  // least chunks (and starts) of a workgroup
 
 // New tokens of request b: cu[b] .. cu[b + 1], held inside [0, T).
 __device__ __forceinline__ void request_tokens(const int32_t* cu, int b, int T, int& start, int& count) {
@@ -93,7 +118,114 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, int B, int T, uint3
   return false;
 }
 
-template <int DT, int L, int R, int NW>
+// Chunks that a request's tiles count in the split form.
+__device__ __forceinline__ uint32_t longest_chunks(int used, int count) {
+  return count > 0 ? ((uint32_t)max(used, 0) + LAT_KEYS - 1) / LAT_KEYS : 0u;
+}
+
+__device__ __forceinline__ uint64_t inclusive_scan64(uint64_t v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint64_t other = __shfl_up((unsigned long long)v, d);
+    if (lane >= d) v += other;
+  }
+  return v;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t uniform64(uint64_t v) {
+  return (uint64_t)(uint32_t)uniform((int)(uint32_t)v) | ((uint64_t)(uint32_t)uniform((int)(uint32_t)(v >> 32)) << 32);
+}
+
+// Where a workgroup of the split form begins.
+struct LatentShare {
+  uint64_t begin, end;       // of the sequence
+  uint64_t total;
+  int32_t workers;           // that have a share
+  int32_t request;
+  uint32_t tile, offset;     // inside the request, inside the tile
+  uint32_t tiles_before;     // of earlier requests
+};
+
+template <int THREADS, int ROWS>
+__device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker, LatentShare& share) {
+  __shared__ uint64_t wave_weight[THREADS / 64];
+  __shared__ uint32_t wave_tiles[THREADS / 64];
+  __shared__ uint32_t found[4];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int per = (a.B + THREADS - 1) / THREADS;  // consecutive requests of a thread
+  auto measure = [&](int b, uint32_t& tiles, uint32_t& each) {
+    int start, count;
+    request_tokens(a.cu, b, a.T, start, count);
+    const int used = (int)min((int64_t)max(a.used[b], 0), (int64_t)a.W << a.page_shift);
+    tiles = ((uint32_t)count * (uint32_t)a.H + ROWS - 1) / ROWS;
+    each = longest_chunks(used, count) + LAT_START;
+  };
+  uint64_t weight = 0;
+  uint32_t tiles = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = tid * per + i;
+    if (b >= a.B) break;
+    uint32_t n, each;
+    measure(b, n, each);
+    weight += (uint64_t)n * each;
+    tiles += n;
+  }
+  const uint64_t upto = inclusive_scan64(weight, lane);
+  const uint32_t tiles_upto = (uint32_t)wave_inclusive_scan((int)tiles);
+  if (lane == 63) {
+    wave_weight[wave] = upto;
+    wave_tiles[wave] = tiles_upto;
+  }
+  __syncthreads();
+  uint64_t before = upto - weight, total = 0;
+  uint32_t tiles_before = tiles_upto - tiles, all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w < wave) {
+      before += wave_weight[w];
+      tiles_before += wave_tiles[w];
+    }
+    total += wave_weight[w];
+    all += wave_tiles[w];
+  }
+  total = uniform64(total);
+  if (worker == 0 && tid == 0) *a.tile_count = all;
+  if (total == 0) return false;
+  const uint64_t most = total / LAT_LEAST;
+  share.workers = most < 1 ? 1 : (most < (uint64_t)a.workers ? (int)most : a.workers);
+  if (worker >= (uint32_t)share.workers) return false;
+  share.total = total;
+  share.begin = total * worker / (uint32_t)share.workers;
+  share.end = total * (worker + 1) / (uint32_t)share.workers;
+  if (share.begin >= before && share.begin < before + weight) {
+    uint64_t at = before;
+    uint32_t done = tiles_before;
+    for (int i = 0; i < per; ++i) {
+      const int b = tid * per + i;
+      uint32_t n, each;
+      measure(b, n, each);
+      if (share.begin < at + (uint64_t)n * each) {
+        const uint32_t inside = (uint32_t)((share.begin - at) / each);
+        found[0] = (uint32_t)b;
+        found[1] = inside;
+        found[2] = (uint32_t)(share.begin - at - (uint64_t)inside * each);
+        found[3] = done;
+        break;
+      }
+      at += (uint64_t)n * each;
+      done += n;
+    }
+  }
+  __syncthreads();
+  share.request = uniform((int)found[0]);
+  share.tile = (uint32_t)uniform((int)found[1]);
+  share.offset = (uint32_t)uniform((int)found[2]);
+  share.tiles_before = (uint32_t)uniform((int)found[3]);
+  return true;
+}
+
+template <int DT, int L, int R, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(LatentArgs a) {
   typedef typename B16<DT>::scalar scalar;
   typedef typename B16<DT>::x8 x8;
@@ -113,18 +245,43 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int g = lane >> 4, i16 = lane & 15;
+  const int H = a.H;
+  // Parts of one tile, and tiles of one request, on one XCD (they share its L2).
+  const uint32_t worker = SPLIT ? xcd_contiguous(blockIdx.x, gridDim.x) : blockIdx.x;
 
   int request;
   uint32_t tile, tiles;
-  const int H = a.H;
-  if (!find_tile<NW * 64>(a.cu, a.B, a.T, blockIdx.x,
-                          [&](int n) { return ((uint32_t)n * (uint32_t)H + ROWS - 1) / ROWS; }, request, tile, tiles))
-    return;
-  if (a.causal) tile = tiles - 1 - tile;  // the longest first
+  LatentShare share;
+  uint64_t left = 0;  // of this workgroup's share
+  if constexpr (SPLIT) {
+    if (!find_share<NW * 64, ROWS>(a, worker, share)) return;
+    request = share.request;
+    tile = share.tile;
+    left = share.end - share.begin;
+  } else {
+    if (!find_tile<NW * 64>(a.cu, a.B, a.T, worker,
+                            [&](int n) { return ((uint32_t)n * (uint32_t)H + ROWS - 1) / ROWS; }, request, tile, tiles))
+      return;
+    if (a.causal) tile = tiles - 1 - tile;  // the longest first
+  }
+  uint32_t offset = SPLIT ? share.offset : 0;
+  const float scale_log2 = a.scale * LAT_LOG2E;
+
+  for (bool first_part = true;; first_part = false) {
+  if (SPLIT && request >= a.B) return;  // never, unless cu_seqlens_q or seqused_kv change under the call
   int start, count;
   request_tokens(a.cu, request, a.T, start, count);
   const int used = (int)min((int64_t)max(a.used[request], 0), (int64_t)a.W << a.page_shift);
   const int rows = count * H;
+  if constexpr (SPLIT) {
+    tiles = ((uint32_t)rows + ROWS - 1) / ROWS;
+    if (tile >= tiles) {  // on to the next request that has tokens (there is one: something is left)
+      share.tiles_before += tiles;
+      tile = 0;
+      ++request;
+      continue;
+    }
+  }
 
   // This lane's (token, head) row, and the keys it sees: [0, limit).
   const int row = (int)tile * ROWS + wave * 16 + i16;
@@ -134,7 +291,32 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   const int limit = valid ? visible(token) : 0;
   const int kv_end = visible((min((int)(tile + 1) * ROWS, rows) - 1) / H);
   const int clean_end = visible((int)tile * ROWS / H);  // no row of the tile hides a key below
-  const int chunks = (kv_end + LAT_KEYS - 1) / LAT_KEYS;
+  const int all_chunks = (kv_end + LAT_KEYS - 1) / LAT_KEYS;
+  int begin = 0, chunks = all_chunks;  // of this part
+  bool whole = true;
+  if constexpr (SPLIT) {
+    // The tile's own chunks, spread over what it counts.
+    const uint32_t counted = longest_chunks(used, count), each = counted + LAT_START;
+    const uint32_t end = (uint32_t)min((uint64_t)each, (uint64_t)offset + left);
+    auto cut = [&](uint32_t x) {
+      return x >= each ? all_chunks : (x <= LAT_START ? 0 : (int)((uint64_t)(x - LAT_START) * (uint32_t)all_chunks / counted));
+    };
+    begin = cut(offset);
+    chunks = cut(end);
+    whole = offset == 0 && end == each;
+    if (offset == 0 && tid == 0) {
+      const uint64_t tile_end = share.end - left + each;  // in the sequence
+      LatentRecord r;
+      r.start = start;
+      r.row = (int)tile * ROWS;
+      r.rows = min(ROWS, rows - (int)tile * ROWS);
+      r.first = (int)worker;
+      r.last = (int)((tile_end * (uint32_t)share.workers - 1) / share.total);
+      a.records[share.tiles_before + tile] = r;
+    }
+    left -= end - offset;
+    if (!first_part) block_barrier();  // the ring is read
+  }
 
   // ---- cache rows to LDS -----------------------------------------------------
   const uint32_t ring_base = lds_address(ring[0]);
@@ -162,7 +344,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     const int page = upper ? next[1] : next[0];
     const int have = (upper ? ok1 : ok0) ? min(max(kv_end - key, 0), RW) : 0;
     const char* from = (const char*)a.cache + ((int64_t)page * (page_mask + 1) + (key & page_mask)) * GROW;
-    const uint32_t slot = ring_base + (uint32_t)(chunk % NS) * SLOT;
+    const uint32_t slot = ring_base + (uint32_t)((chunk - begin) % NS) * SLOT;
     const uint32_t to = opaque_uniform(slot + (uint32_t)(first * LROW));
     const uint32_t to_rope = opaque_uniform(slot + (uint32_t)(ROPE_AT + first * 2 * R));
     if (partial > 0) --partial;
@@ -215,14 +397,13 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   for (int t = 0; t < VTILES; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = -1e30f;  // finite: a chunk that hides all its keys gives p = 0, never NaN
   float l_run = 0.f, l_rounded = 0.f;
-  const float scale_log2 = a.scale * LAT_LOG2E;
 
-  look_up(0);
+  look_up(begin);
 #pragma unroll
   for (int c = 0; c < NS - 1; ++c)
-    if (c < chunks) fetch(c);
+    if (begin + c < chunks) fetch(begin + c);
 
-  for (int c = 0; c < chunks; ++c) {
+  for (int c = begin; c < chunks; ++c) {
     // Chunk c has landed once at most the loads of the NS - 2 younger chunks are
     // in flight; where one of those has fewer loads, or is missing, all must have.
     if (partial == 0 && c + NS - 2 < chunks)
@@ -233,7 +414,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     const int loaded = min(c + NS - 1, chunks);  // chunks fetched so far
     const uint32_t bits = (good >> (2 * (loaded - 1 - c))) & 3u;
     if (c + NS - 1 < chunks) fetch(c + NS - 1);
-    const uint32_t slot = ring_base + (uint32_t)(c % NS) * SLOT;
+    const uint32_t slot = ring_base + (uint32_t)((c - begin) % NS) * SLOT;
 
     f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
     {
@@ -310,18 +491,75 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   }
 
   const float total = sum_over_lane_groups(l_run), applied = sum_over_lane_groups(l_rounded);
-  if (!valid) return;
-  const float inv = applied > 0.f ? 1.0f / applied : 0.f;
-  scalar* out = (scalar*)a.out + (int64_t)(start + token) * a.o_t + (int64_t)head * a.o_h + 4 * g;
+  if (SPLIT && !whole) {
+    // A part of no chunks has sums of 0, and the merge does not read its O.
+    const int64_t part = 2 * (int64_t)worker + (offset == 0 ? 1 : 0), at = part * ROWS + wave * 16 + i16;
+    if (valid && begin < chunks) {
+      float* po = a.partial_o + at * L + 4 * g;
 #pragma unroll
-  for (int t = 0; t < VTILES; ++t) {
-    x4 v;
+      for (int t = 0; t < VTILES; ++t) *(f32x4*)(po + 16 * t) = o[t];
+    }
+    if (valid && g == 0) *(f32x4*)(a.partial_ml + at * 4) = f32x4{m_run, total, applied, 0.f};
+  } else if (valid) {
+    const float inv = applied > 0.f ? 1.0f / applied : 0.f;
+    scalar* out = (scalar*)a.out + (int64_t)(start + token) * a.o_t + (int64_t)head * a.o_h + 4 * g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[t][i] * inv);
-    *(x4*)(out + 16 * t) = v;
+    for (int t = 0; t < VTILES; ++t) {
+      x4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[t][i] * inv);
+      *(x4*)(out + 16 * t) = v;
+    }
+    if (a.lse && g == 0)
+      a.lse[(int64_t)(start + token) * H + head] = total > 0.f ? (m_run + __log2f(total)) * LAT_LN2 : -INFINITY;
   }
-  if (a.lse && g == 0)
-    a.lse[(int64_t)(start + token) * H + head] = total > 0.f ? (m_run + __log2f(total)) * LAT_LN2 : -INFINITY;
+  if (!SPLIT || left == 0) return;
+  offset = 0;
+  ++tile;
+  }
+}
+
+// Combines the parts of the tiles that several workgroups of the split form
+// share: out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, parts in order. One
+// group of L / 4 threads per row; bound by the parts' bytes, which were written
+// just before (2 * 4 L bytes per row and part).
+template <int DT, int L>
+__global__ __launch_bounds__(256) void latent_merge_kernel(LatentArgs a, int tile_rows) {
+  typedef typename B16<DT>::scalar scalar;
+  typedef typename B16<DT>::x4 x4;
+  constexpr int THREADS = L / 4, GROUPS = 256 / THREADS;
+  const int groups = (tile_rows + GROUPS - 1) / GROUPS;
+  const uint32_t tile = blockIdx.x / (uint32_t)groups;
+  const int r = (int)(blockIdx.x % (uint32_t)groups) * GROUPS + (int)threadIdx.x / THREADS;
+  if (tile >= *a.tile_count) return;
+  const LatentRecord record = a.records[tile];
+  if (record.first == record.last || r >= record.rows) return;
+  auto slot = [&](int w) { return (2 * (int64_t)w + (w == record.first ? 1 : 0)) * tile_rows + r; };
+  float top = -1e30f;
+  for (int w = record.first; w <= record.last; ++w) {
+    const f32x4 ml = *(const f32x4*)(a.partial_ml + slot(w) * 4);
+    if (ml[1] > 0.f) top = fmaxf(top, ml[0]);
+  }
+  float total = 0.f, applied = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const int column = 4 * ((int)threadIdx.x % THREADS);
+  for (int w = record.first; w <= record.last; ++w) {
+    const f32x4 ml = *(const f32x4*)(a.partial_ml + slot(w) * 4);
+    if (ml[1] > 0.f) {
+      const float weight = fast_exp2(ml[0] - top);
+      total += weight * ml[1];
+      applied += weight * ml[2];
+      o += weight * *(const f32x4*)(a.partial_o + slot(w) * L + column);
+    }
+  }
+  const int packed = record.row + r, token = packed / a.H, head = packed - token * a.H;
+  const float inv = applied > 0.f ? 1.0f / applied : 0.f;
+  x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[i] * inv);
+  *(x4*)((scalar*)a.out + (int64_t)(record.start + token) * a.o_t + (int64_t)head * a.o_h + column) = v;
+  if (a.lse && column == 0)
+    a.lse[(int64_t)(record.start + token) * a.H + head] = total > 0.f ? (top + __log2f(total)) * LAT_LN2 : -INFINITY;
 }
 
 // Expanded form (latent_attention_expanded), for prompts: keys [k_nope | k_rope]
@@ -631,31 +869,73 @@ int check_latent(const LatentParams* p) {
   return AFA_OK;
 }
 
-// Waves (of 16 rows each) of a tile: 8 where a request has more than 64 rows on average, else 4.
-int latent_waves(const LatentParams* p) { return ((int64_t)p->T + p->B - 1) / p->B * p->H > 64 ? 8 : 4; }
+constexpr int LAT_CUS = 256;
+
+// Form of a call: waves (of 16 rows each) of a tile, 8 where a request has more
+// than 64 rows on average, else 4; and workgroups of the split form, one per CU
+// or two, 0 for the form of one tile per workgroup: where the tiles (at most
+// rows / tile + B of them) would fill the GPU four times over anyway.
+struct LatentPlan {
+  int waves;
+  int workers;
+  int64_t tiles;
+};
+LatentPlan plan_latent(const LatentParams* p) {
+  LatentPlan plan;
+  plan.waves = ((int64_t)p->T + p->B - 1) / p->B * p->H > 64 ? 8 : 4;
+  plan.tiles = (int64_t)p->T * p->H / (16 * plan.waves) + p->B;
+  const int slots = plan.waves == 8 ? LAT_CUS : 2 * LAT_CUS;
+  plan.workers = plan.tiles <= 4 * slots ? slots : 0;
+  return plan;
+}
+
+// Workspace of the split form: parts, their maxima and sums, records, the count of tiles.
+int64_t latent_part_rows(const LatentPlan& plan) { return 2ll * plan.workers * 16 * plan.waves; }
+uint64_t latent_bytes(const LatentParams* p, const LatentPlan& plan) {
+  if (plan.workers == 0 || p->T == 0) return 0;
+  return (uint64_t)(latent_part_rows(plan) * (p->L + 4) * 4 + plan.tiles * (int64_t)sizeof(LatentRecord) + 16);
+}
 
 template <int DT, int L, int R>
-int launch_latent(const LatentArgs& a, int waves, hipStream_t s) {
-  const int64_t tiles = (int64_t)a.T * a.H / (16 * waves) + a.B;  // at least as many as there are
-  if (tiles > 0x7fffffffll) return AFA_E_SHAPE;
-  if (waves == 8)
-    hipLaunchKernelGGL((latent_kernel<DT, L, R, 8>), dim3((unsigned)tiles), dim3(512), 0, s, a);
+int launch_latent(LatentArgs a, const LatentPlan& plan, void* workspace, hipStream_t s) {
+  if (plan.tiles > 0x7fffffffll) return AFA_E_SHAPE;
+  if (plan.workers == 0) {
+    const dim3 grid((unsigned)plan.tiles);
+    if (plan.waves == 8)
+      hipLaunchKernelGGL((latent_kernel<DT, L, R, 8, false>), grid, dim3(512), 0, s, a);
+    else
+      hipLaunchKernelGGL((latent_kernel<DT, L, R, 4, false>), grid, dim3(256), 0, s, a);
+    return (int)hipGetLastError();
+  }
+  const int64_t part_rows = latent_part_rows(plan);
+  a.workers = plan.workers;
+  a.partial_o = (float*)workspace;
+  a.partial_ml = a.partial_o + part_rows * L;
+  a.tile_count = (uint32_t*)(a.partial_ml + part_rows * 4);
+  a.records = (LatentRecord*)(a.tile_count + 4);
+  const dim3 grid((unsigned)plan.workers);
+  if (plan.waves == 8)
+    hipLaunchKernelGGL((latent_kernel<DT, L, R, 8, true>), grid, dim3(512), 0, s, a);
   else
-    hipLaunchKernelGGL((latent_kernel<DT, L, R, 4>), dim3((unsigned)tiles), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((latent_kernel<DT, L, R, 4, true>), grid, dim3(256), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return (int)e;
+  constexpr int GROUPS = 256 / (L / 4);
+  const int rows = 16 * plan.waves, groups = (rows + GROUPS - 1) / GROUPS;
+  hipLaunchKernelGGL((latent_merge_kernel<DT, L>), dim3((unsigned)(plan.tiles * groups)), dim3(256), 0, s, a, rows);
   return (int)hipGetLastError();
 }
 
 template <int DT>
-int dispatch_latent(const LatentArgs& a, const LatentParams* p, hipStream_t s) {
-  const int waves = latent_waves(p);
+int dispatch_latent(const LatentArgs& a, const LatentParams* p, const LatentPlan& plan, void* workspace, hipStream_t s) {
   if (p->R == 64) {
-    if (p->L == 512) return launch_latent<DT, 512, 64>(a, waves, s);
-    if (p->L == 256) return launch_latent<DT, 256, 64>(a, waves, s);
-    return launch_latent<DT, 128, 64>(a, waves, s);
+    if (p->L == 512) return launch_latent<DT, 512, 64>(a, plan, workspace, s);
+    if (p->L == 256) return launch_latent<DT, 256, 64>(a, plan, workspace, s);
+    return launch_latent<DT, 128, 64>(a, plan, workspace, s);
   }
-  if (p->L == 512) return launch_latent<DT, 512, 0>(a, waves, s);
-  if (p->L == 256) return launch_latent<DT, 256, 0>(a, waves, s);
-  return launch_latent<DT, 128, 0>(a, waves, s);
+  if (p->L == 512) return launch_latent<DT, 512, 0>(a, plan, workspace, s);
+  if (p->L == 256) return launch_latent<DT, 256, 0>(a, plan, workspace, s);
+  return launch_latent<DT, 128, 0>(a, plan, workspace, s);
 }
 
 }  // namespace
@@ -663,7 +943,8 @@ int dispatch_latent(const LatentArgs& a, const LatentParams* p, hipStream_t s) {
 
 extern "C" int launch_latent_attention(void* stream, const void* q, const void* q_rope, const void* kv_cache,
                                        const int32_t* block_table, const int32_t* cu_seqlens_q, const int32_t* seqused_kv,
-                                       void* out, float* softmax_lse, const LatentParams* p) {
+                                       void* out, float* softmax_lse, void* workspace, uint64_t workspace_bytes,
+                                       const LatentParams* p) {
   using namespace afa;
   const int status = check_latent(p);
   if (status) return status;
@@ -672,7 +953,11 @@ extern "C" int launch_latent_attention(void* stream, const void* q, const void* 
   if (!rows_fit(q, p->q_stride_t, p->q_stride_h) || !rows_fit(out, p->out_stride_t, p->out_stride_h) ||
       (p->R && !rows_fit(q_rope, p->q_rope_stride_t, p->q_rope_stride_h)) || !rows_fit(kv_cache, 0, 0))
     return AFA_E_SHAPE;
-  LatentArgs a;
+  const LatentPlan plan = plan_latent(p);
+  const uint64_t need = latent_bytes(p, plan);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return AFA_E_WORKSPACE;
+  if ((uintptr_t)workspace & 15) return AFA_E_WORKSPACE;
+  LatentArgs a = {};
   a.q = q;
   a.q_rope = q_rope;
   a.cache = kv_cache;
@@ -695,8 +980,28 @@ extern "C" int launch_latent_attention(void* stream, const void* q, const void* 
   a.blocks = p->BLOCKS;
   a.causal = p->causal ? 1 : 0;
   a.scale = p->scale;
-  return p->dtype == AFA_DTYPE_F16 ? dispatch_latent<DT_F16>(a, p, (hipStream_t)stream)
-                                   : dispatch_latent<DT_BF16>(a, p, (hipStream_t)stream);
+  return p->dtype == AFA_DTYPE_F16 ? dispatch_latent<DT_F16>(a, p, plan, workspace, (hipStream_t)stream)
+                                   : dispatch_latent<DT_BF16>(a, p, plan, workspace, (hipStream_t)stream);
+}
+
+extern "C" int workspace_size_latent_attention(uint64_t* bytes, const LatentParams* p) {
+  using namespace afa;
+  if (!bytes) return AFA_E_NULL;
+  const int status = check_latent(p);
+  if (status) return status;
+  *bytes = latent_bytes(p, plan_latent(p));
+  return AFA_OK;
+}
+
+extern "C" int form_latent_attention(int64_t form[2], const LatentParams* p) {
+  using namespace afa;
+  if (!form) return AFA_E_NULL;
+  const int status = check_latent(p);
+  if (status) return status;
+  const LatentPlan plan = plan_latent(p);
+  form[0] = 16 * plan.waves;
+  form[1] = plan.workers;
+  return AFA_OK;
 }
 
 extern "C" int launch_latent_attention_expanded(void* stream, const void* q, const void* k_nope, const void* k_rope,

@@ -34,17 +34,20 @@ def row_strides(name, tensor):
 
 
 @kept_by_value
-def _params(dtype, T, B, H, L, R, PAGE, W, BLOCKS, qt, qh, rt, rh, ot, oh, SCALE, causal):
-    """Launcher parameters of a call of checked sizes (not changed afterwards)."""
+def _params(lib, dtype, T, B, H, L, R, PAGE, W, BLOCKS, qt, qh, rt, rh, ot, oh, SCALE, causal):
+    """Launcher parameters and workspace bytes of a call of checked sizes (not changed afterwards)."""
     require(H > 0 and B > 0 and W > 0 and BLOCKS > 0, "heads, requests and pages must not be empty")
     require(L in (128, 256, 512), "the latent width (columns of q) must be 128, 256 or 512")
     require(R in (0, 64), "the rotary width must be 64, or 0 without q_rope")
     require(PAGE >= 16 and PAGE & (PAGE - 1) == 0, "PAGE must be a power of two from 16 on")
     require(SCALE > 0, "positive attention scale")
-    return ct.pointer(_native.LatentParams(
+    params = _native.LatentParams(
         dtype=_native.AFA_DTYPE[dtype], causal=int(causal), T=T, B=B, H=H, L=L, R=R, PAGE=PAGE, W=W, BLOCKS=BLOCKS,
         q_stride_t=qt, q_stride_h=qh, q_rope_stride_t=rt, q_rope_stride_h=rh, out_stride_t=ot, out_stride_h=oh,
-        scale=SCALE, reserved=0))
+        scale=SCALE, reserved=0)
+    nbytes = ct.c_uint64(0)
+    _native.check(lib.workspace_size_latent_attention(ct.byref(nbytes), ct.byref(params)), "workspace_size_latent_attention")
+    return ct.pointer(params), nbytes.value
 
 
 def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCALE, q_rope=None, CAUSAL=True, out=None,
@@ -100,14 +103,20 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
         check_apart([("q", q, False), ("q_rope", q_rope, False), ("kv_cache", kv_cache, False),
                      ("block_table", block_table, False), ("cu_seqlens_q", cu_seqlens_q, False),
                      ("seqused_kv", seqused_kv, False), ("out", out, False), ("softmax_lse", softmax_lse, True)])
-    params = _params(_STORAGE[b16], T, B, H, L, R, PAGE, W, BLOCKS, *row_strides("q", q),
+    lib = _native.library()
+    params, nbytes = _params(lib, _STORAGE[b16], T, B, H, L, R, PAGE, W, BLOCKS, *row_strides("q", q),
                      *((0, 0) if q_rope is None else row_strides("q_rope", q_rope)), *row_strides("out", out),
                      float(SCALE), bool(CAUSAL))
     if T:
-        status = launch_on(q.get_device(), _native.library().launch_latent_attention, q.data_ptr(),
+        workspace = None
+        if nbytes:
+            # Partial results; the caching allocator keeps the block for this stream.
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            workspace = scratch.data_ptr()
+        status = launch_on(q.get_device(), lib.launch_latent_attention, q.data_ptr(),
                            None if q_rope is None else q_rope.data_ptr(), kv_cache.data_ptr(), block_table.data_ptr(),
                            cu_seqlens_q.data_ptr(), seqused_kv.data_ptr(), out.data_ptr(),
-                           None if softmax_lse is None else softmax_lse.data_ptr(), params)
+                           None if softmax_lse is None else softmax_lse.data_ptr(), workspace, nbytes, params)
         if status:
             _native.check(status, "launch_latent_attention")
     return out

@@ -378,7 +378,19 @@ typedef struct LatentParams {
 
 int launch_latent_attention(void* stream, const void* q, const void* q_rope, const void* kv_cache,
                             const int32_t* block_table, const int32_t* cu_seqlens_q, const int32_t* seqused_kv,
-                            void* out, float* softmax_lse, const LatentParams* params);
+                            void* out, float* softmax_lse, void* workspace, uint64_t workspace_bytes,
+                            const LatentParams* params);
+
+/* Bytes of device memory, on 16 bytes, that a call of these sizes needs for
+ * partial results (0: none, workspace may be NULL); with less the launcher
+ * returns AFA_E_WORKSPACE before any launch. Calls that may run at the same
+ * time need workspaces of their own. */
+int workspace_size_latent_attention(uint64_t* bytes, const LatentParams* params);
+
+/* Which form a call of these sizes runs: form[0] packed (token, head) rows per
+ * tile, form[1] workgroups that share all tiles' keys evenly, 0 for one tile per
+ * workgroup. For tests and profiles. */
+int form_latent_attention(int64_t form[2], const LatentParams* params);
 
 /* Latent attention, expanded form, ragged requests: for query i of the nq and
  * key j of the nk of request b, head h
