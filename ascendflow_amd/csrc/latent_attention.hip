@@ -71,8 +71,13 @@ struct LatentRecord {
 constexpr uint32_t LAT_START = 2;
 constexpr uint32_t LAT_LEAST = 4;  // least chunks (and starts) of a workgroup
 
+// Metadata in the constant address space, so that uniform reads are scalar loads,
+// whose values stay out of the vector registers and the vector load counter.
+typedef const __attribute__((address_space(4))) int32_t* const_ints;
+__device__ __forceinline__ const_ints constant(const int32_t* p) { return (const_ints)(uintptr_t)p; }
+
 // New tokens of request b: cu[b] .. cu[b + 1], held inside [0, T).
-__device__ __forceinline__ void request_tokens(const int32_t* cu, int b, int T, int& start, int& count) {
+__device__ __forceinline__ void request_tokens(const_ints cu, int b, int T, int& start, int& count) {
   start = min(max(cu[b], 0), T);
   count = max(min(cu[b + 1], T) - start, 0);
 }
@@ -80,7 +85,7 @@ __device__ __forceinline__ void request_tokens(const int32_t* cu, int b, int T, 
 // The request and the tile inside it of tile `index` in the order of requests
 // (tiles_of(tokens) each); false, for the whole workgroup, if there are fewer.
 template <int THREADS, typename F>
-__device__ __forceinline__ bool find_tile(const int32_t* cu, int B, int T, uint32_t index, F&& tiles_of, int& request,
+__device__ __forceinline__ bool find_tile(const_ints cu, int B, int T, uint32_t index, F&& tiles_of, int& request,
                                           uint32_t& tile, uint32_t& tiles) {
   __shared__ uint32_t wave_total[THREADS / 64];
   __shared__ uint32_t found[3];
@@ -156,8 +161,8 @@ __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker,
   const int per = (a.B + THREADS - 1) / THREADS;  // consecutive requests of a thread
   auto measure = [&](int b, uint32_t& tiles, uint32_t& each) {
     int start, count;
-    request_tokens(a.cu, b, a.T, start, count);
-    const int used = (int)min((int64_t)max(a.used[b], 0), (int64_t)a.W << a.page_shift);
+    request_tokens(constant(a.cu), b, a.T, start, count);
+    const int used = (int)min((int64_t)max(constant(a.used)[b], 0), (int64_t)a.W << a.page_shift);
     tiles = ((uint32_t)count * (uint32_t)a.H + ROWS - 1) / ROWS;
     each = longest_chunks(used, count) + LAT_START;
   };
@@ -195,9 +200,10 @@ __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker,
   const uint64_t most = total / LAT_LEAST;
   share.workers = most < 1 ? 1 : (most < (uint64_t)a.workers ? (int)most : a.workers);
   if (worker >= (uint32_t)share.workers) return false;
+  share.workers = uniform(share.workers);
   share.total = total;
-  share.begin = total * worker / (uint32_t)share.workers;
-  share.end = total * (worker + 1) / (uint32_t)share.workers;
+  share.begin = uniform64(total * worker / (uint32_t)share.workers);
+  share.end = uniform64(total * (worker + 1) / (uint32_t)share.workers);
   if (share.begin >= before && share.begin < before + weight) {
     uint64_t at = before;
     uint32_t done = tiles_before;
@@ -259,7 +265,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     tile = share.tile;
     left = share.end - share.begin;
   } else {
-    if (!find_tile<NW * 64>(a.cu, a.B, a.T, worker,
+    if (!find_tile<NW * 64>(constant(a.cu), a.B, a.T, worker,
                             [&](int n) { return ((uint32_t)n * (uint32_t)H + ROWS - 1) / ROWS; }, request, tile, tiles))
       return;
     if (a.causal) tile = tiles - 1 - tile;  // the longest first
@@ -270,8 +276,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   for (bool first_part = true;; first_part = false) {
   if (SPLIT && request >= a.B) return;  // never, unless cu_seqlens_q or seqused_kv change under the call
   int start, count;
-  request_tokens(a.cu, request, a.T, start, count);
-  const int used = (int)min((int64_t)max(a.used[request], 0), (int64_t)a.W << a.page_shift);
+  request_tokens(constant(a.cu), request, a.T, start, count);
+  const int used = (int)min((int64_t)max(constant(a.used)[request], 0), (int64_t)a.W << a.page_shift);
   const int rows = count * H;
   if constexpr (SPLIT) {
     tiles = ((uint32_t)rows + ROWS - 1) / ROWS;
@@ -283,12 +289,15 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     }
   }
 
-  // This lane's (token, head) row, and the keys it sees: [0, limit).
-  const int row = (int)tile * ROWS + wave * 16 + i16;
-  const bool valid = row < rows;
-  const int token = valid ? row / H : 0, head = valid ? row - token * H : 0;
   auto visible = [&](int t) { return a.causal ? min(max(used - count + t + 1, 0), used) : used; };
-  const int limit = valid ? visible(token) : 0;
+  // This lane's (token, head) row. Worked out where it is needed (Q, masks, the
+  // end): kept, it would cost registers that the loop does not have.
+  auto my_row = [&](int& token, int& head) {
+    const int row = (int)(tile * ROWS) + (int)(opaque((uint32_t)tid) >> 6) * 16 + (int)(opaque((uint32_t)tid) & 15u);
+    token = row < rows ? row / H : 0;
+    head = row - token * H;
+    return row < rows;
+  };
   const int kv_end = visible((min((int)(tile + 1) * ROWS, rows) - 1) / H);
   const int clean_end = visible((int)tile * ROWS / H);  // no row of the tile hides a key below
   const int all_chunks = (kv_end + LAT_KEYS - 1) / LAT_KEYS;
@@ -320,10 +329,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 
   // ---- cache rows to LDS -----------------------------------------------------
   const uint32_t ring_base = lds_address(ring[0]);
-  // In the constant address space, so that the uniform reads are scalar loads,
-  // which leave the vector load counter to the ring.
-  typedef const __attribute__((address_space(4))) int32_t* const_ints;
-  const const_ints pages = (const_ints)(uintptr_t)(a.table + (int64_t)request * a.W);
+  const const_ints pages = constant(a.table + (int64_t)request * a.W);
   const int page_mask = (1 << a.page_shift) - 1;
   // Page of the 16-row group that holds `key`; -1 past the end.
   auto page_of = [&](int key) { return key < kv_end ? pages[key >> a.page_shift] : -1; };
@@ -349,24 +355,39 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     const uint32_t to_rope = opaque_uniform(slot + (uint32_t)(ROPE_AT + first * 2 * R));
     if (partial > 0) --partial;
     if (have < RW) partial = NS;
+    const uint32_t ln = opaque((uint32_t)tid) & 63u;  // offsets worked out anew: kept, they would be spilled
+    auto load = [&](uint32_t dst, uint32_t off) {
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                       :: "s"(dst), "v"(off), "s"(from) : "memory");
+    };
+    const int r0 = (int)(ln / (L / 8)), rope_row = (int)(ln >> 3);
+    auto latent_off = [&](int r) {
+      return (uint32_t)(r * GROW) + (((ln % (L / 8)) ^ (uint32_t)((first + r) & 15)) << 4);
+    };
+    auto rope_off = [&]() {
+      return (uint32_t)(rope_row * GROW + LROW) + (((ln & 7u) ^ (uint32_t)(((first + rope_row) >> 1) & 7)) << 4);
+    };
+    if (have == RW) {
 #pragma unroll
-    for (int p = 0; p < LOADS_L; ++p) {
-      const int r = p * LR + lane / (L / 8);
-      const uint32_t off = (uint32_t)(r * GROW + (((lane % (L / 8)) ^ ((first + r) & 15)) << 4));
-      if (r < have)
-        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                         :: "s"(to + (uint32_t)p * 1024u), "v"(off), "s"(from) : "memory");
-      else  // rows past the end or without a page: zeros, which no weight can turn into anything else
-        *(AFA_LDS u32x4*)(uintptr_t)(to + (uint32_t)(p * 1024 + lane * 16)) = u32x4{0u, 0u, 0u, 0u};
-    }
-    if constexpr (R != 0) {
-      const int r = lane >> 3;
-      const uint32_t off = (uint32_t)(r * GROW + LROW + (((lane & 7) ^ (((first + r) >> 1) & 7)) << 4));
-      if (r < have)
-        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                         :: "s"(to_rope), "v"(off), "s"(from) : "memory");
-      else if (r < RW)
-        *(AFA_LDS u32x4*)(uintptr_t)(to_rope + (uint32_t)lane * 16u) = u32x4{0u, 0u, 0u, 0u};
+      for (int p = 0; p < LOADS_L; ++p) load(to + (uint32_t)p * 1024u, latent_off(p * LR + r0));
+      if constexpr (R != 0)
+        if (8 * RW == 64 || rope_row < RW) load(to_rope, rope_off());
+    } else {
+      // Rows past the end or without a page become zeros, which no weight can turn into anything else.
+      const u32x4 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int p = 0; p < LOADS_L; ++p) {
+        if (p * LR + r0 < have)
+          load(to + (uint32_t)p * 1024u, latent_off(p * LR + r0));
+        else
+          *(AFA_LDS u32x4*)(uintptr_t)(to + (uint32_t)p * 1024u + ln * 16u) = zero;
+      }
+      if constexpr (R != 0) {
+        if (rope_row < have)
+          load(to_rope, rope_off());
+        else if (rope_row < RW)
+          *(AFA_LDS u32x4*)(uintptr_t)(to_rope + ln * 16u) = zero;
+      }
     }
     look_up(chunk + 1);
   };
@@ -374,6 +395,9 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   // ---- Q fragments: B operand, columns 32 j + 8 g .. + 7 of row i16 -----------
   x8 qf[KSTEPS + RSTEPS];
   {
+    int token, head;
+    const bool valid = my_row(token, head);
+    if (!valid) head = 0;
     const scalar* q = (const scalar*)a.q + (int64_t)(start + token) * a.q_t + (int64_t)head * a.q_h + 8 * g;
 #pragma unroll
     for (int j = 0; j < KSTEPS; ++j)
@@ -418,7 +442,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 
     f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
     {
-      constexpr int FRAGS = 2 * (KSTEPS + RSTEPS), LOOK = 6;
+      constexpr int FRAGS = 2 * (KSTEPS + RSTEPS), LOOK = L == 512 ? 4 : 6;
       const uint32_t base = opaque(slot + qk_at), rope = opaque(slot + qr_at);
       x8 kf[FRAGS];
       auto load = [&](int f) {  // (step j, key tile t)
@@ -437,7 +461,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     }
     const int key0 = c * LAT_KEYS;
     if (key0 + LAT_KEYS > clean_end || bits != 3u) {  // uniform
-      const int lim = limit - key0;
+      int token, head;
+      const int lim = my_row(token, head) ? visible(token) - key0 : 0;  // this row sees the chunk's keys below it
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -491,6 +516,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   }
 
   const float total = sum_over_lane_groups(l_run), applied = sum_over_lane_groups(l_rounded);
+  int token, head;
+  const bool valid = my_row(token, head);
   if (SPLIT && !whole) {
     // A part of no chunks has sums of 0, and the merge does not read its O.
     const int64_t part = 2 * (int64_t)worker + (offset == 0 ? 1 : 0), at = part * ROWS + wave * 16 + i16;
@@ -605,13 +632,13 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
   const int head = (int)(blockIdx.x % (uint32_t)a.H);
   int request;
   uint32_t tile, tiles;
-  if (!find_tile<512>(a.cu_q, a.B, a.Tq, blockIdx.x / (uint32_t)a.H,
+  if (!find_tile<512>(constant(a.cu_q), a.B, a.Tq, blockIdx.x / (uint32_t)a.H,
                       [&](int n) { return ((uint32_t)n + BQ - 1) / BQ; }, request, tile, tiles))
     return;
   if (a.causal) tile = tiles - 1 - tile;  // the longest first
   int q_start, nq, k_start, nk;
-  request_tokens(a.cu_q, request, a.Tq, q_start, nq);
-  request_tokens(a.cu_k, request, a.Tk, k_start, nk);
+  request_tokens(constant(a.cu_q), request, a.Tq, q_start, nq);
+  request_tokens(constant(a.cu_k), request, a.Tk, k_start, nk);
   const int q0 = (int)tile * BQ;
 
   const scalar* Q = (const scalar*)a.q + (int64_t)q_start * a.q_t + (int64_t)head * a.q_h;
