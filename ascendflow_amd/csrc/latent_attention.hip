@@ -70,6 +70,7 @@ struct LatentRecord {
 // cu_seqlens_q and seqused_kv, alike in every workgroup.
 constexpr uint32_t LAT_START = 2;
 constexpr uint32_t LAT_LEAST = 4;  // least chunks (and starts) of a workgroup
+constexpr int LAT_MAX_WORKERS = 512;
 
 // Metadata in the constant address space, so that uniform reads are scalar loads,
 // whose values stay out of the vector registers and the vector load counter.
@@ -519,9 +520,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   int token, head;
   const bool valid = my_row(token, head);
   if (SPLIT && !whole) {
-    // A part of no chunks has sums of 0, and the merge does not read its O.
     const int64_t part = 2 * (int64_t)worker + (offset == 0 ? 1 : 0), at = part * ROWS + wave * 16 + i16;
-    if (valid && begin < chunks) {
+    if (valid) {
       float* po = a.partial_o + at * L + 4 * g;
 #pragma unroll
       for (int t = 0; t < VTILES; ++t) *(f32x4*)(po + 16 * t) = o[t];
@@ -547,45 +547,76 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 }
 
 // Combines the parts of the tiles that several workgroups of the split form
-// share: out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, parts in order. One
-// group of L / 4 threads per row; bound by the parts' bytes, which were written
-// just before (2 * 4 L bytes per row and part).
-template <int DT, int L>
+// share: out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, in a fixed order. A
+// wave works out the weights of all parts of its row side by side, then sums
+// L / 64 columns a lane over the parts, four parts of loads in flight. Where the
+// tiles are few, the four waves of a workgroup share a row's parts (WAVES = 4,
+// sums joined in wave order), otherwise each takes a row. Bound by the parts'
+// bytes (4 L per row and part, written just before), or, for few tiles, by four
+// dependent loads.
+template <int DT, int L, int WAVES>
 __global__ __launch_bounds__(256) void latent_merge_kernel(LatentArgs a, int tile_rows) {
   typedef typename B16<DT>::scalar scalar;
-  typedef typename B16<DT>::x4 x4;
-  constexpr int THREADS = L / 4, GROUPS = 256 / THREADS;
-  const int groups = (tile_rows + GROUPS - 1) / GROUPS;
-  const uint32_t tile = blockIdx.x / (uint32_t)groups;
-  const int r = (int)(blockIdx.x % (uint32_t)groups) * GROUPS + (int)threadIdx.x / THREADS;
-  if (tile >= *a.tile_count) return;
-  const LatentRecord record = a.records[tile];
-  if (record.first == record.last || r >= record.rows) return;
-  auto slot = [&](int w) { return (2 * (int64_t)w + (w == record.first ? 1 : 0)) * tile_rows + r; };
+  constexpr int ROWS = 4 / WAVES, COLUMNS = L / 64, AHEAD = 4;
+  typedef float vec __attribute__((ext_vector_type(COLUMNS)));
+  typedef scalar out_vec __attribute__((ext_vector_type(COLUMNS)));
+  __shared__ float weights[4][LAT_MAX_WORKERS];
+  __shared__ vec partial[4][64];
+  const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t blocks = (uint32_t)tile_rows / ROWS;  // of a tile
+  const uint32_t tile = blockIdx.x / blocks;
+  const int r = (int)(blockIdx.x % blocks) * ROWS + wave / WAVES, sub = wave % WAVES;
+  const LatentRecord record = a.records[tile];  // there is room for every tile of the grid
+  if (tile >= *a.tile_count || record.first == record.last || r >= record.rows) return;
+  const int parts = record.last - record.first + 1;
+  auto slot = [&](int p) { return (2 * (int64_t)(record.first + p) + (p == 0 ? 1 : 0)) * tile_rows + r; };
+
   float top = -1e30f;
-  for (int w = record.first; w <= record.last; ++w) {
-    const f32x4 ml = *(const f32x4*)(a.partial_ml + slot(w) * 4);
-    if (ml[1] > 0.f) top = fmaxf(top, ml[0]);
-  }
+  for (int p = lane; p < parts; p += 64) top = fmaxf(top, a.partial_ml[slot(p) * 4]);
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
   float total = 0.f, applied = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  const int column = 4 * ((int)threadIdx.x % THREADS);
-  for (int w = record.first; w <= record.last; ++w) {
-    const f32x4 ml = *(const f32x4*)(a.partial_ml + slot(w) * 4);
-    if (ml[1] > 0.f) {
-      const float weight = fast_exp2(ml[0] - top);
-      total += weight * ml[1];
-      applied += weight * ml[2];
-      o += weight * *(const f32x4*)(a.partial_o + slot(w) * L + column);
+  for (int p = lane; p < parts; p += 64) {
+    const f32x4 ml = *(const f32x4*)(a.partial_ml + slot(p) * 4);
+    const float weight = fast_exp2(ml[0] - top);
+    weights[wave][p] = weight;
+    total += weight * ml[1];
+    applied += weight * ml[2];
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) {
+    total += __shfl_xor(total, d);
+    applied += __shfl_xor(applied, d);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the lanes' weights, read by all of them
+
+  vec o = {};
+  for (int p = sub; p < parts; p += AHEAD * WAVES) {
+    vec v[AHEAD];
+    float weight[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int q = min(p + i * WAVES, parts - 1);
+      weight[i] = p + i * WAVES < parts ? weights[wave][q] : 0.f;
+      v[i] = *(const vec*)(a.partial_o + slot(q) * L + lane * COLUMNS);
     }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) o += weight[i] * v[i];
+  }
+  if constexpr (WAVES > 1) {
+    partial[wave][lane] = o;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) o += partial[w][lane];
   }
   const int packed = record.row + r, token = packed / a.H, head = packed - token * a.H;
   const float inv = applied > 0.f ? 1.0f / applied : 0.f;
-  x4 v;
+  out_vec v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[i] * inv);
-  *(x4*)((scalar*)a.out + (int64_t)(record.start + token) * a.o_t + (int64_t)head * a.o_h + column) = v;
-  if (a.lse && column == 0)
+  for (int i = 0; i < COLUMNS; ++i) v[i] = (scalar)(o[i] * inv);
+  *(out_vec*)((scalar*)a.out + (int64_t)(record.start + token) * a.o_t + (int64_t)head * a.o_h + lane * COLUMNS) = v;
+  if (a.lse && lane == 0)
     a.lse[(int64_t)(record.start + token) * a.H + head] = total > 0.f ? (top + __log2f(total)) * LAT_LN2 : -INFINITY;
 }
 
@@ -947,9 +978,12 @@ int launch_latent(LatentArgs a, const LatentPlan& plan, void* workspace, hipStre
     hipLaunchKernelGGL((latent_kernel<DT, L, R, 4, true>), grid, dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  constexpr int GROUPS = 256 / (L / 4);
-  const int rows = 16 * plan.waves, groups = (rows + GROUPS - 1) / GROUPS;
-  hipLaunchKernelGGL((latent_merge_kernel<DT, L>), dim3((unsigned)(plan.tiles * groups)), dim3(256), 0, s, a, rows);
+  // One workgroup per row up to 2048 rows (of 33 parts), else per four rows.
+  const int rows = 16 * plan.waves;
+  if (plan.tiles * rows <= 2048)
+    hipLaunchKernelGGL((latent_merge_kernel<DT, L, 4>), dim3((unsigned)(plan.tiles * rows)), dim3(256), 0, s, a, rows);
+  else
+    hipLaunchKernelGGL((latent_merge_kernel<DT, L, 1>), dim3((unsigned)(plan.tiles * (rows / 4))), dim3(256), 0, s, a, rows);
   return (int)hipGetLastError();
 }
 
