@@ -183,3 +183,53 @@ def launch_on(device_index, launch, *args):
         return launch(raw_stream(device_index), *args)
     with torch.cuda.device(device_index):
         return launch(raw_stream(device_index), *args)
+
+
+def check_operands(names, tensors, optional=()):
+    """Every operand is a tensor, or None where it is optional."""
+    for name, t in zip(names, tensors):
+        if not isinstance(t, torch.Tensor) and not (t is None and name in optional):
+            raise ValueError(f"{name} must be a torch.Tensor")
+
+
+def signature(*tensors):
+    """What the checks of a call go by, None for an absent tensor: shape, strides, type and device of each."""
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
+
+
+class CheckedCalls:
+    """Results of a call's checks, kept by ``signature`` and plain numbers (the
+    last 128). An eager call of a few microseconds on the GPU is otherwise
+    bound by its checks (latent attention 38 -> 17 us of host time). What a
+    signature does not hold, addresses and overlaps, is looked at in every call."""
+
+    __slots__ = ("kept",)
+
+    def __init__(self):
+        self.kept = {}
+
+    def get(self, key):
+        return self.kept.get(key)
+
+    def keep(self, key, value):
+        if len(self.kept) >= 128:
+            self.kept.clear()
+        self.kept[key] = value
+        return value
+
+
+def extents(*tensors):
+    """Bytes from the first to past the last element of each tensor, 0 for None."""
+    spans = [(0, 0) if t is None else memory_span(t) for t in tensors]
+    return tuple(end - start for start, end in spans)
+
+
+def pointers_apart(pointers, sizes, written):
+    """Whether the written ranges (indices) overlap no other one."""
+    for w in written:
+        start = pointers[w]
+        end = start + sizes[w]
+        for i, p in enumerate(pointers):
+            if p < end and start < p + sizes[i] and i != w:
+                return False
+    return True

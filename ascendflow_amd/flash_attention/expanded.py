@@ -16,22 +16,61 @@ import ctypes as ct
 import torch
 
 from .. import _native
-from .._tensors import (DTYPES, check_apart, check_distinct_rows, check_rows, check_tensor, kept_by_value, launch_on,
-                        live_strides, require)
+from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, check_tensor,
+                        extents, launch_on, live_strides, pointers_apart, require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 D, R = 128, 64  # columns of k_nope and v, and of k_rope
 
 
-@kept_by_value
-def _params(dtype, Tq, Tk, B, H, qt, qh, kt, kh, rt, vt, vh, ot, oh, SCALE, causal):
-    """Launcher parameters of a call of checked sizes (not changed afterwards)."""
+NAMES = ("q", "k_nope", "k_rope", "v", "cu_seqlens_q", "cu_seqlens_k", "out", "softmax_lse")
+_calls = CheckedCalls()
+
+
+class _Call:
+    """Checked sizes of a call: launcher parameters and each operand's bytes (none changes afterwards)."""
+
+    __slots__ = ("params", "sizes", "launch")
+
+
+def _check(lib, q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_lse, SCALE, causal):
+    require(q.dim() == 3, f"q must be [Tq, H, {D + R}]")
+    b16 = q.dtype
+    require(b16 in _STORAGE, f"q dtype {b16} is not supported; expected bf16 or f16")
+    Tq, H = q.shape[:2]
+    require(k_rope.dim() == 2, f"k_rope must be [Tk, {R}]")
+    Tk = k_rope.shape[0]
+    check_rows("q", q, (Tq, H, D + R), b16)
+    device = q.device
+    check_rows("k_nope", k_nope, (Tk, H, D), b16, device)
+    check_rows("k_rope", k_rope, (Tk, R), b16, device)
+    check_rows("v", v, (Tk, H, D), b16, device)
+    require(cu_seqlens_q.dim() == 1, "cu_seqlens_q must be int32 [B + 1]")
+    B = cu_seqlens_q.numel() - 1
+    check_tensor("cu_seqlens_q", cu_seqlens_q, (B + 1,), torch.int32, device)
+    check_tensor("cu_seqlens_k", cu_seqlens_k, (B + 1,), torch.int32, device)
+    check_rows("out", out, (Tq, H, D), b16, device)
+    check_distinct_rows("out", out)
+    if softmax_lse is not None:
+        check_tensor("softmax_lse", softmax_lse, (Tq, H), torch.float32, device)
     require(B > 0 and H > 0, "positive request and head counts")
     require(SCALE > 0, "positive attention scale")
-    return ct.pointer(_native.LatentExpandedParams(
-        dtype=_native.AFA_DTYPE[dtype], causal=int(causal), Tq=Tq, Tk=Tk, B=B, H=H, D=D, R=R, q_stride_t=qt,
+    strides = []
+    for name, t in (("q", q), ("k_nope", k_nope), ("k_rope", k_rope), ("v", v), ("out", out)):
+        mine = live_strides(t)[:-1]
+        require(all(s % 8 == 0 for s in mine), f"{name} rows must lie on 16-byte boundaries")
+        if name in ("k_nope", "k_rope", "v"):
+            require(mine[0] < 2**23, f"{name} tokens may lie at most 2^23 - 1 elements apart")
+        strides += mine
+    qt, qh, kt, kh, rt, vt, vh, ot, oh = strides
+    call = _Call()
+    call.params = ct.pointer(_native.LatentExpandedParams(
+        dtype=_native.AFA_DTYPE[_STORAGE[b16]], causal=int(causal), Tq=Tq, Tk=Tk, B=B, H=H, D=D, R=R, q_stride_t=qt,
         q_stride_h=qh, k_stride_t=kt, k_stride_h=kh, k_rope_stride_t=rt, v_stride_t=vt, v_stride_h=vh, out_stride_t=ot,
         out_stride_h=oh, scale=SCALE, reserved=0))
+    call.sizes = extents(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_lse)
+    call.launch = lib.launch_latent_attention_expanded
+    return call
 
 
 def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, *, SCALE, CAUSAL=True, out=None,
@@ -50,45 +89,23 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
     ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``).
     Keys and values that some query of a request sees have to be finite.
     """
-    require(isinstance(q, torch.Tensor) and q.dim() == 3, f"q must be [Tq, H, {D + R}]")
-    b16 = q.dtype
-    require(b16 in _STORAGE, f"q dtype {b16} is not supported; expected bf16 or f16")
-    Tq, H = q.shape[:2]
-    require(isinstance(k_rope, torch.Tensor) and k_rope.dim() == 2, f"k_rope must be [Tk, {R}]")
-    Tk = k_rope.shape[0]
-    check_rows("q", q, (Tq, H, D + R), b16)
-    device = q.device
-    check_rows("k_nope", k_nope, (Tk, H, D), b16, device)
-    check_rows("k_rope", k_rope, (Tk, R), b16, device)
-    check_rows("v", v, (Tk, H, D), b16, device)
-    require(isinstance(cu_seqlens_q, torch.Tensor) and cu_seqlens_q.dim() == 1, "cu_seqlens_q must be int32 [B + 1]")
-    B = cu_seqlens_q.numel() - 1
-    check_tensor("cu_seqlens_q", cu_seqlens_q, (B + 1,), torch.int32, device)
-    check_tensor("cu_seqlens_k", cu_seqlens_k, (B + 1,), torch.int32, device)
-    inputs = [("q", q, False), ("k_nope", k_nope, False), ("k_rope", k_rope, False), ("v", v, False),
-              ("cu_seqlens_q", cu_seqlens_q, False), ("cu_seqlens_k", cu_seqlens_k, False)]
-    if out is None:
-        out = torch.empty((Tq, H, D), dtype=b16, device=device)
-    else:
-        check_rows("out", out, (Tq, H, D), b16, device)
-        check_distinct_rows("out", out)
-        check_apart(inputs + [("out", out, True)])
-    if softmax_lse is not None:
-        check_tensor("softmax_lse", softmax_lse, (Tq, H), torch.float32, device)
-        check_apart(inputs + [("out", out, False), ("softmax_lse", softmax_lse, True)])
-    strides = []
-    for name, t in (("q", q), ("k_nope", k_nope), ("k_rope", k_rope), ("v", v), ("out", out)):
-        mine = live_strides(t)[:-1]
-        require(all(s % 8 == 0 for s in mine) and t.data_ptr() % 16 == 0, f"{name} rows must lie on 16-byte boundaries")
-        if name in ("k_nope", "k_rope", "v"):
-            require(mine[0] < 2**23, f"{name} tokens may lie at most 2^23 - 1 elements apart")
-        strides += mine
-    params = _params(_STORAGE[b16], Tq, Tk, B, H, *strides, float(SCALE), bool(CAUSAL))
-    if Tq:
-        status = launch_on(q.get_device(), _native.library().launch_latent_attention_expanded, q.data_ptr(),
-                           k_nope.data_ptr(), k_rope.data_ptr(), v.data_ptr(), cu_seqlens_q.data_ptr(),
-                           cu_seqlens_k.data_ptr(), out.data_ptr(),
-                           None if softmax_lse is None else softmax_lse.data_ptr(), params)
+    lib = _native.library()
+    new = out is None
+    if new:
+        require(isinstance(q, torch.Tensor) and q.dim() == 3, f"q must be [Tq, H, {D + R}]")
+        out = torch.empty((*q.shape[:2], D), dtype=q.dtype, device=q.device)
+    tensors = (q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_lse)
+    check_operands(NAMES, tensors, optional=("softmax_lse",))
+    SCALE, CAUSAL = float(SCALE), bool(CAUSAL)
+    key = (lib, signature(*tensors), SCALE, CAUSAL)
+    call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, SCALE, CAUSAL))
+    pointers = [0 if t is None else t.data_ptr() for t in tensors]
+    for i in (0, 1, 2, 3, 6):
+        require(pointers[i] % 16 == 0, f"{NAMES[i]} rows must lie on 16-byte boundaries")
+    if not pointers_apart(pointers, call.sizes, (7,) if new and softmax_lse is not None else () if new else (6, 7)):
+        check_apart([(n, t, n in ("out", "softmax_lse")) for n, t in zip(NAMES, tensors)])
+    if q.shape[0]:
+        status = launch_on(q.get_device(), call.launch, *pointers, call.params)
         if status:
             _native.check(status, "launch_latent_attention_expanded")
     return out

@@ -13,28 +13,79 @@ from __future__ import annotations
 
 import ctypes as ct
 import math
+from operator import index
 from typing import Optional
 
 import torch
 
 from .. import _native
-from .._tensors import DTYPES, check_apart, check_rows, check_tensor, kept_by_value, launch_on, live_strides, require
+from .._tensors import (DTYPES, CheckedCalls, check_apart, check_operands, check_rows, check_tensor, extents, launch_on,
+                        live_strides, pointers_apart, require, signature)
 from .rotary import LAYOUTS
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 
 
-@kept_by_value
-def _params(dtype, layout, T, B, W, PAGE, BLOCKS, HKV, DK, DV, R, offset, kt, kh, rt, rh, vt, vh, magnitude):
-    """Launcher parameters of a call of checked sizes (not changed afterwards)."""
+NAMES = ("k", "rope", "v", "block_table", "cu_seqlens_q", "seqused_kv", "frequencies", "k_cache", "v_cache")
+_OPTIONAL = ("rope", "v", "frequencies", "v_cache")
+_calls = CheckedCalls()
+
+
+class _Call:
+    """Checked sizes of a call: launcher parameters and each operand's bytes (none changes afterwards)."""
+
+    __slots__ = ("params", "sizes", "launch")
+
+
+def _check(lib, k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, k_cache, v_cache, layout, offset, magnitude):
+    require(k_cache.dim() == 4, "k_cache must be [BLOCKS, PAGE, HKV, DK]")
+    require(k.dim() == 3, "k must be [T, HKV, columns]")
+    b16 = k_cache.dtype
+    require(b16 in _STORAGE, f"k_cache dtype {b16} is not supported; expected bf16 or f16")
+    BLOCKS, PAGE, HKV, DK = k_cache.shape
+    T = k.shape[0]
+    device = k_cache.device
+    R = 0
+    if frequencies is not None:
+        require(frequencies.dim() == 1 and frequencies.numel() > 0, "frequencies must be a float64 [R / 2] tensor")
+        R = 2 * frequencies.numel()
+    check_tensor("k_cache", k_cache, k_cache.shape, b16)
+    if rope is not None:
+        require(R > 0, "rope needs frequencies")
+        check_rows("rope", rope, (T, HKV, R), b16, device)
+        offset = DK - R
+    check_rows("k", k, (T, HKV, DK - R if rope is not None else DK), b16, device)
+    require((v is None) == (v_cache is None), "v and v_cache go together")
+    DV = 0
+    if v is not None:
+        require(v_cache.dim() == 4, "v_cache must be [BLOCKS, PAGE, HKV, DV]")
+        DV = v_cache.shape[3]
+        check_tensor("v_cache", v_cache, (BLOCKS, PAGE, HKV, DV), b16, device)
+        check_rows("v", v, (T, HKV, DV), b16, device)
+    require(block_table.dim() == 2, "block_table must be int32 [B, W]")
+    B, W = block_table.shape
+    i32 = torch.int32
+    check_tensor("block_table", block_table, (B, W), i32, device)
+    check_tensor("cu_seqlens_q", cu_seqlens_q, (B + 1,), i32, device)
+    check_tensor("seqused_kv", seqused_kv, (B,), i32, device)
+    if frequencies is not None:
+        check_tensor("frequencies", frequencies, (R // 2,), torch.float64, device)
     require(layout in LAYOUTS, 'layout must be "half" or "interleaved"')
     require(R == 0 or 0 <= offset <= DK - R, f"the rotated columns {offset} to {offset + R} must lie inside the row ({DK})")
     require(math.isfinite(magnitude), "magnitude must be finite")
-    require(B > 0 and W > 0 and BLOCKS > 0 and PAGE > 0 and HKV > 0 and DK > 0, "requests, pages, heads and columns must not be empty")
-    return ct.pointer(_native.AppendPagedKvParams(
-        dtype=_native.AFA_DTYPE[dtype], layout=LAYOUTS[layout], T=T, B=B, W=W, PAGE=PAGE, BLOCKS=BLOCKS, HKV=HKV, DK=DK,
-        DV=DV, R=R, offset=offset, k_stride_t=kt, k_stride_h=kh, rope_stride_t=rt, rope_stride_h=rh, v_stride_t=vt,
-        v_stride_h=vh, magnitude=magnitude, reserved=0))
+    require(B > 0 and W > 0 and BLOCKS > 0 and PAGE > 0 and HKV > 0 and DK > 0,
+            "requests, pages, heads and columns must not be empty")
+    kt, kh = live_strides(k)[:2]
+    rt, rh = (0, 0) if rope is None else live_strides(rope)[:2]
+    vt, vh = (0, 0) if v is None else live_strides(v)[:2]
+    call = _Call()
+    call.params = ct.pointer(_native.AppendPagedKvParams(
+        dtype=_native.AFA_DTYPE[_STORAGE[b16]], layout=LAYOUTS[layout], T=T, B=B, W=W, PAGE=PAGE, BLOCKS=BLOCKS, HKV=HKV,
+        DK=DK, DV=DV, R=R, offset=offset if R else 0, k_stride_t=kt, k_stride_h=kh, rope_stride_t=rt, rope_stride_h=rh,
+        v_stride_t=vt, v_stride_h=vh, magnitude=magnitude, reserved=0))
+    call.sizes = extents(k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, k_cache, v_cache)
+    call.launch = lib.launch_append_paged_kv
+    return call
 
 
 def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v_cache=None, *, rope=None,
@@ -58,51 +109,17 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
     name the same row. The call reads no values on the host and can be captured
     in a graph.
     """
-    require(isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4, "k_cache must be [BLOCKS, PAGE, HKV, DK]")
-    require(isinstance(k, torch.Tensor) and k.dim() == 3, "k must be [T, HKV, columns]")
-    b16 = k_cache.dtype
-    require(b16 in _STORAGE, f"k_cache dtype {b16} is not supported; expected bf16 or f16")
-    BLOCKS, PAGE, HKV, DK = k_cache.shape
-    T = k.shape[0]
-    device = k_cache.device
-    R = 0
-    if frequencies is not None:
-        require(isinstance(frequencies, torch.Tensor) and frequencies.dim() == 1 and frequencies.numel() > 0,
-                "frequencies must be a float64 [R / 2] tensor")
-        R = 2 * frequencies.numel()
-    check_tensor("k_cache", k_cache, k_cache.shape, b16)
-    if rope is not None:
-        require(R > 0, "rope needs frequencies")
-        check_rows("rope", rope, (T, HKV, R), b16, device)
-        offset = DK - R
-    check_rows("k", k, (T, HKV, DK - R if rope is not None else DK), b16, device)
-    require((v is None) == (v_cache is None), "v and v_cache go together")
-    DV = 0
-    if v is not None:
-        require(isinstance(v_cache, torch.Tensor) and v_cache.dim() == 4, "v_cache must be [BLOCKS, PAGE, HKV, DV]")
-        DV = v_cache.shape[3]
-        check_tensor("v_cache", v_cache, (BLOCKS, PAGE, HKV, DV), b16, device)
-        check_rows("v", v, (T, HKV, DV), b16, device)
-    require(isinstance(block_table, torch.Tensor) and block_table.dim() == 2, "block_table must be int32 [B, W]")
-    B, W = block_table.shape
-    i32 = torch.int32
-    check_tensor("block_table", block_table, (B, W), i32, device)
-    check_tensor("cu_seqlens_q", cu_seqlens_q, (B + 1,), i32, device)
-    check_tensor("seqused_kv", seqused_kv, (B,), i32, device)
-    if frequencies is not None:
-        check_tensor("frequencies", frequencies, (R // 2,), torch.float64, device)
-    check_apart([("k", k, False), ("rope", rope, False), ("v", v, False), ("block_table", block_table, False),
-                 ("cu_seqlens_q", cu_seqlens_q, False), ("seqused_kv", seqused_kv, False),
-                 ("frequencies", frequencies, False), ("k_cache", k_cache, True), ("v_cache", v_cache, True)])
-    params = _params(_STORAGE[b16], layout, T, B, W, PAGE, BLOCKS, HKV, DK, DV, R, offset, *live_strides(k)[:2],
-                     *((0, 0) if rope is None else live_strides(rope)[:2]), *((0, 0) if v is None else live_strides(v)[:2]),
-                     float(magnitude))
-    if T:
-        status = launch_on(k_cache.get_device(), _native.library().launch_append_paged_kv, k.data_ptr(),
-                           None if rope is None else rope.data_ptr(), None if v is None else v.data_ptr(),
-                           block_table.data_ptr(), cu_seqlens_q.data_ptr(), seqused_kv.data_ptr(),
-                           None if frequencies is None else frequencies.data_ptr(), k_cache.data_ptr(),
-                           None if v is None else v_cache.data_ptr(), params)
+    lib = _native.library()
+    tensors = (k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, k_cache, v_cache)
+    check_operands(NAMES, tensors, _OPTIONAL)
+    offset, magnitude = index(offset), float(magnitude)
+    key = (lib, signature(*tensors), layout, offset, magnitude)
+    call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, layout, offset, magnitude))
+    pointers = [0 if t is None else t.data_ptr() for t in tensors]
+    if not pointers_apart(pointers, call.sizes, (7, 8)):
+        check_apart([(n, t, n in ("k_cache", "v_cache")) for n, t in zip(NAMES, tensors)])
+    if k.shape[0]:
+        status = launch_on(k_cache.get_device(), call.launch, *pointers, call.params)
         if status:
             _native.check(status, "launch_append_paged_kv")
     return k_cache if v is None else (k_cache, v_cache)

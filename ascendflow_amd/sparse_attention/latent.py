@@ -20,54 +20,30 @@ from typing import Optional
 import torch
 
 from .. import _native
-from .._tensors import (DTYPES, check_apart, check_distinct_rows, check_rows, check_tensor, kept_by_value, launch_on,
-                        live_strides, require)
+from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, check_tensor,
+                        extents, launch_on, live_strides, pointers_apart, require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
+
+
+NAMES = ("q", "q_rope", "kv_cache", "block_table", "cu_seqlens_q", "seqused_kv", "out", "softmax_lse")
+_calls = CheckedCalls()
 
 
 def row_strides(name, tensor):
     """(token, head) strides of a tensor whose rows the kernels read in 16-byte pieces."""
     t, h = live_strides(tensor)[:2]
-    require(t % 8 == 0 and h % 8 == 0 and tensor.data_ptr() % 16 == 0, f"{name} rows must lie on 16-byte boundaries")
+    require(t % 8 == 0 and h % 8 == 0, f"{name} rows must lie on 16-byte boundaries")
     return t, h
 
 
-@kept_by_value
-def _params(lib, dtype, T, B, H, L, R, PAGE, W, BLOCKS, qt, qh, rt, rh, ot, oh, SCALE, causal):
-    """Launcher parameters and workspace bytes of a call of checked sizes (not changed afterwards)."""
-    require(H > 0 and B > 0 and W > 0 and BLOCKS > 0, "heads, requests and pages must not be empty")
-    require(L in (128, 256, 512), "the latent width (columns of q) must be 128, 256 or 512")
-    require(R in (0, 64), "the rotary width must be 64, or 0 without q_rope")
-    require(PAGE >= 16 and PAGE & (PAGE - 1) == 0, "PAGE must be a power of two from 16 on")
-    require(SCALE > 0, "positive attention scale")
-    params = _native.LatentParams(
-        dtype=_native.AFA_DTYPE[dtype], causal=int(causal), T=T, B=B, H=H, L=L, R=R, PAGE=PAGE, W=W, BLOCKS=BLOCKS,
-        q_stride_t=qt, q_stride_h=qh, q_rope_stride_t=rt, q_rope_stride_h=rh, out_stride_t=ot, out_stride_h=oh,
-        scale=SCALE, reserved=0)
-    nbytes = ct.c_uint64(0)
-    _native.check(lib.workspace_size_latent_attention(ct.byref(nbytes), ct.byref(params)), "workspace_size_latent_attention")
-    return ct.pointer(params), nbytes.value
+class _Call:
+    """Checked sizes of a call: launcher parameters, workspace bytes and each operand's bytes (none changes afterwards)."""
+
+    __slots__ = ("params", "nbytes", "sizes", "launch")
 
 
-def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCALE, q_rope=None, CAUSAL=True, out=None,
-                     softmax_lse=None):
-    """Returns ``out`` [T, H, L]: dense attention of every token over its request's cache rows.
-
-    ``q`` [T, H, L] (L 128, 256 or 512) and ``q_rope`` [T, H, 64], or None:
-    bf16 or f16, any strides of tokens and heads, rows on 16 bytes. ``kv_cache``
-    [BLOCKS, PAGE, 1, L + R], contiguous, R the width of ``q_rope`` or 0, PAGE a
-    power of two from 16 on. ``block_table`` int32 [B, W], ``cu_seqlens_q`` int32
-    [B + 1], ``seqused_kv`` int32 [B]: rows of each request, the new tokens'
-    included (``append_paged_kv`` writes them). With ``CAUSAL`` token j of a
-    request's n sees rows up to ``seqused_kv[b] - n + j``, without all of them.
-    ``softmax_lse`` (optional float32 [T, H]) receives ln(sum_j exp(s_j)).
-
-    A token that sees no row gets zeros and -inf; tokens at or past
-    ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``).
-    Rows behind ``seqused_kv`` are never read and pages outside the cache hold no
-    keys, but the rows that some token of a request sees have to be finite.
-    """
+def _check(lib, q, q_rope, kv_cache, block_table, cu_seqlens_q, seqused_kv, out, softmax_lse, SCALE, causal):
     require(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [T, H, L]")
     b16 = q.dtype
     require(b16 in _STORAGE, f"q dtype {b16} is not supported; expected bf16 or f16")
@@ -89,34 +65,71 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
     check_tensor("seqused_kv", seqused_kv, (B,), i32, device)
     if q_rope is not None:
         check_rows("q_rope", q_rope, (T, H, R), b16, device)
+    check_rows("out", out, (T, H, L), b16, device)
+    check_distinct_rows("out", out)
     if softmax_lse is not None:
         check_tensor("softmax_lse", softmax_lse, (T, H), torch.float32, device)
-    if out is None:
-        out = torch.empty((T, H, L), dtype=b16, device=device)
-    else:
-        check_rows("out", out, (T, H, L), b16, device)
-        check_distinct_rows("out", out)
-        check_apart([("q", q, False), ("q_rope", q_rope, False), ("kv_cache", kv_cache, False),
-                     ("block_table", block_table, False), ("cu_seqlens_q", cu_seqlens_q, False),
-                     ("seqused_kv", seqused_kv, False), ("out", out, True)])
-    if softmax_lse is not None:
-        check_apart([("q", q, False), ("q_rope", q_rope, False), ("kv_cache", kv_cache, False),
-                     ("block_table", block_table, False), ("cu_seqlens_q", cu_seqlens_q, False),
-                     ("seqused_kv", seqused_kv, False), ("out", out, False), ("softmax_lse", softmax_lse, True)])
+    require(H > 0 and B > 0 and W > 0 and BLOCKS > 0, "heads, requests and pages must not be empty")
+    require(L in (128, 256, 512), "the latent width (columns of q) must be 128, 256 or 512")
+    require(R in (0, 64), "the rotary width must be 64, or 0 without q_rope")
+    require(PAGE >= 16 and PAGE & (PAGE - 1) == 0, "PAGE must be a power of two from 16 on")
+    require(SCALE > 0, "positive attention scale")
+    qt, qh = row_strides("q", q)
+    rt, rh = (0, 0) if q_rope is None else row_strides("q_rope", q_rope)
+    ot, oh = row_strides("out", out)
+    params = _native.LatentParams(
+        dtype=_native.AFA_DTYPE[_STORAGE[b16]], causal=int(causal), T=T, B=B, H=H, L=L, R=R, PAGE=PAGE, W=W,
+        BLOCKS=BLOCKS, q_stride_t=qt, q_stride_h=qh, q_rope_stride_t=rt, q_rope_stride_h=rh, out_stride_t=ot,
+        out_stride_h=oh, scale=SCALE, reserved=0)
+    nbytes = ct.c_uint64(0)
+    _native.check(lib.workspace_size_latent_attention(ct.byref(nbytes), ct.byref(params)), "workspace_size_latent_attention")
+    call = _Call()
+    call.params, call.nbytes = ct.pointer(params), nbytes.value
+    call.sizes = extents(q, q_rope, kv_cache, block_table, cu_seqlens_q, seqused_kv, out, softmax_lse)
+    call.launch = lib.launch_latent_attention
+    return call
+
+
+def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCALE, q_rope=None, CAUSAL=True, out=None,
+                     softmax_lse=None):
+    """Returns ``out`` [T, H, L]: dense attention of every token over its request's cache rows.
+
+    ``q`` [T, H, L] (L 128, 256 or 512) and ``q_rope`` [T, H, 64], or None:
+    bf16 or f16, any strides of tokens and heads, rows on 16 bytes. ``kv_cache``
+    [BLOCKS, PAGE, 1, L + R], contiguous, R the width of ``q_rope`` or 0, PAGE a
+    power of two from 16 on. ``block_table`` int32 [B, W], ``cu_seqlens_q`` int32
+    [B + 1], ``seqused_kv`` int32 [B]: rows of each request, the new tokens'
+    included (``append_paged_kv`` writes them). With ``CAUSAL`` token j of a
+    request's n sees rows up to ``seqused_kv[b] - n + j``, without all of them.
+    ``softmax_lse`` (optional float32 [T, H]) receives ln(sum_j exp(s_j)).
+
+    A token that sees no row gets zeros and -inf; tokens at or past
+    ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``).
+    Rows behind ``seqused_kv`` are never read and pages outside the cache hold no
+    keys, but the rows that some token of a request sees have to be finite.
+    """
     lib = _native.library()
-    params, nbytes = _params(lib, _STORAGE[b16], T, B, H, L, R, PAGE, W, BLOCKS, *row_strides("q", q),
-                     *((0, 0) if q_rope is None else row_strides("q_rope", q_rope)), *row_strides("out", out),
-                     float(SCALE), bool(CAUSAL))
-    if T:
+    new = out is None
+    if new:
+        require(isinstance(q, torch.Tensor), "q must be [T, H, L]")
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    tensors = (q, q_rope, kv_cache, block_table, cu_seqlens_q, seqused_kv, out, softmax_lse)
+    check_operands(NAMES, tensors, optional=("q_rope", "softmax_lse"))
+    SCALE, CAUSAL = float(SCALE), bool(CAUSAL)
+    key = (lib, signature(*tensors), SCALE, CAUSAL)
+    call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, SCALE, CAUSAL))
+    pointers = [0 if t is None else t.data_ptr() for t in tensors]
+    for i in (0, 1, 2, 6):
+        require(pointers[i] % 16 == 0, f"{NAMES[i]} rows must lie on 16-byte boundaries")
+    if not pointers_apart(pointers, call.sizes, (7,) if new and softmax_lse is not None else () if new else (6, 7)):
+        check_apart([(n, t, n in ("out", "softmax_lse")) for n, t in zip(NAMES, tensors)])
+    if q.shape[0]:
         workspace = None
-        if nbytes:
+        if call.nbytes:
             # Partial results; the caching allocator keeps the block for this stream.
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            scratch = torch.empty(call.nbytes, dtype=torch.uint8, device=q.device)
             workspace = scratch.data_ptr()
-        status = launch_on(q.get_device(), lib.launch_latent_attention, q.data_ptr(),
-                           None if q_rope is None else q_rope.data_ptr(), kv_cache.data_ptr(), block_table.data_ptr(),
-                           cu_seqlens_q.data_ptr(), seqused_kv.data_ptr(), out.data_ptr(),
-                           None if softmax_lse is None else softmax_lse.data_ptr(), workspace, nbytes, params)
+        status = launch_on(q.get_device(), call.launch, *pointers, workspace, call.nbytes, call.params)
         if status:
             _native.check(status, "launch_latent_attention")
     return out

@@ -16,11 +16,13 @@ from __future__ import annotations
 
 import ctypes as ct
 import math
+from operator import index
 
 import torch
 
 from .. import _native
-from .._tensors import DTYPES, check_apart, check_distinct_rows, check_rows, kept_by_value, launch_on, live_strides, require
+from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, extents,
+                        launch_on, live_strides, pointers_apart, require, signature)
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
@@ -61,54 +63,68 @@ def rotary_magnitude(factor, coefficient=1.0):
     return 0.1 * coefficient * math.log(factor) + 1.0 if factor > 1.0 else 1.0
 
 
-@kept_by_value
-def _params(dtype, layout, inverse, position_bytes, H, D, R, offset, B, S, xb, xs, xh, ob, os, oh, position_stride, magnitude):
-    """Launcher parameters of a call of checked sizes (not changed afterwards)."""
-    require(layout in LAYOUTS, 'layout must be "half" or "interleaved"')
-    require(R >= 2 and 0 <= offset <= D - R, f"the rotated columns {offset} to {offset + R} must lie inside the head ({D})")
-    require(math.isfinite(magnitude), "magnitude must be finite")
-    return ct.pointer(_native.RotaryParams(
-        dtype=_native.AFA_DTYPE[dtype], layout=LAYOUTS[layout], inverse=int(inverse), position_bytes=position_bytes,
-        H=H, D=D, R=R, offset=offset, B=B, S=S, x_stride_b=xb, x_stride_s=xs, x_stride_h=xh, out_stride_b=ob,
-        out_stride_s=os, out_stride_h=oh, position_stride_b=position_stride, magnitude=magnitude, reserved=0))
+NAMES = ("x", "positions", "frequencies", "out")
+_calls = CheckedCalls()
 
 
-def _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out):
-    require(isinstance(x, torch.Tensor) and x.dim() in (3, 4), "x must be [T, H, D] or [B, H, S, D]")
+class _Call:
+    """Checked sizes of a call: launcher parameters and each operand's bytes (none changes afterwards)."""
+
+    __slots__ = ("params", "sizes", "launch")
+
+
+def _check(lib, x, positions, frequencies, out, layout, offset, magnitude, inverse):
+    require(x.dim() in (3, 4), "x must be [T, H, D] or [B, H, S, D]")
     require(x.dtype in _STORAGE, f"x dtype {x.dtype} is not supported; expected bf16 or f16")
     if x.dim() == 3:
         (S, H, D), B = x.shape, 1
     else:
         B, H, S, D = x.shape
     require(H > 0 and D > 0, "x must have heads and columns")
-    require(isinstance(positions, torch.Tensor) and positions.dtype in (torch.int32, torch.int64),
-            "positions must be an int32 or int64 tensor")
+    require(positions.dtype in (torch.int32, torch.int64), "positions must be an int32 or int64 tensor")
     require(tuple(positions.shape) == (S,) or (x.dim() == 4 and tuple(positions.shape) == (B, S)),
             f"positions shape {tuple(positions.shape)} does not fit x {tuple(x.shape)}")
-    require(isinstance(frequencies, torch.Tensor) and frequencies.dim() == 1 and frequencies.numel() > 0,
-            "frequencies must be a float64 [R / 2] tensor")
+    require(frequencies.dim() == 1 and frequencies.numel() > 0, "frequencies must be a float64 [R / 2] tensor")
     check_rows("x", x, x.shape, x.dtype)
     device = x.device
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=device)
-    elif out is not x:
-        check_rows("out", out, x.shape, x.dtype, device)
+    check_rows("out", out, x.shape, x.dtype, device)
     check_rows("positions", positions, positions.shape, positions.dtype, device)
     check_rows("frequencies", frequencies, frequencies.shape, torch.float64, device)
-    in_place = out is x or (out.data_ptr() == x.data_ptr() and out.stride() == x.stride())
     check_distinct_rows("out", out)
-    check_apart([("x", None if in_place else x, False), ("positions", positions, False),
-                 ("frequencies", frequencies, False), ("out", out, True)])
+    R = 2 * frequencies.numel()
+    require(layout in LAYOUTS, 'layout must be "half" or "interleaved"')
+    require(0 <= offset <= D - R, f"the rotated columns {offset} to {offset + R} must lie inside the head ({D})")
+    require(math.isfinite(magnitude), "magnitude must be finite")
     xs, os = live_strides(x), live_strides(out)
-    if x.dim() == 3:
-        xs, os = (0, xs[0], xs[1]), (0, os[0], os[1])
-    else:
-        xs, os = (xs[0], xs[2], xs[1]), (os[0], os[2], os[1])
-    params = _params(_STORAGE[x.dtype], layout, bool(inverse), positions.element_size(), H, D, 2 * frequencies.numel(),
-                     offset, B, S, *xs, *os, live_strides(positions)[0] if positions.dim() == 2 else 0, float(magnitude))
+    xs, os = ((0, xs[0], xs[1]), (0, os[0], os[1])) if x.dim() == 3 else ((xs[0], xs[2], xs[1]), (os[0], os[2], os[1]))
+    call = _Call()
+    call.params = ct.pointer(_native.RotaryParams(
+        dtype=_native.AFA_DTYPE[_STORAGE[x.dtype]], layout=LAYOUTS[layout], inverse=int(inverse),
+        position_bytes=positions.element_size(), H=H, D=D, R=R, offset=offset, B=B, S=S, x_stride_b=xs[0],
+        x_stride_s=xs[1], x_stride_h=xs[2], out_stride_b=os[0], out_stride_s=os[1], out_stride_h=os[2],
+        position_stride_b=live_strides(positions)[0] if positions.dim() == 2 else 0, magnitude=magnitude, reserved=0))
+    call.sizes = extents(x, positions, frequencies, out)
+    call.launch = lib.launch_apply_rotary
+    return call
+
+
+def _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out):
+    lib = _native.library()
+    new = out is None
+    if new:
+        require(isinstance(x, torch.Tensor), "x must be a torch.Tensor")
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    tensors = (x, positions, frequencies, out)
+    check_operands(NAMES, tensors)
+    key = (lib, signature(*tensors), layout, offset, magnitude, inverse)
+    call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, layout, offset, magnitude, inverse))
+    pointers = [t.data_ptr() for t in tensors]
+    if not new and not pointers_apart(pointers, call.sizes, (3,)):
+        in_place = pointers[0] == pointers[3] and x.stride() == out.stride()
+        check_apart([("x", None if in_place else x, False), ("positions", positions, False),
+                     ("frequencies", frequencies, False), ("out", out, True)])
     if x.numel():
-        status = launch_on(x.get_device(), _native.library().launch_apply_rotary, x.data_ptr(), positions.data_ptr(),
-                           frequencies.data_ptr(), out.data_ptr(), params)
+        status = launch_on(x.get_device(), call.launch, *pointers, call.params)
         if status:
             _native.check(status, "launch_apply_rotary")
     return out
@@ -146,7 +162,13 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         layout, offset, magnitude, inverse = ctx.how
-        return _Rotary.apply(_dense_rows(grad), *ctx.saved_tensors, layout, offset, magnitude, not inverse), *[None] * 6
+        positions, frequencies = ctx.saved_tensors
+        grad = _dense_rows(grad)
+        if not torch.is_grad_enabled():
+            turned = _rotate(grad, positions, frequencies, layout, offset, magnitude, not inverse, None)
+        else:
+            turned = _Rotary.apply(grad, positions, frequencies, layout, offset, magnitude, not inverse)
+        return turned, None, None, None, None, None, None
 
 
 def _dense_rows(grad):
@@ -171,10 +193,11 @@ def apply_rotary(x, positions, frequencies, *, layout="half", offset=0, magnitud
     place, otherwise memory apart from it) it is written there, without one.
     Raises ``ValueError`` for shapes, types, devices or overlaps that do not fit.
     """
+    offset = index(offset)
     if out is not None or not (torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad):
         require(out is None or not (torch.is_grad_enabled() and (x.requires_grad or out.requires_grad)),
                 "out cannot be given where a gradient is recorded")
-        return _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out)
+        return _rotate(x, positions, frequencies, layout, offset, float(magnitude), bool(inverse), out)
     return _Rotary.apply(x, positions, frequencies, layout, offset, float(magnitude), bool(inverse))
 
 
