@@ -30,7 +30,12 @@ namespace afa {
 
 constexpr float LAT_LOG2E = 1.4426950408889634f, LAT_LN2 = 0.6931471805599453f;
 constexpr float LAT_TAU = 8.0f;
-constexpr int LAT_KEYS = 32;  // cache rows per chunk
+// Cache rows per chunk. Eight waves (one workgroup per CU): 64, two slots; a
+// barrier, a fetch and a reduction per 64 rows instead of 32 and four chains of
+// dependent matrix instructions instead of two (128 heads, 4 chunks of 512 tokens
+// behind 8K: 4317 -> XXXX us). Four waves: 32, two slots in each of the CU's two
+// workgroups.
+template <int NW> __host__ __device__ constexpr int lat_keys() { return NW == 8 ? 64 : 32; }
 
 struct LatentArgs {
   const void* q;
@@ -63,13 +68,13 @@ struct LatentRecord {
 // Split form: the chunks of all tiles, in order, are one sequence that the
 // workgroups share evenly, so that few or unequal requests fill the GPU and end
 // together. A tile counts its chunks (those of its request's last token) and
-// LAT_START chunks for its start and end. A workgroup takes at most one tile's
+// 64 rows' worth for its start and end. A workgroup takes at most one tile's
 // end, whole tiles and one tile's beginning; parts go to the workspace (slot
 // 2 w the end, 2 w + 1 the beginning) as float32 and latent_merge_kernel
 // combines them in order. Everything is computed on the device from
 // cu_seqlens_q and seqused_kv, alike in every workgroup.
-constexpr uint32_t LAT_START = 2;
-constexpr uint32_t LAT_LEAST = 4;  // least chunks (and starts) of a workgroup
+template <int NW> __device__ constexpr uint32_t lat_start() { return 64 / lat_keys<NW>(); }
+template <int NW> __device__ constexpr uint32_t lat_least() { return 128 / lat_keys<NW>(); }  // least of a workgroup
 constexpr int LAT_MAX_WORKERS = 512;
 
 // Metadata in the constant address space, so that uniform reads are scalar loads,
@@ -125,8 +130,8 @@ __device__ __forceinline__ bool find_tile(const_ints cu, int B, int T, uint32_t 
 }
 
 // Chunks that a request's tiles count in the split form.
-__device__ __forceinline__ uint32_t longest_chunks(int used, int count) {
-  return count > 0 ? ((uint32_t)max(used, 0) + LAT_KEYS - 1) / LAT_KEYS : 0u;
+template <int NW> __device__ __forceinline__ uint32_t longest_chunks(int used, int count) {
+  return count > 0 ? ((uint32_t)max(used, 0) + lat_keys<NW>() - 1) / lat_keys<NW>() : 0u;
 }
 
 __device__ __forceinline__ uint64_t inclusive_scan64(uint64_t v, int lane) {
@@ -153,8 +158,9 @@ struct LatentShare {
   uint32_t tiles_before;     // of earlier requests
 };
 
-template <int THREADS, int ROWS>
+template <int NW>
 __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker, LatentShare& share) {
+  constexpr int THREADS = NW * 64, ROWS = NW * 16;
   __shared__ uint64_t wave_weight[THREADS / 64];
   __shared__ uint32_t wave_tiles[THREADS / 64];
   __shared__ uint32_t found[4];
@@ -165,7 +171,7 @@ __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker,
     request_tokens(constant(a.cu), b, a.T, start, count);
     const int used = (int)min((int64_t)max(constant(a.used)[b], 0), (int64_t)a.W << a.page_shift);
     tiles = ((uint32_t)count * (uint32_t)a.H + ROWS - 1) / ROWS;
-    each = longest_chunks(used, count) + LAT_START;
+    each = longest_chunks<NW>(used, count) + lat_start<NW>();
   };
   uint64_t weight = 0;
   uint32_t tiles = 0;
@@ -198,7 +204,7 @@ __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker,
   total = uniform64(total);
   if (worker == 0 && tid == 0) *a.tile_count = all;
   if (total == 0) return false;
-  const uint64_t most = total / LAT_LEAST;
+  const uint64_t most = total / lat_least<NW>();
   share.workers = most < 1 ? 1 : (most < (uint64_t)a.workers ? (int)most : a.workers);
   if (worker >= (uint32_t)share.workers) return false;
   share.workers = uniform(share.workers);
@@ -241,10 +247,12 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   constexpr int ROWS = 16 * NW;
   constexpr int LROW = 2 * L;                  // bytes of a latent row in LDS
   constexpr int GROW = 2 * (L + R);            // bytes of a cache row
-  constexpr int ROPE_AT = LAT_KEYS * LROW;     // the rotary parts follow the latents
-  constexpr int SLOT = LAT_KEYS * GROW;
-  constexpr int NS = NW == 8 ? 4 : 2;          // ring slots: one workgroup per CU, or two
-  constexpr int RW = LAT_KEYS / NW;            // rows that one wave loads
+  constexpr int KEYS = lat_keys<NW>(), KT = KEYS / 16;
+  constexpr int ROPE_AT = KEYS * LROW;         // the rotary parts follow the latents
+  constexpr int SLOT = KEYS * GROW;
+  constexpr int NS = NW == 8 && L < 512 ? 3 : 2;  // ring slots: what 160 KiB hold for one workgroup per CU, or two
+  constexpr int RW = 8;                        // rows that one wave loads
+  static_assert(RW * NW == KEYS, "a chunk is loaded by all waves");
   constexpr int LR = 512 / L, LOADS_L = RW / LR, LOADS = LOADS_L + (R ? 1 : 0);
   constexpr int KSTEPS = L / 32, RSTEPS = R / 32, VTILES = L / 16;
   __shared__ __attribute__((aligned(256))) uint8_t ring[NS][SLOT];
@@ -261,7 +269,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   LatentShare share;
   uint64_t left = 0;  // of this workgroup's share
   if constexpr (SPLIT) {
-    if (!find_share<NW * 64, ROWS>(a, worker, share)) return;
+    if (!find_share<NW>(a, worker, share)) return;
     request = share.request;
     tile = share.tile;
     left = share.end - share.begin;
@@ -301,15 +309,16 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   };
   const int kv_end = visible((min((int)(tile + 1) * ROWS, rows) - 1) / H);
   const int clean_end = visible((int)tile * ROWS / H);  // no row of the tile hides a key below
-  const int all_chunks = (kv_end + LAT_KEYS - 1) / LAT_KEYS;
+  const int all_chunks = (kv_end + KEYS - 1) / KEYS;
   int begin = 0, chunks = all_chunks;  // of this part
   bool whole = true;
   if constexpr (SPLIT) {
     // The tile's own chunks, spread over what it counts.
-    const uint32_t counted = longest_chunks(used, count), each = counted + LAT_START;
+    constexpr uint32_t START = lat_start<NW>();
+    const uint32_t counted = longest_chunks<NW>(used, count), each = counted + START;
     const uint32_t end = (uint32_t)min((uint64_t)each, (uint64_t)offset + left);
     auto cut = [&](uint32_t x) {
-      return x >= each ? all_chunks : (x <= LAT_START ? 0 : (int)((uint64_t)(x - LAT_START) * (uint32_t)all_chunks / counted));
+      return x >= each ? all_chunks : (x <= START ? 0 : (int)((uint64_t)(x - START) * (uint32_t)all_chunks / counted));
     };
     begin = cut(offset);
     chunks = cut(end);
@@ -332,25 +341,34 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   const uint32_t ring_base = lds_address(ring[0]);
   const const_ints pages = constant(a.table + (int64_t)request * a.W);
   const int page_mask = (1 << a.page_shift) - 1;
-  // Page of the 16-row group that holds `key`; -1 past the end.
-  auto page_of = [&](int key) { return key < kv_end ? pages[key >> a.page_shift] : -1; };
   auto inside = [&](int page) { return (uint32_t)page < (uint32_t)a.blocks; };
-  int next[2];         // pages of the two 16-row groups of the next chunk to load
-  uint32_t good = 0;   // two bits per chunk loaded, the latest lowest: its groups' pages lie in the cache
+  int page[KT];        // of the 16-row groups of the next chunk to load, -1 past the end
+  uint32_t good = 0;   // KT bits per chunk loaded, the latest lowest: its groups' pages lie in the cache
   int partial = 0;     // chunks until every one in flight has all its loads
   auto look_up = [&](int chunk) {
-    next[0] = page_of(chunk * LAT_KEYS);
-    next[1] = page_of(chunk * LAT_KEYS + 16);
+    const int key = chunk * KEYS;
+    if (a.page_shift >= (KEYS == 64 ? 6 : 5)) {  // one page
+      page[0] = key < kv_end ? pages[key >> a.page_shift] : -1;
+#pragma unroll
+      for (int i = 1; i < KT; ++i) page[i] = key + 16 * i < kv_end ? page[0] : -1;
+    } else {
+#pragma unroll
+      for (int i = 0; i < KT; ++i) page[i] = key + 16 * i < kv_end ? pages[(key + 16 * i) >> a.page_shift] : -1;
+    }
   };
   auto fetch = [&](int chunk) {
-    const bool ok0 = inside(next[0]), ok1 = inside(next[1]);
-    good = (good << 2) | (ok0 ? 1u : 0u) | (ok1 ? 2u : 0u);
-    const int first = wave * RW;  // of the chunk's rows
-    const int key = chunk * LAT_KEYS + first;
-    const bool upper = first >= 16;
-    const int page = upper ? next[1] : next[0];
-    const int have = (upper ? ok1 : ok0) ? min(max(kv_end - key, 0), RW) : 0;
-    const char* from = (const char*)a.cache + ((int64_t)page * (page_mask + 1) + (key & page_mask)) * GROW;
+    const int first = wave * RW, group = first >> 4;  // of the chunk's rows
+    const int key = chunk * KEYS + first;
+    int mine = page[0];
+    uint32_t bits = inside(page[0]) ? 1u : 0u;
+#pragma unroll
+    for (int i = 1; i < KT; ++i) {
+      bits |= inside(page[i]) ? 1u << i : 0u;
+      mine = group == i ? page[i] : mine;
+    }
+    good = (good << KT) | bits;
+    const int have = (bits >> group) & 1u ? min(max(kv_end - key, 0), RW) : 0;
+    const char* from = (const char*)a.cache + (((int64_t)mine << a.page_shift) + (key & page_mask)) * GROW;
     const uint32_t slot = ring_base + (uint32_t)((chunk - begin) % NS) * SLOT;
     const uint32_t to = opaque_uniform(slot + (uint32_t)(first * LROW));
     const uint32_t to_rope = opaque_uniform(slot + (uint32_t)(ROPE_AT + first * 2 * R));
@@ -372,7 +390,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 #pragma unroll
       for (int p = 0; p < LOADS_L; ++p) load(to + (uint32_t)p * 1024u, latent_off(p * LR + r0));
       if constexpr (R != 0)
-        if (8 * RW == 64 || rope_row < RW) load(to_rope, rope_off());
+        load(to_rope, rope_off());
     } else {
       // Rows past the end or without a page become zeros, which no weight can turn into anything else.
       const u32x4 zero = {0u, 0u, 0u, 0u};
@@ -386,11 +404,10 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
       if constexpr (R != 0) {
         if (rope_row < have)
           load(to_rope, rope_off());
-        else if (rope_row < RW)
+        else
           *(AFA_LDS u32x4*)(uintptr_t)(to_rope + ln * 16u) = zero;
       }
     }
-    look_up(chunk + 1);
   };
 
   // ---- Q fragments: B operand, columns 32 j + 8 g .. + 7 of row i16 -----------
@@ -423,12 +440,16 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   float m_run = -1e30f;  // finite: a chunk that hides all its keys gives p = 0, never NaN
   float l_run = 0.f, l_rounded = 0.f;
 
-  look_up(begin);
 #pragma unroll
   for (int c = 0; c < NS - 1; ++c)
-    if (begin + c < chunks) fetch(begin + c);
+    if (begin + c < chunks) {
+      look_up(begin + c);
+      fetch(begin + c);
+    }
 
   for (int c = begin; c < chunks; ++c) {
+    const bool more = c + NS - 1 < chunks;
+    if (more) look_up(c + NS - 1);
     // Chunk c has landed once at most the loads of the NS - 2 younger chunks are
     // in flight; where one of those has fewer loads, or is missing, all must have.
     if (partial == 0 && c + NS - 2 < chunks)
@@ -437,42 +458,44 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
       wait_vmcnt<0>();
     block_barrier();  // every wave's part of chunk c is there, and chunk c - 1 is read
     const int loaded = min(c + NS - 1, chunks);  // chunks fetched so far
-    const uint32_t bits = (good >> (2 * (loaded - 1 - c))) & 3u;
-    if (c + NS - 1 < chunks) fetch(c + NS - 1);
+    const uint32_t bits = (good >> (KT * (loaded - 1 - c))) & ((1u << KT) - 1u);
+    if (more) fetch(c + NS - 1);
     const uint32_t slot = ring_base + (uint32_t)((c - begin) % NS) * SLOT;
 
-    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    f32x4 s[KT];
     {
-      constexpr int FRAGS = 2 * (KSTEPS + RSTEPS), LOOK = L == 512 ? 4 : 6;
+      constexpr int FRAGS = KT * (KSTEPS + RSTEPS), LOOK = L == 512 ? 4 : 6;
       const uint32_t base = opaque(slot + qk_at), rope = opaque(slot + qr_at);
       x8 kf[FRAGS];
       auto load = [&](int f) {  // (step j, key tile t)
-        const int j = f / 2, t = f % 2;
+        const int j = f / KT, t = f % KT;
         kf[f] = j < KSTEPS ? *(const AFA_LDS x8*)(lds_at<uint8_t>(base ^ (uint32_t)((j & 3) << 6)) + (j >> 2) * 256 + t * 16 * LROW)
                            : *(const AFA_LDS x8*)(lds_at<uint8_t>(rope ^ (uint32_t)((j - KSTEPS) << 6)) + t * 16 * 2 * R);
       };
+#pragma unroll
+      for (int t = 0; t < KT; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int f = 0; f < LOOK; ++f) load(f);
 #pragma unroll
       for (int f = 0; f < FRAGS; ++f) {
         if (f + LOOK < FRAGS) load(f + LOOK);
-        s[f % 2] = B16<DT>::mfma(kf[f], qf[f / 2], s[f % 2]);
+        s[f % KT] = B16<DT>::mfma(kf[f], qf[f / KT], s[f % KT]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    const int key0 = c * LAT_KEYS;
-    if (key0 + LAT_KEYS > clean_end || bits != 3u) {  // uniform
+    const int key0 = c * KEYS;
+    if (key0 + KEYS > clean_end || bits != (1u << KT) - 1u) {  // uniform
       int token, head;
       const int lim = my_row(token, head) ? visible(token) - key0 : 0;  // this row sees the chunk's keys below it
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           s[t][i] = 16 * t + sigma(4 * g + i) < lim && ((bits >> t) & 1u) ? s[t][i] : -INFINITY;
     }
     float top = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
     const float m_new = fmaxf(m_run, max_over_lane_groups(top) * scale_log2);
@@ -484,33 +507,34 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
       for (int t = 0; t < VTILES; ++t) o[t] *= alpha;
       m_run = m_new;
     }
-    x8 pf;
+    x8 pf[KT / 2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float p = fast_exp2(__builtin_fmaf(s[t][i], scale_log2, -m_run));
         const scalar r = (scalar)p;
         l_run += p;
         l_rounded += (float)r;
-        pf[4 * t + i] = r;
+        pf[t / 2][4 * (t % 2) + i] = r;
       }
     {
-      constexpr int LOOK = 3;
+      constexpr int FRAGS = KT / 2 * VTILES, LOOK = 3;
       const uint32_t base = opaque(slot + tr_at);
-      x4 lo[VTILES], hi[VTILES];
-      auto load = [&](int t) {
-        const AFA_LDS uint8_t* p = lds_at<uint8_t>(base ^ (uint32_t)((t & 7) << 5)) + (t >> 3) * 256;
-        lo[t] = B16<DT>::read_tr((const AFA_LDS void*)p);
-        hi[t] = B16<DT>::read_tr((const AFA_LDS void*)(p + 16 * LROW));
+      x4 lo[FRAGS], hi[FRAGS];
+      auto load = [&](int f) {  // (32 rows ks, column tile t)
+        const int ks = f / VTILES, t = f % VTILES;
+        const AFA_LDS uint8_t* p = lds_at<uint8_t>(base ^ (uint32_t)((t & 7) << 5)) + (t >> 3) * 256 + ks * 32 * LROW;
+        lo[f] = B16<DT>::read_tr((const AFA_LDS void*)p);
+        hi[f] = B16<DT>::read_tr((const AFA_LDS void*)(p + 16 * LROW));
       };
 #pragma unroll
-      for (int t = 0; t < LOOK; ++t) load(t);
+      for (int f = 0; f < LOOK; ++f) load(f);
 #pragma unroll
-      for (int t = 0; t < VTILES; ++t) {
-        if (t + LOOK < VTILES) load(t + LOOK);
-        const x8 vf = {lo[t][0], lo[t][1], lo[t][2], lo[t][3], hi[t][0], hi[t][1], hi[t][2], hi[t][3]};
-        o[t] = B16<DT>::mfma(vf, pf, o[t]);
+      for (int f = 0; f < FRAGS; ++f) {
+        if (f + LOOK < FRAGS) load(f + LOOK);
+        const x8 vf = {lo[f][0], lo[f][1], lo[f][2], lo[f][3], hi[f][0], hi[f][1], hi[f][2], hi[f][3]};
+        o[f % VTILES] = B16<DT>::mfma(vf, pf[f / VTILES], o[f % VTILES]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
