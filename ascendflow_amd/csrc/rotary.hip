@@ -9,11 +9,15 @@
 // and the cosine and sine of the rest are float32. The rotation runs in float32
 // and rounds once, to the storage type.
 //
-// Both kernels move each byte once and are bound by HBM (few long calls) or by
-// the launch and a chain of dependent loads (decode). A thread takes 8 pairs
-// (two 16-byte pieces, in either layout) of a token, computes their cosines
-// once and goes over several heads with them; rows that no 16-byte piece fits
-// (odd widths, offsets or strides) take one pair at a time.
+// Both kernels move each byte once and are bound by HBM (many tokens) or by the
+// launch and a chain of dependent loads (decode). A workgroup takes a few
+// tokens: it works out their cosines and sines once, one pair a thread, into
+// LDS, then goes over the rows in pieces of 8 pairs (two 16-byte accesses, in
+// either layout); rows that no 16-byte piece fits (odd widths, offsets or
+// strides) are taken one pair at a time. 8192 tokens of 64 heads x 64 columns take
+// 27.6 us (4.9 TB/s, the rate of a large copy), 4260 ragged prompt tokens of 8
+// heads x 256 columns into pages 11.9 us (22.5 where each thread worked out the
+// cosines of its own 8 pairs), 384 decode tokens of one 576-column row 3.9 (6.1).
 #include <algorithm>
 
 #include "common.h"
@@ -51,21 +55,23 @@ __device__ __forceinline__ void store_piece(typename B16<DT>::scalar* p, const P
   }
 }
 
-// Cosines and sines, magnitude included, of VEC pairs from `pair` on.
-template <int VEC>
-__device__ __forceinline__ void pair_angles(const double* frequencies, int pair, int64_t position, float magnitude,
-                                            bool inverse, float (&c)[VEC], float (&s)[VEC]) {
-#pragma clang fp contract(off)  // the same angles whatever VEC is
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const double turns = (double)position * (frequencies[pair + i] * 0.15915494309189535);  // 1 / 2 pi
-    const float rest = (float)(turns - __builtin_rint(turns));
-    float sine, cosine;
-    sincospif(2.0f * rest, &sine, &cosine);
-    c[i] = magnitude * cosine;
-    s[i] = inverse ? -magnitude * sine : magnitude * sine;
-  }
+constexpr int ROT_MAX_PAIRS = 512, ROT_TOKENS = 8;  // pairs of a row, tokens of a workgroup
+constexpr int ROT_LDS_PAIRS = 1024;                 // pairs of all its tokens
+constexpr int ROT_MAX_D = 16384;                    // columns of a row
+
+// Cosine and sine of a pair, magnitude included.
+__device__ __forceinline__ float2 pair_angle(double frequency, int64_t position, float magnitude, bool inverse) {
+#pragma clang fp contract(off)
+  const double turns = (double)position * (frequency * 0.15915494309189535);  // 1 / 2 pi
+  const float rest = (float)(turns - __builtin_rint(turns));
+  float sine, cosine;
+  sincospif(2.0f * rest, &sine, &cosine);
+  return make_float2(magnitude * cosine, inverse ? -magnitude * sine : magnitude * sine);
 }
+
+// index / n for index * n < 2^32, with m = ceil(2^32 / n): the product exceeds
+// index / n by index (m n - 2^32) / (2^32 n) < 1 / n. n = 1 has m = 0.
+__device__ __forceinline__ uint32_t divide(uint32_t index, uint32_t m) { return m ? __umulhi(index, m) : index; }
 
 // Columns of the two pieces of pair group g inside the rotated part.
 template <int VEC, int LAYOUT>
@@ -82,8 +88,7 @@ __device__ __forceinline__ void piece_columns(int g, int R, int& lo, int& hi) {
 // Rotates the VEC pairs held by the two pieces: halves pair element i of both,
 // interleaved pairs neighbours (of the concatenated pieces).
 template <int DT, int VEC, int LAYOUT>
-__device__ __forceinline__ void rotate_pieces(Piece<DT, VEC>& lo, Piece<DT, VEC>& hi, const float (&c)[VEC],
-                                              const float (&s)[VEC]) {
+__device__ __forceinline__ void rotate_pieces(Piece<DT, VEC>& lo, Piece<DT, VEC>& hi, const float2* angles) {
   typedef typename B16<DT>::scalar scalar;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
@@ -93,10 +98,11 @@ __device__ __forceinline__ void rotate_pieces(Piece<DT, VEC>& lo, Piece<DT, VEC>
       u = 2 * i < VEC ? &lo.e[2 * i] : &hi.e[2 * i - VEC];
       v = u + 1;
     }
+    const float2 t = angles[i];
     const float a = (float)*u, b = (float)*v;
     // Written as fused operations: left to the compiler, their order differs between VEC = 8 and 1.
-    *u = (scalar)__builtin_fmaf(a, c[i], -(b * s[i]));
-    *v = (scalar)__builtin_fmaf(a, s[i], b * c[i]);
+    *u = (scalar)__builtin_fmaf(a, t.x, -(b * t.y));
+    *v = (scalar)__builtin_fmaf(a, t.y, b * t.x);
   }
 }
 
@@ -105,11 +111,11 @@ struct RotaryArgs {
   void* out;
   const void* positions;
   const double* frequencies;
-  int64_t first;  // token index of item 0 (calls of more than 2^31 items are launched in parts)
-  int64_t S, x_b, x_s, x_h, out_b, out_s, out_h, position_b;
-  uint32_t items;        // tokens * slots * groups of this launch
-  int32_t slots, groups;  // head slots per token (head slot i takes heads i, i + slots, ...), groups per row
-  int32_t rotary_groups;  // the first ones of a row; the rest copy the other columns (not in place)
+  int64_t tokens, S, x_b, x_s, x_h, out_b, out_s, out_h, position_b;
+  int32_t block_tokens, block_heads, head_blocks;  // of a workgroup; workgroups per token block
+  int32_t groups;         // pieces of a row: the rotated ones, then (not in place) the other columns
+  int32_t rotary_groups;
+  uint32_t groups_m, heads_m;  // for divide(): by groups, by block_heads
   int32_t H, R, offset;
   int32_t wide_positions, inverse;
   float magnitude;
@@ -118,36 +124,48 @@ struct RotaryArgs {
 template <int DT, int VEC, int LAYOUT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   typedef typename B16<DT>::scalar scalar;
-  const uint32_t item = blockIdx.x * 256u + threadIdx.x;
-  if (item >= a.items) return;
-  const uint32_t row = item / (uint32_t)a.groups;
-  const int g = (int)(item - row * (uint32_t)a.groups);
-  const uint32_t local = row / (uint32_t)a.slots;
-  const int slot = (int)(row - local * (uint32_t)a.slots);
-  const int64_t token = a.first + local;
-  const int64_t b = a.S > token ? 0 : token / a.S, s = token - b * a.S;
-  const scalar* x = (const scalar*)a.x + b * a.x_b + s * a.x_s;
-  scalar* out = (scalar*)a.out + b * a.out_b + s * a.out_s;
-  if (g >= a.rotary_groups) {
-    int column = (g - a.rotary_groups) * VEC;
-    if (column >= a.offset) column += a.R;
-    for (int h = slot; h < a.H; h += a.slots)
-      store_piece<DT, VEC>(out + h * a.out_h + column, load_piece<DT, VEC>(x + h * a.x_h + column));
-    return;
+  __shared__ float2 angles[ROT_LDS_PAIRS];
+  const int pairs = a.R / 2;
+  const int64_t token0 = (int64_t)(blockIdx.x / (uint32_t)a.head_blocks) * a.block_tokens;
+  const int head0 = (int)(blockIdx.x % (uint32_t)a.head_blocks) * a.block_heads;
+  const int tokens = (int)min((int64_t)a.block_tokens, a.tokens - token0);
+  auto place = [&](int t, int64_t& b, int64_t& s) {
+    const int64_t token = token0 + t;
+    b = a.S > token ? 0 : token / a.S;
+    s = token - b * a.S;
+  };
+  for (int i = threadIdx.x; i < tokens * pairs; i += 256) {
+    const int t = i / pairs;
+    int64_t b, s;
+    place(t, b, s);
+    const int64_t at = b * a.position_b + s;
+    const int64_t position = a.wide_positions ? ((const int64_t*)a.positions)[at] : ((const int32_t*)a.positions)[at];
+    angles[i] = pair_angle(a.frequencies[i - t * pairs], position, a.magnitude, a.inverse != 0);
   }
-  const int64_t at = b * a.position_b + s;
-  const int64_t position = a.wide_positions ? ((const int64_t*)a.positions)[at] : ((const int32_t*)a.positions)[at];
-  float c[VEC], sn[VEC];
-  pair_angles<VEC>(a.frequencies, g * VEC, position, a.magnitude, a.inverse != 0, c, sn);
-  int lo, hi;
-  piece_columns<VEC, LAYOUT>(g, a.R, lo, hi);
-  lo += a.offset;
-  hi += a.offset;
-  for (int h = slot; h < a.H; h += a.slots) {
-    Piece<DT, VEC> u = load_piece<DT, VEC>(x + h * a.x_h + lo), v = load_piece<DT, VEC>(x + h * a.x_h + hi);
-    rotate_pieces<DT, VEC, LAYOUT>(u, v, c, sn);
-    store_piece<DT, VEC>(out + h * a.out_h + lo, u);
-    store_piece<DT, VEC>(out + h * a.out_h + hi, v);
+  __syncthreads();
+  const uint32_t items = (uint32_t)(tokens * a.block_heads * a.groups);
+  for (uint32_t item = threadIdx.x; item < items; item += 256) {
+    const uint32_t row = divide(item, a.groups_m), t = divide(row, a.heads_m);
+    const int g = (int)(item - row * (uint32_t)a.groups), h = head0 + (int)(row - t * (uint32_t)a.block_heads);
+    if (h >= a.H) continue;
+    int64_t b, s;
+    place((int)t, b, s);
+    const scalar* x = (const scalar*)a.x + b * a.x_b + s * a.x_s + h * a.x_h;
+    scalar* out = (scalar*)a.out + b * a.out_b + s * a.out_s + h * a.out_h;
+    if (g < a.rotary_groups) {
+      int lo, hi;
+      piece_columns<VEC, LAYOUT>(g, a.R, lo, hi);
+      lo += a.offset;
+      hi += a.offset;
+      Piece<DT, VEC> u = load_piece<DT, VEC>(x + lo), v = load_piece<DT, VEC>(x + hi);
+      rotate_pieces<DT, VEC, LAYOUT>(u, v, angles + (int)t * pairs + g * VEC);
+      store_piece<DT, VEC>(out + lo, u);
+      store_piece<DT, VEC>(out + hi, v);
+    } else {
+      int column = (g - a.rotary_groups) * VEC;
+      if (column >= a.offset) column += a.R;
+      store_piece<DT, VEC>(out + column, load_piece<DT, VEC>(x + column));
+    }
   }
 }
 
@@ -163,52 +181,71 @@ struct AppendArgs {
   const double* frequencies;
   int64_t k_t, k_h, rope_t, rope_h, v_t, v_h;
   int32_t T, B, W, PAGE, BLOCKS, HKV, DK, DV, R, offset;
-  int32_t rotary_groups, copy_groups, value_groups;  // per head
+  int32_t block_tokens;
+  int32_t rotary_groups, copy_groups, groups;  // pieces per head: rotated, other key columns, all (the values' last)
+  uint32_t groups_m, heads_m;                  // for divide(): by groups, by HKV
   float magnitude;
 };
 
-// One wave per new token. Its request is the number of boundaries cu[1..B] at
-// or below it (64 compared at a time), its position seqused - n + j; token rows
-// at or past cu[B], positions outside the table's width and pages outside the
-// cache write nothing.
+// A workgroup of four waves takes block_tokens new tokens. One wave finds a
+// token's place: its request is the number of boundaries cu[1..B] at or below
+// it (64 compared at a time), its position seqused - n + j; token rows at or past
+// cu[B], positions outside the table's width and pages outside the cache have none.
 template <int DT, int VEC, int LAYOUT>
 __global__ __launch_bounds__(256) void append_paged_kv_kernel(AppendArgs a) {
   typedef typename B16<DT>::scalar scalar;
+  __shared__ float2 angles[ROT_LDS_PAIRS];
+  __shared__ int64_t slots[ROT_TOKENS], positions[ROT_TOKENS];  // cache row, -1: none
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t token = (int64_t)blockIdx.x * 4 + wave;
-  if (token >= a.T) return;
-  int request = 0;
-  for (int first = 1; first <= a.B; first += 64) {
-    const int i = first + lane;
-    const int below = __popcll(__ballot(i <= a.B && a.cu[min(i, a.B)] <= token));
-    request += below;
-    if (below < 64) break;
+  const int64_t token0 = (int64_t)blockIdx.x * a.block_tokens;
+  const int tokens = (int)min((int64_t)a.block_tokens, (int64_t)a.T - token0);
+  const int pairs = a.R / 2;
+  auto find = [&](int64_t token, int64_t& position) -> int64_t {
+    int request = 0;
+    for (int first = 1; first <= a.B; first += 64) {
+      const int i = first + lane;
+      const int below = __popcll(__ballot(i <= a.B && a.cu[min(i, a.B)] <= token));
+      request += below;
+      if (below < 64) break;
+    }
+    position = -1;
+    if (request >= a.B) return -1;
+    position = (int64_t)a.used[request] - a.cu[request + 1] + token;
+    if (position < 0) return -1;
+    const int64_t page = position / a.PAGE;
+    if (page >= a.W) return -1;
+    const int block = a.table[(int64_t)request * a.W + page];
+    if (block < 0 || block >= a.BLOCKS) return -1;
+    return (int64_t)block * a.PAGE + (position - page * a.PAGE);
+  };
+  for (int t = wave; t < tokens; t += 4) {
+    int64_t position;
+    const int64_t slot = find(token0 + t, position);
+    if (lane == 0) {
+      slots[t] = slot;
+      positions[t] = position;
+    }
   }
-  if (request >= a.B) return;
-  const int end = a.cu[request + 1];
-  const int64_t position = (int64_t)a.used[request] - end + token;
-  if (position < 0) return;
-  const int64_t page = position / a.PAGE;
-  if (page >= a.W) return;
-  const int block = a.table[(int64_t)request * a.W + page];
-  if (block < 0 || block >= a.BLOCKS) return;
-  const int64_t slot = (int64_t)block * a.PAGE + (position - page * a.PAGE);
-
-  const int per_head = a.rotary_groups + a.copy_groups + a.value_groups;
-  const uint32_t items = (uint32_t)per_head * (uint32_t)a.HKV;
-  for (uint32_t item = lane; item < items; item += 64) {
-    const int h = (int)(item / (uint32_t)per_head);
-    const int g = (int)(item - (uint32_t)h * (uint32_t)per_head);
+  __syncthreads();
+  for (int i = threadIdx.x; i < tokens * pairs; i += 256) {
+    const int t = i / pairs;
+    angles[i] = pair_angle(a.frequencies[i - t * pairs], positions[t], a.magnitude, false);
+  }
+  __syncthreads();
+  const uint32_t items = (uint32_t)(tokens * a.HKV * a.groups);
+  for (uint32_t item = threadIdx.x; item < items; item += 256) {
+    const uint32_t head_row = divide(item, a.groups_m), t = divide(head_row, a.heads_m);
+    const int g = (int)(item - head_row * (uint32_t)a.groups), h = (int)(head_row - t * (uint32_t)a.HKV);
+    const int64_t slot = slots[t], token = token0 + t;
+    if (slot < 0) continue;
     const scalar* k = (const scalar*)a.k + token * a.k_t + h * a.k_h;
     scalar* row = (scalar*)a.k_cache + (slot * a.HKV + h) * a.DK;
     if (g < a.rotary_groups) {
-      float c[VEC], s[VEC];
-      pair_angles<VEC>(a.frequencies, g * VEC, position, a.magnitude, false, c, s);
       int lo, hi;
       piece_columns<VEC, LAYOUT>(g, a.R, lo, hi);
       const scalar* from = a.rope ? (const scalar*)a.rope + token * a.rope_t + h * a.rope_h : k + a.offset;
       Piece<DT, VEC> u = load_piece<DT, VEC>(from + lo), w = load_piece<DT, VEC>(from + hi);
-      rotate_pieces<DT, VEC, LAYOUT>(u, w, c, s);
+      rotate_pieces<DT, VEC, LAYOUT>(u, w, angles + (int)t * pairs + g * VEC);
       store_piece<DT, VEC>(row + a.offset + lo, u);
       store_piece<DT, VEC>(row + a.offset + hi, w);
     } else if (g < a.rotary_groups + a.copy_groups) {
@@ -232,28 +269,22 @@ bool pieces_fit(int R, int offset, int layout) {
   return offset % 8 == 0 && R % 16 == 0 && (layout == ROTARY_INTERLEAVED || (R / 2) % 8 == 0);
 }
 
+// Multiplier of divide() for n.
+uint32_t divider(int64_t n) { return n == 1 ? 0u : (uint32_t)(((1ull << 32) + n - 1) / n); }
+
 template <int DT, int VEC>
-int launch_rotary(RotaryArgs a, int layout, int64_t tokens, hipStream_t s) {
-  // Launches of at most 2^30 items: a token has at most H * (D / VEC) of them.
-  const int64_t per_token = (int64_t)a.slots * a.groups;
-  const int64_t most = std::max<int64_t>(1, (1ll << 30) / per_token);
-  for (int64_t first = 0; first < tokens; first += most) {
-    a.first = first;
-    a.items = (uint32_t)(std::min(most, tokens - first) * per_token);
-    const dim3 grid((a.items + 255u) / 256u), block(256);
-    if (layout == ROTARY_HALF)
-      hipLaunchKernelGGL((rotary_kernel<DT, VEC, ROTARY_HALF>), grid, block, 0, s, a);
-    else
-      hipLaunchKernelGGL((rotary_kernel<DT, VEC, ROTARY_INTERLEAVED>), grid, block, 0, s, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-  }
-  return AFA_OK;
+int launch_rotary(const RotaryArgs& a, int layout, int64_t blocks, hipStream_t s) {
+  const dim3 grid((unsigned)blocks), block(256);
+  if (layout == ROTARY_HALF)
+    hipLaunchKernelGGL((rotary_kernel<DT, VEC, ROTARY_HALF>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((rotary_kernel<DT, VEC, ROTARY_INTERLEAVED>), grid, block, 0, s, a);
+  return (int)hipGetLastError();
 }
 
 template <int DT, int VEC>
 int launch_append(const AppendArgs& a, int layout, hipStream_t s) {
-  const dim3 grid((unsigned)((a.T + 3) / 4)), block(256);
+  const dim3 grid((unsigned)(((int64_t)a.T + a.block_tokens - 1) / a.block_tokens)), block(256);
   if (layout == ROTARY_HALF)
     hipLaunchKernelGGL((append_paged_kv_kernel<DT, VEC, ROTARY_HALF>), grid, block, 0, s, a);
   else
@@ -269,7 +300,7 @@ extern "C" int launch_apply_rotary(void* stream, const void* x, const void* posi
   using namespace afa;
   if (!p || !x || !positions || !frequencies || !out) return AFA_E_NULL;
   if (p->dtype != AFA_DTYPE_BF16 && p->dtype != AFA_DTYPE_F16) return AFA_E_DTYPE;
-  if (p->B < 0 || p->S < 0 || p->H <= 0 || p->D <= 0 || p->H > (1 << 20) || p->D > (1 << 16)) return AFA_E_SHAPE;
+  if (p->B < 0 || p->S < 0 || p->H <= 0 || p->D <= 0 || p->D > ROT_MAX_D || p->R > 2 * ROT_MAX_PAIRS) return AFA_E_SHAPE;
   if (p->R < 2 || p->R % 2 || p->offset < 0 || p->offset > p->D - p->R) return AFA_E_SHAPE;
   if ((p->layout != ROTARY_HALF && p->layout != ROTARY_INTERLEAVED) || (p->position_bytes != 4 && p->position_bytes != 8))
     return AFA_E_SHAPE;
@@ -302,16 +333,26 @@ extern "C" int launch_apply_rotary(void* stream, const void* x, const void* posi
   a.wide_positions = p->position_bytes == 8;
   a.inverse = p->inverse ? 1 : 0;
   a.magnitude = p->magnitude;
-  // Heads per thread: as many share a thread's cosines as leave two waves per SIMD.
+  // Workgroups of a few tokens and all heads (at most 2^15 pieces, which
+  // divide() holds), of fewer heads, then of fewer tokens, until there are four
+  // per CU.
   const int64_t tokens = p->B * p->S;
-  int heads = 1;
-  while (heads < 8 && heads < p->H && tokens * ((p->H + 2 * heads - 1) / (2 * heads)) * a.groups >= 256ll * 512) heads *= 2;
-  a.slots = (p->H + heads - 1) / heads;
-  if ((int64_t)a.slots * a.groups > (1ll << 30)) return AFA_E_SHAPE;
+  int64_t block_tokens = std::min<int64_t>(ROT_TOKENS, ROT_LDS_PAIRS / (p->R / 2));
+  int64_t heads = std::min<int64_t>(p->H, std::max<int64_t>(1, (1 << 15) / (block_tokens * a.groups)));
+  auto count = [&] { return (tokens + block_tokens - 1) / block_tokens * ((p->H + heads - 1) / heads); };
+  while (heads > 1 && count() < 1024) heads = (heads + 1) / 2;
+  while (block_tokens > 1 && (count() < 1024 || block_tokens * heads * a.groups > (1 << 15))) block_tokens /= 2;
+  if (count() > 0x7fffffffll) return AFA_E_SHAPE;
+  a.tokens = tokens;
+  a.block_tokens = (int32_t)block_tokens;
+  a.block_heads = (int32_t)heads;
+  a.head_blocks = (int32_t)((p->H + heads - 1) / heads);
+  a.groups_m = divider(a.groups);
+  a.heads_m = divider(heads);
   hipStream_t s = (hipStream_t)stream;
   if (p->dtype == AFA_DTYPE_F16)
-    return wide ? launch_rotary<DT_F16, 8>(a, p->layout, tokens, s) : launch_rotary<DT_F16, 1>(a, p->layout, tokens, s);
-  return wide ? launch_rotary<DT_BF16, 8>(a, p->layout, tokens, s) : launch_rotary<DT_BF16, 1>(a, p->layout, tokens, s);
+    return wide ? launch_rotary<DT_F16, 8>(a, p->layout, count(), s) : launch_rotary<DT_F16, 1>(a, p->layout, count(), s);
+  return wide ? launch_rotary<DT_BF16, 8>(a, p->layout, count(), s) : launch_rotary<DT_BF16, 1>(a, p->layout, count(), s);
 }
 
 extern "C" int launch_append_paged_kv(void* stream, const void* k, const void* rope, const void* v,
@@ -323,7 +364,7 @@ extern "C" int launch_append_paged_kv(void* stream, const void* k, const void* r
   if (p->dtype != AFA_DTYPE_BF16 && p->dtype != AFA_DTYPE_F16) return AFA_E_DTYPE;
   if (p->T < 0 || p->B <= 0 || p->W <= 0 || p->PAGE <= 0 || p->BLOCKS <= 0 || p->HKV <= 0 || p->DK <= 0 || p->DV < 0)
     return AFA_E_SHAPE;
-  if (p->HKV > (1 << 16) || p->DK > (1 << 14) || p->DV > (1 << 14)) return AFA_E_SHAPE;
+  if (p->DK > ROT_MAX_D || p->DV > ROT_MAX_D || p->R > 2 * ROT_MAX_PAIRS) return AFA_E_SHAPE;
   if (p->R < 0 || p->R % 2 || p->offset < 0 || p->R > p->DK || p->offset > p->DK - p->R) return AFA_E_SHAPE;
   if (p->layout != ROTARY_HALF && p->layout != ROTARY_INTERLEAVED) return AFA_E_SHAPE;
   if (rope && (p->R == 0 || p->offset != p->DK - p->R)) return AFA_E_SHAPE;
@@ -364,7 +405,16 @@ extern "C" int launch_append_paged_kv(void* stream, const void* k, const void* r
   a.offset = p->offset;
   a.rotary_groups = R / 2 / vec;
   a.copy_groups = (p->DK - R) / vec;
-  a.value_groups = p->DV / vec;
+  a.groups = a.rotary_groups + a.copy_groups + p->DV / vec;
+  // divide() needs the items of a workgroup times groups and heads below 2^32.
+  const int64_t items = (int64_t)p->HKV * a.groups;
+  if (items * std::max<int64_t>(a.groups, p->HKV) > 0x1fffffffll) return AFA_E_SHAPE;
+  // One token a workgroup up to four workgroups per CU, then up to eight.
+  int64_t block_tokens = R ? std::min<int64_t>(ROT_TOKENS, ROT_LDS_PAIRS / (R / 2)) : ROT_TOKENS;
+  while (block_tokens > 1 && p->T / block_tokens < 1024) block_tokens /= 2;
+  a.block_tokens = (int32_t)block_tokens;
+  a.groups_m = divider(a.groups);
+  a.heads_m = divider(p->HKV);
   a.magnitude = p->magnitude;
   hipStream_t s = (hipStream_t)stream;
   if (p->dtype == AFA_DTYPE_F16)

@@ -70,6 +70,7 @@ def _check(lib, k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, 
     check_tensor("seqused_kv", seqused_kv, (B,), i32, device)
     if frequencies is not None:
         check_tensor("frequencies", frequencies, (R // 2,), torch.float64, device)
+    require(R <= 1024 and DK <= 16384 and DV <= 16384, "at most 1024 rotated and 16384 columns")
     require(layout in LAYOUTS, 'layout must be "half" or "interleaved"')
     require(R == 0 or 0 <= offset <= DK - R, f"the rotated columns {offset} to {offset + R} must lie inside the row ({DK})")
     require(math.isfinite(magnitude), "magnitude must be finite")

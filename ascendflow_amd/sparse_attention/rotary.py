@@ -80,7 +80,7 @@ def _check(lib, x, positions, frequencies, out, layout, offset, magnitude, inver
         (S, H, D), B = x.shape, 1
     else:
         B, H, S, D = x.shape
-    require(H > 0 and D > 0, "x must have heads and columns")
+    require(H > 0 and 0 < D <= 16384, "x must have heads, and at most 16384 columns")
     require(positions.dtype in (torch.int32, torch.int64), "positions must be an int32 or int64 tensor")
     require(tuple(positions.shape) == (S,) or (x.dim() == 4 and tuple(positions.shape) == (B, S)),
             f"positions shape {tuple(positions.shape)} does not fit x {tuple(x.shape)}")
@@ -92,6 +92,7 @@ def _check(lib, x, positions, frequencies, out, layout, offset, magnitude, inver
     check_rows("frequencies", frequencies, frequencies.shape, torch.float64, device)
     check_distinct_rows("out", out)
     R = 2 * frequencies.numel()
+    require(R <= 1024, "at most 1024 columns can be rotated")
     require(layout in LAYOUTS, 'layout must be "half" or "interleaved"')
     require(0 <= offset <= D - R, f"the rotated columns {offset} to {offset + R} must lie inside the head ({D})")
     require(math.isfinite(magnitude), "magnitude must be finite")

@@ -311,7 +311,8 @@ int form_sparse_topk_indices(int64_t form[3], const SparseTopkParams* params, in
  * with strides in elements, columns contiguous; the other columns are copied,
  * or, where out is x (equal strides), not touched. positions int32 or int64
  * (position_bytes 4 or 8) [S], position_stride_b elements apart for each b.
- * 16-byte accesses where R % 16, offset, D and the strides allow them. */
+ * R up to 1024, D up to 16384. 16-byte accesses where R % 16, offset, D and the
+ * strides allow them. */
 typedef struct RotaryParams {
   int32_t dtype;
   int32_t layout;          /* 0 halves, 1 interleaved */
@@ -340,7 +341,7 @@ int launch_apply_rotary(void* stream, const void* x, const void* positions, cons
  * [BLOCKS][PAGE][HKV][DV] (DV = 0: none). Strides in elements, columns
  * contiguous. Tokens at or past cu_seqlens_q[B], positions below 0 or beyond W
  * pages, and pages outside [0, BLOCKS) write nothing. No two new tokens may
- * name the same cache row. */
+ * name the same cache row. R up to 1024, DK and DV up to 16384. */
 typedef struct AppendPagedKvParams {
   int32_t dtype;
   int32_t layout;
