@@ -54,6 +54,8 @@ EXPORTS = (
     "workspace_size_latent_attention",
     "form_latent_attention",
     "launch_latent_attention_expanded",
+    "workspace_size_latent_attention_expanded",
+    "form_latent_attention_expanded",
     "launch_cache_flush",
     "launch_clock_probe",
     "ascendflow_amd_version",
@@ -185,7 +187,9 @@ _SIGNATURES = {
     "launch_latent_attention": ([_P] * 10 + [ct.c_uint64, ct.POINTER(LatentParams)], ct.c_int),
     "workspace_size_latent_attention": ([ct.POINTER(ct.c_uint64), ct.POINTER(LatentParams)], ct.c_int),
     "form_latent_attention": ([ct.POINTER(ct.c_int64), ct.POINTER(LatentParams)], ct.c_int),
-    "launch_latent_attention_expanded": ([_P] * 9 + [ct.POINTER(LatentExpandedParams)], ct.c_int),
+    "launch_latent_attention_expanded": ([_P] * 10 + [ct.c_uint64, ct.POINTER(LatentExpandedParams)], ct.c_int),
+    "workspace_size_latent_attention_expanded": ([ct.POINTER(ct.c_uint64), ct.POINTER(LatentExpandedParams)], ct.c_int),
+    "form_latent_attention_expanded": ([ct.POINTER(ct.c_int64), ct.POINTER(LatentExpandedParams)], ct.c_int),
     "launch_cache_flush": ([_P, _P, ct.c_uint64], ct.c_int),
     "launch_clock_probe": ([_P, _P, ct.c_int32], ct.c_int),
     "ascendflow_amd_version": ([], ct.c_char_p),

@@ -22,6 +22,7 @@
 // weights that were applied add up to one; the log-sum-exp takes the sum before
 // rounding.
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 #include "../../include/ascendflow_amd.h"
@@ -30,6 +31,7 @@ namespace afa {
 
 constexpr float LAT_LOG2E = 1.4426950408889634f, LAT_LN2 = 0.6931471805599453f;
 constexpr float LAT_TAU = 8.0f;
+constexpr int EXP_MAX_SPLITS = 64;
 // Cache rows per chunk. Eight waves (one workgroup per CU): 64, two slots; a
 // barrier, a fetch and a reduction per 64 rows instead of 32 and four chains of
 // dependent matrix instructions instead of two (128 heads, 4 chunks of 512 tokens
@@ -92,9 +94,9 @@ __device__ __forceinline__ void request_tokens(const_ints cu, int b, int T, int&
 // (tiles_of(tokens) each); false, for the whole workgroup, if there are fewer.
 template <int THREADS, typename F>
 __device__ __forceinline__ bool find_tile(const_ints cu, int B, int T, uint32_t index, F&& tiles_of, int& request,
-                                          uint32_t& tile, uint32_t& tiles) {
-  __shared__ uint32_t wave_total[THREADS / 64];
-  __shared__ uint32_t found[3];
+                                          uint32_t& tile, uint32_t& tiles, uint32_t* words) {
+  uint32_t* const wave_total = words;                // LDS, THREADS / 64 + 3 words
+  uint32_t* const found = words + THREADS / 64;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   uint32_t before = 0;
   for (int base = 0; base < B; base += THREADS) {
@@ -278,8 +280,10 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     left = share.end - share.begin;
   } else {
     if (!find_tile<NW * 64>(constant(a.cu), a.B, a.T, worker,
-                            [&](int n) { return ((uint32_t)n * (uint32_t)H + ROWS - 1) / ROWS; }, request, tile, tiles))
+                            [&](int n) { return ((uint32_t)n * (uint32_t)H + ROWS - 1) / ROWS; }, request, tile, tiles,
+                            (uint32_t*)ring[0]))
       return;
+    __syncthreads();  // the words are read before loads land on them
     if (a.causal) tile = tiles - 1 - tile;  // the longest first
   }
   uint32_t offset = SPLIT ? share.offset : 0;
@@ -657,11 +661,15 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(LatentArgs a, int til
 // 2 (128 + 64 + 128) flops a pair instead of the absorbed 2 (2 L + 64), for keys
 // and values that the caller expands once per prompt. The two parts of a key are
 // read from where they lie, so no concatenated, per-head copy of k_rope is made.
-// One workgroup per (request, head, 256 query rows): 8 waves of two 16-row tiles
-// with Q resident; 64-key chunks of k_nope, k_rope and v stream through a
-// three-slot LDS ring two chunks ahead. QK of chunk c + 1 is issued ahead of the
-// softmax of chunk c, whose exponentials run in the shadow of the matrix
-// instructions of QK (c + 1) and PV (c).
+// One workgroup of NW waves per (request, head, NW * QT * 16 query rows), QT
+// 16-row tiles a wave with Q resident; 64-key chunks of k_nope, k_rope and v
+// stream through an LDS ring: three slots each, two chunks ahead, for NW = 8; two
+// for NW = 4, keys two chunks ahead and values one, so that two workgroups fit a
+// CU (128- or 64-row tiles: less of short, ragged or few prompts is padding or an
+// idle CU, more loads per row). QK of chunk c + 1 is issued ahead of the softmax of
+// chunk c, whose exponentials run in the shadow of the matrix instructions of QK
+// (c + 1) and PV (c). Where even small tiles leave CUs idle, `splits` workgroups
+// share a tile's keys and expanded_merge_kernel joins their float32 parts in order.
 struct ExpandedArgs {
   const void* q;
   const void* k;
@@ -673,30 +681,41 @@ struct ExpandedArgs {
   float* lse;  // [Tq][H] or NULL
   int64_t q_t, q_h, k_t, k_h, kr_t, v_t, v_h, o_t, o_h;
   int32_t Tq, Tk, B, H, causal;
+  int32_t splits;
   float scale;
+  float* partial_o;   // [splits][Tq * H][128], not normalised
+  float* partial_ml;  // [splits][Tq * H][4]: running maximum (log2), sum, sum of rounded weights
 };
 
-template <int DT>
-__global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
+template <int DT, int NW, int QT, bool SPLIT>
+__global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(ExpandedArgs a) {
   typedef typename B16<DT>::scalar scalar;
   typedef typename B16<DT>::x8 x8;
   typedef typename B16<DT>::x4 x4;
-  constexpr int NW = 8, QT = 2, BQ = NW * QT * 16, KC = 64, KT = KC / 16, NS = 3;
+  constexpr int BQ = NW * QT * 16, KC = 64, KT = KC / 16, NS = NW == 8 ? 3 : 2;
   constexpr int D = 128, R = 64, ROW_BYTES = 2 * D, ROPE_BYTES = 2 * R;
-  constexpr int ROPE_AT = KC * ROW_BYTES, V_AT = ROPE_AT + KC * ROPE_BYTES, SLOT = V_AT + KC * ROW_BYTES;
+  constexpr int ROPE_AT = KC * ROW_BYTES, K_TILE = ROPE_AT + KC * ROPE_BYTES, V_TILE = KC * ROW_BYTES;
   constexpr int KSTEPS = D / 32, STEPS = KSTEPS + R / 32;
-  constexpr int LOADS = 5;  // wave loads per chunk: two of k_nope, two of v (4 rows each), one of k_rope (8 rows)
-  __shared__ __attribute__((aligned(256))) uint8_t ring[NS][SLOT];
+  // Wave loads per chunk: k_nope and v (4 rows each), k_rope (8 rows).
+  constexpr int LOADS = KC / 4 / NW, ROPE_LOADS = KC / 8 / NW;
+  // The whole 160 KiB for two workgroups of NW = 4: find_tile's few words lie in it too.
+  __shared__ __attribute__((aligned(256))) uint8_t ring[NS * (K_TILE + V_TILE)];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int g = lane >> 4, i16 = lane & 15;
+  // Heads first: consecutive workgroups go to different XCDs, and a head's tiles
+  // to the same one where H is a multiple of 8, which then shares its L2.
   const int head = (int)(blockIdx.x % (uint32_t)a.H);
+  uint32_t index = blockIdx.x / (uint32_t)a.H;
+  const int split = SPLIT ? (int)(index % (uint32_t)a.splits) : 0;
+  if (SPLIT) index /= (uint32_t)a.splits;
   int request;
   uint32_t tile, tiles;
-  if (!find_tile<512>(constant(a.cu_q), a.B, a.Tq, blockIdx.x / (uint32_t)a.H,
-                      [&](int n) { return ((uint32_t)n + BQ - 1) / BQ; }, request, tile, tiles))
+  if (!find_tile<NW * 64>(constant(a.cu_q), a.B, a.Tq, index,
+                          [&](int n) { return ((uint32_t)n + BQ - 1) / BQ; }, request, tile, tiles, (uint32_t*)ring))
     return;
+  __syncthreads();             // the words are read before loads land on them
   if (a.causal) tile = tiles - 1 - tile;  // the longest first
   int q_start, nq, k_start, nk;
   request_tokens(constant(a.cu_q), request, a.Tq, q_start, nq);
@@ -710,12 +729,11 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
 
   // Query i sees keys [0, nk - nq + i + 1) (causal, aligned at the end) or all.
   auto visible = [&](int i) { return a.causal ? min(max(nk - nq + i + 1, 0), nk) : nk; };
-  int limit[QT];
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt) limit[qt] = visible(min(q0 + (wave * QT + qt) * 16 + i16, nq - 1));
   const int kv_end = visible(min(q0 + BQ, nq) - 1);
   const int clean_end = visible(q0);
-  const int chunks = (kv_end + KC - 1) / KC, clean_chunks = clean_end / KC;
+  const int all_chunks = (kv_end + KC - 1) / KC, clean_chunks = clean_end / KC;
+  const int begin = SPLIT ? (int)((int64_t)all_chunks * split / a.splits) : 0;
+  const int chunks = SPLIT ? (int)((int64_t)all_chunks * (split + 1) / a.splits) : all_chunks;
 
   x8 qf[QT][STEPS];
 #pragma unroll
@@ -726,38 +744,47 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
       qf[qt][j] = row < nq ? *(const x8*)(Q + row * a.q_t + 32 * j + 8 * g) : __builtin_bit_cast(x8, u32x4{0u, 0u, 0u, 0u});
   }
 
-  const uint32_t ring_base = lds_address(ring[0]);
-  auto slot_of = [&](int chunk) { return opaque_uniform(ring_base + (uint32_t)(chunk % NS) * SLOT); };
-  // Rows past the last key read the last key instead (masked later). 32-bit row
-  // offsets: the host holds 64 rows of any stride below 2^31 bytes.
-  const uint32_t k_row = (uint32_t)(2 * a.k_t), v_row = (uint32_t)(2 * a.v_t), r_row = (uint32_t)(2 * a.kr_t);
-  auto fetch = [&](int chunk) {
-    const int key0 = chunk * KC;
-    const char* kbase = K + (int64_t)key0 * (2 * a.k_t);
-    const char* vbase = V + (int64_t)key0 * (2 * a.v_t);
-    const char* rbase = KR + (int64_t)key0 * (2 * a.kr_t);
-    const int last = nk - 1 - key0;
-    const uint32_t slot = slot_of(chunk);
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int r = (wave * 2 + p) * 4 + (lane >> 4);
-      const uint32_t rr = (uint32_t)min(r, last), unit = (uint32_t)(((lane & 15) ^ (r & 15)) << 4);
-      const uint32_t to = slot + (uint32_t)((wave * 2 + p) * 4 * ROW_BYTES);
-      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                       :: "s"(to), "v"(rr * k_row + unit), "s"(kbase) : "memory");
-      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                       :: "s"(to + (uint32_t)V_AT), "v"(rr * v_row + unit), "s"(vbase) : "memory");
-    }
-    const int r = wave * 8 + (lane >> 3);
-    const uint32_t off = (uint32_t)min(r, last) * r_row + (uint32_t)(((lane & 7) ^ ((r >> 1) & 7)) << 4);
-    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                     :: "s"(slot + (uint32_t)(ROPE_AT + wave * 8 * ROPE_BYTES)), "v"(off), "s"(rbase) : "memory");
+  const uint32_t ring_base = lds_address(ring);
+  auto k_slot = [&](int chunk) { return opaque_uniform(ring_base + (uint32_t)(chunk % NS) * K_TILE); };
+  auto v_slot = [&](int chunk) { return opaque_uniform(ring_base + (uint32_t)(NS * K_TILE) + (uint32_t)(chunk % NS) * V_TILE); };
+  auto load = [](uint32_t to, uint32_t off, const char* from) {
+    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(off), "s"(from) : "memory");
   };
+  // Rows of 128 columns: load p of this wave lands on rows 4 (wave * LOADS + p) ..
+  // + 3, unit u of row r at u ^ (r & 15). Rows past the last key read the last key instead
+  // (masked later). 32-bit row offsets: the host holds 64 rows below 2^31 bytes.
+  const uint32_t k_row = (uint32_t)(2 * a.k_t), v_row = (uint32_t)(2 * a.v_t), r_row = (uint32_t)(2 * a.kr_t);
+  auto fetch_rows = [&](uint32_t slot, const char* rows, uint32_t row_bytes, int key0) {
+    const char* base = rows + (int64_t)key0 * row_bytes;
+    const int last = nk - 1 - key0;
+    const uint32_t ln = opaque((uint32_t)tid) & 63u;
+#pragma unroll
+    for (int p = 0; p < LOADS; ++p) {
+      const int r = (wave * LOADS + p) * 4 + (int)(ln >> 4);
+      load(slot + (uint32_t)((wave * LOADS + p) * 4 * ROW_BYTES),
+           (uint32_t)min(r, last) * row_bytes + (((ln & 15u) ^ (uint32_t)(r & 15)) << 4), base);
+    }
+  };
+  auto fetch_k = [&](int chunk) {
+    const int key0 = chunk * KC;
+    const uint32_t slot = k_slot(chunk);
+    fetch_rows(slot, K, k_row, key0);
+    const char* base = KR + (int64_t)key0 * r_row;
+    const int last = nk - 1 - key0;
+    const uint32_t ln = opaque((uint32_t)tid) & 63u;
+#pragma unroll
+    for (int p = 0; p < ROPE_LOADS; ++p) {
+      const int r = (wave * ROPE_LOADS + p) * 8 + (int)(ln >> 3);
+      load(slot + (uint32_t)(ROPE_AT + (wave * ROPE_LOADS + p) * 8 * ROPE_BYTES),
+           (uint32_t)min(r, last) * r_row + (((ln & 7u) ^ (uint32_t)((r >> 1) & 7)) << 4), base);
+    }
+  };
+  auto fetch_v = [&](int chunk) { fetch_rows(v_slot(chunk), V, v_row, chunk * KC); };
 
   const int ra = sigma(i16), rt = sigma(4 * g + (i16 >> 2));
   const uint32_t qk_at = (uint32_t)(ra * ROW_BYTES + ((g ^ (ra & 15)) << 4));
   const uint32_t qr_at = (uint32_t)(ROPE_AT + ra * ROPE_BYTES + ((g ^ ((ra >> 1) & 7)) << 4));
-  const uint32_t tr_at = (uint32_t)(V_AT + rt * ROW_BYTES + ((((i16 & 3) >> 1) ^ (rt & 15)) << 4) + (i16 & 1) * 8);
+  const uint32_t tr_at = (uint32_t)(rt * ROW_BYTES + ((((i16 & 3) >> 1) ^ (rt & 15)) << 4) + (i16 & 1) * 8);
 
   f32x4 o[QT][D / 16];
   float m_run[QT], l_run[QT], l_rounded[QT];
@@ -770,9 +797,9 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
   }
   const float scale_log2 = a.scale * LAT_LOG2E;
 
-  constexpr int QK_FRAGS = STEPS * KT, LOOK = 6;
+  constexpr int QK_FRAGS = STEPS * KT, LOOK = 5;
   auto qk_chunk = [&](int chunk, f32x4 (&s)[KT][QT], auto&& between) {
-    const uint32_t slot = slot_of(chunk);
+    const uint32_t slot = k_slot(chunk);
     const uint32_t base = opaque(slot + qk_at), rope = opaque(slot + qr_at);
     x8 kf[QK_FRAGS];
     auto load = [&](int f) {  // (step j, key tile t)
@@ -797,7 +824,7 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
   };
   constexpr int PV_FRAGS = (KC / 32) * (D / 16);
   auto pv_chunk = [&](int chunk, x8 (&pf)[QT][KC / 32], auto&& between) {
-    const uint32_t base = opaque(slot_of(chunk) + tr_at);
+    const uint32_t base = opaque(v_slot(chunk) + tr_at);
     constexpr int VLOOK = 3;
     x4 lo[PV_FRAGS], hi[PV_FRAGS];
     auto load = [&](int f) {  // (32 keys ks, column tile t)
@@ -822,7 +849,8 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
   auto mask = [&](int chunk, f32x4 (&s)[KT][QT]) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      const int lim = limit[qt] - chunk * KC;
+      const int row = q0 + (wave * QT + qt) * 16 + (int)(opaque((uint32_t)tid) & 15u);
+      const int lim = visible(min(row, nq - 1)) - chunk * KC;
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -832,22 +860,26 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
 
   constexpr int HALF = QT * 8, QK_EXP0 = QT + 2, PV_EXP_STEPS = PV_FRAGS / 2 - 1;
   f32x4 s_a[KT][QT], s_b[KT][QT];
-  if (chunks > 0) {
-    fetch(0);
-    if (chunks > 1) {
-      fetch(1);
-      wait_vmcnt<LOADS>();
+  if (begin < chunks) {
+    fetch_k(begin);
+    fetch_v(begin);
+    if (begin + 1 < chunks) {
+      fetch_k(begin + 1);
+      if constexpr (NS == 3) fetch_v(begin + 1);
+      wait_vmcnt<LOADS + ROPE_LOADS + (NS == 3 ? LOADS : 0)>();
     } else {
       wait_vmcnt<0>();
     }
     block_barrier();
-    qk_chunk(0, s_a, [](int) {});
+    qk_chunk(begin, s_a, [](int) {});
   }
   auto iteration = [&](int c, f32x4 (&cur)[KT][QT], f32x4 (&nxt)[KT][QT]) {
-    // Chunk c + 1 has landed, and every wave is past QK (c) and PV (c - 1).
+    // Keys of chunk c + 1 and values of c have landed, and every wave is past QK (c)
+    // and PV (c - 1), whose slots are free.
     wait_vmcnt<0>();
     block_barrier();
-    if (c + 2 < chunks) fetch(c + 2);
+    if (c + 2 < chunks) fetch_k(c + 2);
+    if (c + NS - 1 < chunks) fetch_v(c + NS - 1);
     if (c >= clean_chunks) mask(c, cur);
     x8 pf[QT][KC / 32];
     float top[QT], m_new[QT], psum[QT], rsum[QT];
@@ -917,7 +949,7 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
     __builtin_amdgcn_s_setprio(1);
     pv_chunk(c, pf, pv_between);
   };
-  for (int c = 0; c < chunks; c += 2) {
+  for (int c = begin; c < chunks; c += 2) {
     iteration(c, s_a, s_b);
     if (c + 1 < chunks) iteration(c + 1, s_b, s_a);
   }
@@ -926,8 +958,14 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
   for (int qt = 0; qt < QT; ++qt) {
     const int row = q0 + (wave * QT + qt) * 16 + i16;
     const float total = sum_over_lane_groups(l_run[qt]), applied = sum_over_lane_groups(l_rounded[qt]);
-    const float inv = applied > 0.f ? 1.0f / applied : 0.f;
-    if (row < nq) {
+    if (row >= nq) continue;
+    if constexpr (SPLIT) {
+      const int64_t at = ((int64_t)split * a.Tq + q_start + row) * a.H + head;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) *(f32x4*)(a.partial_o + at * D + 16 * t + 4 * g) = o[qt][t];
+      if (g == 0) *(f32x4*)(a.partial_ml + at * 4) = f32x4{m_run[qt], total, applied, 0.f};
+    } else {
+      const float inv = applied > 0.f ? 1.0f / applied : 0.f;
       scalar* out = (scalar*)a.out + (int64_t)(q_start + row) * a.o_t + (int64_t)head * a.o_h + 4 * g;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
@@ -940,6 +978,45 @@ __global__ __launch_bounds__(512, 1) void expanded_kernel(ExpandedArgs a) {
         a.lse[(int64_t)(q_start + row) * a.H + head] = total > 0.f ? (m_run[qt] + __log2f(total)) * LAT_LN2 : -INFINITY;
     }
   }
+}
+
+// Joins the parts of split keys, in order: half a wave per (query, head) row, four
+// columns a lane, four parts of loads in flight.
+template <int DT>
+__global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedArgs a) {
+  typedef typename B16<DT>::scalar scalar;
+  typedef typename B16<DT>::x4 x4;
+  constexpr int AHEAD = 4;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (int64_t)a.Tq * a.H;
+  const int column = 4 * (threadIdx.x & 31);
+  const int end = min(max(constant(a.cu_q)[a.B], 0), a.Tq);  // rows of no request stay as they are
+  if (row >= rows || row / a.H >= end || row / a.H < constant(a.cu_q)[0]) return;
+  float top = -1e30f;
+  for (int p = 0; p < a.splits; ++p) top = fmaxf(top, a.partial_ml[(p * rows + row) * 4]);
+  float total = 0.f, applied = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < a.splits; p += AHEAD) {
+    f32x4 ml[AHEAD], v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int64_t at = min(p + i, a.splits - 1) * rows + row;
+      ml[i] = *(const f32x4*)(a.partial_ml + at * 4);
+      v[i] = *(const f32x4*)(a.partial_o + at * 128 + column);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const float weight = p + i < a.splits ? fast_exp2(ml[i][0] - top) : 0.f;
+      total += weight * ml[i][1];
+      applied += weight * ml[i][2];
+      o += weight * v[i];
+    }
+  }
+  const float inv = applied > 0.f ? 1.0f / applied : 0.f;
+  x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[i] * inv);
+  *(x4*)((scalar*)a.out + row / a.H * a.o_t + row % a.H * a.o_h + column) = v;
+  if (a.lse && column == 0) a.lse[row] = total > 0.f ? (top + __log2f(total)) * LAT_LN2 : -INFINITY;
 }
 
 namespace {
@@ -1104,15 +1181,97 @@ extern "C" int form_latent_attention(int64_t form[2], const LatentParams* p) {
   return AFA_OK;
 }
 
-extern "C" int launch_latent_attention_expanded(void* stream, const void* q, const void* k_nope, const void* k_rope,
-                                                const void* v, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                                                void* out, float* softmax_lse, const LatentExpandedParams* p) {
-  using namespace afa;
-  if (!p || !q || !cu_seqlens_q || !cu_seqlens_k || !out) return AFA_E_NULL;
+namespace afa {
+namespace {
+
+// Form of an expanded call: rows of a tile (256, 128 or 64) and key splits.
+struct ExpandedPlan {
+  int rows;
+  int splits;
+};
+
+int check_expanded(const LatentExpandedParams* p) {
+  if (!p) return AFA_E_NULL;
   if (p->dtype != AFA_DTYPE_BF16 && p->dtype != AFA_DTYPE_F16) return AFA_E_DTYPE;
   if (p->Tq < 0 || p->Tk < 0 || p->B <= 0 || p->H <= 0 || p->Tq > 0x7fffff00 || p->Tk > 0x7fffff00) return AFA_E_SHAPE;
   if (p->D != 128 || p->R != 64 || !(p->scale > 0.0f)) return AFA_E_SHAPE;
-  if (p->Tk > 0 && (!k_nope || !k_rope || !v)) return AFA_E_NULL;
+  if (((int64_t)p->Tq / 64 + p->B) * p->H > 0x7fffffffll / EXP_MAX_SPLITS) return AFA_E_SHAPE;
+  return AFA_OK;
+}
+
+// The form that a cost model finds cheapest (us), fixed at 256 CUs, with mean
+// request lengths (the launcher reads no device memory). A tile's 64-key chunk
+// costs ALONE where it has its CU to itself and FULL with the CU's workgroups at
+// work (one of 256 rows, two of 128 or 64); a round of workgroups START. Measured
+// at 256 / 128 / 64 rows: 1 x 8192 causal, 32 heads 726 / 741 / 921 us; 1 x 1500,
+// 128 heads 160 / 144 / 181; 5 x 235..470 behind up to 2000, 16 heads 79 / 69 / 56;
+// 1 x 2048, 16 heads 83 / 64 / 55. Split keys add a launch and their float32 parts
+// written and read at 3 TB/s: 64 rows in 1 / 2 / 4 / 8 parts, 8 x 20 behind 3000, 8 heads
+// 60 / 38 / 28 / 30; 1 x 500 behind 4000, 32 heads 90 / 68 / 76 / 98.
+ExpandedPlan plan_expanded(const LatentExpandedParams* p) {
+  constexpr int FORMS = 3, ROWS[FORMS] = {256, 128, 64}, SLOTS[FORMS] = {256, 512, 512};
+  constexpr double ALONE[FORMS] = {2.0, 1.5, 1.2}, FULL[FORMS] = {2.75, 3.0, 1.65}, START[FORMS] = {12.0, 9.0, 7.5};
+  constexpr double MERGE = 5.0, MERGE_RATE = 3e6;  // us, bytes a us
+  const int64_t nq = std::max<int64_t>(1, (p->Tq + p->B - 1) / p->B), nk = std::max<int64_t>(1, (p->Tk + p->B - 1) / p->B);
+  const double chunks = std::ceil(nk / 64.0);
+  // Mean keys of a query over those of the last.
+  const double mean = p->causal && nk > 1 ? 1.0 - 0.5 * std::min(1.0, (double)(nq - 1) / nk) : 1.0;
+  auto cost = [&](int form, int splits) {
+    const double blocks = (double)((nq + ROWS[form] - 1) / ROWS[form]) * p->B * p->H * splits;
+    const double rounds = blocks / SLOTS[form], each = std::ceil(chunks / splits);
+    const double full = (p->causal ? rounds : std::ceil(rounds)) * mean * each * FULL[form] *
+                        std::min(1.0, std::max(rounds, 256.0 / SLOTS[form]));
+    return START[form] * (0.5 + 0.5 * std::ceil(rounds)) + std::max(each * ALONE[form], full) +
+           (splits > 1 ? MERGE + (double)splits * p->Tq * p->H * (2 * 132 * 4) / MERGE_RATE : 0.0);
+  };
+  ExpandedPlan plan{ROWS[0], 1};
+  double best = cost(0, 1);
+  for (int form = 1; form < FORMS; ++form)
+    if (cost(form, 1) < best) {
+      best = cost(form, 1);
+      plan.rows = ROWS[form];
+    }
+  const int64_t most = std::min<int64_t>(EXP_MAX_SPLITS, (int64_t)chunks / 4);  // at least 256 keys each
+  for (int splits = 2; splits <= most; ++splits)
+    if (cost(2, splits) < best) {
+      best = cost(2, splits);
+      plan = ExpandedPlan{64, splits};
+    }
+  return plan;
+}
+
+uint64_t expanded_bytes(const LatentExpandedParams* p, const ExpandedPlan& plan) {
+  return plan.splits > 1 ? (uint64_t)plan.splits * p->Tq * p->H * (128 + 4) * 4 : 0;
+}
+
+template <int DT>
+int launch_expanded(const ExpandedArgs& a, const ExpandedPlan& plan, hipStream_t s) {
+  const dim3 grid((unsigned)(((int64_t)a.Tq / plan.rows + a.B) * a.H * plan.splits));
+  if (plan.splits > 1)
+    hipLaunchKernelGGL((expanded_kernel<DT, 4, 1, true>), grid, dim3(256), 0, s, a);
+  else if (plan.rows == 256)
+    hipLaunchKernelGGL((expanded_kernel<DT, 8, 2, false>), grid, dim3(512), 0, s, a);
+  else if (plan.rows == 128)
+    hipLaunchKernelGGL((expanded_kernel<DT, 4, 2, false>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((expanded_kernel<DT, 4, 1, false>), grid, dim3(256), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || plan.splits == 1) return (int)e;
+  hipLaunchKernelGGL(expanded_merge_kernel<DT>, dim3((unsigned)(((int64_t)a.Tq * a.H + 7) / 8)), dim3(256), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+}  // namespace afa
+
+extern "C" int launch_latent_attention_expanded(void* stream, const void* q, const void* k_nope, const void* k_rope,
+                                                const void* v, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                                void* out, float* softmax_lse, void* workspace, uint64_t workspace_bytes,
+                                                const LatentExpandedParams* p) {
+  using namespace afa;
+  const int status = check_expanded(p);
+  if (status) return status;
+  if (!q || !cu_seqlens_q || !cu_seqlens_k || !out || (p->Tk > 0 && (!k_nope || !k_rope || !v))) return AFA_E_NULL;
   if (!rows_fit(q, p->q_stride_t, p->q_stride_h) || !rows_fit(out, p->out_stride_t, p->out_stride_h) ||
       !rows_fit(k_nope, p->k_stride_t, p->k_stride_h) || !rows_fit(k_rope, p->k_rope_stride_t, 0) ||
       !rows_fit(v, p->v_stride_t, p->v_stride_h))
@@ -1120,8 +1279,9 @@ extern "C" int launch_latent_attention_expanded(void* stream, const void* q, con
   for (int64_t stride : {p->k_stride_t, p->k_rope_stride_t, p->v_stride_t})
     if (stride < 0 || stride >= (1ll << 23)) return AFA_E_SHAPE;  // 64 rows span less than 2^31 bytes
   if (p->Tq == 0) return AFA_OK;
-  const int64_t blocks = ((int64_t)p->Tq / 256 + p->B) * p->H;
-  if (blocks > 0x7fffffffll) return AFA_E_SHAPE;
+  const ExpandedPlan plan = plan_expanded(p);
+  const uint64_t need = expanded_bytes(p, plan);
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return AFA_E_WORKSPACE;
   ExpandedArgs a;
   a.q = q;
   a.k = k_nope;
@@ -1145,10 +1305,30 @@ extern "C" int launch_latent_attention_expanded(void* stream, const void* q, con
   a.B = p->B;
   a.H = p->H;
   a.causal = p->causal ? 1 : 0;
+  a.splits = plan.splits;
   a.scale = p->scale;
-  if (p->dtype == AFA_DTYPE_F16)
-    hipLaunchKernelGGL(expanded_kernel<DT_F16>, dim3((unsigned)blocks), dim3(512), 0, (hipStream_t)stream, a);
-  else
-    hipLaunchKernelGGL(expanded_kernel<DT_BF16>, dim3((unsigned)blocks), dim3(512), 0, (hipStream_t)stream, a);
-  return (int)hipGetLastError();
+  a.partial_o = (float*)workspace;
+  a.partial_ml = (float*)workspace + (need ? (int64_t)plan.splits * p->Tq * p->H * 128 : 0);
+  return p->dtype == AFA_DTYPE_F16 ? launch_expanded<DT_F16>(a, plan, (hipStream_t)stream)
+                                   : launch_expanded<DT_BF16>(a, plan, (hipStream_t)stream);
+}
+
+extern "C" int workspace_size_latent_attention_expanded(uint64_t* bytes, const LatentExpandedParams* p) {
+  using namespace afa;
+  if (!bytes) return AFA_E_NULL;
+  const int status = check_expanded(p);
+  if (status) return status;
+  *bytes = expanded_bytes(p, plan_expanded(p));
+  return AFA_OK;
+}
+
+extern "C" int form_latent_attention_expanded(int64_t form[2], const LatentExpandedParams* p) {
+  using namespace afa;
+  if (!form) return AFA_E_NULL;
+  const int status = check_expanded(p);
+  if (status) return status;
+  const ExpandedPlan plan = plan_expanded(p);
+  form[0] = plan.rows;
+  form[1] = plan.splits;
+  return AFA_OK;
 }

@@ -15,7 +15,7 @@
 // LDS, then goes over the rows in pieces of 8 pairs (two 16-byte accesses, in
 // either layout); rows that no 16-byte piece fits (odd widths, offsets or
 // strides) are taken one pair at a time. 8192 tokens of 64 heads x 64 columns take
-// 27.6 us (4.9 TB/s, the rate of a large copy), 4260 ragged prompt tokens of 8
+// 27.6 us (4.9 TB/s, the rate of a large copy), 4209 ragged prompt tokens of 8
 // heads x 256 columns into pages 11.9 us (22.5 where each thread worked out the
 // cosines of its own 8 pairs), 384 decode tokens of one 576-column row 3.9 (6.1).
 #include <algorithm>

@@ -28,9 +28,9 @@ _calls = CheckedCalls()
 
 
 class _Call:
-    """Checked sizes of a call: launcher parameters and each operand's bytes (none changes afterwards)."""
+    """Checked sizes of a call: launcher parameters, workspace bytes and each operand's bytes (none changes afterwards)."""
 
-    __slots__ = ("params", "sizes", "launch")
+    __slots__ = ("params", "nbytes", "sizes", "launch")
 
 
 def _check(lib, q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_lse, SCALE, causal):
@@ -63,11 +63,15 @@ def _check(lib, q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_l
             require(mine[0] < 2**23, f"{name} tokens may lie at most 2^23 - 1 elements apart")
         strides += mine
     qt, qh, kt, kh, rt, vt, vh, ot, oh = strides
-    call = _Call()
-    call.params = ct.pointer(_native.LatentExpandedParams(
+    params = _native.LatentExpandedParams(
         dtype=_native.AFA_DTYPE[_STORAGE[b16]], causal=int(causal), Tq=Tq, Tk=Tk, B=B, H=H, D=D, R=R, q_stride_t=qt,
         q_stride_h=qh, k_stride_t=kt, k_stride_h=kh, k_rope_stride_t=rt, v_stride_t=vt, v_stride_h=vh, out_stride_t=ot,
-        out_stride_h=oh, scale=SCALE, reserved=0))
+        out_stride_h=oh, scale=SCALE, reserved=0)
+    nbytes = ct.c_uint64(0)
+    _native.check(lib.workspace_size_latent_attention_expanded(ct.byref(nbytes), ct.byref(params)),
+                  "workspace_size_latent_attention_expanded")
+    call = _Call()
+    call.params, call.nbytes = ct.pointer(params), nbytes.value
     call.sizes = extents(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_lse)
     call.launch = lib.launch_latent_attention_expanded
     return call
@@ -105,7 +109,12 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
     if not pointers_apart(pointers, call.sizes, (7,) if new and softmax_lse is not None else () if new else (6, 7)):
         check_apart([(n, t, n in ("out", "softmax_lse")) for n, t in zip(NAMES, tensors)])
     if q.shape[0]:
-        status = launch_on(q.get_device(), call.launch, *pointers, call.params)
+        workspace = None
+        if call.nbytes:
+            # Partial results of split keys; the caching allocator keeps the block for this stream.
+            scratch = torch.empty(call.nbytes, dtype=torch.uint8, device=q.device)
+            workspace = scratch.data_ptr()
+        status = launch_on(q.get_device(), call.launch, *pointers, workspace, call.nbytes, call.params)
         if status:
             _native.check(status, "launch_latent_attention_expanded")
     return out

@@ -412,7 +412,13 @@ typedef struct LatentExpandedParams {
 
 int launch_latent_attention_expanded(void* stream, const void* q, const void* k_nope, const void* k_rope, const void* v,
                                      const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, void* out,
-                                     float* softmax_lse, const LatentExpandedParams* params);
+                                     float* softmax_lse, void* workspace, uint64_t workspace_bytes,
+                                     const LatentExpandedParams* params);
+
+/* As workspace_size_latent_attention and form_latent_attention: form[0] query
+ * rows per tile, form[1] key splits (1: no workspace, no second launch). */
+int workspace_size_latent_attention_expanded(uint64_t* bytes, const LatentExpandedParams* params);
+int form_latent_attention_expanded(int64_t form[2], const LatentExpandedParams* params);
 
 /* Measurement helpers (no reference kernel; the reference sweeps a >= 4x L2
  * buffer before each timed launch, benchmarks/cache.py:13-92 and
