@@ -53,7 +53,7 @@ struct LatentArgs {
   float scale;
   // Split form (below): workgroups, and its workspace.
   int32_t workers;
-  float* partial_o;         // [2 * workers][rows of a tile][L], not normalised
+  float* partial_o;         // [2 * workers][rows of a tile / 16][L / 16][64][4], not normalised, as a wave holds it
   float* partial_ml;        // [2 * workers][rows of a tile][4]: running maximum (log2), sum, sum of rounded weights
   struct LatentRecord* records;  // [tiles]
   uint32_t* tile_count;
@@ -77,7 +77,6 @@ struct LatentRecord {
 // cu_seqlens_q and seqused_kv, alike in every workgroup.
 template <int NW> __device__ constexpr uint32_t lat_start() { return 64 / lat_keys<NW>(); }
 template <int NW> __device__ constexpr uint32_t lat_least() { return 128 / lat_keys<NW>(); }  // least of a workgroup
-constexpr int LAT_MAX_WORKERS = 512;
 
 // Metadata in the constant address space, so that uniform reads are scalar loads,
 // whose values stay out of the vector registers and the vector load counter.
@@ -211,8 +210,13 @@ __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker,
   if (worker >= (uint32_t)share.workers) return false;
   share.workers = uniform(share.workers);
   share.total = total;
-  share.begin = uniform64(total * worker / (uint32_t)share.workers);
-  share.end = uniform64(total * (worker + 1) / (uint32_t)share.workers);
+  if (total < (1u << 22)) {  // 32-bit products with at most 512 workers: a 64-bit division costs microseconds
+    share.begin = (uint32_t)total * worker / (uint32_t)share.workers;
+    share.end = (uint32_t)total * (worker + 1) / (uint32_t)share.workers;
+  } else {
+    share.begin = uniform64(total * worker / (uint32_t)share.workers);
+    share.end = uniform64(total * (worker + 1) / (uint32_t)share.workers);
+  }
   if (share.begin >= before && share.begin < before + weight) {
     uint64_t at = before;
     uint32_t done = tiles_before;
@@ -316,6 +320,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   };
   const int kv_end = visible((min((int)(tile + 1) * ROWS, rows) - 1) / H);
   const int clean_end = visible((int)tile * ROWS / H);  // no row of the tile hides a key below
+  const bool idle = (int)(tile * ROWS) + wave * 16 >= rows;  // this wave has no rows: it only loads
   const int all_chunks = (kv_end + KEYS - 1) / KEYS;
   int begin = 0, chunks = all_chunks;  // of this part
   bool whole = true;
@@ -337,7 +342,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
       r.row = (int)tile * ROWS;
       r.rows = min(ROWS, rows - (int)tile * ROWS);
       r.first = (int)worker;
-      r.last = (int)((tile_end * (uint32_t)share.workers - 1) / share.total);
+      r.last = share.total < (1u << 22) ? (int)(((uint32_t)tile_end * (uint32_t)share.workers - 1) / (uint32_t)share.total)
+                                        : (int)((tile_end * (uint32_t)share.workers - 1) / share.total);
       a.records[share.tiles_before + tile] = r;
     }
     left -= end - offset;
@@ -471,6 +477,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     const int loaded = min(c + NS - 1, chunks);  // chunks fetched so far
     const uint32_t bits = (good >> (KT * (loaded - 1 - c))) & ((1u << KT) - 1u);
     if (more) fetch(c + NS - 1);
+    if (idle) continue;
     const uint32_t slot = ring_base + (uint32_t)((c - begin) % NS) * SLOT;
 
     f32x4 s[KT];
@@ -555,13 +562,14 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   int token, head;
   const bool valid = my_row(token, head);
   if (SPLIT && !whole) {
-    const int64_t part = 2 * (int64_t)worker + (offset == 0 ? 1 : 0), at = part * ROWS + wave * 16 + i16;
-    if (valid) {
-      float* po = a.partial_o + at * L + 4 * g;
+    // As the registers hold it, [16-row group][column tile][lane] of four columns: whole kilobytes per store.
+    const int64_t group = (2 * (int64_t)worker + (offset == 0 ? 1 : 0)) * NW + wave;
+    float* po = a.partial_o + (group * VTILES * 64 + lane) * 4;
+    if (!idle) {
 #pragma unroll
-      for (int t = 0; t < VTILES; ++t) *(f32x4*)(po + 16 * t) = o[t];
+      for (int t = 0; t < VTILES; ++t) *(f32x4*)(po + t * 256) = o[t];
     }
-    if (valid && g == 0) *(f32x4*)(a.partial_ml + at * 4) = f32x4{m_run, total, applied, 0.f};
+    if (!idle && g == 0) *(f32x4*)(a.partial_ml + (group * 16 + i16) * 4) = f32x4{m_run, total, applied, 0.f};
   } else if (valid) {
     const float inv = applied > 0.f ? 1.0f / applied : 0.f;
     scalar* out = (scalar*)a.out + (int64_t)(start + token) * a.o_t + (int64_t)head * a.o_h + 4 * g;
@@ -583,75 +591,96 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 
 // Combines the parts of the tiles that several workgroups of the split form
 // share: out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, in a fixed order. A
-// wave works out the weights of all parts of its row side by side, then sums
-// L / 64 columns a lane over the parts, four parts of loads in flight. Where the
-// tiles are few, the four waves of a workgroup share a row's parts (WAVES = 4,
-// sums joined in wave order), otherwise each takes a row. Bound by the parts'
-// bytes (4 L per row and part, written just before), or, for few tiles, by four
-// dependent loads.
+// wave takes 16 rows and 16 * TILES columns in the layout that a wave of the main
+// kernel holds them in: its lane groups first go over a quarter of the parts'
+// maxima each, then every lane sums its columns over the parts, AHEAD parts of
+// loads in flight. Many tiles (WAVES = 1): four such waves a workgroup, bound by
+// the parts' bytes (4 L per row and part, written just before). Few tiles, whose
+// parts are many: 16 waves share the parts of 16 columns and are joined through
+// LDS; bound by a few dependent loads.
 template <int DT, int L, int WAVES>
-__global__ __launch_bounds__(256) void latent_merge_kernel(LatentArgs a, int tile_rows) {
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void latent_merge_kernel(LatentArgs a, int tile_rows) {
   typedef typename B16<DT>::scalar scalar;
-  constexpr int ROWS = 4 / WAVES, COLUMNS = L / 64, AHEAD = 4;
-  typedef float vec __attribute__((ext_vector_type(COLUMNS)));
-  typedef scalar out_vec __attribute__((ext_vector_type(COLUMNS)));
-  __shared__ float weights[4][LAT_MAX_WORKERS];
-  __shared__ vec partial[4][64];
-  const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const uint32_t blocks = (uint32_t)tile_rows / ROWS;  // of a tile
-  const uint32_t tile = blockIdx.x / blocks;
-  const int r = (int)(blockIdx.x % blocks) * ROWS + wave / WAVES, sub = wave % WAVES;
-  const LatentRecord record = a.records[tile];  // there is room for every tile of the grid
-  if (tile >= *a.tile_count || record.first == record.last || r >= record.rows) return;
-  const int parts = record.last - record.first + 1;
-  auto slot = [&](int p) { return (2 * (int64_t)(record.first + p) + (p == 0 ? 1 : 0)) * tile_rows + r; };
+  typedef typename B16<DT>::x4 x4;
+  constexpr int VTILES = L / 16, TILES = WAVES == 1 ? 4 : 1, AHEAD = WAVES == 1 ? 4 : 8, SHARES = VTILES / TILES;
+  __shared__ f32x4 joined_o[WAVES == 1 ? 1 : WAVES][64];
+  __shared__ f32x4 joined_sums[WAVES == 1 ? 1 : WAVES][16];
+  const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
+  const uint32_t job = WAVES == 1 ? blockIdx.x * 4u + (uint32_t)wave : blockIdx.x, groups = (uint32_t)tile_rows / 16;
+  const uint32_t tile = job / (groups * SHARES), rest = job % (groups * SHARES);
+  const int group = (int)(rest / SHARES), t0 = (int)(rest % SHARES) * TILES;
+  if (tile >= *constant((const int32_t*)a.tile_count)) return;
+  const LatentRecord record = a.records[tile];
+  if (record.first == record.last || group * 16 >= record.rows) return;
+  const int parts = record.last - record.first + 1, sub = WAVES == 1 ? 0 : wave;
+  const int mine = (parts - sub + WAVES - 1) / WAVES;  // parts sub, sub + WAVES, ...
+  auto slot = [&](int k) {
+    const int p = sub + k * WAVES;
+    return (2 * (int64_t)(record.first + p) + (p == 0 ? 1 : 0)) * groups + group;
+  };
+  auto sums = [&](int k) { return *(const f32x4*)(a.partial_ml + (slot(k) * 16 + i16) * 4); };
 
   float top = -1e30f;
-  for (int p = lane; p < parts; p += 64) top = fmaxf(top, a.partial_ml[slot(p) * 4]);
-#pragma unroll
-  for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+#pragma unroll 4
+  for (int k = g; k < mine; k += 4) top = fmaxf(top, sums(k)[0]);
+  top = max_over_lane_groups(top);
   float total = 0.f, applied = 0.f;
-  for (int p = lane; p < parts; p += 64) {
-    const f32x4 ml = *(const f32x4*)(a.partial_ml + slot(p) * 4);
-    const float weight = fast_exp2(ml[0] - top);
-    weights[wave][p] = weight;
-    total += weight * ml[1];
-    applied += weight * ml[2];
-  }
+  f32x4 o[TILES];
 #pragma unroll
-  for (int d = 32; d > 0; d /= 2) {
-    total += __shfl_xor(total, d);
-    applied += __shfl_xor(applied, d);
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the lanes' weights, read by all of them
-
-  vec o = {};
-  for (int p = sub; p < parts; p += AHEAD * WAVES) {
-    vec v[AHEAD];
-    float weight[AHEAD];
+  for (int t = 0; t < TILES; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < mine; k += AHEAD) {
+    f32x4 ml[AHEAD], v[AHEAD][TILES];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const int q = min(p + i * WAVES, parts - 1);
-      weight[i] = p + i * WAVES < parts ? weights[wave][q] : 0.f;
-      v[i] = *(const vec*)(a.partial_o + slot(q) * L + lane * COLUMNS);
+      const int q = min(k + i, mine - 1);
+      ml[i] = sums(q);
+      const float* po = a.partial_o + ((slot(q) * VTILES + t0) * 64 + lane) * 4;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) v[i][t] = *(const f32x4*)(po + t * 256);
     }
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) o += weight[i] * v[i];
+    for (int i = 0; i < AHEAD; ++i) {
+      const float weight = k + i < mine ? fast_exp2(ml[i][0] - top) : 0.f;
+      total += weight * ml[i][1];
+      applied += weight * ml[i][2];
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) o[t] += weight * v[i][t];
+    }
   }
   if constexpr (WAVES > 1) {
-    partial[wave][lane] = o;
+    joined_o[wave][lane] = o[0];
+    if (g == 0) joined_sums[wave][i16] = f32x4{top, total, applied, 0.f};
     __syncthreads();
     if (wave != 0) return;
+    const float own = top;
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) o += partial[w][lane];
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, joined_sums[w][i16][0]);
+    const float scale = fast_exp2(own - top);
+    total *= scale;
+    applied *= scale;
+    o[0] *= scale;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      const f32x4 ml = joined_sums[w][i16];
+      const float weight = fast_exp2(ml[0] - top);
+      total += weight * ml[1];
+      applied += weight * ml[2];
+      o[0] += weight * joined_o[w][lane];
+    }
   }
+  const int r = group * 16 + i16;
+  if (r >= record.rows) return;
   const int packed = record.row + r, token = packed / a.H, head = packed - token * a.H;
   const float inv = applied > 0.f ? 1.0f / applied : 0.f;
-  out_vec v;
+  scalar* out = (scalar*)a.out + (int64_t)(record.start + token) * a.o_t + (int64_t)head * a.o_h + 16 * t0 + 4 * g;
 #pragma unroll
-  for (int i = 0; i < COLUMNS; ++i) v[i] = (scalar)(o[i] * inv);
-  *(out_vec*)((scalar*)a.out + (int64_t)(record.start + token) * a.o_t + (int64_t)head * a.o_h + lane * COLUMNS) = v;
-  if (a.lse && lane == 0)
+  for (int t = 0; t < TILES; ++t) {
+    x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[t][i] * inv);
+    *(x4*)(out + 16 * t) = v;
+  }
+  if (a.lse && t0 == 0 && g == 0)
     a.lse[(int64_t)(record.start + token) * a.H + head] = total > 0.f ? (top + __log2f(total)) * LAT_LN2 : -INFINITY;
 }
 
@@ -1037,6 +1066,7 @@ int check_latent(const LatentParams* p) {
 
 constexpr int LAT_CUS = 256;
 constexpr int64_t LAT_STREAM_BYTES = 128ll << 20;
+constexpr int64_t LAT_FEW_JOBS = 2048;
 
 // Form of a call: waves (of 16 rows each) of a tile, 8 where a request has more
 // than 64 rows on average, else 4; and workgroups of the split form, one per CU
@@ -1094,12 +1124,12 @@ int launch_latent(LatentArgs a, const LatentPlan& plan, void* workspace, hipStre
     hipLaunchKernelGGL((latent_kernel<DT, L, R, 4, true, false>), grid, dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  // One workgroup per row up to 2048 rows (of 33 parts), else per four rows.
   const int rows = 16 * plan.waves;
-  if (plan.tiles * rows <= 2048)
-    hipLaunchKernelGGL((latent_merge_kernel<DT, L, 4>), dim3((unsigned)(plan.tiles * rows)), dim3(256), 0, s, a, rows);
+  const int64_t jobs = plan.tiles * plan.waves * (L / 16);  // of 16 rows and 16 columns
+  if (jobs <= LAT_FEW_JOBS)
+    hipLaunchKernelGGL((latent_merge_kernel<DT, L, 16>), dim3((unsigned)jobs), dim3(1024), 0, s, a, rows);
   else
-    hipLaunchKernelGGL((latent_merge_kernel<DT, L, 1>), dim3((unsigned)(plan.tiles * (rows / 4))), dim3(256), 0, s, a, rows);
+    hipLaunchKernelGGL((latent_merge_kernel<DT, L, 1>), dim3((unsigned)((jobs / 4 + 3) / 4)), dim3(256), 0, s, a, rows);
   return (int)hipGetLastError();
 }
 
