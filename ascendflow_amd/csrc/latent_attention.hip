@@ -1240,7 +1240,7 @@ int check_expanded(const LatentExpandedParams* p) {
 // 60 / 38 / 28 / 30; 1 x 500 behind 4000, 32 heads 90 / 68 / 76 / 98.
 ExpandedPlan plan_expanded(const LatentExpandedParams* p) {
   constexpr int FORMS = 3, ROWS[FORMS] = {256, 128, 64}, SLOTS[FORMS] = {256, 512, 512};
-  constexpr double ALONE[FORMS] = {2.0, 1.5, 1.2}, FULL[FORMS] = {2.75, 3.0, 1.65}, START[FORMS] = {12.0, 9.0, 7.5};
+  constexpr double ALONE[FORMS] = {2.0, 1.5, 1.2}, FULL[FORMS] = {2.85, 2.9, 1.65}, START[FORMS] = {12.0, 11.0, 7.5};
   constexpr double MERGE = 5.0, MERGE_RATE = 3e6;  // us, bytes a us
   const int64_t nq = std::max<int64_t>(1, (p->Tq + p->B - 1) / p->B), nk = std::max<int64_t>(1, (p->Tk + p->B - 1) / p->B);
   const double chunks = std::ceil(nk / 64.0);
