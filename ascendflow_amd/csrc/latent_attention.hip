@@ -18,9 +18,12 @@
 // Online softmax in float32, exp2 domain: the running maximum m is raised only
 // when a row's maximum exceeds it by more than LAT_TAU (log2 units), so that O
 // is rescaled rarely; P <= 2^LAT_TAU is rounded to the storage type (a matrix
-// operand has to be), and O is divided by the sum of the rounded P, so that the
-// weights that were applied add up to one; the log-sum-exp takes the sum before
-// rounding.
+// operand has to be), at most half a step of each weight, while O is divided by
+// the sum of the weights before rounding. (The sum of the rounded ones would
+// cancel that error where one key takes all, but costs a conversion and an
+// addition a score: in the expanded form, which the vector units bound, 700
+// instead of 635 us for 8192 causal tokens of 32 heads. A maximum raised at every
+// growth, whose own weight is exactly 1: 665.)
 #include <algorithm>
 #include <cmath>
 
@@ -54,7 +57,7 @@ struct LatentArgs {
   // Split form (below): workgroups, and its workspace.
   int32_t workers;
   float* partial_o;         // [2 * workers][rows of a tile / 16][L / 16][64][4], not normalised, as a wave holds it
-  float* partial_ml;        // [2 * workers][rows of a tile][4]: running maximum (log2), sum, sum of rounded weights
+  float* partial_ml;        // [2 * workers][rows of a tile][2]: running maximum (log2), sum of weights
   struct LatentRecord* records;  // [tiles]
   uint32_t* tile_count;
 };
@@ -320,7 +323,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   };
   const int kv_end = visible((min((int)(tile + 1) * ROWS, rows) - 1) / H);
   const int clean_end = visible((int)tile * ROWS / H);  // no row of the tile hides a key below
-  const bool idle = (int)(tile * ROWS) + wave * 16 >= rows;  // this wave has no rows: it only loads
+  // This wave has no rows: it only loads (the direct form, whose tiles are nearly all full, spills with the branch).
+  const bool idle = SPLIT && (int)(tile * ROWS) + wave * 16 >= rows;
   const int all_chunks = (kv_end + KEYS - 1) / KEYS;
   int begin = 0, chunks = all_chunks;  // of this part
   bool whole = true;
@@ -410,7 +414,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
         load(to_rope, rope_off());
     } else {
       // Rows past the end or without a page become zeros, which no weight can turn into anything else.
-      const u32x4 zero = {0u, 0u, 0u, 0u};
+      const uint32_t none = opaque(0u);  // not a register kept through the loop
+      const u32x4 zero = {none, none, none, none};
 #pragma unroll
       for (int p = 0; p < LOADS_L; ++p) {
         if (p * LR + r0 < have)
@@ -455,7 +460,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 #pragma unroll
   for (int t = 0; t < VTILES; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = -1e30f;  // finite: a chunk that hides all its keys gives p = 0, never NaN
-  float l_run = 0.f, l_rounded = 0.f;
+  float l_run = 0.f;
 
 #pragma unroll
   for (int c = 0; c < NS - 1; ++c)
@@ -520,7 +525,6 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     if (__ballot(m_new > m_run + LAT_TAU) != 0ull) {
       const float alpha = fast_exp2(m_run - m_new);
       l_run *= alpha;
-      l_rounded *= alpha;
 #pragma unroll
       for (int t = 0; t < VTILES; ++t) o[t] *= alpha;
       m_run = m_new;
@@ -531,10 +535,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float p = fast_exp2(__builtin_fmaf(s[t][i], scale_log2, -m_run));
-        const scalar r = (scalar)p;
         l_run += p;
-        l_rounded += (float)r;
-        pf[t / 2][4 * (t % 2) + i] = r;
+        pf[t / 2][4 * (t % 2) + i] = (scalar)p;
       }
     {
       constexpr int FRAGS = KT / 2 * VTILES, LOOK = 3;
@@ -558,7 +560,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     }
   }
 
-  const float total = sum_over_lane_groups(l_run), applied = sum_over_lane_groups(l_rounded);
+  const float total = sum_over_lane_groups(l_run);
   int token, head;
   const bool valid = my_row(token, head);
   if (SPLIT && !whole) {
@@ -569,9 +571,9 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 #pragma unroll
       for (int t = 0; t < VTILES; ++t) *(f32x4*)(po + t * 256) = o[t];
     }
-    if (!idle && g == 0) *(f32x4*)(a.partial_ml + (group * 16 + i16) * 4) = f32x4{m_run, total, applied, 0.f};
+    if (!idle && g == 0) *(float2*)(a.partial_ml + (group * 16 + i16) * 2) = make_float2(m_run, total);
   } else if (valid) {
-    const float inv = applied > 0.f ? 1.0f / applied : 0.f;
+    const float inv = total > 0.f ? 1.0f / total : 0.f;
     scalar* out = (scalar*)a.out + (int64_t)(start + token) * a.o_t + (int64_t)head * a.o_h + 4 * g;
 #pragma unroll
     for (int t = 0; t < VTILES; ++t) {
@@ -604,7 +606,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void latent_merge_ke
   typedef typename B16<DT>::x4 x4;
   constexpr int VTILES = L / 16, TILES = WAVES == 1 ? 4 : 1, AHEAD = WAVES == 1 ? 4 : 8, SHARES = VTILES / TILES;
   __shared__ f32x4 joined_o[WAVES == 1 ? 1 : WAVES][64];
-  __shared__ f32x4 joined_sums[WAVES == 1 ? 1 : WAVES][16];
+  __shared__ float2 joined_sums[WAVES == 1 ? 1 : WAVES][16];
   const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
   const uint32_t job = WAVES == 1 ? blockIdx.x * 4u + (uint32_t)wave : blockIdx.x, groups = (uint32_t)tile_rows / 16;
   const uint32_t tile = job / (groups * SHARES), rest = job % (groups * SHARES);
@@ -618,18 +620,19 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void latent_merge_ke
     const int p = sub + k * WAVES;
     return (2 * (int64_t)(record.first + p) + (p == 0 ? 1 : 0)) * groups + group;
   };
-  auto sums = [&](int k) { return *(const f32x4*)(a.partial_ml + (slot(k) * 16 + i16) * 4); };
+  auto sums = [&](int k) { return *(const float2*)(a.partial_ml + (slot(k) * 16 + i16) * 2); };
 
   float top = -1e30f;
 #pragma unroll 4
-  for (int k = g; k < mine; k += 4) top = fmaxf(top, sums(k)[0]);
+  for (int k = g; k < mine; k += 4) top = fmaxf(top, sums(k).x);
   top = max_over_lane_groups(top);
-  float total = 0.f, applied = 0.f;
+  float total = 0.f;
   f32x4 o[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int k = 0; k < mine; k += AHEAD) {
-    f32x4 ml[AHEAD], v[AHEAD][TILES];
+    float2 ml[AHEAD];
+    f32x4 v[AHEAD][TILES];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int q = min(k + i, mine - 1);
@@ -640,38 +643,35 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void latent_merge_ke
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const float weight = k + i < mine ? fast_exp2(ml[i][0] - top) : 0.f;
-      total += weight * ml[i][1];
-      applied += weight * ml[i][2];
+      const float weight = k + i < mine ? fast_exp2(ml[i].x - top) : 0.f;
+      total += weight * ml[i].y;
 #pragma unroll
       for (int t = 0; t < TILES; ++t) o[t] += weight * v[i][t];
     }
   }
   if constexpr (WAVES > 1) {
     joined_o[wave][lane] = o[0];
-    if (g == 0) joined_sums[wave][i16] = f32x4{top, total, applied, 0.f};
+    if (g == 0) joined_sums[wave][i16] = make_float2(top, total);
     __syncthreads();
     if (wave != 0) return;
     const float own = top;
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, joined_sums[w][i16][0]);
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, joined_sums[w][i16].x);
     const float scale = fast_exp2(own - top);
     total *= scale;
-    applied *= scale;
     o[0] *= scale;
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) {
-      const f32x4 ml = joined_sums[w][i16];
-      const float weight = fast_exp2(ml[0] - top);
-      total += weight * ml[1];
-      applied += weight * ml[2];
+      const float2 ml = joined_sums[w][i16];
+      const float weight = fast_exp2(ml.x - top);
+      total += weight * ml.y;
       o[0] += weight * joined_o[w][lane];
     }
   }
   const int r = group * 16 + i16;
   if (r >= record.rows) return;
   const int packed = record.row + r, token = packed / a.H, head = packed - token * a.H;
-  const float inv = applied > 0.f ? 1.0f / applied : 0.f;
+  const float inv = total > 0.f ? 1.0f / total : 0.f;
   scalar* out = (scalar*)a.out + (int64_t)(record.start + token) * a.o_t + (int64_t)head * a.o_h + 16 * t0 + 4 * g;
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
@@ -713,7 +713,7 @@ struct ExpandedArgs {
   int32_t splits;
   float scale;
   float* partial_o;   // [splits][Tq * H][128], not normalised
-  float* partial_ml;  // [splits][Tq * H][4]: running maximum (log2), sum, sum of rounded weights
+  float* partial_ml;  // [splits][Tq * H][2]: running maximum (log2), sum of weights
 };
 
 template <int DT, int NW, int QT, bool SPLIT>
@@ -816,11 +816,11 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(Expa
   const uint32_t tr_at = (uint32_t)(rt * ROW_BYTES + ((((i16 & 3) >> 1) ^ (rt & 15)) << 4) + (i16 & 1) * 8);
 
   f32x4 o[QT][D / 16];
-  float m_run[QT], l_run[QT], l_rounded[QT];
+  float m_run[QT], l_run[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     m_run[qt] = -1e30f;
-    l_run[qt] = l_rounded[qt] = 0.f;
+    l_run[qt] = 0.f;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -911,14 +911,12 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(Expa
     if (c + NS - 1 < chunks) fetch_v(c + NS - 1);
     if (c >= clean_chunks) mask(c, cur);
     x8 pf[QT][KC / 32];
-    float top[QT], m_new[QT], psum[QT], rsum[QT];
+    float top[QT], m_new[QT], psum[QT];
     auto exp_element = [&](int e) {  // (half, qt, key tile of the half, i)
       const int h = e / HALF, qt = (e / 8) % QT, t = 2 * h + (e / 4) % 2, i = e % 4;
       const float p = fast_exp2(__builtin_fmaf(cur[t][qt][i], scale_log2, -m_run[qt]));
-      const scalar r = (scalar)p;
       psum[qt] += p;
-      rsum[qt] += (float)r;
-      pf[qt][h][(t & 1) * 4 + i] = r;
+      pf[qt][h][(t & 1) * 4 + i] = (scalar)p;
     };
     auto qk_between = [&](int f) {
       if (f == QK_FRAGS / 2 - 1) __builtin_amdgcn_s_setprio(2);
@@ -933,7 +931,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(Expa
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
           m_new[qt] = fmaxf(m_run[qt], max_over_lane_groups(top[qt]) * scale_log2);
-          psum[qt] = rsum[qt] = 0.f;
+          psum[qt] = 0.f;
         }
       } else if (f == QT + 1) {
         bool grow = false;
@@ -944,7 +942,6 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(Expa
           for (int qt = 0; qt < QT; ++qt) {
             const float alpha = fast_exp2(m_run[qt] - m_new[qt]);
             l_run[qt] *= alpha;
-            l_rounded[qt] *= alpha;
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) o[qt][t] *= alpha;
             m_run[qt] = m_new[qt];
@@ -964,10 +961,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(Expa
           if (e * PV_EXP_STEPS / HALF == f) exp_element(HALF + e);
       } else if (f == PV_EXP_STEPS + 1) {
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          l_run[qt] += psum[qt];
-          l_rounded[qt] += rsum[qt];
-        }
+        for (int qt = 0; qt < QT; ++qt) l_run[qt] += psum[qt];
       }
     };
     // Wave priority steps down with the wave's progress through a chunk: of the
@@ -986,15 +980,15 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(Expa
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const int row = q0 + (wave * QT + qt) * 16 + i16;
-    const float total = sum_over_lane_groups(l_run[qt]), applied = sum_over_lane_groups(l_rounded[qt]);
+    const float total = sum_over_lane_groups(l_run[qt]);
     if (row >= nq) continue;
     if constexpr (SPLIT) {
       const int64_t at = ((int64_t)split * a.Tq + q_start + row) * a.H + head;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) *(f32x4*)(a.partial_o + at * D + 16 * t + 4 * g) = o[qt][t];
-      if (g == 0) *(f32x4*)(a.partial_ml + at * 4) = f32x4{m_run[qt], total, applied, 0.f};
+      if (g == 0) *(float2*)(a.partial_ml + at * 2) = make_float2(m_run[qt], total);
     } else {
-      const float inv = applied > 0.f ? 1.0f / applied : 0.f;
+      const float inv = total > 0.f ? 1.0f / total : 0.f;
       scalar* out = (scalar*)a.out + (int64_t)(q_start + row) * a.o_t + (int64_t)head * a.o_h + 4 * g;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
@@ -1021,26 +1015,26 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedArgs a) {
   const int end = min(max(constant(a.cu_q)[a.B], 0), a.Tq);  // rows of no request stay as they are
   if (row >= rows || row / a.H >= end || row / a.H < constant(a.cu_q)[0]) return;
   float top = -1e30f;
-  for (int p = 0; p < a.splits; ++p) top = fmaxf(top, a.partial_ml[(p * rows + row) * 4]);
-  float total = 0.f, applied = 0.f;
+  for (int p = 0; p < a.splits; ++p) top = fmaxf(top, a.partial_ml[(p * rows + row) * 2]);
+  float total = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int p = 0; p < a.splits; p += AHEAD) {
-    f32x4 ml[AHEAD], v[AHEAD];
+    float2 ml[AHEAD];
+    f32x4 v[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int64_t at = min(p + i, a.splits - 1) * rows + row;
-      ml[i] = *(const f32x4*)(a.partial_ml + at * 4);
+      ml[i] = *(const float2*)(a.partial_ml + at * 2);
       v[i] = *(const f32x4*)(a.partial_o + at * 128 + column);
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const float weight = p + i < a.splits ? fast_exp2(ml[i][0] - top) : 0.f;
-      total += weight * ml[i][1];
-      applied += weight * ml[i][2];
+      const float weight = p + i < a.splits ? fast_exp2(ml[i].x - top) : 0.f;
+      total += weight * ml[i].y;
       o += weight * v[i];
     }
   }
-  const float inv = applied > 0.f ? 1.0f / applied : 0.f;
+  const float inv = total > 0.f ? 1.0f / total : 0.f;
   x4 v;
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[i] * inv);
@@ -1093,7 +1087,7 @@ LatentPlan plan_latent(const LatentParams* p) {
 int64_t latent_part_rows(const LatentPlan& plan) { return 2ll * plan.workers * 16 * plan.waves; }
 uint64_t latent_bytes(const LatentParams* p, const LatentPlan& plan) {
   if (plan.workers == 0 || p->T == 0) return 0;
-  return (uint64_t)(latent_part_rows(plan) * (p->L + 4) * 4 + plan.tiles * (int64_t)sizeof(LatentRecord) + 16);
+  return (uint64_t)(latent_part_rows(plan) * (p->L + 2) * 4 + plan.tiles * (int64_t)sizeof(LatentRecord) + 16);
 }
 
 template <int DT, int L, int R>
@@ -1111,7 +1105,7 @@ int launch_latent(LatentArgs a, const LatentPlan& plan, void* workspace, hipStre
   a.workers = plan.workers;
   a.partial_o = (float*)workspace;
   a.partial_ml = a.partial_o + part_rows * L;
-  a.tile_count = (uint32_t*)(a.partial_ml + part_rows * 4);
+  a.tile_count = (uint32_t*)(a.partial_ml + part_rows * 2);
   a.records = (LatentRecord*)(a.tile_count + 4);
   const dim3 grid((unsigned)plan.workers);
   if (plan.waves == 8 && plan.stream)
@@ -1252,7 +1246,7 @@ ExpandedPlan plan_expanded(const LatentExpandedParams* p) {
     const double full = (p->causal ? rounds : std::ceil(rounds)) * mean * each * FULL[form] *
                         std::min(1.0, std::max(rounds, 256.0 / SLOTS[form]));
     return START[form] * (0.5 + 0.5 * std::ceil(rounds)) + std::max(each * ALONE[form], full) +
-           (splits > 1 ? MERGE + (double)splits * p->Tq * p->H * (2 * 132 * 4) / MERGE_RATE : 0.0);
+           (splits > 1 ? MERGE + (double)splits * p->Tq * p->H * (2 * 130 * 4) / MERGE_RATE : 0.0);
   };
   ExpandedPlan plan{ROWS[0], 1};
   double best = cost(0, 1);
@@ -1271,7 +1265,7 @@ ExpandedPlan plan_expanded(const LatentExpandedParams* p) {
 }
 
 uint64_t expanded_bytes(const LatentExpandedParams* p, const ExpandedPlan& plan) {
-  return plan.splits > 1 ? (uint64_t)plan.splits * p->Tq * p->H * (128 + 4) * 4 : 0;
+  return plan.splits > 1 ? (uint64_t)plan.splits * p->Tq * p->H * (128 + 2) * 4 : 0;
 }
 
 template <int DT>

@@ -130,9 +130,9 @@ def test_latent_forms(lib, sizes, form):
     rows, workers = form
     if workers == 0:
         assert size.value == 0
-    else:  # parts of 512 columns, a maximum and two sums per row; a record per tile and their count
+    else:  # parts of 512 columns, a maximum and a sum per row; a record per tile and their count
         tiles = sizes["T"] * sizes["H"] // rows + sizes["B"]
-        assert size.value == 2 * workers * rows * (512 + 4) * 4 + tiles * 20 + 16
+        assert size.value == 2 * workers * rows * (512 + 2) * 4 + tiles * 20 + 16
     assert lib.form_latent_attention(None, ct.byref(latent())) == -1 and lib.form_latent_attention(got, None) == -1
 
 
@@ -159,7 +159,7 @@ def test_expanded_forms(lib, sizes, form):
     assert got[0] == form[0] and (got[1] > 1 if form[1] is None else got[1] == form[1])
     size = ct.c_uint64(1)
     assert lib.workspace_size_latent_attention_expanded(ct.byref(size), ct.byref(expanded(**sizes))) == 0
-    assert size.value == (got[1] * sizes["Tq"] * sizes["H"] * 132 * 4 if got[1] > 1 else 0)
+    assert size.value == (got[1] * sizes["Tq"] * sizes["H"] * 130 * 4 if got[1] > 1 else 0)
     if size.value:
         args = [None] + [P(16)] * 7 + [None]
         for workspace, nbytes in ((None, size.value), (P(16), size.value - 1), (P(8), size.value)):
