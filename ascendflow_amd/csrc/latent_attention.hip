@@ -510,11 +510,12 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     if (key0 + KEYS > clean_end || bits != (1u << KT) - 1u) {  // uniform
       int token, head;
       const int lim = my_row(token, head) ? visible(token) - key0 : 0;  // this row sees the chunk's keys below it
+      const int quad = 4 * (int)((opaque((uint32_t)tid) >> 4) & 3u);
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          s[t][i] = 16 * t + sigma(4 * g + i) < lim && ((bits >> t) & 1u) ? s[t][i] : -INFINITY;
+          s[t][i] = 16 * t + sigma(quad + i) < lim && ((bits >> t) & 1u) ? s[t][i] : -INFINITY;
     }
     float top = -INFINITY;
 #pragma unroll
