@@ -38,7 +38,7 @@ constexpr int EXP_MAX_SPLITS = 64;
 // Cache rows per chunk. Eight waves (one workgroup per CU): 64, two slots; a
 // barrier, a fetch and a reduction per 64 rows instead of 32 and four chains of
 // dependent matrix instructions instead of two (128 heads, 4 chunks of 512 tokens
-// behind 8K: 4317 -> XXXX us). Four waves: 32, two slots in each of the CU's two
+// behind 8K: 4317 -> 3660 us). Four waves: 32, two slots in each of the CU's two
 // workgroups.
 template <int NW> __host__ __device__ constexpr int lat_keys() { return NW == 8 ? 64 : 32; }
 
@@ -60,6 +60,7 @@ struct LatentArgs {
   float* partial_ml;        // [2 * workers][rows of a tile][2]: running maximum (log2), sum of weights
   struct LatentRecord* records;  // [tiles]
   uint32_t* tile_count;
+  uint32_t tiles;           // the most that monotone cu_seqlens_q can give
 };
 
 // A tile of the split form as its merge needs it: its first row is row `row` of
@@ -72,14 +73,16 @@ struct LatentRecord {
 
 // Split form: the chunks of all tiles, in order, are one sequence that the
 // workgroups share evenly, so that few or unequal requests fill the GPU and end
-// together. A tile counts its chunks (those of its request's last token) and
-// 64 rows' worth for its start and end. A workgroup takes at most one tile's
-// end, whole tiles and one tile's beginning; parts go to the workspace (slot
-// 2 w the end, 2 w + 1 the beginning) as float32 and latent_merge_kernel
-// combines them in order. Everything is computed on the device from
-// cu_seqlens_q and seqused_kv, alike in every workgroup.
-template <int NW> __device__ constexpr uint32_t lat_start() { return 64 / lat_keys<NW>(); }
-template <int NW> __device__ constexpr uint32_t lat_least() { return 128 / lat_keys<NW>(); }  // least of a workgroup
+// together. A tile counts its chunks and 64 rows' worth for its start and end.
+// Causal tiles of a request have unequal numbers of them: tiles i and n - 1 - i
+// follow each other (the longer first) and count, together, what the first and
+// the last tile do, so that any place in the sequence is found by a division.
+// A workgroup takes at most one tile's end, whole tiles and one tile's
+// beginning; parts go to the workspace (slot 2 w the end, 2 w + 1 the beginning)
+// as float32 and latent_merge_kernel combines them in order. Everything is
+// computed on the device from cu_seqlens_q and seqused_kv, alike in every workgroup.
+template <int NW> __host__ __device__ constexpr uint32_t lat_start() { return 64 / lat_keys<NW>(); }
+template <int NW> __host__ __device__ constexpr uint32_t lat_least() { return 128 / lat_keys<NW>(); }  // least of a workgroup
 
 // Metadata in the constant address space, so that uniform reads are scalar loads,
 // whose values stay out of the vector registers and the vector load counter.
@@ -133,10 +136,44 @@ __device__ __forceinline__ bool find_tile(const_ints cu, int B, int T, uint32_t 
   return false;
 }
 
-// Chunks that a request's tiles count in the split form.
-template <int NW> __device__ __forceinline__ uint32_t longest_chunks(int used, int count) {
-  return count > 0 ? ((uint32_t)max(used, 0) + lat_keys<NW>() - 1) / lat_keys<NW>() : 0u;
-}
+// The part of the split form's sequence that a request takes.
+template <int NW> struct LatentSpan {
+  static constexpr uint32_t ROWS = 16 * NW, START = lat_start<NW>();
+  int H, used, count, causal;
+  uint32_t tiles;
+  uint32_t pair, middle;  // what two paired tiles count, and the one left over
+  __device__ __forceinline__ uint32_t chunks(uint32_t tile) const {
+    const uint32_t last = min((tile + 1) * ROWS, (uint32_t)(count * H)) - 1;
+    const int seen = causal ? min(max(used - count + (int)(last / (uint32_t)H) + 1, 0), used) : used;
+    return ((uint32_t)seen + lat_keys<NW>() - 1) / lat_keys<NW>();
+  }
+  __device__ __forceinline__ LatentSpan(const LatentArgs& a, int b) : H((int)opaque_uniform((uint32_t)a.H)), causal(a.causal) {
+    int start;
+    request_tokens(constant(a.cu), b, a.T, start, count);
+    used = (int)min((int64_t)max(constant(a.used)[b], 0), (int64_t)a.W << a.page_shift);
+    tiles = ((uint32_t)(count * H) + ROWS - 1) / ROWS;
+    const uint32_t most = ((uint32_t)used + lat_keys<NW>() - 1) / lat_keys<NW>() + START;
+    pair = 2 * most;
+    middle = most;
+    if (causal && tiles > 1) {
+      pair = most + chunks(0) + START;
+      middle = chunks(tiles / 2) + START;
+    }
+  }
+  __device__ __forceinline__ uint32_t longest() const {
+    return tiles == 0 ? 0u : causal && tiles > 1 ? pair - chunks(0) - START : middle;
+  }
+  __device__ __forceinline__ uint64_t weight() const { return (uint64_t)(tiles / 2) * pair + (tiles % 2 ? middle : 0u); }
+  // The tile at place `at` of the request's, and what it counts.
+  __device__ __forceinline__ uint32_t tile(uint32_t at) const { return at % 2 || at + 1 == tiles ? at / 2 : tiles - 1 - at / 2; }
+  __device__ __forceinline__ uint32_t longer(uint32_t p) const {
+    return causal ? min(chunks(tiles - 1 - p) + START, pair - 1) : pair / 2;
+  }
+  __device__ __forceinline__ uint32_t counts(uint32_t at) const {
+    if (at + 1 == tiles && tiles % 2) return middle;
+    return at % 2 ? pair - longer(at / 2) : longer(at / 2);
+  }
+};
 
 __device__ __forceinline__ uint64_t inclusive_scan64(uint64_t v, int lane) {
 #pragma unroll
@@ -147,55 +184,71 @@ __device__ __forceinline__ uint64_t inclusive_scan64(uint64_t v, int lane) {
   return v;
 }
 
+// Maximum of the wave, in lane 63.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  auto with = [&](uint32_t other) { v = max(v, other); };
+  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));  // row_shr:1
+  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));  // row_shr:2
+  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));  // row_shr:4
+  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));  // row_shr:8
+  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));  // row_bcast:31
+  return v;
+}
+
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ uint64_t uniform64(uint64_t v) {
   return (uint64_t)(uint32_t)uniform((int)(uint32_t)v) | ((uint64_t)(uint32_t)uniform((int)(uint32_t)(v >> 32)) << 32);
 }
+
+// Sharing tiles costs the parts' bytes and the join, LAT_JOIN chunks' worth, and
+// chunks take longer the more of the GPU is at work (3.2 us with half its CUs, 4.3
+// with all: 128 rows of 512 columns are bound by power and by the L2s). Tiles are
+// therefore kept whole where the longest of them, or the rounds that they need,
+// take LAT_APART times as many chunks as an even share and the join.
+constexpr float LAT_APART = 0.875f;
+template <int NW> constexpr float LAT_JOIN = NW == 8 ? 5.0f : 10.0f;
 
 // Where a workgroup of the split form begins.
 struct LatentShare {
   uint64_t begin, end;       // of the sequence
   uint64_t total;
   int32_t workers;           // that have a share
+  bool apart;                // tiles are not shared: a tile is whoever's its beginning is
   int32_t request;
-  uint32_t tile, offset;     // inside the request, inside the tile
+  uint32_t place, offset;    // of the tile among the request's, inside the tile
   uint32_t tiles_before;     // of earlier requests
 };
 
 template <int NW>
 __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker, LatentShare& share) {
-  constexpr int THREADS = NW * 64, ROWS = NW * 16;
+  constexpr int THREADS = NW * 64;
   __shared__ uint64_t wave_weight[THREADS / 64];
-  __shared__ uint32_t wave_tiles[THREADS / 64];
+  __shared__ uint32_t wave_tiles[THREADS / 64], wave_longest[THREADS / 64];
   __shared__ uint32_t found[4];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int per = (a.B + THREADS - 1) / THREADS;  // consecutive requests of a thread
-  auto measure = [&](int b, uint32_t& tiles, uint32_t& each) {
-    int start, count;
-    request_tokens(constant(a.cu), b, a.T, start, count);
-    const int used = (int)min((int64_t)max(constant(a.used)[b], 0), (int64_t)a.W << a.page_shift);
-    tiles = ((uint32_t)count * (uint32_t)a.H + ROWS - 1) / ROWS;
-    each = longest_chunks<NW>(used, count) + lat_start<NW>();
-  };
   uint64_t weight = 0;
-  uint32_t tiles = 0;
+  uint32_t tiles = 0, longest = 0;
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;
     if (b >= a.B) break;
-    uint32_t n, each;
-    measure(b, n, each);
-    weight += (uint64_t)n * each;
-    tiles += n;
+    const LatentSpan<NW> span(a, b);
+    weight += span.weight();
+    tiles += span.tiles;
+    longest = max(longest, span.longest());
   }
   const uint64_t upto = inclusive_scan64(weight, lane);
   const uint32_t tiles_upto = (uint32_t)wave_inclusive_scan((int)tiles);
+  longest = wave_max(longest);
   if (lane == 63) {
     wave_weight[wave] = upto;
     wave_tiles[wave] = tiles_upto;
+    wave_longest[wave] = longest;
   }
   __syncthreads();
   uint64_t before = upto - weight, total = 0;
-  uint32_t tiles_before = tiles_upto - tiles, all = 0;
+  uint32_t tiles_before = tiles_upto - tiles, all = 0, most_chunks = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / 64; ++w) {
     if (w < wave) {
@@ -204,44 +257,80 @@ __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker,
     }
     total += wave_weight[w];
     all += wave_tiles[w];
+    most_chunks = max(most_chunks, wave_longest[w]);
   }
   total = uniform64(total);
-  if (worker == 0 && tid == 0) *a.tile_count = all;
-  if (total == 0) return false;
+  if (total == 0) {
+    if (worker == 0 && tid == 0) *a.tile_count = 0;
+    return false;
+  }
   const uint64_t most = total / lat_least<NW>();
   share.workers = most < 1 ? 1 : (most < (uint64_t)a.workers ? (int)most : a.workers);
-  if (worker >= (uint32_t)share.workers) return false;
   share.workers = uniform(share.workers);
+  all = (uint32_t)uniform((int)all);
+  longest = (uint32_t)uniform((int)most_chunks);
+  const float each = (float)total / (float)share.workers;
+  const float whole = (float)((all + (uint32_t)share.workers - 1) / (uint32_t)share.workers) * ((float)total / (float)all);
+  share.apart = __ballot(LAT_APART * fmaxf((float)longest, whole) <= each + LAT_JOIN<NW>) != 0;
+  const bool one = share.apart && all <= (uint32_t)a.workers;  // a tile each, spread over the XCDs
+  worker = (uint32_t)uniform((int)(one ? blockIdx.x : worker));
+  if (worker >= (one ? all : (uint32_t)share.workers)) return false;
+  if (worker == 0 && tid == 0) *a.tile_count = share.apart ? 0u : all;
   share.total = total;
   if (total < (1u << 22)) {  // 32-bit products with at most 512 workers: a 64-bit division costs microseconds
-    share.begin = (uint32_t)total * worker / (uint32_t)share.workers;
-    share.end = (uint32_t)total * (worker + 1) / (uint32_t)share.workers;
+    share.begin = (uint32_t)uniform((int)((uint32_t)total * worker / (uint32_t)share.workers));
+    share.end = (uint32_t)uniform((int)((uint32_t)total * (worker + 1) / (uint32_t)share.workers));
   } else {
     share.begin = uniform64(total * worker / (uint32_t)share.workers);
     share.end = uniform64(total * (worker + 1) / (uint32_t)share.workers);
   }
-  if (share.begin >= before && share.begin < before + weight) {
+  if (one) {
+    if (worker >= tiles_before && worker < tiles_before + tiles) {
+      uint32_t place = worker - tiles_before;
+      for (int i = 0; i < per; ++i) {
+        const int b = tid * per + i;
+        const uint32_t mine = LatentSpan<NW>(a, b).tiles;
+        if (place < mine) {
+          found[0] = (uint32_t)b;
+          found[1] = place;
+          found[2] = 0;
+          found[3] = 0;
+          break;
+        }
+        place -= mine;
+      }
+    }
+  } else if (share.begin >= before && share.begin < before + weight) {
     uint64_t at = before;
     uint32_t done = tiles_before;
     for (int i = 0; i < per; ++i) {
       const int b = tid * per + i;
-      uint32_t n, each;
-      measure(b, n, each);
-      if (share.begin < at + (uint64_t)n * each) {
-        const uint32_t inside = (uint32_t)((share.begin - at) / each);
+      const LatentSpan<NW> span(a, b);
+      if (share.begin < at + span.weight()) {
+        const uint64_t inside = share.begin - at;
+        const uint32_t pairs = (uint32_t)min(inside / span.pair, (uint64_t)(span.tiles / 2));
+        uint32_t offset = (uint32_t)(inside - (uint64_t)pairs * span.pair), place = 2 * pairs;
+        if (pairs < span.tiles / 2) {
+          const uint32_t longer = span.longer(pairs);
+          if (offset >= longer) {
+            offset -= longer;
+            ++place;
+          }
+        }
         found[0] = (uint32_t)b;
-        found[1] = inside;
-        found[2] = (uint32_t)(share.begin - at - (uint64_t)inside * each);
+        found[1] = place;
+        found[2] = offset;
         found[3] = done;
         break;
       }
-      at += (uint64_t)n * each;
-      done += n;
+      at += span.weight();
+      done += span.tiles;
     }
   }
   __syncthreads();
+  if (one) share.end = share.begin + 1;
   share.request = uniform((int)found[0]);
-  share.tile = (uint32_t)uniform((int)found[1]);
+  share.place = (uint32_t)uniform((int)found[1]);
   share.offset = (uint32_t)uniform((int)found[2]);
   share.tiles_before = (uint32_t)uniform((int)found[3]);
   return true;
@@ -278,12 +367,13 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 
   int request;
   uint32_t tile, tiles;
+  uint32_t place = 0;  // of the tile among its request's in the split form's order
   LatentShare share;
-  uint64_t left = 0;  // of this workgroup's share
+  uint64_t left = 0;   // of this workgroup's share
   if constexpr (SPLIT) {
     if (!find_share<NW>(a, worker, share)) return;
     request = share.request;
-    tile = share.tile;
+    place = share.place;
     left = share.end - share.begin;
   } else {
     if (!find_tile<NW * 64>(constant(a.cu), a.B, a.T, worker,
@@ -302,12 +392,22 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   request_tokens(constant(a.cu), request, a.T, start, count);
   const int used = (int)min((int64_t)max(constant(a.used)[request], 0), (int64_t)a.W << a.page_shift);
   const int rows = count * H;
+  uint32_t each = 0;  // what the tile counts
   if constexpr (SPLIT) {
-    tiles = ((uint32_t)rows + ROWS - 1) / ROWS;
-    if (tile >= tiles) {  // on to the next request that has tokens (there is one: something is left)
-      share.tiles_before += tiles;
-      tile = 0;
+    const LatentSpan<NW> span(a, request);
+    if (place >= span.tiles) {  // on to the next request that has tokens (there is one: something is left)
+      share.tiles_before += span.tiles;
+      place = 0;
       ++request;
+      continue;
+    }
+    tile = (uint32_t)uniform((int)span.tile(place));
+    each = (uint32_t)uniform((int)span.counts(place));
+    if (share.apart && offset > 0) {  // an earlier workgroup's tile
+      if (left <= each - offset) return;
+      left -= each - offset;
+      offset = 0;
+      ++place;
       continue;
     }
   }
@@ -331,26 +431,27 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   if constexpr (SPLIT) {
     // The tile's own chunks, spread over what it counts.
     constexpr uint32_t START = lat_start<NW>();
-    const uint32_t counted = longest_chunks<NW>(used, count), each = counted + START;
-    const uint32_t end = (uint32_t)min((uint64_t)each, (uint64_t)offset + left);
+    const uint32_t end = share.apart ? each : (uint32_t)min((uint64_t)each, (uint64_t)offset + left);
     auto cut = [&](uint32_t x) {
-      return x >= each ? all_chunks : (x <= START ? 0 : (int)((uint64_t)(x - START) * (uint32_t)all_chunks / counted));
+      return x >= each ? all_chunks : (x <= START ? 0 : (int)((uint64_t)(x - START) * (uint32_t)all_chunks / (each - START)));
     };
     begin = cut(offset);
     chunks = cut(end);
     whole = offset == 0 && end == each;
-    if (offset == 0 && tid == 0) {
+    if (!share.apart && offset == 0 && tid == 0 && share.tiles_before + place < a.tiles) {
       const uint64_t tile_end = share.end - left + each;  // in the sequence
       LatentRecord r;
       r.start = start;
       r.row = (int)tile * ROWS;
       r.rows = min(ROWS, rows - (int)tile * ROWS);
       r.first = (int)worker;
-      r.last = share.total < (1u << 22) ? (int)(((uint32_t)tile_end * (uint32_t)share.workers - 1) / (uint32_t)share.total)
-                                        : (int)((tile_end * (uint32_t)share.workers - 1) / share.total);
-      a.records[share.tiles_before + tile] = r;
+      // Divisions from scratch: their divisors' reciprocals, kept, would be spilled.
+      const uint32_t low = opaque_uniform((uint32_t)share.total), high = opaque_uniform((uint32_t)(share.total >> 32));
+      r.last = share.total < (1u << 22) ? (int)(((uint32_t)tile_end * (uint32_t)share.workers - 1) / low)
+                                        : (int)((tile_end * (uint32_t)share.workers - 1) / ((uint64_t)high << 32 | low));
+      a.records[share.tiles_before + place] = r;
     }
-    left -= end - offset;
+    left -= min(left, (uint64_t)(end - offset));
     if (!first_part) block_barrier();  // the ring is read
   }
 
@@ -588,7 +689,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   }
   if (!SPLIT || left == 0) return;
   offset = 0;
-  ++tile;
+  ++place;
   }
 }
 
@@ -1064,9 +1165,13 @@ constexpr int64_t LAT_STREAM_BYTES = 128ll << 20;
 constexpr int64_t LAT_FEW_JOBS = 2048;
 
 // Form of a call: waves (of 16 rows each) of a tile, 8 where a request has more
-// than 64 rows on average, else 4; and workgroups of the split form, one per CU
-// or two, 0 for the form of one tile per workgroup: where the tiles (at most
-// rows / tile + B of them) would fill the GPU four times over anyway.
+// than 64 rows on average, else 4 (64 decode requests of 8000 rows, 128 heads 179 us
+// with 8, 195 with 4; 4 chunks of 512 behind them 3597 and 3818; one of 4096 rows
+// 31.0 and 30.0); and workgroups of the split form, one per CU or two, 0 for the
+// form of one tile per workgroup: where the tiles (at most rows / tile + B of
+// them) would fill the GPU four times over anyway, or a single request's fill 85%
+// of their rounds (128 heads behind 8000 rows: 230 tokens 459 us directly, 504
+// split; 400 tokens 869 and 848; 500 tokens 907 and 1032).
 struct LatentPlan {
   int waves;
   int workers;
@@ -1078,7 +1183,9 @@ LatentPlan plan_latent(const LatentParams* p) {
   plan.waves = ((int64_t)p->T + p->B - 1) / p->B * p->H > 64 ? 8 : 4;
   plan.tiles = (int64_t)p->T * p->H / (16 * plan.waves) + p->B;
   const int slots = plan.waves == 8 ? LAT_CUS : 2 * LAT_CUS;
-  plan.workers = plan.tiles <= 4 * slots ? slots : 0;
+  const int64_t single = ((int64_t)p->T * p->H + 16 * plan.waves - 1) / (16 * plan.waves);  // a single request's tiles
+  const bool even = p->B == 1 && 20 * single >= 17 * ((single + slots - 1) / slots) * slots;
+  plan.workers = plan.tiles <= 4 * slots && !even ? slots : 0;
   plan.stream = (int64_t)p->T * p->H <= (int64_t)p->B * 16 * plan.waves &&
                 (int64_t)p->BLOCKS * p->PAGE * (p->L + p->R) * 2 >= LAT_STREAM_BYTES;
   return plan;
@@ -1108,6 +1215,7 @@ int launch_latent(LatentArgs a, const LatentPlan& plan, void* workspace, hipStre
   a.partial_ml = a.partial_o + part_rows * L;
   a.tile_count = (uint32_t*)(a.partial_ml + part_rows * 2);
   a.records = (LatentRecord*)(a.tile_count + 4);
+  a.tiles = (uint32_t)plan.tiles;
   const dim3 grid((unsigned)plan.workers);
   if (plan.waves == 8 && plan.stream)
     hipLaunchKernelGGL((latent_kernel<DT, L, R, 8, true, true>), grid, dim3(512), 0, s, a);

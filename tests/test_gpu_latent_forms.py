@@ -206,3 +206,57 @@ def test_random_ragged_prompts(device, seed):
     nq = [int(torch.randint(0, min(n, 400) + 1, (1,), generator=gen)) for n in nk]
     nq[0] = max(1, nq[0])
     check_expanded(device, nq, nk, H, pick(True, False), pick("bf16", "f16"), seed, pick(0, 3))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("counts,lengths,H", [
+    ([150], [1500], 96),                  # 113 tiles that token boundaries cut, shared
+    ([151, 0, 3, 40], [151, 70, 3000, 2000], 128),
+    ([70, 33], [40, 33], 80),             # queries before their request's first row
+])
+def test_unequal_tiles_of_a_request_are_shared(device, counts, lengths, H, causal):
+    """Causal tiles of a request, paired from both ends, odd and even numbers of them."""
+    t = paged(device, counts, lengths, H=H, L=128, R=64, page=32, spare_tokens=2)
+    assert form_of(t) == [128, 256]
+    check_on_device(device, t, counts, lengths, causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("counts,lengths,H", [
+    ([128], [128], 128),                  # a tile a workgroup
+    ([1] * 200, [500] * 200, 128),
+    ([100, 101, 0, 99], [100, 101, 5, 99], 128),  # some a workgroup
+    ([70] * 7, list(range(70, 77)), 96),
+])
+def test_short_tiles_are_kept_whole(device, counts, lengths, H, causal):
+    t = paged(device, counts, lengths, H=H, L=128, R=64, page=16, spare_tokens=3)
+    assert form_of(t) == [128, 256]
+    check_on_device(device, t, counts, lengths, causal)
+
+
+def test_whole_and_shared_tiles_of_one_captured_call(device):
+    """Which of the two a call does follows from its lengths on the device, at each replay of a graph."""
+    t = paged(device, [1] * 40, [900] * 40, H=16, L=128, R=64, page=64)
+    assert form_of(t) == [64, 512]
+    scale = 128 ** -0.5
+    out, lse = torch.empty_like(t["q"]), torch.empty(40, 16, device=device)
+    call(t, scale, True, out, lse)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(t, scale, True, out, lse)
+    for lengths in ([900] * 40, [30] * 40, [900] + [1] * 39, [0] * 40, [64] * 40):
+        t["seqused_kv"].copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed, replayed_lse = out.clone(), lse.clone()
+        expected = lr.latent_attention(t["q"], t["q_rope"], t["kv_cache"], t["block_table"].cpu(), t["cu_seqlens_q"].cpu(),
+                                       t["seqused_kv"].cpu(), scale, True)
+        finite = t["kv_cache"][torch.isfinite(t["kv_cache"])]
+        compare(replayed, replayed_lse, expected, B16["bf16"], max(1, *lengths), finite.abs().max().item())
+
+
+def test_a_single_request_that_fills_its_rounds(device):
+    t = paged(device, [230], [260], H=128, L=128, R=64, page=32)
+    assert form_of(t) == [128, 0]
+    check_on_device(device, t, [230], [260])
