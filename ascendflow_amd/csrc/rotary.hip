@@ -189,8 +189,8 @@ struct AppendArgs {
 
 // A workgroup of four waves takes block_tokens new tokens. One wave finds a
 // token's place: its request is the number of boundaries cu[1..B] at or below
-// it (64 compared at a time), its position seqused - n + j; token rows at or past
-// cu[B], positions outside the table's width and pages outside the cache have none.
+// it (64 compared at a time), its position seqused - n + j; token rows below cu[0], at
+// or past cu[B], positions outside the table's width and pages outside the cache have none.
 template <int DT, int VEC, int LAYOUT>
 __global__ __launch_bounds__(256) void append_paged_kv_kernel(AppendArgs a) {
   typedef typename B16<DT>::scalar scalar;
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256) void append_paged_kv_kernel(AppendArgs a) {
       if (below < 64) break;
     }
     position = -1;
-    if (request >= a.B) return -1;
+    if (request >= a.B || token < a.cu[0]) return -1;
     position = (int64_t)a.used[request] - a.cu[request + 1] + token;
     if (position < 0) return -1;
     const int64_t page = position / a.PAGE;

@@ -105,7 +105,7 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
     of the row (``offset`` is not read), and ``k`` holds the DK - R others: the
     latent and the rotary key of a token as two tensors.
 
-    Tokens at or past ``cu_seqlens_q[B]``, negative positions, positions beyond
+    Tokens of no request (at or past ``cu_seqlens_q[B]``), negative positions, positions beyond
     the table and pages outside the cache write nothing. Two new tokens must not
     name the same row. The call reads no values on the host and can be captured
     in a graph.

@@ -180,3 +180,11 @@ def test_refusals(device):
             append_paged_kv(**{**t, **extra, **change})
     with pytest.raises(ValueError, match="overlap"):
         append_paged_kv(**{**t, **extra, "k": t["k_cache"].view(-1, 2, 64)[:5]})
+
+
+def test_tokens_ahead_of_the_first_request_write_nothing(device):
+    t, extra = inputs(device, [4, 3], [9, 20], spare=2)
+    t["cu_seqlens_q"] = t["cu_seqlens_q"] + 2  # two tokens of no request, then seven
+    got = check(t, extra)
+    changed = (got != t["k_cache"].cpu()).any(-1).flatten(1).any(-1)
+    assert changed.sum() <= 3  # the pages of the seven rows

@@ -102,3 +102,24 @@ def test_rotation_and_append_feed_the_sparse_operator(device):
     positions = torch.cat([torch.arange(297, 300, device=device)] * 2)
     back = apply_rotary(first, positions, frequencies, offset=448, inverse=True)
     assert torch.isfinite(back.float()).all() and torch.equal(back[..., :448], first[..., :448])
+
+
+@pytest.mark.parametrize("H", [16, 128])
+def test_tokens_ahead_of_the_first_request_stay_as_they_were(device, H):
+    from tests import test_gpu_latent_expanded as expanded
+    from tests.latent_helpers import call, paged
+
+    t = paged(device, [1, 2], [90, 300], H=H, spare_tokens=3)
+    shifted = {**t, "cu_seqlens_q": t["cu_seqlens_q"] + 3,
+               "q": torch.cat([t["q"][3:], t["q"][:3]]), "q_rope": torch.cat([t["q_rope"][3:], t["q_rope"][:3]])}
+    want, got = torch.full_like(t["q"], 7.0), torch.full_like(t["q"], 7.0)
+    call(t, 0.07, True, want)
+    call(shifted, 0.07, True, got)
+    assert torch.equal(got[3:], want[:3]) and (got[:3] == 7).all()
+
+    t = expanded.inputs(device, [1, 2], [900, 700], H=4, spare=3)  # split keys, joined by a second launch
+    shifted = {**t, "cu_q": t["cu_q"] + 3, "q": torch.cat([t["q"][3:], t["q"][:3]])}
+    want, got = (torch.full((6, 4, 128), 7.0, dtype=torch.bfloat16, device=device) for _ in range(2))
+    expanded.call(t, out=want)
+    expanded.call(shifted, out=got)
+    assert torch.equal(got[3:], want[:3]) and (got[:3] == 7).all()
