@@ -8,7 +8,7 @@
 // so a row is read once and serves as key and as value. The rows of a request's
 // (token, head) pairs are packed token by token into tiles of 16 * NW rows; each
 // wave owns 16 of them, whose Q (L + R columns) and O (L columns, float32) stay
-// in registers. Cache rows stream in chunks of 32 through an LDS ring filled by
+// in registers. Cache rows stream in chunks of 64 or 32 through an LDS ring filled by
 // the load-to-LDS path, XOR-swizzled on the global side, and every wave reads
 // every row twice: S^T[keys, rows] = K Q^T with ds_read_b128, O^T[columns, rows]
 // += V^T P^T with the transposing ds_read_b64_tr_b16. P stays in the wave's
@@ -338,7 +338,8 @@ __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker,
 
 // STREAM: non-temporal loads, for requests of one tile each (nothing is read
 // twice) over a cache too large to stay in the 256 MiB Infinity Cache between
-// calls (64 requests of 32K: 128 heads 664 -> 639 us, 16 heads 435 -> 420).
+// calls (64 requests of 32K with 128 heads 633 -> 617 us, 32 with 16 heads 223 -> 204;
+// 64 of 2K with 16 heads, 150 MB, 44.7 -> 44.9).
 template <int DT, int L, int R, int NW, bool SPLIT, bool STREAM>
 __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(LatentArgs a) {
   typedef typename B16<DT>::scalar scalar;
@@ -1156,12 +1157,15 @@ int check_latent(const LatentParams* p) {
   if (p->PAGE < 16 || p->PAGE > (1 << 20) || (p->PAGE & (p->PAGE - 1))) return AFA_E_SHAPE;
   // Packed rows, tiles and positions are 32-bit numbers.
   if ((int64_t)p->T * p->H > 0x7fffff00ll || (int64_t)p->W * p->PAGE > 0x7fffff00ll || p->B > 0x3fffffff) return AFA_E_SHAPE;
-  if (!(p->scale > 0.0f)) return AFA_E_SHAPE;
+  if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return AFA_E_SHAPE;
   return AFA_OK;
 }
 
 constexpr int LAT_CUS = 256;
 constexpr int64_t LAT_STREAM_BYTES = 128ll << 20;
+// Merge jobs of 16 waves each up to here, of one wave above: one request of 4K rows
+// (256 jobs) 23 and 27 us, of 64K rows 46 and 144; 16 of 4K rows with 16 heads (2560)
+// 31.5 and 30.1, 8 x 4 tokens of 64 heads (6144) 78 and 45.
 constexpr int64_t LAT_FEW_JOBS = 2048;
 
 // Form of a call: waves (of 16 rows each) of a tile, 8 where a request has more
@@ -1327,7 +1331,7 @@ int check_expanded(const LatentExpandedParams* p) {
   if (!p) return AFA_E_NULL;
   if (p->dtype != AFA_DTYPE_BF16 && p->dtype != AFA_DTYPE_F16) return AFA_E_DTYPE;
   if (p->Tq < 0 || p->Tk < 0 || p->B <= 0 || p->H <= 0 || p->Tq > 0x7fffff00 || p->Tk > 0x7fffff00) return AFA_E_SHAPE;
-  if (p->D != 128 || p->R != 64 || !(p->scale > 0.0f)) return AFA_E_SHAPE;
+  if (p->D != 128 || p->R != 64 || !(p->scale > 0.0f) || !std::isfinite(p->scale)) return AFA_E_SHAPE;
   if (((int64_t)p->Tq / 64 + p->B) * p->H > 0x7fffffffll / EXP_MAX_SPLITS) return AFA_E_SHAPE;
   return AFA_OK;
 }
@@ -1336,11 +1340,12 @@ int check_expanded(const LatentExpandedParams* p) {
 // request lengths (the launcher reads no device memory). A tile's 64-key chunk
 // costs ALONE where it has its CU to itself and FULL with the CU's workgroups at
 // work (one of 256 rows, two of 128 or 64); a round of workgroups START. Measured
-// at 256 / 128 / 64 rows: 1 x 8192 causal, 32 heads 726 / 741 / 921 us; 1 x 1500,
-// 128 heads 160 / 144 / 181; 5 x 235..470 behind up to 2000, 16 heads 79 / 69 / 56;
-// 1 x 2048, 16 heads 83 / 64 / 55. Split keys add a launch and their float32 parts
+// at 256 / 128 / 64 rows: 1 x 8192 causal, 32 heads 639 / 653 / 845 us; 1 x 1500,
+// 128 heads 133 / 124 / 151; 5 x 235..470 behind up to 2000, 16 heads 67 / 59 / 49;
+// 1 x 2048, 16 heads 70 / 54 / 47. Split keys add a launch and their float32 parts
 // written and read at 3 TB/s: 64 rows in 1 / 2 / 4 / 8 parts, 8 x 20 behind 3000, 8 heads
-// 60 / 38 / 28 / 30; 1 x 500 behind 4000, 32 heads 90 / 68 / 76 / 98.
+// 54 / 37 / 27 / 29; 1 x 500 behind 4000, 32 heads 76 / 69 / 76 / 96; one query of 8192
+// keys, 16 heads 136 / 78 / 43 / 27.
 ExpandedPlan plan_expanded(const LatentExpandedParams* p) {
   constexpr int FORMS = 3, ROWS[FORMS] = {256, 128, 64}, SLOTS[FORMS] = {256, 512, 512};
   constexpr double ALONE[FORMS] = {2.0, 1.5, 1.2}, FULL[FORMS] = {2.85, 2.9, 1.65}, START[FORMS] = {12.0, 11.0, 7.5};

@@ -12,6 +12,7 @@ are read from where they lie: no per-head copy of ``k_rope`` is made.
 from __future__ import annotations
 
 import ctypes as ct
+import math
 
 import torch
 
@@ -54,7 +55,7 @@ def _check(lib, q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_l
     if softmax_lse is not None:
         check_tensor("softmax_lse", softmax_lse, (Tq, H), torch.float32, device)
     require(B > 0 and H > 0, "positive request and head counts")
-    require(SCALE > 0, "positive attention scale")
+    require(0 < SCALE < math.inf, "positive, finite attention scale")
     strides = []
     for name, t in (("q", q), ("k_nope", k_nope), ("k_rope", k_rope), ("v", v), ("out", out)):
         mine = live_strides(t)[:-1]

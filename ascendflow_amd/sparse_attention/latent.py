@@ -15,6 +15,7 @@ decode, verification of several tokens a request, and chunks of prompts
 from __future__ import annotations
 
 import ctypes as ct
+import math
 from typing import Optional
 
 import torch
@@ -73,7 +74,7 @@ def _check(lib, q, q_rope, kv_cache, block_table, cu_seqlens_q, seqused_kv, out,
     require(L in (128, 256, 512), "the latent width (columns of q) must be 128, 256 or 512")
     require(R in (0, 64), "the rotary width must be 64, or 0 without q_rope")
     require(PAGE >= 16 and PAGE & (PAGE - 1) == 0, "PAGE must be a power of two from 16 on")
-    require(SCALE > 0, "positive attention scale")
+    require(0 < SCALE < math.inf, "positive, finite attention scale")
     qt, qh = row_strides("q", q)
     rt, rh = (0, 0) if q_rope is None else row_strides("q_rope", q_rope)
     ot, oh = row_strides("out", out)

@@ -389,7 +389,8 @@ int launch_latent_attention(void* stream, const void* q, const void* q_rope, con
 int workspace_size_latent_attention(uint64_t* bytes, const LatentParams* params);
 
 /* Which form a call of these sizes runs: form[0] packed (token, head) rows per
- * tile, form[1] workgroups that share all tiles' keys evenly, 0 for one tile per
+ * tile, form[1] workgroups that share the tiles (their keys, or, where that does not
+ * pay at the lengths found on the device, whole tiles), 0 for one tile per
  * workgroup. For tests and profiles. */
 int form_latent_attention(int64_t form[2], const LatentParams* params);
 

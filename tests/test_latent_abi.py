@@ -231,3 +231,9 @@ def test_absorbed_and_expanded_definitions_agree():
     absorbed = torch.einsum("nhd,hld->nhl", q[..., :128], w_k)
     o, lse2, *_ = lr.latent_attention(absorbed, q[..., 128:], cache, torch.tensor([[0, 1]]), cu, torch.tensor([s]), 0.07)
     assert torch.allclose(lse, lse2, atol=1e-12) and torch.allclose(torch.einsum("nhl,hld->nhd", o, w_v), out, atol=1e-12)
+
+
+def test_infinite_scales_are_refused(lib):
+    args = [None] + [P(16)] * 7 + [None, P(16), 1 << 40]
+    assert lib.launch_latent_attention(*args, ct.byref(latent(scale=math.inf))) == -2
+    assert lib.launch_latent_attention_expanded(*args, ct.byref(expanded(scale=math.inf))) == -2
