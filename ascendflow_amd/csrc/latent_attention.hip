@@ -95,6 +95,16 @@ __device__ __forceinline__ void request_tokens(const_ints cu, int b, int T, int&
   count = max(min(cu[b + 1], T) - start, 0);
 }
 
+// Cache rows of request b that its table holds, and those ahead of its first new
+// token (fewer than none where it has more tokens than rows). The tokens' places
+// and so the causal limit go by the length itself, which may pass the table:
+// token t sees rows up to ahead + t of the `used`.
+__device__ __forceinline__ void request_rows(const LatentArgs& a, int b, int start, int& used, int& ahead) {
+  const int length = max(constant(a.used)[b], 0);
+  used = (int)min((int64_t)length, (int64_t)a.W << a.page_shift);
+  ahead = length - (max(constant(a.cu)[b + 1], start) - start);
+}
+
 // The request and the tile inside it of tile `index` in the order of requests
 // (tiles_of(tokens) each); false, for the whole workgroup, if there are fewer.
 template <int THREADS, typename F>
@@ -139,18 +149,18 @@ __device__ __forceinline__ bool find_tile(const_ints cu, int B, int T, uint32_t 
 // The part of the split form's sequence that a request takes.
 template <int NW> struct LatentSpan {
   static constexpr uint32_t ROWS = 16 * NW, START = lat_start<NW>();
-  int H, used, count, causal;
+  int H, used, ahead, count, causal;
   uint32_t tiles;
   uint32_t pair, middle;  // what two paired tiles count, and the one left over
   __device__ __forceinline__ uint32_t chunks(uint32_t tile) const {
     const uint32_t last = min((tile + 1) * ROWS, (uint32_t)(count * H)) - 1;
-    const int seen = causal ? min(max(used - count + (int)(last / (uint32_t)H) + 1, 0), used) : used;
+    const int seen = causal ? min(max(ahead + (int)(last / (uint32_t)H) + 1, 0), used) : used;
     return ((uint32_t)seen + lat_keys<NW>() - 1) / lat_keys<NW>();
   }
   __device__ __forceinline__ LatentSpan(const LatentArgs& a, int b) : H((int)opaque_uniform((uint32_t)a.H)), causal(a.causal) {
     int start;
     request_tokens(constant(a.cu), b, a.T, start, count);
-    used = (int)min((int64_t)max(constant(a.used)[b], 0), (int64_t)a.W << a.page_shift);
+    request_rows(a, b, start, used, ahead);
     tiles = ((uint32_t)(count * H) + ROWS - 1) / ROWS;
     const uint32_t most = ((uint32_t)used + lat_keys<NW>() - 1) / lat_keys<NW>() + START;
     pair = 2 * most;
@@ -391,7 +401,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   if (SPLIT && request >= a.B) return;  // never, unless cu_seqlens_q or seqused_kv change under the call
   int start, count;
   request_tokens(constant(a.cu), request, a.T, start, count);
-  const int used = (int)min((int64_t)max(constant(a.used)[request], 0), (int64_t)a.W << a.page_shift);
+  int used, ahead;
+  request_rows(a, request, start, used, ahead);
   const int rows = count * H;
   uint32_t each = 0;  // what the tile counts
   if constexpr (SPLIT) {
@@ -413,7 +424,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     }
   }
 
-  auto visible = [&](int t) { return a.causal ? min(max(used - count + t + 1, 0), used) : used; };
+  auto visible = [&](int t) { return a.causal ? min(max(ahead + t + 1, 0), used) : used; };
   // This lane's (token, head) row. Worked out where it is needed (Q, masks, the
   // end): kept, it would cost registers that the loop does not have.
   auto my_row = [&](int& token, int& head) {

@@ -102,6 +102,7 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
     [B + 1], ``seqused_kv`` int32 [B]: rows of each request, the new tokens'
     included (``append_paged_kv`` writes them). With ``CAUSAL`` token j of a
     request's n sees rows up to ``seqused_kv[b] - n + j``, without all of them.
+    Rows past the table are not there; the limit goes by ``seqused_kv[b]`` as it is, as the append's places do.
     ``softmax_lse`` (optional float32 [T, H]) receives ln(sum_j exp(s_j)).
 
     A token that sees no row gets zeros and -inf; tokens at or past

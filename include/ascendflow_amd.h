@@ -360,7 +360,8 @@ int launch_append_paged_kv(void* stream, const void* k, const void* rope, const 
  * L + R columns, kv_cache [BLOCKS][PAGE][L + R]: for token t, head h of request b
  *   s_j = scale (q[t][h] . c_j + q_rope[t][h] . k_rope_j),  out[t][h] = softmax(s) c,
  * over the rows j < seqused_kv[b], and, causal, j <= seqused_kv[b] - n + i for
- * the i-th of the request's n tokens. L 128, 256 or 512, R 0 or 64, PAGE a power
+ * the i-th of the request's n tokens (a length past the table's W * PAGE rows has no
+ * rows there, but keeps this limit). L 128, 256 or 512, R 0 or 64, PAGE a power
  * of two from 16 on. q and out [T][H][L], q_rope [T][H][R] with strides in
  * elements (multiples of 8; rows contiguous and on 16 bytes). Rows behind
  * seqused_kv are not read; pages outside [0, BLOCKS) hold no keys; a token that

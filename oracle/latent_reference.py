@@ -73,7 +73,8 @@ def latent_attention(q, q_rope, cache, table, cu, used, scale, causal=True):
     whole = q.double() if q_rope is None else torch.cat([q.double(), q_rope.double()], -1)
     for b in range(table.shape[0]):
         start, end = int(cu[b]), int(cu[b + 1])
-        n, s = end - start, max(0, min(int(used[b]), table.shape[1] * page))
+        n, length = end - start, max(0, int(used[b]))
+        s = min(length, table.shape[1] * page)  # rows that the table holds; the tokens' places go by the length itself
         if n == 0:
             continue
         ids = table[b].tolist()
@@ -81,7 +82,7 @@ def latent_attention(q, q_rope, cache, table, cu, used, scale, causal=True):
         block = torch.tensor([ids[j // page] for j in there], dtype=torch.long, device=q.device)
         slot = torch.tensor([j % page for j in there], dtype=torch.long, device=q.device)
         rows = cache[block, slot].double()  # [keys, 1, L + R]
-        limit = [sum(1 for j in there if j < (s - n + i + 1 if causal else s)) for i in range(n)]
+        limit = [sum(1 for j in there if j < (length - n + i + 1 if causal else s)) for i in range(n)]
         part = _attend(whole[start:end], rows, rows[..., :L], scale, limit)
         for whole_result, piece in zip(result, part):
             whole_result[start:end] = piece
