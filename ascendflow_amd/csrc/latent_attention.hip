@@ -84,6 +84,17 @@ struct LatentRecord {
 template <int NW> __host__ __device__ constexpr uint32_t lat_start() { return 64 / lat_keys<NW>(); }
 template <int NW> __host__ __device__ constexpr uint32_t lat_least() { return 128 / lat_keys<NW>(); }  // least of a workgroup
 
+// A row's ln(sum of e^scores) from its maximum m (log2) and its sum of weights:
+// -inf for a sum of nothing. A sum that is not a number (scores that are none, or
+// overflow to +inf) stays one, beside an output that is none either; it is told by its
+// bits, since device code is built without NaN semantics of comparisons.
+__device__ __forceinline__ float row_lse(float m, float total) {
+  const uint32_t bits = __float_as_uint(total);
+  uint32_t lse = __float_as_uint((m + __log2f(total)) * LAT_LN2);
+  lse = (bits & 0x7fffffffu) > 0x7f800000u ? 0x7fc00000u : lse;
+  return __uint_as_float(bits == 0u ? 0xff800000u : lse);
+}
+
 // Metadata in the constant address space, so that uniform reads are scalar loads,
 // whose values stay out of the vector registers and the vector load counter.
 typedef const __attribute__((address_space(4))) int32_t* const_ints;
@@ -697,7 +708,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
       *(x4*)(out + 16 * t) = v;
     }
     if (a.lse && g == 0)
-      a.lse[(int64_t)(start + token) * H + head] = total > 0.f ? (m_run + __log2f(total)) * LAT_LN2 : -INFINITY;
+      a.lse[(int64_t)(start + token) * H + head] = row_lse(m_run, total);
   }
   if (!SPLIT || left == 0) return;
   offset = 0;
@@ -795,7 +806,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void latent_merge_ke
     *(x4*)(out + 16 * t) = v;
   }
   if (a.lse && t0 == 0 && g == 0)
-    a.lse[(int64_t)(record.start + token) * a.H + head] = total > 0.f ? (top + __log2f(total)) * LAT_LN2 : -INFINITY;
+    a.lse[(int64_t)(record.start + token) * a.H + head] = row_lse(top, total);
 }
 
 // Expanded form (latent_attention_expanded), for prompts: keys [k_nope | k_rope]
@@ -1112,7 +1123,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(Expa
         *(x4*)(out + 16 * t) = v;
       }
       if (a.lse && g == 0)
-        a.lse[(int64_t)(q_start + row) * a.H + head] = total > 0.f ? (m_run[qt] + __log2f(total)) * LAT_LN2 : -INFINITY;
+        a.lse[(int64_t)(q_start + row) * a.H + head] = row_lse(m_run[qt], total);
     }
   }
 }
@@ -1153,7 +1164,7 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedArgs a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[i] * inv);
   *(x4*)((scalar*)a.out + row / a.H * a.o_t + row % a.H * a.o_h + column) = v;
-  if (a.lse && column == 0) a.lse[row] = total > 0.f ? (top + __log2f(total)) * LAT_LN2 : -INFINITY;
+  if (a.lse && column == 0) a.lse[row] = row_lse(top, total);
 }
 
 namespace {

@@ -91,7 +91,8 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
     [Tq, H]) receives ln(sum_j exp(s_j)).
 
     A query that sees no key gets zeros and -inf; queries at or past
-    ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``).
+    ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``). One
+    whose scores are NaN or overflow to +inf gets NaN in both.
     Keys and values that some query of a request sees have to be finite.
     """
     lib = _native.library()

@@ -106,7 +106,8 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
     ``softmax_lse`` (optional float32 [T, H]) receives ln(sum_j exp(s_j)).
 
     A token that sees no row gets zeros and -inf; tokens at or past
-    ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``).
+    ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``). One
+    whose scores are NaN or overflow to +inf gets NaN in both.
     Rows behind ``seqused_kv`` are never read and pages outside the cache hold no
     keys, but the rows that some token of a request sees have to be finite.
     """

@@ -367,6 +367,7 @@ int launch_append_paged_kv(void* stream, const void* k, const void* rope, const 
  * seqused_kv are not read; pages outside [0, BLOCKS) hold no keys; a token that
  * sees no key gets zeros; tokens at or past cu_seqlens_q[B] are left as they
  * were. softmax_lse f32 [T][H] or NULL: ln(sum_j e^(s_j)), -inf without a key.
+ * Scores of a (token, head) that are NaN or overflow to +inf give NaN in both of its results.
  * Values of a row that some token of the request sees have to be finite. */
 typedef struct LatentParams {
   int32_t dtype;
