@@ -120,19 +120,20 @@ def rotation_bound(x, positions, frequencies, dtype, magnitude=1.0):
 def attention_bound(out, spread, reach, dtype, keys, values):
     """Largest error of an attention with products of 16-bit operands accumulated in float32 and P rounded to ``dtype``.
 
-    With u half a step: P = p (1 + d), |d| <= u, applied and summed alike, moves
-    out = sum P v / sum P by at most u / (1 - u) sum w |v - out| <= u (spread + |out|) / (1 - u);
-    a score summed in float32 over blocks of 32 columns, at most 18 of them, is off by at most
-    (18 + 5) 2^-24 reach, its exponent (scale, difference, exp2) by 4 2^-24 (reach + |m|) more, |m| <= reach:
-    64 2^-24 reach covers both, which moves w by twice that; sums of P v over `keys` in float32
-    add (keys / 32 + 8) 2^-24 spread; float16's P below 2^-14 is off by 2^-25, next to a sum of at least 1 or so
-    (the running maximum may lag by 2^8, which only enlarges P); the result rounds once more.
+    With u half a step: P = p (1 + d), |d| <= u, in the products only, the denominator being the sum of the p, moves
+    out = sum P v / sum p by at most u spread; a score summed in float32 over blocks of 32 columns, at most 18 of them, is
+    off by at most (18 + 5) 2^-24 reach, its exponent (scale, difference, exp2) by 4 2^-24 (reach + |m|) more,
+    |m| <= reach: 64 2^-24 reach covers both, which moves w by twice that and out by as much of spread + |out|; sums of P v
+    over `keys` in float32 add (keys / 32 + 8) 2^-24 spread, the sum of the p, a quarter of them one after the other,
+    (keys / 4 + 8) 2^-24 |out|; float16's P below 2^-14 is off by 2^-25 (all of it where it becomes 0), next to a sum of
+    at least 1 (the maximum's own weight, or more where the running maximum lags); the result rounds once more.
     """
     u = torch.finfo(dtype).eps / 2
     score = 2 * 64 * 2.0 ** -24 * reach[..., None]
-    bound = (u / (1 - u) + score) * (spread + out.abs()) * (1 + 1e-2) + (keys / 32 + 8) * 2.0 ** -24 * spread
+    bound = (u * spread + score * (spread + out.abs())) * (1 + 1e-2)
+    bound = bound + 2.0 ** -24 * ((keys / 32 + 8) * spread + (keys / 4 + 8) * out.abs())
     if dtype == torch.float16:
-        bound = bound + 2 * keys * 2.0 ** -25 * values
+        bound = bound + keys * 2.0 ** -25 * values
     return bound * (1 + u) + u * out.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
 
 
