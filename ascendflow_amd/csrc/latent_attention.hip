@@ -15,15 +15,17 @@
 // registers (the accumulator layout of S^T is the operand layout of P^T, up to
 // an order of keys that both sides share), so a chunk costs one barrier.
 //
-// Online softmax in float32, exp2 domain: the running maximum m is raised only
-// when a row's maximum exceeds it by more than LAT_TAU (log2 units), so that O
-// is rescaled rarely; P <= 2^LAT_TAU is rounded to the storage type (a matrix
-// operand has to be), at most half a step of each weight, while O is divided by
-// the sum of the weights before rounding. (The sum of the rounded ones would
-// cancel that error where one key takes all, but costs a conversion and an
-// addition a score: in the expanded form, which the vector units bound, 700
-// instead of 635 us for 8192 causal tokens of 32 heads. A maximum raised at every
-// growth, whose own weight is exactly 1: 665.)
+// Online softmax in float32, exp2 domain: the running maximum m is raised when a
+// row's maximum exceeds it by more than lat_tau (log2 units): 8 with float16, so
+// that O is rescaled rarely, 0 with bfloat16. P <= 2^lat_tau is rounded to the
+// storage type (a matrix operand has to be), at most half a step of each weight,
+// while O is divided by the sum of the weights before rounding. Of a row that one
+// key dominates that key's own rounding is the error: none where it holds the
+// maximum (its weight is 1), up to half a step where the maximum lags, 2^-11 in
+// float16 but 2^-8 in bfloat16. (Raising it at any growth costs 5% of 8192 causal
+// tokens of 32 heads, expanded, 604 -> 633 us, and 0 to 3% of the absorbed calls.
+// The sum of the rounded weights would cancel that error too, but costs a
+// conversion and an addition a score: 700 us.)
 #include <algorithm>
 #include <cmath>
 
@@ -33,7 +35,7 @@
 namespace afa {
 
 constexpr float LAT_LOG2E = 1.4426950408889634f, LAT_LN2 = 0.6931471805599453f;
-constexpr float LAT_TAU = 8.0f;
+template <int DT> __device__ constexpr float lat_tau() { return DT == DT_F16 ? 8.0f : 0.0f; }
 constexpr int EXP_MAX_SPLITS = 64;
 // Cache rows per chunk. Eight waves (one workgroup per CU): 64, two slots; a
 // barrier, a fetch and a reduction per 64 rows instead of 32 and four chains of
@@ -647,7 +649,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
     const float m_new = fmaxf(m_run, max_over_lane_groups(top) * scale_log2);
-    if (__ballot(m_new > m_run + LAT_TAU) != 0ull) {
+    if (__ballot(m_new > m_run + lat_tau<DT>()) != 0ull) {
       const float alpha = fast_exp2(m_run - m_new);
       l_run *= alpha;
 #pragma unroll
@@ -1061,7 +1063,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(Expa
       } else if (f == QT + 1) {
         bool grow = false;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) grow |= m_new[qt] > m_run[qt] + LAT_TAU;
+        for (int qt = 0; qt < QT; ++qt) grow |= m_new[qt] > m_run[qt] + lat_tau<DT>();
         if (__ballot(grow) != 0ull) {
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
