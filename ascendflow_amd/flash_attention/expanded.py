@@ -18,7 +18,7 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, check_tensor,
-                        extents, launch_on, live_strides, pointers_apart, require, signature)
+                        extents, launch_on, live_strides, mark_written, pointers_apart, require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 D, R = 128, 64  # columns of k_nope and v, and of k_rope
@@ -119,6 +119,8 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
         status = launch_on(q.get_device(), call.launch, *pointers, workspace, call.nbytes, call.params)
         if status:
             _native.check(status, "launch_latent_attention_expanded")
+        if not new or softmax_lse is not None:
+            mark_written(None if new else out, softmax_lse)
     return out
 
 

@@ -20,7 +20,7 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, check_apart, check_operands, check_rows, check_tensor, extents, launch_on,
-                        live_strides, pointers_apart, require, signature)
+                        live_strides, mark_written, pointers_apart, require, signature)
 from .rotary import LAYOUTS
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
@@ -123,6 +123,7 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
         status = launch_on(k_cache.get_device(), call.launch, *pointers, call.params)
         if status:
             _native.check(status, "launch_append_paged_kv")
+        mark_written(k_cache, v_cache)
     return k_cache if v is None else (k_cache, v_cache)
 
 

@@ -22,7 +22,7 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, check_tensor,
-                        extents, launch_on, live_strides, pointers_apart, require, signature)
+                        extents, launch_on, live_strides, mark_written, pointers_apart, require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 
@@ -135,6 +135,8 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
         status = launch_on(q.get_device(), call.launch, *pointers, workspace, call.nbytes, call.params)
         if status:
             _native.check(status, "launch_latent_attention")
+        if not new or softmax_lse is not None:
+            mark_written(None if new else out, softmax_lse)
     return out
 
 

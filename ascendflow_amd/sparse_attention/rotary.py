@@ -22,7 +22,7 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, extents,
-                        launch_on, live_strides, pointers_apart, require, signature)
+                        launch_on, live_strides, mark_written, pointers_apart, require, signature)
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
@@ -128,6 +128,8 @@ def _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out):
         status = launch_on(x.get_device(), call.launch, *pointers, call.params)
         if status:
             _native.check(status, "launch_apply_rotary")
+        if not new:
+            mark_written(out)
     return out
 
 
