@@ -12,6 +12,7 @@ import ctypes as ct
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
 
@@ -183,6 +184,25 @@ def launch_on(device_index, launch, *args):
         return launch(raw_stream(device_index), *args)
     with torch.cuda.device(device_index):
         return launch(raw_stream(device_index), *args)
+
+
+def has_tangent(*tensors):
+    """Whether forward-mode differentiation is under way and one of the tensors carries a tangent."""
+    return forward_ad._current_level >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def refuse_tangents(name, *tensors):
+    """For a call without a forward-mode derivative: what it writes would carry no tangent, as if it were constant."""
+    if has_tangent(*tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
+def refuse_forward_mode(name):
+    """``refuse_tangents`` for the body of a custom op, which may see its operands without their tangents."""
+    if forward_ad._current_level >= 0:
+        raise NotImplementedError(f"torch.ops.ascendflow_amd.{name} has no forward-mode derivative and cannot be called "
+                                  "where one is being taken")
 
 
 def mark_written(*tensors):

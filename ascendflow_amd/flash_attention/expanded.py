@@ -18,7 +18,8 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, check_tensor,
-                        extents, launch_on, live_strides, mark_written, pointers_apart, require, signature)
+                        extents, launch_on, live_strides, mark_written, pointers_apart, refuse_forward_mode, refuse_tangents,
+                        require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 D, R = 128, 64  # columns of k_nope and v, and of k_rope
@@ -102,6 +103,7 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
         out = torch.empty((*q.shape[:2], D), dtype=q.dtype, device=q.device)
     tensors = (q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_lse)
     check_operands(NAMES, tensors, optional=("softmax_lse",))
+    refuse_tangents("latent_attention_expanded", *tensors)
     SCALE, CAUSAL = float(SCALE), bool(CAUSAL)
     key = (lib, signature(*tensors), SCALE, CAUSAL)
     call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, SCALE, CAUSAL))
@@ -136,6 +138,7 @@ def latent_attention_expanded_op(
     causal: bool = True,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Framework-facing form of ``latent_attention_expanded``: returns (out, softmax_lse float32 [Tq, H])."""
+    refuse_forward_mode("latent_attention_expanded")
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     out = latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, SCALE=softmax_scale, CAUSAL=causal,
                                     softmax_lse=lse)

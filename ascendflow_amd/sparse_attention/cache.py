@@ -20,7 +20,7 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, check_apart, check_operands, check_rows, check_tensor, extents, launch_on,
-                        live_strides, mark_written, pointers_apart, require, signature)
+                        live_strides, mark_written, pointers_apart, refuse_forward_mode, refuse_tangents, require, signature)
 from .rotary import LAYOUTS
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
@@ -113,6 +113,7 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
     lib = _native.library()
     tensors = (k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, k_cache, v_cache)
     check_operands(NAMES, tensors, _OPTIONAL)
+    refuse_tangents("append_paged_kv", *tensors)
     offset, magnitude = index(offset), float(magnitude)
     key = (lib, signature(*tensors), layout, offset, magnitude)
     call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, layout, offset, magnitude))
@@ -143,5 +144,6 @@ def append_paged_kv_op(
     magnitude: float = 1.0,
 ) -> None:
     """Framework-facing form of ``append_paged_kv``."""
+    refuse_forward_mode("append_paged_kv")
     append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v, v_cache, rope=rope, frequencies=frequencies,
                     layout=layout, offset=offset, magnitude=magnitude)

@@ -22,7 +22,8 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, check_tensor,
-                        extents, launch_on, live_strides, mark_written, pointers_apart, require, signature)
+                        extents, launch_on, live_strides, mark_written, pointers_apart, refuse_forward_mode, refuse_tangents,
+                        require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 
@@ -118,6 +119,7 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     tensors = (q, q_rope, kv_cache, block_table, cu_seqlens_q, seqused_kv, out, softmax_lse)
     check_operands(NAMES, tensors, optional=("q_rope", "softmax_lse"))
+    refuse_tangents("latent_attention", *tensors)
     SCALE, CAUSAL = float(SCALE), bool(CAUSAL)
     key = (lib, signature(*tensors), SCALE, CAUSAL)
     call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, SCALE, CAUSAL))
@@ -152,6 +154,7 @@ def latent_attention_op(
     causal: bool = True,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Framework-facing form of ``latent_attention``: returns (out [T, H, L], softmax_lse float32 [T, H])."""
+    refuse_forward_mode("latent_attention")
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     out = latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, SCALE=softmax_scale, q_rope=q_rope,
                            CAUSAL=causal, softmax_lse=lse)

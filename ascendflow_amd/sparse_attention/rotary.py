@@ -22,7 +22,8 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, extents,
-                        launch_on, live_strides, mark_written, pointers_apart, require, signature)
+                        has_tangent, launch_on, live_strides, mark_written, pointers_apart, refuse_forward_mode, require,
+                        signature)
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
@@ -159,6 +160,7 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, x, positions, frequencies, layout, offset, magnitude, inverse):
         _watch_leaf(ctx)
         ctx.save_for_backward(positions, frequencies)
+        ctx.save_for_forward(positions, frequencies)
         ctx.how = layout, offset, magnitude, inverse
         return _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, None)
 
@@ -173,9 +175,14 @@ class _Rotary(torch.autograd.Function):
             turned = _Rotary.apply(grad, positions, frequencies, layout, offset, magnitude, not inverse)
         return turned, None, None, None, None, None, None
 
+    @staticmethod
+    def jvp(ctx, tangent, *constants):
+        positions, frequencies = ctx.saved_tensors
+        return _Rotary.apply(_dense_rows(tangent), positions, frequencies, *ctx.how)
+
 
 def _dense_rows(grad):
-    """A gradient with contiguous rows (a sum's arrives expanded from one element)."""
+    """A gradient or tangent with contiguous rows (a sum's arrives expanded from one element)."""
     return grad if grad.shape[-1] <= 1 or grad.stride(-1) == 1 else grad.contiguous()
 
 
@@ -191,13 +198,17 @@ def apply_rotary(x, positions, frequencies, *, layout="half", offset=0, magnitud
     of their type, negative ones included; angles are formed in float64.
 
     Without ``out`` the result is a new contiguous tensor and carries its
-    gradient with respect to ``x`` (a captured backward pass of a leaf needs the
+    gradient, or forward-mode tangent, with respect to ``x`` (a captured backward pass of a leaf needs the
     leaf's eager graphs gone, and is refused otherwise); with ``out`` (``x`` itself for a rotation in
     place, otherwise memory apart from it) it is written there, without one.
     Raises ``ValueError`` for shapes, types, devices or overlaps that do not fit.
     """
     offset = index(offset)
-    if out is not None or not (torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad):
+    if has_tangent(x, frequencies, out):
+        require(out is None, "out cannot be given where a tangent is carried")
+        if has_tangent(frequencies):
+            raise NotImplementedError("apply_rotary has no derivative with respect to frequencies")
+    elif out is not None or not (torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad):
         require(out is None or not (torch.is_grad_enabled() and (x.requires_grad or out.requires_grad)),
                 "out cannot be given where a gradient is recorded")
         return _rotate(x, positions, frequencies, layout, offset, float(magnitude), bool(inverse), out)
@@ -214,7 +225,8 @@ def apply_rotary_op(
     magnitude: float = 1.0,
     inverse: bool = False,
 ) -> torch.Tensor:
-    """Framework-facing form of ``apply_rotary``: returns a new contiguous tensor."""
+    """Framework-facing form of ``apply_rotary``: returns a new contiguous tensor; no forward-mode derivative."""
+    refuse_forward_mode("apply_rotary")
     return _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, None)
 
 
