@@ -205,6 +205,20 @@ def refuse_forward_mode(name):
                                   "where one is being taken")
 
 
+class ForwardOnly(torch.autograd.Function):
+    """The result of a call that computes no gradient, for operands that would record one: a backward pass that reaches it
+    raises, where a plain tensor would end it as a constant does."""
+
+    @staticmethod
+    def forward(ctx, name, result, *operands):
+        ctx.name = name
+        return result.detach()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} is forward only: it computes no gradient")
+
+
 def mark_written(*tensors):
     """Counts a new version of each tensor that a launch wrote (None is left out), as an operation of torch in place does:
     a backward pass that saved one of them raises instead of using its new values. (What

@@ -17,9 +17,9 @@ import math
 import torch
 
 from .. import _native
-from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, check_tensor,
-                        extents, launch_on, live_strides, mark_written, pointers_apart, refuse_forward_mode, refuse_tangents,
-                        require, signature)
+from .._tensors import (DTYPES, CheckedCalls, ForwardOnly, check_apart, check_distinct_rows, check_operands,
+                        check_rows, check_tensor, extents, launch_on, live_strides, mark_written, pointers_apart,
+                        refuse_forward_mode, refuse_tangents, require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 D, R = 128, 64  # columns of k_nope and v, and of k_rope
@@ -95,6 +95,9 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
     ``cu_seqlens_q[B]`` are left as they were (uninitialised in a new ``out``). One
     whose scores are NaN or overflow to +inf gets NaN in both.
     Keys and values that some query of a request sees have to be finite.
+
+    Forward only: a backward pass that reaches the result raises; with ``out`` or
+    ``softmax_lse`` the call is refused where a gradient would be recorded.
     """
     lib = _native.library()
     new = out is None
@@ -104,6 +107,9 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
     tensors = (q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_lse)
     check_operands(NAMES, tensors, optional=("softmax_lse",))
     refuse_tangents("latent_attention_expanded", *tensors)
+    graph = torch.is_grad_enabled() and any(
+        [t is not None and t.requires_grad for t in (q, k_nope, k_rope, v, out, softmax_lse)])
+    require(not graph or (new and softmax_lse is None), "out and softmax_lse cannot be given where a gradient is recorded")
     SCALE, CAUSAL = float(SCALE), bool(CAUSAL)
     key = (lib, signature(*tensors), SCALE, CAUSAL)
     call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, SCALE, CAUSAL))
@@ -123,7 +129,7 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
             _native.check(status, "launch_latent_attention_expanded")
         if not new or softmax_lse is not None:
             mark_written(None if new else out, softmax_lse)
-    return out
+    return ForwardOnly.apply("latent_attention_expanded", out, q, k_nope, k_rope, v) if graph else out
 
 
 @torch.library.custom_op("ascendflow_amd::latent_attention_expanded", mutates_args=())

@@ -107,13 +107,16 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
 
     Tokens of no request (at or past ``cu_seqlens_q[B]``), negative positions, positions beyond
     the table and pages outside the cache write nothing. Two new tokens must not
-    name the same row. The call reads no values on the host and can be captured
+    name the same row. Forward only: refused where a gradient would be recorded. The call reads no values on the host and can be captured
     in a graph.
     """
     lib = _native.library()
     tensors = (k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, k_cache, v_cache)
     check_operands(NAMES, tensors, _OPTIONAL)
     refuse_tangents("append_paged_kv", *tensors)
+    if torch.is_grad_enabled():
+        require(not any([t is not None and t.requires_grad for t in (k, rope, v, frequencies, k_cache, v_cache)]),
+                "append_paged_kv records no gradient: call it under torch.no_grad(), or on detached tensors")
     offset, magnitude = index(offset), float(magnitude)
     key = (lib, signature(*tensors), layout, offset, magnitude)
     call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, layout, offset, magnitude))
@@ -143,7 +146,7 @@ def append_paged_kv_op(
     offset: int = 0,
     magnitude: float = 1.0,
 ) -> None:
-    """Framework-facing form of ``append_paged_kv``."""
+    """Framework-facing form of ``append_paged_kv``, without its refusal of gradients: torch takes the rows as constants."""
     refuse_forward_mode("append_paged_kv")
     append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v, v_cache, rope=rope, frequencies=frequencies,
                     layout=layout, offset=offset, magnitude=magnitude)

@@ -21,9 +21,9 @@ from typing import Optional
 import torch
 
 from .. import _native
-from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, check_tensor,
-                        extents, launch_on, live_strides, mark_written, pointers_apart, refuse_forward_mode, refuse_tangents,
-                        require, signature)
+from .._tensors import (DTYPES, CheckedCalls, ForwardOnly, check_apart, check_distinct_rows, check_operands,
+                        check_rows, check_tensor, extents, launch_on, live_strides, mark_written, pointers_apart,
+                        refuse_forward_mode, refuse_tangents, require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 
@@ -111,6 +111,9 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
     whose scores are NaN or overflow to +inf gets NaN in both.
     Rows behind ``seqused_kv`` are never read and pages outside the cache hold no
     keys, but the rows that some token of a request sees have to be finite.
+
+    Forward only: a backward pass that reaches the result raises; with ``out`` or
+    ``softmax_lse`` the call is refused where a gradient would be recorded.
     """
     lib = _native.library()
     new = out is None
@@ -120,6 +123,9 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
     tensors = (q, q_rope, kv_cache, block_table, cu_seqlens_q, seqused_kv, out, softmax_lse)
     check_operands(NAMES, tensors, optional=("q_rope", "softmax_lse"))
     refuse_tangents("latent_attention", *tensors)
+    graph = torch.is_grad_enabled() and any(
+        [t is not None and t.requires_grad for t in (q, q_rope, kv_cache, out, softmax_lse)])
+    require(not graph or (new and softmax_lse is None), "out and softmax_lse cannot be given where a gradient is recorded")
     SCALE, CAUSAL = float(SCALE), bool(CAUSAL)
     key = (lib, signature(*tensors), SCALE, CAUSAL)
     call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, SCALE, CAUSAL))
@@ -139,7 +145,7 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
             _native.check(status, "launch_latent_attention")
         if not new or softmax_lse is not None:
             mark_written(None if new else out, softmax_lse)
-    return out
+    return ForwardOnly.apply("latent_attention", out, q, q_rope, kv_cache) if graph else out
 
 
 @torch.library.custom_op("ascendflow_amd::latent_attention", mutates_args=())

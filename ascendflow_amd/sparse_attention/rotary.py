@@ -153,12 +153,17 @@ def _watch_leaf(ctx):
                            "drop its results before the capture")
 
 
+def _refuse_frequencies(wanted):
+    require(not wanted, "no gradient with respect to frequencies is computed: detach them")
+
+
 class _Rotary(torch.autograd.Function):
     """The rotation as a differentiable map of x: its gradient is the inverse rotation, magnitude kept."""
 
     @staticmethod
     def forward(ctx, x, positions, frequencies, layout, offset, magnitude, inverse):
         _watch_leaf(ctx)
+        _refuse_frequencies(ctx.needs_input_grad[2])
         ctx.save_for_backward(positions, frequencies)
         ctx.save_for_forward(positions, frequencies)
         ctx.how = layout, offset, magnitude, inverse
@@ -199,7 +204,8 @@ def apply_rotary(x, positions, frequencies, *, layout="half", offset=0, magnitud
 
     Without ``out`` the result is a new contiguous tensor and carries its
     gradient, or forward-mode tangent, with respect to ``x`` (a captured backward pass of a leaf needs the
-    leaf's eager graphs gone, and is refused otherwise); with ``out`` (``x`` itself for a rotation in
+    leaf's eager graphs gone, and is refused otherwise; ``frequencies`` that require
+    one are refused too); with ``out`` (``x`` itself for a rotation in
     place, otherwise memory apart from it) it is written there, without one.
     Raises ``ValueError`` for shapes, types, devices or overlaps that do not fit.
     """
@@ -209,6 +215,8 @@ def apply_rotary(x, positions, frequencies, *, layout="half", offset=0, magnitud
         if has_tangent(frequencies):
             raise NotImplementedError("apply_rotary has no derivative with respect to frequencies")
     elif out is not None or not (torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad):
+        if torch.is_grad_enabled() and isinstance(frequencies, torch.Tensor):
+            _refuse_frequencies(frequencies.requires_grad)
         require(out is None or not (torch.is_grad_enabled() and (x.requires_grad or out.requires_grad)),
                 "out cannot be given where a gradient is recorded")
         return _rotate(x, positions, frequencies, layout, offset, float(magnitude), bool(inverse), out)
@@ -238,6 +246,7 @@ def _(x, positions, frequencies, layout="half", offset=0, magnitude=1.0, inverse
 def _op_context(ctx, inputs, output):
     _, positions, frequencies, *how = inputs
     _watch_leaf(ctx)
+    _refuse_frequencies(ctx.needs_input_grad[2])
     ctx.save_for_backward(positions, frequencies)
     ctx.how = how
 

@@ -109,3 +109,68 @@ def test_forward_mode_refusals_of_the_append(device, name):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 entry(**with_tangent(t, name))
         append_paged_kv(**t)
+
+
+def test_gradients_of_the_frequencies_are_refused(device):
+    x, positions, frequencies = rotary(device)
+    learned = frequencies.clone().requires_grad_(True)
+    for leaf in (x, x.clone().requires_grad_(True)):
+        for entry in (apply_rotary, torch.ops.ascendflow_amd.apply_rotary):
+            with pytest.raises(ValueError, match="frequencies"):
+                entry(leaf, positions, learned)
+    with pytest.raises(ValueError, match="frequencies"):
+        apply_rotary(x, positions, learned, out=torch.empty_like(x))
+    with torch.no_grad():
+        assert torch.equal(apply_rotary(x, positions, learned), apply_rotary(x, positions, frequencies))
+
+
+def wanting(tensors, name):
+    return {**tensors, name: tensors[name].clone().requires_grad_(True)}
+
+
+def check_forward_only(run, tensors, name):
+    """``run(tensors, **outputs)``: the plain result, whose backward pass raises; no result is written without a word."""
+    plain = run(tensors)
+    t = wanting(tensors, name)
+    out = run(t)
+    assert torch.equal(out, plain)
+    with pytest.raises(RuntimeError, match="forward only"):
+        (out.sum() + t[name].sum()).backward()
+    for given in (dict(out=torch.empty_like(plain)),
+                  dict(softmax_lse=torch.empty(plain.shape[:2], dtype=torch.float32, device=plain.device))):
+        with pytest.raises(ValueError, match="gradient"):
+            run(t, **given)
+        with torch.no_grad():
+            assert torch.equal(run(t, **given), plain)
+    with torch.inference_mode():
+        assert torch.equal(run(t), plain)
+
+
+@pytest.mark.parametrize("name", ["q", "q_rope", "kv_cache"])
+def test_the_absorbed_form_is_forward_only(device, name):
+    t = paged(device, [1, 2], [40, 70], H=8, page=64)
+    check_forward_only(lambda t, out=None, softmax_lse=None: call(t, 0.1, True, out, softmax_lse), t, name)
+    t = wanting(t, name)
+    out, _ = torch.ops.ascendflow_amd.latent_attention(t["q"], t["q_rope"], t["kv_cache"], t["block_table"], t["cu_seqlens_q"],
+                                                       t["seqused_kv"], 0.1)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("name", ["q", "k_nope", "k_rope", "v"])
+def test_the_expanded_form_is_forward_only(device, name):
+    t = expanded.inputs(device, [5, 3], [40, 30], H=8)
+    check_forward_only(lambda t, **kw: expanded.call(t, **kw), t, name)
+    t = wanting(t, name)
+    out, _ = torch.ops.ascendflow_amd.latent_attention_expanded(t["q"], t["k_nope"], t["k_rope"], t["v"], t["cu_q"], t["cu_k"], 0.1)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("name", ["k", "rope", "v", "frequencies", "k_cache", "v_cache"])
+def test_the_append_records_no_gradient(device, name):
+    t = wanting(append_inputs(device), name)
+    with pytest.raises(ValueError, match="gradient"):
+        append_paged_kv(**t)
+    with torch.no_grad():
+        append_paged_kv(**t)
