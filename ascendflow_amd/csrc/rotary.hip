@@ -58,6 +58,7 @@ __device__ __forceinline__ void store_piece(typename B16<DT>::scalar* p, const P
 constexpr int ROT_MAX_PAIRS = 512, ROT_TOKENS = 8;  // pairs of a row, tokens of a workgroup
 constexpr int ROT_LDS_PAIRS = 1024;                 // pairs of all its tokens
 constexpr int ROT_MAX_D = 16384;                    // columns of a row
+constexpr int ROT_MAX_HKV = 32768;                  // heads of a cache
 
 // Cosine and sine of a pair, magnitude included.
 __device__ __forceinline__ float2 pair_angle(double frequency, int64_t position, float magnitude, bool inverse) {
@@ -181,13 +182,14 @@ struct AppendArgs {
   const double* frequencies;
   int64_t k_t, k_h, rope_t, rope_h, v_t, v_h;
   int32_t T, B, W, PAGE, BLOCKS, HKV, DK, DV, R, offset;
-  int32_t block_tokens;
+  int32_t block_tokens, block_heads;  // of a workgroup
   int32_t rotary_groups, copy_groups, groups;  // pieces per head: rotated, other key columns, all (the values' last)
-  uint32_t groups_m, heads_m;                  // for divide(): by groups, by HKV
+  uint32_t groups_m, heads_m;                  // for divide(): by groups, by block_heads
   float magnitude;
 };
 
-// A workgroup of four waves takes block_tokens new tokens. One wave finds a
+// A workgroup of four waves takes block_tokens new tokens, with all heads but
+// for rows so wide that divide() cannot hold them all. One wave finds a
 // token's place: its request is the number of boundaries cu[1..B] at or below
 // it (64 compared at a time), its position seqused - n + j; token rows below cu[0], at
 // or past cu[B], positions outside the table's width and pages outside the cache have none.
@@ -232,12 +234,13 @@ __global__ __launch_bounds__(256) void append_paged_kv_kernel(AppendArgs a) {
     angles[i] = pair_angle(a.frequencies[i - t * pairs], positions[t], a.magnitude, false);
   }
   __syncthreads();
-  const uint32_t items = (uint32_t)(tokens * a.HKV * a.groups);
+  const int head0 = (int)blockIdx.y * a.block_heads;
+  const uint32_t items = (uint32_t)(tokens * a.block_heads * a.groups);
   for (uint32_t item = threadIdx.x; item < items; item += 256) {
     const uint32_t head_row = divide(item, a.groups_m), t = divide(head_row, a.heads_m);
-    const int g = (int)(item - head_row * (uint32_t)a.groups), h = (int)(head_row - t * (uint32_t)a.HKV);
+    const int g = (int)(item - head_row * (uint32_t)a.groups), h = head0 + (int)(head_row - t * (uint32_t)a.block_heads);
     const int64_t slot = slots[t], token = token0 + t;
-    if (slot < 0) continue;
+    if (slot < 0 || h >= a.HKV) continue;
     const scalar* k = (const scalar*)a.k + token * a.k_t + h * a.k_h;
     scalar* row = (scalar*)a.k_cache + (slot * a.HKV + h) * a.DK;
     if (g < a.rotary_groups) {
@@ -284,7 +287,9 @@ int launch_rotary(const RotaryArgs& a, int layout, int64_t blocks, hipStream_t s
 
 template <int DT, int VEC>
 int launch_append(const AppendArgs& a, int layout, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.T + a.block_tokens - 1) / a.block_tokens)), block(256);
+  const dim3 grid((unsigned)(((int64_t)a.T + a.block_tokens - 1) / a.block_tokens),
+                  (unsigned)((a.HKV + a.block_heads - 1) / a.block_heads));
+  const dim3 block(256);
   if (layout == ROTARY_HALF)
     hipLaunchKernelGGL((append_paged_kv_kernel<DT, VEC, ROTARY_HALF>), grid, block, 0, s, a);
   else
@@ -364,6 +369,7 @@ extern "C" int launch_append_paged_kv(void* stream, const void* k, const void* r
   if (p->dtype != AFA_DTYPE_BF16 && p->dtype != AFA_DTYPE_F16) return AFA_E_DTYPE;
   if (p->T < 0 || p->B <= 0 || p->W <= 0 || p->PAGE <= 0 || p->BLOCKS <= 0 || p->HKV <= 0 || p->DK <= 0 || p->DV < 0)
     return AFA_E_SHAPE;
+  if (p->HKV > ROT_MAX_HKV) return AFA_E_SHAPE;
   if (p->DK > ROT_MAX_D || p->DV > ROT_MAX_D || p->R > 2 * ROT_MAX_PAIRS) return AFA_E_SHAPE;
   if (p->R < 0 || p->R % 2 || p->offset < 0 || p->R > p->DK || p->offset > p->DK - p->R) return AFA_E_SHAPE;
   if (p->layout != ROTARY_HALF && p->layout != ROTARY_INTERLEAVED) return AFA_E_SHAPE;
@@ -406,15 +412,19 @@ extern "C" int launch_append_paged_kv(void* stream, const void* k, const void* r
   a.rotary_groups = R / 2 / vec;
   a.copy_groups = (p->DK - R) / vec;
   a.groups = a.rotary_groups + a.copy_groups + p->DV / vec;
-  // divide() needs the items of a workgroup times groups and heads below 2^32.
-  const int64_t items = (int64_t)p->HKV * a.groups;
-  if (items * std::max<int64_t>(a.groups, p->HKV) > 0x1fffffffll) return AFA_E_SHAPE;
-  // One token a workgroup up to four workgroups per CU, then up to eight.
+  // One token a workgroup up to four workgroups per CU, then up to eight; fewer,
+  // then fewer heads (at most 2^15 groups leave three), until divide() holds
+  // a workgroup's items by groups and its rows by heads.
   int64_t block_tokens = R ? std::min<int64_t>(ROT_TOKENS, ROT_LDS_PAIRS / (R / 2)) : ROT_TOKENS;
-  while (block_tokens > 1 && p->T / block_tokens < 1024) block_tokens /= 2;
+  int64_t heads = p->HKV;
+  const int64_t by_groups = (int64_t)a.groups * a.groups;
+  auto held = [&] { return block_tokens * heads * std::max(by_groups, heads) < (1ll << 32); };
+  while (block_tokens > 1 && (p->T / block_tokens < 1024 || !held())) block_tokens /= 2;
+  while (!held()) heads = (heads + 1) / 2;
   a.block_tokens = (int32_t)block_tokens;
+  a.block_heads = (int32_t)heads;
   a.groups_m = divider(a.groups);
-  a.heads_m = divider(p->HKV);
+  a.heads_m = divider(heads);
   a.magnitude = p->magnitude;
   hipStream_t s = (hipStream_t)stream;
   if (p->dtype == AFA_DTYPE_F16)

@@ -70,7 +70,8 @@ def _check(lib, k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, 
     check_tensor("seqused_kv", seqused_kv, (B,), i32, device)
     if frequencies is not None:
         check_tensor("frequencies", frequencies, (R // 2,), torch.float64, device)
-    require(R <= 1024 and DK <= 16384 and DV <= 16384, "at most 1024 rotated and 16384 columns")
+    require(R <= 1024 and DK <= 16384 and DV <= 16384 and HKV <= 32768,
+            "at most 1024 rotated and 16384 columns, and 32768 heads")
     require(layout in LAYOUTS, 'layout must be "half" or "interleaved"')
     require(R == 0 or 0 <= offset <= DK - R, f"the rotated columns {offset} to {offset + R} must lie inside the row ({DK})")
     require(math.isfinite(magnitude), "magnitude must be finite")
@@ -94,9 +95,9 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
     """Writes new rows ``k`` (and ``v``) into the paged ``k_cache`` (and ``v_cache``); returns the cache or both.
 
     ``k_cache`` [BLOCKS, PAGE, HKV, DK], ``v_cache`` [BLOCKS, PAGE, HKV, DV]:
-    contiguous, bf16 or f16. ``k`` [T, HKV, DK] and ``v`` [T, HKV, DV]: any
-    strides of tokens and heads. ``block_table`` int32 [B, W], ``cu_seqlens_q``
-    int32 [B + 1], ``seqused_kv`` int32 [B]. Token j of the n new ones of request
+    contiguous, bf16 or f16, at most 16384 columns and 32768 heads. ``k`` [T, HKV,
+    DK] and ``v`` [T, HKV, DV]: any strides of tokens and heads. ``block_table``
+    int32 [B, W], ``cu_seqlens_q`` int32 [B + 1], ``seqused_kv`` int32 [B]. Token j of the n new ones of request
     b goes to position ``seqused_kv[b] - n + j``.
 
     With ``frequencies`` (float64 [R / 2], as for ``apply_rotary``) the R columns
@@ -105,10 +106,10 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
     of the row (``offset`` is not read), and ``k`` holds the DK - R others: the
     latent and the rotary key of a token as two tensors.
 
-    Tokens of no request (at or past ``cu_seqlens_q[B]``), negative positions, positions beyond
-    the table and pages outside the cache write nothing. Two new tokens must not
-    name the same row. Forward only: refused where a gradient would be recorded. The call reads no values on the host and can be captured
-    in a graph.
+    Tokens of no request (at or past ``cu_seqlens_q[B]``), negative positions,
+    positions beyond the table and pages outside the cache write nothing. Two new
+    tokens must not name the same row. Forward only: refused where a gradient would
+    be recorded. The call reads no values on the host and can be captured in a graph.
     """
     lib = _native.library()
     tensors = (k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, k_cache, v_cache)

@@ -341,7 +341,7 @@ int launch_apply_rotary(void* stream, const void* x, const void* positions, cons
  * [BLOCKS][PAGE][HKV][DV] (DV = 0: none). Strides in elements, columns
  * contiguous. Tokens at or past cu_seqlens_q[B], positions below 0 or beyond W
  * pages, and pages outside [0, BLOCKS) write nothing. No two new tokens may
- * name the same cache row. R up to 1024, DK and DV up to 16384. */
+ * name the same cache row. R up to 1024, DK and DV up to 16384, HKV up to 32768. */
 typedef struct AppendPagedKvParams {
   int32_t dtype;
   int32_t layout;
