@@ -1171,6 +1171,9 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedArgs a) {
 
 namespace {
 
+// Whether a launch, which counts its threads in 32 bits, can have so many workgroups.
+bool launchable(int64_t workgroups, int threads) { return workgroups <= 0xffffffffll / threads; }
+
 bool rows_fit(const void* p, int64_t a, int64_t b) { return ((uintptr_t)p & 15) == 0 && (a | b) % 8 == 0; }
 
 int check_latent(const LatentParams* p) {
@@ -1228,7 +1231,7 @@ uint64_t latent_bytes(const LatentParams* p, const LatentPlan& plan) {
 
 template <int DT, int L, int R>
 int launch_latent(LatentArgs a, const LatentPlan& plan, void* workspace, hipStream_t s) {
-  if (plan.tiles > 0x7fffffffll) return AFA_E_SHAPE;
+  if (!launchable(plan.tiles, 64 * plan.waves)) return AFA_E_SHAPE;
   if (plan.workers == 0) {
     const dim3 grid((unsigned)plan.tiles);
     if (plan.waves == 8)
@@ -1408,7 +1411,10 @@ uint64_t expanded_bytes(const LatentExpandedParams* p, const ExpandedPlan& plan)
 
 template <int DT>
 int launch_expanded(const ExpandedArgs& a, const ExpandedPlan& plan, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.Tq / plan.rows + a.B) * a.H * plan.splits));
+  const int64_t workgroups = ((int64_t)a.Tq / plan.rows + a.B) * a.H * plan.splits;
+  const int64_t merge = ((int64_t)a.Tq * a.H + 7) / 8;
+  if (!launchable(workgroups, plan.rows == 256 ? 512 : 256) || (plan.splits > 1 && !launchable(merge, 256))) return AFA_E_SHAPE;
+  const dim3 grid((unsigned)workgroups);
   if (plan.splits > 1)
     hipLaunchKernelGGL((expanded_kernel<DT, 4, 1, true>), grid, dim3(256), 0, s, a);
   else if (plan.rows == 256)
@@ -1419,7 +1425,7 @@ int launch_expanded(const ExpandedArgs& a, const ExpandedPlan& plan, hipStream_t
     hipLaunchKernelGGL((expanded_kernel<DT, 4, 1, false>), grid, dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || plan.splits == 1) return (int)e;
-  hipLaunchKernelGGL(expanded_merge_kernel<DT>, dim3((unsigned)(((int64_t)a.Tq * a.H + 7) / 8)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(expanded_merge_kernel<DT>, dim3((unsigned)merge), dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
 

@@ -59,6 +59,9 @@ constexpr int ROT_MAX_PAIRS = 512, ROT_TOKENS = 8;  // pairs of a row, tokens of
 constexpr int ROT_LDS_PAIRS = 1024;                 // pairs of all its tokens
 constexpr int ROT_MAX_D = 16384;                    // columns of a row
 constexpr int ROT_MAX_HKV = 32768;                  // heads of a cache
+// Workgroups of 256 threads along one dimension of a grid, whose threads a launch
+// counts in 32 bits: a call with more of them has further slices.
+constexpr int64_t ROT_SLICE = 1 << 23;
 
 // Cosine and sine of a pair, magnitude included.
 __device__ __forceinline__ float2 pair_angle(double frequency, int64_t position, float magnitude, bool inverse) {
@@ -127,8 +130,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   typedef typename B16<DT>::scalar scalar;
   __shared__ float2 angles[ROT_LDS_PAIRS];
   const int pairs = a.R / 2;
-  const int64_t token0 = (int64_t)(blockIdx.x / (uint32_t)a.head_blocks) * a.block_tokens;
-  const int head0 = (int)(blockIdx.x % (uint32_t)a.head_blocks) * a.block_heads;
+  const uint32_t block = blockIdx.y * (uint32_t)ROT_SLICE + blockIdx.x;
+  const int64_t token0 = (int64_t)(block / (uint32_t)a.head_blocks) * a.block_tokens;
+  const int head0 = (int)(block % (uint32_t)a.head_blocks) * a.block_heads;
+  if (token0 >= a.tokens) return;  // the last slice's end
   const int tokens = (int)min((int64_t)a.block_tokens, a.tokens - token0);
   auto place = [&](int t, int64_t& b, int64_t& s) {
     const int64_t token = token0 + t;
@@ -199,7 +204,8 @@ __global__ __launch_bounds__(256) void append_paged_kv_kernel(AppendArgs a) {
   __shared__ float2 angles[ROT_LDS_PAIRS];
   __shared__ int64_t slots[ROT_TOKENS], positions[ROT_TOKENS];  // cache row, -1: none
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t token0 = (int64_t)blockIdx.x * a.block_tokens;
+  const int64_t token0 = (blockIdx.z * ROT_SLICE + blockIdx.x) * a.block_tokens;
+  if (token0 >= a.T) return;  // the last slice's end
   const int tokens = (int)min((int64_t)a.block_tokens, (int64_t)a.T - token0);
   const int pairs = a.R / 2;
   auto find = [&](int64_t token, int64_t& position) -> int64_t {
@@ -277,7 +283,7 @@ uint32_t divider(int64_t n) { return n == 1 ? 0u : (uint32_t)(((1ull << 32) + n 
 
 template <int DT, int VEC>
 int launch_rotary(const RotaryArgs& a, int layout, int64_t blocks, hipStream_t s) {
-  const dim3 grid((unsigned)blocks), block(256);
+  const dim3 grid((unsigned)std::min(blocks, ROT_SLICE), (unsigned)((blocks + ROT_SLICE - 1) / ROT_SLICE)), block(256);
   if (layout == ROTARY_HALF)
     hipLaunchKernelGGL((rotary_kernel<DT, VEC, ROTARY_HALF>), grid, block, 0, s, a);
   else
@@ -287,8 +293,9 @@ int launch_rotary(const RotaryArgs& a, int layout, int64_t blocks, hipStream_t s
 
 template <int DT, int VEC>
 int launch_append(const AppendArgs& a, int layout, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.T + a.block_tokens - 1) / a.block_tokens),
-                  (unsigned)((a.HKV + a.block_heads - 1) / a.block_heads));
+  const int64_t blocks = ((int64_t)a.T + a.block_tokens - 1) / a.block_tokens;
+  const dim3 grid((unsigned)std::min(blocks, ROT_SLICE), (unsigned)((a.HKV + a.block_heads - 1) / a.block_heads),
+                  (unsigned)((blocks + ROT_SLICE - 1) / ROT_SLICE));
   const dim3 block(256);
   if (layout == ROTARY_HALF)
     hipLaunchKernelGGL((append_paged_kv_kernel<DT, VEC, ROTARY_HALF>), grid, block, 0, s, a);
