@@ -19,6 +19,7 @@
 // heads x 256 columns into pages 11.9 us (22.5 where each thread worked out the
 // cosines of its own 8 pairs), 384 decode tokens of one 576-column row 3.9 (6.1).
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 #include "../../include/ascendflow_amd.h"
@@ -316,6 +317,7 @@ extern "C" int launch_apply_rotary(void* stream, const void* x, const void* posi
   if (p->R < 2 || p->R % 2 || p->offset < 0 || p->offset > p->D - p->R) return AFA_E_SHAPE;
   if ((p->layout != ROTARY_HALF && p->layout != ROTARY_INTERLEAVED) || (p->position_bytes != 4 && p->position_bytes != 8))
     return AFA_E_SHAPE;
+  if (!std::isfinite(p->magnitude)) return AFA_E_SHAPE;
   if (p->B == 0 || p->S == 0) return AFA_OK;
   if (p->B > INT64_MAX / p->S) return AFA_E_SHAPE;
   const bool in_place = x == out;
@@ -380,6 +382,7 @@ extern "C" int launch_append_paged_kv(void* stream, const void* k, const void* r
   if (p->DK > ROT_MAX_D || p->DV > ROT_MAX_D || p->R > 2 * ROT_MAX_PAIRS) return AFA_E_SHAPE;
   if (p->R < 0 || p->R % 2 || p->offset < 0 || p->R > p->DK || p->offset > p->DK - p->R) return AFA_E_SHAPE;
   if (p->layout != ROTARY_HALF && p->layout != ROTARY_INTERLEAVED) return AFA_E_SHAPE;
+  if (!std::isfinite(p->magnitude)) return AFA_E_SHAPE;
   if (rope && (p->R == 0 || p->offset != p->DK - p->R)) return AFA_E_SHAPE;
   if (!block_table || !cu_seqlens_q || !seqused_kv || !k_cache || (p->R > 0 && !frequencies)) return AFA_E_NULL;
   if ((!k && !(rope && p->R == p->DK)) || (p->DV > 0 && (!v || !v_cache))) return AFA_E_NULL;

@@ -74,7 +74,7 @@ def _check(lib, k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, 
             "at most 1024 rotated and 16384 columns, and 32768 heads")
     require(layout in LAYOUTS, 'layout must be "half" or "interleaved"')
     require(R == 0 or 0 <= offset <= DK - R, f"the rotated columns {offset} to {offset + R} must lie inside the row ({DK})")
-    require(math.isfinite(magnitude), "magnitude must be finite")
+    require(math.isfinite(ct.c_float(magnitude).value), "magnitude must be finite, as a float32 too")
     require(B > 0 and W > 0 and BLOCKS > 0 and PAGE > 0 and HKV > 0 and DK > 0,
             "requests, pages, heads and columns must not be empty")
     kt, kh = live_strides(k)[:2]

@@ -96,7 +96,7 @@ def _check(lib, x, positions, frequencies, out, layout, offset, magnitude, inver
     require(R <= 1024, "at most 1024 columns can be rotated")
     require(layout in LAYOUTS, 'layout must be "half" or "interleaved"')
     require(0 <= offset <= D - R, f"the rotated columns {offset} to {offset + R} must lie inside the head ({D})")
-    require(math.isfinite(magnitude), "magnitude must be finite")
+    require(math.isfinite(ct.c_float(magnitude).value), "magnitude must be finite, as a float32 too")
     xs, os = live_strides(x), live_strides(out)
     xs, os = ((0, xs[0], xs[1]), (0, os[0], os[1])) if x.dim() == 3 else ((xs[0], xs[2], xs[1]), (os[0], os[2], os[1]))
     call = _Call()
