@@ -122,7 +122,7 @@ def _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out):
     call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, layout, offset, magnitude, inverse))
     pointers = [t.data_ptr() for t in tensors]
     if not new and not pointers_apart(pointers, call.sizes, (3,)):
-        in_place = pointers[0] == pointers[3] and x.stride() == out.stride()
+        in_place = pointers[0] == pointers[3] and live_strides(x) == live_strides(out)
         check_apart([("x", None if in_place else x, False), ("positions", positions, False),
                      ("frequencies", frequencies, False), ("out", out, True)])
     if x.numel():
