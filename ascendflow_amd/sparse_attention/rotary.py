@@ -114,10 +114,8 @@ def _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out):
     lib = _native.library()
     new = out is None
     if new:
-        require(isinstance(x, torch.Tensor), "x must be a torch.Tensor")
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     tensors = (x, positions, frequencies, out)
-    check_operands(NAMES, tensors)
     key = (lib, signature(*tensors), layout, offset, magnitude, inverse)
     call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, layout, offset, magnitude, inverse))
     pointers = [t.data_ptr() for t in tensors]
@@ -137,14 +135,14 @@ def _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out):
 _EAGER = "ascendflow_amd_eager_graph"
 
 
-def _watch_leaf(ctx):
+def _watch_leaf(ctx, x):
     """Marks the node that takes the gradient of a leaf as part of an eager graph, or, under capture, refuses it if marked.
 
     That node remembers the stream it was made on for as long as some graph holds
     it. A backward pass captured into a HIP graph would record an event on that
     other stream, which breaks the capture and ends the process."""
     node = ctx.next_functions[0][0] if ctx.next_functions else None
-    if node is None or node.next_functions:  # x is no leaf
+    if node is None or node.next_functions or not x.is_cuda:  # x is no leaf, or refused later on
         return
     if not torch.cuda.is_current_stream_capturing():
         node.metadata[_EAGER] = True
@@ -162,7 +160,7 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, positions, frequencies, layout, offset, magnitude, inverse):
-        _watch_leaf(ctx)
+        _watch_leaf(ctx, x)
         _refuse_frequencies(ctx.needs_input_grad[2])
         ctx.save_for_backward(positions, frequencies)
         ctx.save_for_forward(positions, frequencies)
@@ -210,15 +208,16 @@ def apply_rotary(x, positions, frequencies, *, layout="half", offset=0, magnitud
     Raises ``ValueError`` for shapes, types, devices or overlaps that do not fit.
     """
     offset = index(offset)
+    check_operands(NAMES, (x, positions, frequencies, out), optional=("out",))
     if has_tangent(x, frequencies, out):
         require(out is None, "out cannot be given where a tangent is carried")
         if has_tangent(frequencies):
             raise NotImplementedError("apply_rotary has no derivative with respect to frequencies")
-    elif out is not None or not (torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad):
-        if torch.is_grad_enabled() and isinstance(frequencies, torch.Tensor):
+    elif out is not None or not (torch.is_grad_enabled() and x.requires_grad):
+        if torch.is_grad_enabled():
             _refuse_frequencies(frequencies.requires_grad)
-        require(out is None or not (torch.is_grad_enabled() and (x.requires_grad or out.requires_grad)),
-                "out cannot be given where a gradient is recorded")
+            require(out is None or not (x.requires_grad or out.requires_grad),
+                    "out cannot be given where a gradient is recorded")
         return _rotate(x, positions, frequencies, layout, offset, float(magnitude), bool(inverse), out)
     return _Rotary.apply(x, positions, frequencies, layout, offset, float(magnitude), bool(inverse))
 
@@ -244,8 +243,8 @@ def _(x, positions, frequencies, layout="half", offset=0, magnitude=1.0, inverse
 
 
 def _op_context(ctx, inputs, output):
-    _, positions, frequencies, *how = inputs
-    _watch_leaf(ctx)
+    x, positions, frequencies, *how = inputs
+    _watch_leaf(ctx, x)
     _refuse_frequencies(ctx.needs_input_grad[2])
     ctx.save_for_backward(positions, frequencies)
     ctx.how = how
