@@ -53,6 +53,7 @@ EXPORTS = (
     "launch_latent_attention",
     "workspace_size_latent_attention",
     "form_latent_attention",
+    "split_form_latent_attention",
     "launch_latent_attention_expanded",
     "workspace_size_latent_attention_expanded",
     "form_latent_attention_expanded",
@@ -186,6 +187,7 @@ _SIGNATURES = {
     "launch_append_paged_kv": ([_P] * 10 + [ct.POINTER(AppendPagedKvParams)], ct.c_int),
     "launch_latent_attention": ([_P] * 10 + [ct.c_uint64, ct.POINTER(LatentParams)], ct.c_int),
     "workspace_size_latent_attention": ([ct.POINTER(ct.c_uint64), ct.POINTER(LatentParams)], ct.c_int),
+    "split_form_latent_attention": ([ct.POINTER(ct.c_int64), ct.POINTER(LatentParams)], ct.c_int),
     "form_latent_attention": ([ct.POINTER(ct.c_int64), ct.POINTER(LatentParams)], ct.c_int),
     "launch_latent_attention_expanded": ([_P] * 10 + [ct.c_uint64, ct.POINTER(LatentExpandedParams)], ct.c_int),
     "workspace_size_latent_attention_expanded": ([ct.POINTER(ct.c_uint64), ct.POINTER(LatentExpandedParams)], ct.c_int),

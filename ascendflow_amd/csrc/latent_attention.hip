@@ -1222,6 +1222,9 @@ LatentPlan plan_latent(const LatentParams* p) {
   return plan;
 }
 
+// Merge jobs of 16 rows and 16 columns.
+int64_t latent_merge_jobs(const LatentPlan& plan, int L) { return plan.tiles * plan.waves * (L / 16); }
+
 // Workspace of the split form: parts, their maxima and sums, records, the count of tiles.
 int64_t latent_part_rows(const LatentPlan& plan) { return 2ll * plan.workers * 16 * plan.waves; }
 uint64_t latent_bytes(const LatentParams* p, const LatentPlan& plan) {
@@ -1259,7 +1262,7 @@ int launch_latent(LatentArgs a, const LatentPlan& plan, void* workspace, hipStre
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   const int rows = 16 * plan.waves;
-  const int64_t jobs = plan.tiles * plan.waves * (L / 16);  // of 16 rows and 16 columns
+  const int64_t jobs = latent_merge_jobs(plan, L);
   if (jobs <= LAT_FEW_JOBS)
     hipLaunchKernelGGL((latent_merge_kernel<DT, L, 16>), dim3((unsigned)jobs), dim3(1024), 0, s, a, rows);
   else
@@ -1342,6 +1345,17 @@ extern "C" int form_latent_attention(int64_t form[2], const LatentParams* p) {
   const LatentPlan plan = plan_latent(p);
   form[0] = 16 * plan.waves;
   form[1] = plan.workers;
+  return AFA_OK;
+}
+
+extern "C" int split_form_latent_attention(int64_t form[2], const LatentParams* p) {
+  using namespace afa;
+  if (!form) return AFA_E_NULL;
+  const int status = check_latent(p);
+  if (status) return status;
+  const LatentPlan plan = plan_latent(p);
+  form[0] = plan.workers > 0 && plan.stream ? 1 : 0;
+  form[1] = plan.workers == 0 ? 0 : latent_merge_jobs(plan, p->L) <= LAT_FEW_JOBS ? 16 : 1;
   return AFA_OK;
 }
 

@@ -396,6 +396,14 @@ int workspace_size_latent_attention(uint64_t* bytes, const LatentParams* params)
  * workgroup. For tests and profiles. */
 int form_latent_attention(int64_t form[2], const LatentParams* params);
 
+/* The same of a call whose tiles are shared: form[0] 1 for cache loads that stay
+ * out of the caches (0: ordinary), form[1] waves that join one part of a tile, 16
+ * or 1; both 0 for one tile per workgroup. Whether such a call shares keys or whole
+ * tiles follows from the lengths: the 32-bit word behind its parts, at byte
+ * 2 form_latent_attention[1] * form_latent_attention[0] * (L + 2) * 4 of the
+ * workspace, holds the number of tiles afterwards, 0 if they stayed whole. */
+int split_form_latent_attention(int64_t form[2], const LatentParams* params);
+
 /* Latent attention, expanded form, ragged requests: for query i of the nq and
  * key j of the nk of request b, head h
  *   s_j = scale (q[i][h][0:D] . k_nope[j][h] + q[i][h][D:D+R] . k_rope[j]),  out[i][h] = softmax(s) v[:, h],
