@@ -186,10 +186,13 @@ def launch_on(device_index, launch, *args):
         return launch(raw_stream(device_index), *args)
 
 
+def forward_mode() -> bool:
+    """Whether forward-mode differentiation is under way."""
+    return forward_ad._current_level >= 0
+
+
 def has_tangent(*tensors):
-    """Whether forward-mode differentiation is under way and one of the tensors carries a tangent."""
-    return forward_ad._current_level >= 0 and any(
-        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def refuse_tangents(name, *tensors):
@@ -200,7 +203,7 @@ def refuse_tangents(name, *tensors):
 
 def refuse_forward_mode(name):
     """``refuse_tangents`` for the body of a custom op, which may see its operands without their tangents."""
-    if forward_ad._current_level >= 0:
+    if forward_mode():
         raise NotImplementedError(f"torch.ops.ascendflow_amd.{name} has no forward-mode derivative and cannot be called "
                                   "where one is being taken")
 
@@ -219,11 +222,11 @@ class ForwardOnly(torch.autograd.Function):
         raise RuntimeError(f"{ctx.name} is forward only: it computes no gradient")
 
 
-def mark_written(*tensors):
-    """Counts a new version of each tensor that a launch wrote (None is left out), as an operation of torch in place does:
-    a backward pass that saved one of them raises instead of using its new values. (What
-    ``torch.autograd.graph.increment_version`` calls, without its 0.6 us of host time.)"""
-    torch._C._increment_version([t for t in tensors if t is not None])
+# mark_written(tensors) counts a new version of each tensor that a launch wrote, as an
+# operation of torch in place does: a backward pass that saved one of them raises
+# instead of using its new values. (What torch.autograd.graph.increment_version
+# calls, without 0.6 us of host time.)
+mark_written = torch._C._increment_version
 
 
 def check_operands(names, tensors, optional=()):

@@ -18,8 +18,8 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, ForwardOnly, check_apart, check_distinct_rows, check_operands,
-                        check_rows, check_tensor, extents, launch_on, live_strides, mark_written, pointers_apart,
-                        refuse_forward_mode, refuse_tangents, require, signature)
+                        check_rows, check_tensor, extents, forward_mode, launch_on, live_strides, mark_written,
+                        pointers_apart, refuse_forward_mode, refuse_tangents, require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 D, R = 128, 64  # columns of k_nope and v, and of k_rope
@@ -106,9 +106,11 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
         out = torch.empty((*q.shape[:2], D), dtype=q.dtype, device=q.device)
     tensors = (q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, out, softmax_lse)
     check_operands(NAMES, tensors, optional=("softmax_lse",))
-    refuse_tangents("latent_attention_expanded", *tensors)
-    graph = torch.is_grad_enabled() and any(
-        [t is not None and t.requires_grad for t in (q, k_nope, k_rope, v, out, softmax_lse)])
+    if forward_mode():
+        refuse_tangents("latent_attention_expanded", *tensors)
+    graph = torch.is_grad_enabled() and (
+        q.requires_grad or k_nope.requires_grad or k_rope.requires_grad or v.requires_grad
+        or out.requires_grad or (softmax_lse is not None and softmax_lse.requires_grad))
     require(not graph or (new and softmax_lse is None), "out and softmax_lse cannot be given where a gradient is recorded")
     SCALE, CAUSAL = float(SCALE), bool(CAUSAL)
     key = (lib, signature(*tensors), SCALE, CAUSAL)
@@ -128,7 +130,7 @@ def latent_attention_expanded(q, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, 
         if status:
             _native.check(status, "launch_latent_attention_expanded")
         if not new or softmax_lse is not None:
-            mark_written(None if new else out, softmax_lse)
+            mark_written([t for t in (None if new else out, softmax_lse) if t is not None])
     return ForwardOnly.apply("latent_attention_expanded", out, q, k_nope, k_rope, v) if graph else out
 
 

@@ -19,8 +19,9 @@ from typing import Optional
 import torch
 
 from .. import _native
-from .._tensors import (DTYPES, CheckedCalls, check_apart, check_operands, check_rows, check_tensor, extents, launch_on,
-                        live_strides, mark_written, pointers_apart, refuse_forward_mode, refuse_tangents, require, signature)
+from .._tensors import (DTYPES, CheckedCalls, check_apart, check_operands, check_rows, check_tensor, extents,
+                        forward_mode, launch_on, live_strides, mark_written, pointers_apart, refuse_forward_mode,
+                        refuse_tangents, require, signature)
 from .rotary import LAYOUTS
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
@@ -114,10 +115,13 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
     lib = _native.library()
     tensors = (k, rope, v, block_table, cu_seqlens_q, seqused_kv, frequencies, k_cache, v_cache)
     check_operands(NAMES, tensors, _OPTIONAL)
-    refuse_tangents("append_paged_kv", *tensors)
-    if torch.is_grad_enabled():
-        require(not any([t is not None and t.requires_grad for t in (k, rope, v, frequencies, k_cache, v_cache)]),
-                "append_paged_kv records no gradient: call it under torch.no_grad(), or on detached tensors")
+    if forward_mode():
+        refuse_tangents("append_paged_kv", *tensors)
+    if torch.is_grad_enabled() and (
+            k.requires_grad or k_cache.requires_grad or (rope is not None and rope.requires_grad)
+            or (frequencies is not None and frequencies.requires_grad)
+            or (v is not None and v.requires_grad) or (v_cache is not None and v_cache.requires_grad)):
+        raise ValueError("append_paged_kv records no gradient: call it under torch.no_grad(), or on detached tensors")
     offset, magnitude = index(offset), float(magnitude)
     key = (lib, signature(*tensors), layout, offset, magnitude)
     call = _calls.get(key) or _calls.keep(key, _check(lib, *tensors, layout, offset, magnitude))
@@ -128,7 +132,7 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
         status = launch_on(k_cache.get_device(), call.launch, *pointers, call.params)
         if status:
             _native.check(status, "launch_append_paged_kv")
-        mark_written(k_cache, v_cache)
+        mark_written([k_cache] if v is None else [k_cache, v_cache])
     return k_cache if v is None else (k_cache, v_cache)
 
 

@@ -22,8 +22,8 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, ForwardOnly, check_apart, check_distinct_rows, check_operands,
-                        check_rows, check_tensor, extents, launch_on, live_strides, mark_written, pointers_apart,
-                        refuse_forward_mode, refuse_tangents, require, signature)
+                        check_rows, check_tensor, extents, forward_mode, launch_on, live_strides, mark_written,
+                        pointers_apart, refuse_forward_mode, refuse_tangents, require, signature)
 
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
 
@@ -122,9 +122,11 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     tensors = (q, q_rope, kv_cache, block_table, cu_seqlens_q, seqused_kv, out, softmax_lse)
     check_operands(NAMES, tensors, optional=("q_rope", "softmax_lse"))
-    refuse_tangents("latent_attention", *tensors)
-    graph = torch.is_grad_enabled() and any(
-        [t is not None and t.requires_grad for t in (q, q_rope, kv_cache, out, softmax_lse)])
+    if forward_mode():
+        refuse_tangents("latent_attention", *tensors)
+    graph = torch.is_grad_enabled() and (
+        q.requires_grad or kv_cache.requires_grad or (q_rope is not None and q_rope.requires_grad)
+        or out.requires_grad or (softmax_lse is not None and softmax_lse.requires_grad))
     require(not graph or (new and softmax_lse is None), "out and softmax_lse cannot be given where a gradient is recorded")
     SCALE, CAUSAL = float(SCALE), bool(CAUSAL)
     key = (lib, signature(*tensors), SCALE, CAUSAL)
@@ -144,7 +146,7 @@ def latent_attention(q, kv_cache, block_table, cu_seqlens_q, seqused_kv, *, SCAL
         if status:
             _native.check(status, "launch_latent_attention")
         if not new or softmax_lse is not None:
-            mark_written(None if new else out, softmax_lse)
+            mark_written([t for t in (None if new else out, softmax_lse) if t is not None])
     return ForwardOnly.apply("latent_attention", out, q, q_rope, kv_cache) if graph else out
 
 

@@ -22,8 +22,8 @@ import torch
 
 from .. import _native
 from .._tensors import (DTYPES, CheckedCalls, check_apart, check_distinct_rows, check_operands, check_rows, extents,
-                        has_tangent, launch_on, live_strides, mark_written, pointers_apart, refuse_forward_mode, require,
-                        signature)
+                        forward_mode, has_tangent, launch_on, live_strides, mark_written, pointers_apart,
+                        refuse_forward_mode, require, signature)
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 _STORAGE = {dt: name for name, dt in DTYPES.items()}
@@ -128,7 +128,7 @@ def _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, out):
         if status:
             _native.check(status, "launch_apply_rotary")
         if not new:
-            mark_written(out)
+            mark_written([out])
     return out
 
 
@@ -209,7 +209,7 @@ def apply_rotary(x, positions, frequencies, *, layout="half", offset=0, magnitud
     """
     offset = index(offset)
     check_operands(NAMES, (x, positions, frequencies, out), optional=("out",))
-    if has_tangent(x, frequencies, out):
+    if forward_mode() and has_tangent(x, frequencies, out):
         require(out is None, "out cannot be given where a tangent is carried")
         if has_tangent(frequencies):
             raise NotImplementedError("apply_rotary has no derivative with respect to frequencies")
