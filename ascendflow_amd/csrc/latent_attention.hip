@@ -40,7 +40,7 @@ constexpr int EXP_MAX_SPLITS = 64;
 // Cache rows per chunk. Eight waves (one workgroup per CU): 64, two slots; a
 // barrier, a fetch and a reduction per 64 rows instead of 32 and four chains of
 // dependent matrix instructions instead of two (128 heads, 4 chunks of 512 tokens
-// behind 8K: 4317 -> 3660 us). Four waves: 32, two slots in each of the CU's two
+// behind 8K: 4317 -> 3865 us when it was taken). Four waves: 32, two slots in each of the CU's two
 // workgroups.
 template <int NW> __host__ __device__ constexpr int lat_keys() { return NW == 8 ? 64 : 32; }
 
@@ -361,8 +361,8 @@ __device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker,
 
 // STREAM: non-temporal loads, for requests of one tile each (nothing is read
 // twice) over a cache too large to stay in the 256 MiB Infinity Cache between
-// calls (64 requests of 32K with 128 heads 633 -> 617 us, 32 with 16 heads 223 -> 204;
-// 64 of 2K with 16 heads, 150 MB, 44.7 -> 44.9).
+// calls (64 requests of 32K with 128 heads 627 -> 616 us, 32 with 16 heads 222 -> 200;
+// 64 of 2K with 16 heads, 150 MB, 43.6 -> 43.9).
 template <int DT, int L, int R, int NW, bool SPLIT, bool STREAM>
 __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(LatentArgs a) {
   typedef typename B16<DT>::scalar scalar;
@@ -1191,18 +1191,19 @@ int check_latent(const LatentParams* p) {
 constexpr int LAT_CUS = 256;
 constexpr int64_t LAT_STREAM_BYTES = 128ll << 20;
 // Merge jobs of 16 waves each up to here, of one wave above: one request of 4K rows
-// (256 jobs) 23 and 27 us, of 64K rows 46 and 144; 16 of 4K rows with 16 heads (2560)
-// 31.5 and 30.1, 8 x 4 tokens of 64 heads (6144) 78 and 45.
+// (256 jobs) 23.5 and 27.7 us, of 64K rows 45 and 144; 16 of 4K rows with 16 heads (2560)
+// 31.8 and 30.5, 8 x 4 tokens of 64 heads over 4K rows (6144) 78 and 47.
 constexpr int64_t LAT_FEW_JOBS = 2048;
 
 // Form of a call: waves (of 16 rows each) of a tile, 8 where a request has more
-// than 64 rows on average, else 4 (64 decode requests of 8000 rows, 128 heads 179 us
-// with 8, 195 with 4; 4 chunks of 512 behind them 3597 and 3818; one of 4096 rows
-// 31.0 and 30.0); and workgroups of the split form, one per CU or two, 0 for the
+// than 64 rows on average, else 4 (64 decode requests of 8000 rows, 128 heads 170 us
+// with 8, 195 with 4; 4 chunks of 512 behind 8K 4079 and 4403; one of 4096 rows
+// 30.5 and 30.8); and workgroups of the split form, one per CU or two, 0 for the
 // form of one tile per workgroup: where the tiles (at most rows / tile + B of
 // them) would fill the GPU four times over anyway, or a single request's fill 85%
-// of their rounds (128 heads behind 8000 rows: 230 tokens 459 us directly, 504
-// split; 400 tokens 869 and 848; 500 tokens 907 and 1032).
+// of their rounds (128 heads behind 8000 rows: 230 tokens 460 us directly, 461
+// split; 500 tokens 971 and 989; 400 tokens, whose second round is half empty, 890
+// and 856; 1000 tokens with no context 180 and 186).
 struct LatentPlan {
   int waves;
   int workers;
@@ -1381,12 +1382,12 @@ int check_expanded(const LatentExpandedParams* p) {
 // request lengths (the launcher reads no device memory). A tile's 64-key chunk
 // costs ALONE where it has its CU to itself and FULL with the CU's workgroups at
 // work (one of 256 rows, two of 128 or 64); a round of workgroups START. Measured
-// at 256 / 128 / 64 rows: 1 x 8192 causal, 32 heads 639 / 653 / 845 us; 1 x 1500,
-// 128 heads 133 / 124 / 151; 5 x 235..470 behind up to 2000, 16 heads 67 / 59 / 49;
-// 1 x 2048, 16 heads 70 / 54 / 47. Split keys add a launch and their float32 parts
+// at 256 / 128 / 64 rows, bfloat16: 1 x 8192 causal, 32 heads 648 / 666 / 854 us; 1 x 1500,
+// 128 heads 132 / 127 / 159; 5 x 235..470 behind up to 2000, 16 heads 74 / 56 / 47;
+// 1 x 2048, 16 heads 75 / 56 / 46. Split keys add a launch and their float32 parts
 // written and read at 3 TB/s: 64 rows in 1 / 2 / 4 / 8 parts, 8 x 20 behind 3000, 8 heads
-// 54 / 37 / 27 / 29; 1 x 500 behind 4000, 32 heads 76 / 69 / 76 / 96; one query of 8192
-// keys, 16 heads 136 / 78 / 43 / 27.
+// 55 / 35 / 26 / 28; 1 x 500 behind 4000, 32 heads 82 / 67 / 79 / 101; one query of 8192
+// keys, 16 heads 133 / 77 / 42 / 26.5 (22.5 in 16).
 ExpandedPlan plan_expanded(const LatentExpandedParams* p) {
   constexpr int FORMS = 3, ROWS[FORMS] = {256, 128, 64}, SLOTS[FORMS] = {256, 512, 512};
   constexpr double ALONE[FORMS] = {2.0, 1.5, 1.2}, FULL[FORMS] = {2.85, 2.9, 1.65}, START[FORMS] = {12.0, 11.0, 7.5};

@@ -163,7 +163,8 @@ class _Rotary(torch.autograd.Function):
         _watch_leaf(ctx, x)
         _refuse_frequencies(ctx.needs_input_grad[2])
         ctx.save_for_backward(positions, frequencies)
-        ctx.save_for_forward(positions, frequencies)
+        if forward_mode():
+            ctx.save_for_forward(positions, frequencies)
         ctx.how = layout, offset, magnitude, inverse
         return _rotate(x, positions, frequencies, layout, offset, magnitude, inverse, None)
 
