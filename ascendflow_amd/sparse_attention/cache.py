@@ -98,8 +98,8 @@ def append_paged_kv(k, k_cache, block_table, cu_seqlens_q, seqused_kv, v=None, v
     ``k_cache`` [BLOCKS, PAGE, HKV, DK], ``v_cache`` [BLOCKS, PAGE, HKV, DV]:
     contiguous, bf16 or f16, at most 16384 columns and 32768 heads. ``k`` [T, HKV,
     DK] and ``v`` [T, HKV, DV]: any strides of tokens and heads. ``block_table``
-    int32 [B, W], ``cu_seqlens_q`` int32 [B + 1], ``seqused_kv`` int32 [B]. Token j of the n new ones of request
-    b goes to position ``seqused_kv[b] - n + j``.
+    int32 [B, W], ``cu_seqlens_q`` int32 [B + 1], ``seqused_kv`` int32 [B]. Token j
+    of the n new ones of request b goes to position ``seqused_kv[b] - n + j``.
 
     With ``frequencies`` (float64 [R / 2], as for ``apply_rotary``) the R columns
     from ``offset`` on of every key row are rotated by that position. With

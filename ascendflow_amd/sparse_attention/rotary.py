@@ -202,10 +202,11 @@ def apply_rotary(x, positions, frequencies, *, layout="half", offset=0, magnitud
     of their type, negative ones included; angles are formed in float64.
 
     Without ``out`` the result is a new contiguous tensor and carries its
-    gradient, or forward-mode tangent, with respect to ``x`` (a captured backward pass of a leaf needs the
-    leaf's eager graphs gone, and is refused otherwise; ``frequencies`` that require
-    one are refused too); with ``out`` (``x`` itself for a rotation in
-    place, otherwise memory apart from it) it is written there, without one.
+    gradient, or forward-mode tangent, with respect to ``x`` (a captured backward
+    pass of a leaf needs the leaf's eager graphs gone, and is refused otherwise;
+    ``frequencies`` that require a gradient are refused too); with ``out`` (``x``
+    itself for a rotation in place, otherwise memory apart from it) it is written
+    there, without one.
     Raises ``ValueError`` for shapes, types, devices or overlaps that do not fit.
     """
     offset = index(offset)
