@@ -29,12 +29,11 @@
 #include <algorithm>
 #include <cmath>
 
-#include "common.h"
+#include "shares.h"
 #include "../../include/ascendflow_amd.h"
 
 namespace afa {
 
-constexpr float LAT_LOG2E = 1.4426950408889634f, LAT_LN2 = 0.6931471805599453f;
 template <int DT> __device__ constexpr float lat_tau() { return DT == DT_F16 ? 8.0f : 0.0f; }
 constexpr int EXP_MAX_SPLITS = 64;
 // Cache rows per chunk. Eight waves (one workgroup per CU): 64, two slots; a
@@ -60,304 +59,20 @@ struct LatentArgs {
   int32_t workers;
   float* partial_o;         // [2 * workers][rows of a tile / 16][L / 16][64][4], not normalised, as a wave holds it
   float* partial_ml;        // [2 * workers][rows of a tile][2]: running maximum (log2), sum of weights
-  struct LatentRecord* records;  // [tiles]
+  TileRecord* records;  // [tiles]
   uint32_t* tile_count;
   uint32_t tiles;           // the most that monotone cu_seqlens_q can give
 };
 
-// A tile of the split form as its merge needs it: its first row is row `row` of
-// the packed rows of the request that starts at token `start`; workgroups
-// first .. last hold parts of it (first == last: the tile is whole and written).
-struct LatentRecord {
-  int32_t start, row, rows;
-  int32_t first, last;
+// The split form of the absorbed attention: a tile counts its chunks and 64 rows'
+// worth for its start and end, a workgroup takes 128 rows' worth at least.
+template <int NW> struct LatentForm {
+  static constexpr int ROWS = 16 * NW, KEYS = lat_keys<NW>(), THREADS = 64 * NW;
+  static constexpr uint32_t START = 64 / KEYS, LEAST = 128 / KEYS;
+  static constexpr float JOIN = NW == 8 ? 5.0f : 10.0f;
 };
+template <int NW> using LatentSpan = TileSpan<LatentForm<NW>, LatentArgs>;
 
-// Split form: the chunks of all tiles, in order, are one sequence that the
-// workgroups share evenly, so that few or unequal requests fill the GPU and end
-// together. A tile counts its chunks and 64 rows' worth for its start and end.
-// Causal tiles of a request have unequal numbers of them: tiles i and n - 1 - i
-// follow each other (the longer first) and count, together, what the first and
-// the last tile do, so that any place in the sequence is found by a division.
-// A workgroup takes at most one tile's end, whole tiles and one tile's
-// beginning; parts go to the workspace (slot 2 w the end, 2 w + 1 the beginning)
-// as float32 and latent_merge_kernel combines them in order. Everything is
-// computed on the device from cu_seqlens_q and seqused_kv, alike in every workgroup.
-template <int NW> __host__ __device__ constexpr uint32_t lat_start() { return 64 / lat_keys<NW>(); }
-template <int NW> __host__ __device__ constexpr uint32_t lat_least() { return 128 / lat_keys<NW>(); }  // least of a workgroup
-
-// A row's ln(sum of e^scores) from its maximum m (log2) and its sum of weights:
-// -inf for a sum of nothing. A sum that is not a number (scores that are none, or
-// overflow to +inf) stays one, beside an output that is none either; it is told by its
-// bits, since device code is built without NaN semantics of comparisons.
-__device__ __forceinline__ float row_lse(float m, float total) {
-  const uint32_t bits = __float_as_uint(total);
-  uint32_t lse = __float_as_uint((m + __log2f(total)) * LAT_LN2);
-  lse = (bits & 0x7fffffffu) > 0x7f800000u ? 0x7fc00000u : lse;
-  return __uint_as_float(bits == 0u ? 0xff800000u : lse);
-}
-
-// Metadata in the constant address space, so that uniform reads are scalar loads,
-// whose values stay out of the vector registers and the vector load counter.
-typedef const __attribute__((address_space(4))) int32_t* const_ints;
-__device__ __forceinline__ const_ints constant(const int32_t* p) { return (const_ints)(uintptr_t)p; }
-
-// New tokens of request b: cu[b] .. cu[b + 1], held inside [0, T).
-__device__ __forceinline__ void request_tokens(const_ints cu, int b, int T, int& start, int& count) {
-  start = min(max(cu[b], 0), T);
-  count = max(min(cu[b + 1], T) - start, 0);
-}
-
-// Cache rows of request b that its table holds, and those ahead of its first new
-// token (fewer than none where it has more tokens than rows). The tokens' places
-// and so the causal limit go by the length itself, which may pass the table:
-// token t sees rows up to ahead + t of the `used`.
-__device__ __forceinline__ void request_rows(const LatentArgs& a, int b, int start, int& used, int& ahead) {
-  const int length = max(constant(a.used)[b], 0);
-  used = (int)min((int64_t)length, (int64_t)a.W << a.page_shift);
-  ahead = length - (max(constant(a.cu)[b + 1], start) - start);
-}
-
-// The request and the tile inside it of tile `index` in the order of requests
-// (tiles_of(tokens) each); false, for the whole workgroup, if there are fewer.
-template <int THREADS, typename F>
-__device__ __forceinline__ bool find_tile(const_ints cu, int B, int T, uint32_t index, F&& tiles_of, int& request,
-                                          uint32_t& tile, uint32_t& tiles, uint32_t* words) {
-  uint32_t* const wave_total = words;                // LDS, THREADS / 64 + 3 words
-  uint32_t* const found = words + THREADS / 64;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  uint32_t before = 0;
-  for (int base = 0; base < B; base += THREADS) {
-    const int b = base + tid;
-    int start = 0, count = 0;
-    if (b < B) request_tokens(cu, b, T, start, count);
-    const uint32_t mine = b < B ? tiles_of(count) : 0u;
-    const uint32_t upto = (uint32_t)wave_inclusive_scan((int)mine);
-    if (lane == 63) wave_total[wave] = upto;
-    __syncthreads();
-    uint32_t first = before, all = before;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-      if (w < wave) first += wave_total[w];
-      all += wave_total[w];
-    }
-    const uint32_t begin = first + upto - mine;
-    if (index >= begin && index < begin + mine) {
-      found[0] = (uint32_t)b;
-      found[1] = index - begin;
-      found[2] = mine;
-    }
-    __syncthreads();
-    if (index < all) {
-      request = __builtin_amdgcn_readfirstlane((int)found[0]);
-      tile = (uint32_t)__builtin_amdgcn_readfirstlane((int)found[1]);
-      tiles = (uint32_t)__builtin_amdgcn_readfirstlane((int)found[2]);
-      return true;
-    }
-    before = all;
-  }
-  return false;
-}
-
-// The part of the split form's sequence that a request takes.
-template <int NW> struct LatentSpan {
-  static constexpr uint32_t ROWS = 16 * NW, START = lat_start<NW>();
-  int H, used, ahead, count, causal;
-  uint32_t tiles;
-  uint32_t pair, middle;  // what two paired tiles count, and the one left over
-  __device__ __forceinline__ uint32_t chunks(uint32_t tile) const {
-    const uint32_t last = min((tile + 1) * ROWS, (uint32_t)(count * H)) - 1;
-    const int seen = causal ? min(max(ahead + (int)(last / (uint32_t)H) + 1, 0), used) : used;
-    return ((uint32_t)seen + lat_keys<NW>() - 1) / lat_keys<NW>();
-  }
-  __device__ __forceinline__ LatentSpan(const LatentArgs& a, int b) : H((int)opaque_uniform((uint32_t)a.H)), causal(a.causal) {
-    int start;
-    request_tokens(constant(a.cu), b, a.T, start, count);
-    request_rows(a, b, start, used, ahead);
-    tiles = ((uint32_t)(count * H) + ROWS - 1) / ROWS;
-    const uint32_t most = ((uint32_t)used + lat_keys<NW>() - 1) / lat_keys<NW>() + START;
-    pair = 2 * most;
-    middle = most;
-    if (causal && tiles > 1) {
-      pair = most + chunks(0) + START;
-      middle = chunks(tiles / 2) + START;
-    }
-  }
-  __device__ __forceinline__ uint32_t longest() const {
-    return tiles == 0 ? 0u : causal && tiles > 1 ? pair - chunks(0) - START : middle;
-  }
-  __device__ __forceinline__ uint64_t weight() const { return (uint64_t)(tiles / 2) * pair + (tiles % 2 ? middle : 0u); }
-  // The tile at place `at` of the request's, and what it counts.
-  __device__ __forceinline__ uint32_t tile(uint32_t at) const { return at % 2 || at + 1 == tiles ? at / 2 : tiles - 1 - at / 2; }
-  __device__ __forceinline__ uint32_t longer(uint32_t p) const {
-    return causal ? min(chunks(tiles - 1 - p) + START, pair - 1) : pair / 2;
-  }
-  __device__ __forceinline__ uint32_t counts(uint32_t at) const {
-    if (at + 1 == tiles && tiles % 2) return middle;
-    return at % 2 ? pair - longer(at / 2) : longer(at / 2);
-  }
-};
-
-__device__ __forceinline__ uint64_t inclusive_scan64(uint64_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t other = __shfl_up((unsigned long long)v, d);
-    if (lane >= d) v += other;
-  }
-  return v;
-}
-
-// Maximum of the wave, in lane 63.
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-  auto with = [&](uint32_t other) { v = max(v, other); };
-  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));  // row_shr:1
-  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));  // row_shr:2
-  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));  // row_shr:4
-  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));  // row_shr:8
-  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));  // row_bcast:15
-  with((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));  // row_bcast:31
-  return v;
-}
-
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ uint64_t uniform64(uint64_t v) {
-  return (uint64_t)(uint32_t)uniform((int)(uint32_t)v) | ((uint64_t)(uint32_t)uniform((int)(uint32_t)(v >> 32)) << 32);
-}
-
-// Sharing tiles costs the parts' bytes and the join, LAT_JOIN chunks' worth, and
-// chunks take longer the more of the GPU is at work (3.2 us with half its CUs, 4.3
-// with all: 128 rows of 512 columns are bound by power and by the L2s). Tiles are
-// therefore kept whole where the longest of them, or the rounds that they need,
-// take LAT_APART times as many chunks as an even share and the join.
-constexpr float LAT_APART = 0.875f;
-template <int NW> constexpr float LAT_JOIN = NW == 8 ? 5.0f : 10.0f;
-
-// Where a workgroup of the split form begins.
-struct LatentShare {
-  uint64_t begin, end;       // of the sequence
-  uint64_t total;
-  int32_t workers;           // that have a share
-  bool apart;                // tiles are not shared: a tile is whoever's its beginning is
-  int32_t request;
-  uint32_t place, offset;    // of the tile among the request's, inside the tile
-  uint32_t tiles_before;     // of earlier requests
-};
-
-template <int NW>
-__device__ __forceinline__ bool find_share(const LatentArgs& a, uint32_t worker, LatentShare& share) {
-  constexpr int THREADS = NW * 64;
-  __shared__ uint64_t wave_weight[THREADS / 64];
-  __shared__ uint32_t wave_tiles[THREADS / 64], wave_longest[THREADS / 64];
-  __shared__ uint32_t found[4];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int per = (a.B + THREADS - 1) / THREADS;  // consecutive requests of a thread
-  uint64_t weight = 0;
-  uint32_t tiles = 0, longest = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i;
-    if (b >= a.B) break;
-    const LatentSpan<NW> span(a, b);
-    weight += span.weight();
-    tiles += span.tiles;
-    longest = max(longest, span.longest());
-  }
-  const uint64_t upto = inclusive_scan64(weight, lane);
-  const uint32_t tiles_upto = (uint32_t)wave_inclusive_scan((int)tiles);
-  longest = wave_max(longest);
-  if (lane == 63) {
-    wave_weight[wave] = upto;
-    wave_tiles[wave] = tiles_upto;
-    wave_longest[wave] = longest;
-  }
-  __syncthreads();
-  uint64_t before = upto - weight, total = 0;
-  uint32_t tiles_before = tiles_upto - tiles, all = 0, most_chunks = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    if (w < wave) {
-      before += wave_weight[w];
-      tiles_before += wave_tiles[w];
-    }
-    total += wave_weight[w];
-    all += wave_tiles[w];
-    most_chunks = max(most_chunks, wave_longest[w]);
-  }
-  total = uniform64(total);
-  if (total == 0) {
-    if (worker == 0 && tid == 0) *a.tile_count = 0;
-    return false;
-  }
-  const uint64_t most = total / lat_least<NW>();
-  share.workers = most < 1 ? 1 : (most < (uint64_t)a.workers ? (int)most : a.workers);
-  share.workers = uniform(share.workers);
-  all = (uint32_t)uniform((int)all);
-  longest = (uint32_t)uniform((int)most_chunks);
-  const float each = (float)total / (float)share.workers;
-  const float whole = (float)((all + (uint32_t)share.workers - 1) / (uint32_t)share.workers) * ((float)total / (float)all);
-  share.apart = __ballot(LAT_APART * fmaxf((float)longest, whole) <= each + LAT_JOIN<NW>) != 0;
-  const bool one = share.apart && all <= (uint32_t)a.workers;  // a tile each, spread over the XCDs
-  worker = (uint32_t)uniform((int)(one ? blockIdx.x : worker));
-  if (worker >= (one ? all : (uint32_t)share.workers)) return false;
-  if (worker == 0 && tid == 0) *a.tile_count = share.apart ? 0u : all;
-  share.total = total;
-  if (total < (1u << 22)) {  // 32-bit products with at most 512 workers: a 64-bit division costs microseconds
-    share.begin = (uint32_t)uniform((int)((uint32_t)total * worker / (uint32_t)share.workers));
-    share.end = (uint32_t)uniform((int)((uint32_t)total * (worker + 1) / (uint32_t)share.workers));
-  } else {
-    share.begin = uniform64(total * worker / (uint32_t)share.workers);
-    share.end = uniform64(total * (worker + 1) / (uint32_t)share.workers);
-  }
-  if (one) {
-    if (worker >= tiles_before && worker < tiles_before + tiles) {
-      uint32_t place = worker - tiles_before;
-      for (int i = 0; i < per; ++i) {
-        const int b = tid * per + i;
-        const uint32_t mine = LatentSpan<NW>(a, b).tiles;
-        if (place < mine) {
-          found[0] = (uint32_t)b;
-          found[1] = place;
-          found[2] = 0;
-          found[3] = 0;
-          break;
-        }
-        place -= mine;
-      }
-    }
-  } else if (share.begin >= before && share.begin < before + weight) {
-    uint64_t at = before;
-    uint32_t done = tiles_before;
-    for (int i = 0; i < per; ++i) {
-      const int b = tid * per + i;
-      const LatentSpan<NW> span(a, b);
-      if (share.begin < at + span.weight()) {
-        const uint64_t inside = share.begin - at;
-        const uint32_t pairs = (uint32_t)min(inside / span.pair, (uint64_t)(span.tiles / 2));
-        uint32_t offset = (uint32_t)(inside - (uint64_t)pairs * span.pair), place = 2 * pairs;
-        if (pairs < span.tiles / 2) {
-          const uint32_t longer = span.longer(pairs);
-          if (offset >= longer) {
-            offset -= longer;
-            ++place;
-          }
-        }
-        found[0] = (uint32_t)b;
-        found[1] = place;
-        found[2] = offset;
-        found[3] = done;
-        break;
-      }
-      at += span.weight();
-      done += span.tiles;
-    }
-  }
-  __syncthreads();
-  if (one) share.end = share.begin + 1;
-  share.request = uniform((int)found[0]);
-  share.place = (uint32_t)uniform((int)found[1]);
-  share.offset = (uint32_t)uniform((int)found[2]);
-  share.tiles_before = (uint32_t)uniform((int)found[3]);
-  return true;
-}
 
 // STREAM: non-temporal loads, for requests of one tile each (nothing is read
 // twice) over a cache too large to stay in the 256 MiB Infinity Cache between
@@ -392,10 +107,10 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   int request;
   uint32_t tile, tiles;
   uint32_t place = 0;  // of the tile among its request's in the split form's order
-  LatentShare share;
+  TileShare share;
   uint64_t left = 0;   // of this workgroup's share
   if constexpr (SPLIT) {
-    if (!find_share<NW>(a, worker, share)) return;
+    if (!find_share<LatentForm<NW>>(a, worker, blockIdx.x, share)) return;
     request = share.request;
     place = share.place;
     left = share.end - share.begin;
@@ -408,7 +123,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     if (a.causal) tile = tiles - 1 - tile;  // the longest first
   }
   uint32_t offset = SPLIT ? share.offset : 0;
-  const float scale_log2 = a.scale * LAT_LOG2E;
+  const float scale_log2 = a.scale * LOG2E;
 
   for (bool first_part = true;; first_part = false) {
   if (SPLIT && request >= a.B) return;  // never, unless cu_seqlens_q or seqused_kv change under the call
@@ -455,7 +170,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
   bool whole = true;
   if constexpr (SPLIT) {
     // The tile's own chunks, spread over what it counts.
-    constexpr uint32_t START = lat_start<NW>();
+    constexpr uint32_t START = LatentForm<NW>::START;
     const uint32_t end = share.apart ? each : (uint32_t)min((uint64_t)each, (uint64_t)offset + left);
     auto cut = [&](uint32_t x) {
       return x >= each ? all_chunks : (x <= START ? 0 : (int)((uint64_t)(x - START) * (uint32_t)all_chunks / (each - START)));
@@ -465,7 +180,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void latent_kernel(Latent
     whole = offset == 0 && end == each;
     if (!share.apart && offset == 0 && tid == 0 && share.tiles_before + place < a.tiles) {
       const uint64_t tile_end = share.end - left + each;  // in the sequence
-      LatentRecord r;
+      TileRecord r;
       r.start = start;
       r.row = (int)tile * ROWS;
       r.rows = min(ROWS, rows - (int)tile * ROWS);
@@ -739,7 +454,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void latent_merge_ke
   const uint32_t tile = job / (groups * SHARES), rest = job % (groups * SHARES);
   const int group = (int)(rest / SHARES), t0 = (int)(rest % SHARES) * TILES;
   if (tile >= *constant((const int32_t*)a.tile_count)) return;
-  const LatentRecord record = a.records[tile];
+  const TileRecord record = a.records[tile];
   if (record.first == record.last || group * 16 >= record.rows) return;
   const int parts = record.last - record.first + 1, sub = WAVES == 1 ? 0 : wave;
   const int mine = (parts - sub + WAVES - 1) / WAVES;  // parts sub, sub + WAVES, ...
@@ -951,7 +666,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void expanded_kernel(Expa
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const float scale_log2 = a.scale * LAT_LOG2E;
+  const float scale_log2 = a.scale * LOG2E;
 
   constexpr int QK_FRAGS = STEPS * KT, LOOK = 5;
   auto qk_chunk = [&](int chunk, f32x4 (&s)[KT][QT], auto&& between) {
@@ -1230,7 +945,7 @@ int64_t latent_merge_jobs(const LatentPlan& plan, int L) { return plan.tiles * p
 int64_t latent_part_rows(const LatentPlan& plan) { return 2ll * plan.workers * 16 * plan.waves; }
 uint64_t latent_bytes(const LatentParams* p, const LatentPlan& plan) {
   if (plan.workers == 0 || p->T == 0) return 0;
-  return (uint64_t)(latent_part_rows(plan) * (p->L + 2) * 4 + plan.tiles * (int64_t)sizeof(LatentRecord) + 16);
+  return (uint64_t)(latent_part_rows(plan) * (p->L + 2) * 4 + plan.tiles * (int64_t)sizeof(TileRecord) + 16);
 }
 
 template <int DT, int L, int R>
@@ -1249,7 +964,7 @@ int launch_latent(LatentArgs a, const LatentPlan& plan, void* workspace, hipStre
   a.partial_o = (float*)workspace;
   a.partial_ml = a.partial_o + part_rows * L;
   a.tile_count = (uint32_t*)(a.partial_ml + part_rows * 2);
-  a.records = (LatentRecord*)(a.tile_count + 4);
+  a.records = (TileRecord*)(a.tile_count + 4);
   a.tiles = (uint32_t)plan.tiles;
   const dim3 grid((unsigned)plan.workers);
   if (plan.waves == 8 && plan.stream)
