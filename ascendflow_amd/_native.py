@@ -14,6 +14,7 @@ LIB_NAME = "libascendflow_amd.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 
 AFA_DTYPE = {"bf16": 0, "f16": 1}
+AFA_CODE = {"e4m3": 0, "int8": 1}
 SCRATCH_BYTES = 32 << 20  # AFA_SCRATCH_BYTES: the allocation-free entry's static workspace per GPU
 STATUS = {
     -1: "AFA_E_NULL: a required pointer is NULL",
@@ -57,6 +58,15 @@ EXPORTS = (
     "launch_latent_attention_expanded",
     "workspace_size_latent_attention_expanded",
     "form_latent_attention_expanded",
+    "launch_append_quantized_kv",
+    "launch_quantized_attention",
+    "workspace_size_quantized_attention",
+    "form_quantized_attention",
+    "launch_copy_pages",
+    "launch_fork_pages",
+    "workspace_size_fork_pages",
+    "launch_compact_pages",
+    "workspace_size_compact_pages",
     "launch_cache_flush",
     "launch_clock_probe",
     "ascendflow_amd_version",
@@ -136,6 +146,29 @@ class LatentExpandedParams(ct.Structure):
     )
 
 
+class AppendQuantizedKvParams(ct.Structure):
+    _fields_ = (
+        [(n, ct.c_int32) for n in ("dtype", "code", "T", "B", "W", "PAGE", "GROUP", "BLOCKS", "HKV", "D")]
+        + [(n, ct.c_int64) for n in ("k_stride_t", "k_stride_h", "v_stride_t", "v_stride_h")]
+    )
+
+
+class QuantizedParams(ct.Structure):
+    _fields_ = (
+        [(n, ct.c_int32) for n in ("dtype", "code", "causal", "T", "B", "HQ", "HKV", "D", "PAGE", "GROUP", "W", "BLOCKS")]
+        + [(n, ct.c_int64) for n in ("q_stride_t", "q_stride_h", "out_stride_t", "out_stride_h")]
+        + [("scale", ct.c_float), ("reserved", ct.c_int32)]
+    )
+
+
+class ForkPagesParams(ct.Structure):
+    _fields_ = [(n, ct.c_int32) for n in ("B", "W", "PAGE", "BLOCKS", "reserve")]
+
+
+class CompactPagesParams(ct.Structure):
+    _fields_ = [(n, ct.c_int32) for n in ("B", "W", "BLOCKS")]
+
+
 _P = ct.c_void_p
 _SIGNATURES = {
     "launch_sparse_mla": ([_P] * 15 + [ct.POINTER(SparseMlaParams)], ct.c_int),
@@ -192,6 +225,18 @@ _SIGNATURES = {
     "launch_latent_attention_expanded": ([_P] * 10 + [ct.c_uint64, ct.POINTER(LatentExpandedParams)], ct.c_int),
     "workspace_size_latent_attention_expanded": ([ct.POINTER(ct.c_uint64), ct.POINTER(LatentExpandedParams)], ct.c_int),
     "form_latent_attention_expanded": ([ct.POINTER(ct.c_int64), ct.POINTER(LatentExpandedParams)], ct.c_int),
+    "launch_append_quantized_kv": ([_P] * 10 + [ct.POINTER(AppendQuantizedKvParams)], ct.c_int),
+    "launch_quantized_attention": ([_P] * 12 + [ct.c_uint64, ct.POINTER(QuantizedParams)], ct.c_int),
+    "workspace_size_quantized_attention": ([ct.POINTER(ct.c_uint64), ct.POINTER(QuantizedParams)], ct.c_int),
+    "form_quantized_attention": ([ct.POINTER(ct.c_int64), ct.POINTER(QuantizedParams)], ct.c_int),
+    "launch_copy_pages": (
+        [_P, ct.POINTER(_P), ct.POINTER(ct.c_uint64), ct.c_int32, _P, _P, ct.c_int32, ct.c_int32],
+        ct.c_int,
+    ),
+    "launch_fork_pages": ([_P] * 9 + [ct.c_uint64, ct.POINTER(ForkPagesParams)], ct.c_int),
+    "workspace_size_fork_pages": ([ct.POINTER(ct.c_uint64), ct.POINTER(ForkPagesParams)], ct.c_int),
+    "launch_compact_pages": ([_P] * 6 + [ct.c_uint64, ct.POINTER(CompactPagesParams)], ct.c_int),
+    "workspace_size_compact_pages": ([ct.POINTER(ct.c_uint64), ct.POINTER(CompactPagesParams)], ct.c_int),
     "launch_cache_flush": ([_P, _P, ct.c_uint64], ct.c_int),
     "launch_clock_probe": ([_P, _P, ct.c_int32], ct.c_int),
     "ascendflow_amd_version": ([], ct.c_char_p),

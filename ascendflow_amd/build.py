@@ -41,7 +41,7 @@ HIP_FLAGS = (
 # signalling NaNs. Host code keeps IEEE NaN semantics (the launchers' argument checks).
 NO_NAN_FLAGS = ("-Xarch_device", "-fno-honor-nans")
 # Sources whose kernels pass NaNs of their inputs on.
-NAN_SOURCES = ("rotary",)
+NAN_SOURCES = ("quantized_cache", "rotary")
 
 
 def hipcc() -> str:

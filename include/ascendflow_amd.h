@@ -40,6 +40,9 @@ enum {
 
 enum { AFA_DTYPE_BF16 = 0, AFA_DTYPE_F16 = 1 };
 
+/* 8-bit codes of a quantised cache. */
+enum { AFA_CODE_E4M3 = 0, AFA_CODE_INT8 = 1 };
+
 /* Sizes and policy of one sparse_mla call
  * (examples/sparse_attention/attention.py:225-245). */
 typedef struct SparseMlaParams {
@@ -430,6 +433,104 @@ int launch_latent_attention_expanded(void* stream, const void* q, const void* k_
  * rows per tile, form[1] key splits (1: no workspace, no second launch). */
 int workspace_size_latent_attention_expanded(uint64_t* bytes, const LatentExpandedParams* params);
 int form_latent_attention_expanded(int64_t form[2], const LatentExpandedParams* params);
+
+/* Append of new tokens to a paged cache held in 8 bits, codes c of scale s
+ * standing for c s. k and v [T][HKV][D] (strides in elements, columns
+ * contiguous) go to the places that launch_append_paged_kv names, in k_cache and
+ * v_cache [BLOCKS][PAGE][HKV][D]. GROUP tokens of a page and one head share a
+ * scale, float32 k_scale and v_scale [BLOCKS][PAGE / GROUP][HKV]. With A the
+ * largest finite magnitude of a block's new rows and C the largest code (448 for
+ * e4m3, 127 for int8), need = 2^max(ceil(log2(A / C)), -80); a block whose first
+ * row is new gets s = need, another max(need, its s), and the rows that it held
+ * before the new ones are rounded anew where that is larger. Codes are x * (1 / s)
+ * to nearest, ties to even, held inside [-C, C]; a NaN is e4m3's NaN, or 0. Rows
+ * behind the new ones are left as they are. No two new tokens may name the same
+ * row, and no two requests append to the same block. PAGE and GROUP are powers
+ * of two, 16 <= GROUP <= PAGE, GROUP up to 1024, D up to 1024, HKV up to 32768,
+ * T below 2^23. */
+typedef struct AppendQuantizedKvParams {
+  int32_t dtype;
+  int32_t code;            /* AFA_CODE_* */
+  int32_t T, B, W, PAGE, GROUP, BLOCKS, HKV, D;
+  int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+} AppendQuantizedKvParams;
+
+int launch_append_quantized_kv(void* stream, const void* k, const void* v, const int32_t* block_table,
+                               const int32_t* cu_seqlens_q, const int32_t* seqused_kv, void* k_cache, void* v_cache,
+                               float* k_scale, float* v_scale, const AppendQuantizedKvParams* params);
+
+/* Attention of grouped query heads over such a cache: for token t, head h of
+ * request b, with kv = h / (HQ / HKV) and the blocks' scales ks and vs
+ *   s_j = scale ks_j (q[t][h] . k_j[kv]),  out[t][h] = sum_j e^(s_j) vs_j v_j[kv] / sum_j e^(s_j),
+ * over the rows that launch_latent_attention names, causal or not. D 64, 128 or
+ * 256, PAGE and GROUP as above. q and out [T][HQ][D] with strides in elements
+ * (multiples of 8; rows contiguous and on 16 bytes). softmax_lse f32 [T][HQ] or
+ * NULL. Empty rows, pages outside the cache, tokens of no request and scores
+ * that are not finite as there; scales of rows that a token of the request sees
+ * have to be finite and positive, and value scales below 2^-80 count as that.
+ * The workspace holds partial results; calls that may run at the same time need
+ * workspaces of their own. */
+typedef struct QuantizedParams {
+  int32_t dtype;
+  int32_t code;            /* AFA_CODE_* */
+  int32_t causal;
+  int32_t T, B, HQ, HKV, D;
+  int32_t PAGE, GROUP, W, BLOCKS;
+  int64_t q_stride_t, q_stride_h, out_stride_t, out_stride_h;
+  float scale;
+  int32_t reserved;
+} QuantizedParams;
+
+int launch_quantized_attention(void* stream, const void* q, const void* k_cache, const void* v_cache,
+                               const float* k_scale, const float* v_scale, const int32_t* block_table,
+                               const int32_t* cu_seqlens_q, const int32_t* seqused_kv, void* out, float* softmax_lse,
+                               void* workspace, uint64_t workspace_bytes, const QuantizedParams* params);
+
+/* Bytes of that workspace, on 16 bytes, and which form a call of these sizes
+ * runs: form[0] packed (token, head) rows per tile, form[1] workgroups of a
+ * key/value head that share the tiles. */
+int workspace_size_quantized_attention(uint64_t* bytes, const QuantizedParams* params);
+int form_quantized_attention(int64_t form[2], const QuantizedParams* params);
+
+/* Copies page source[i] to page destination[i], i < pairs, in each of n_caches
+ * tensors of BLOCKS pages (caches: device pointers, page_bytes: bytes of a page,
+ * both arrays on the host). Pairs with a number outside [0, BLOCKS) copy
+ * nothing. No destination may be named twice or be a source as well. */
+int launch_copy_pages(void* stream, const void* const* caches, const uint64_t* page_bytes, int32_t n_caches,
+                      const int32_t* source, const int32_t* destination, int32_t pairs, int32_t BLOCKS);
+
+/* Forks requests: row b of block_table [B][W] becomes a copy of row parents[b]
+ * as it was before the call, or empty (-1 throughout) where that is outside
+ * [0, B). seqused_kv[b] is the length of the new row: it keeps the pages of its
+ * tokens, and gets pages for `reserve` tokens more. A page that row b will go on
+ * writing to (seqused_kv[b] % PAGE tokens of it are used) and that others hold
+ * too is replaced by a new one, to be copied from the old: source[b],
+ * destination[b], both -1 where nothing is copied. Of rows that will write to
+ * one page the lowest keeps it, unless somebody else holds it. page_counts
+ * [BLOCKS], the references of each page, follows all of it; free pages (count 0)
+ * are handed out from the lowest up, row by row, the copy first. missing[0]
+ * counts the pages that were wanted beyond the free ones or beyond the table's
+ * width (2^31 - 1 at most); their entries are -1. B up to 8192, PAGE a power of two. */
+typedef struct ForkPagesParams {
+  int32_t B, W, PAGE, BLOCKS, reserve;
+} ForkPagesParams;
+
+int workspace_size_fork_pages(uint64_t* bytes, const ForkPagesParams* params);
+int launch_fork_pages(void* stream, int32_t* block_table, int32_t* page_counts, const int32_t* parents,
+                      const int32_t* seqused_kv, int32_t* source, int32_t* destination, int32_t* missing,
+                      void* workspace, uint64_t workspace_bytes, const ForkPagesParams* params);
+
+/* Compacts: with n pages in use (count above 0), the k-th of those from page n on
+ * is renamed to the k-th free page below n, in block_table [B][W] and in
+ * page_counts [BLOCKS]; source and destination [BLOCKS / 2] list the moves, to be
+ * copied, behind them -1. Afterwards pages 0 .. n - 1 are in use. */
+typedef struct CompactPagesParams {
+  int32_t B, W, BLOCKS;
+} CompactPagesParams;
+
+int workspace_size_compact_pages(uint64_t* bytes, const CompactPagesParams* params);
+int launch_compact_pages(void* stream, int32_t* block_table, int32_t* page_counts, int32_t* source, int32_t* destination,
+                         void* workspace, uint64_t workspace_bytes, const CompactPagesParams* params);
 
 /* Measurement helpers (no reference kernel; the reference sweeps a >= 4x L2
  * buffer before each timed launch, benchmarks/cache.py:13-92 and
