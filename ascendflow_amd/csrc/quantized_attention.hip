@@ -49,8 +49,8 @@ struct QuantizedArgs {
   int32_t T, B, HKV, W, page_shift, group_shift, blocks, causal;
   int32_t H;  // query heads of a key/value head: the packed rows of a token
   float scale;
-  int32_t workers;          // workgroups of a key/value head
-  float* partial_o;         // [2 * workers][HKV][ROWS][D], not normalised
+  int32_t workers;          // workgroups of the same key/value heads
+  float* partial_o;         // [2 * workers][HKV][ROWS / 16][D / 16][64][4], not normalised, as a wave holds it
   float* partial_ml;        // [2 * workers][HKV][ROWS][2]: running maximum (log2), sum of weights
   TileRecord* records;      // [tiles], alike for every head
   uint32_t* tile_count;
@@ -112,51 +112,79 @@ template <> struct Codes<DT_BF16, AFA_CODE_INT8> {
 // ---- stream form ---------------------------------------------------------------
 //
 // For the few rows of decode and verification: a tile is 16 QT packed rows of one
-// key/value head, a chunk 128 cache rows, 32 for each of four waves. Waves are on their
-// own until a tile ends: no barrier, no LDS; each keeps all rows' queries and an output of
-// its own, and its codes go from memory to registers, a chunk ahead of their use.
-// S^T[keys, rows] = K Q^T: a lane loads 16 bytes of a key row (the order of columns is
-// free, queries follow it). O^T[columns, rows] += V^T P^T: lane (g, i) needs a column's
-// values of the eight keys that its P holds, which lie a row apart, so it loads D / 16
-// columns of those eight rows and transposes bytes in registers; the tiles of columns
-// that come out interleave, which leaves each lane with D / 4 consecutive ones.
-template <int QT> struct StreamForm {
-  static constexpr int ROWS = 16 * QT, KEYS = 128, THREADS = 256;
+// key/value head. A workgroup's four waves take HW heads, whose rows of a token lie side
+// by side in memory, and 4 / HW runs of 32 cache rows of a chunk. Waves are on their own
+// until a tile ends: each keeps all rows' queries, an output of its own and a ring of LDS
+// slots that the load-to-LDS path fills ahead of their use, without a barrier or a
+// register; it waits for its own loads only.
+// S^T[keys, rows] = K Q^T: a lane reads 16 bytes of a key row (the order of columns is
+// free, queries follow it). O^T[columns, rows] += V^T P^T: the accumulator layout of S^T
+// is the operand layout of P^T, and ds_read_b64_tr_b8 gives a lane a column's codes of the
+// eight keys whose weights it holds. Codes become 16-bit values between LDS and the
+// matrix instructions.
+template <int QT, int HW> struct StreamForm {
+  static constexpr int ROWS = 16 * QT, KEYS = 128 / HW, THREADS = 256;
   static constexpr uint32_t START = 1, LEAST = 2;
   static constexpr float JOIN = 4.0f;
 };
+// Slots of a wave's ring, 64 D bytes each, for two workgroups per CU (D = 256: one).
+template <int D> __host__ __device__ constexpr int q8_slots() { return D == 64 ? 4 : 2; }
+template <int D> __host__ __device__ constexpr int q8_groups() { return D == 256 ? 1 : 2; }  // workgroups of a CU
 
 template <int BYTES> struct Bytes;
-template <> struct Bytes<4> { typedef uint32_t type __attribute__((ext_vector_type(1))); };
 template <> struct Bytes<8> { typedef u32x2 type; };
 template <> struct Bytes<16> { typedef u32x4 type; };
 
-// 4 x 4 bytes, rows to columns.
-__device__ __forceinline__ void transpose4(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t* c) {
-  const uint32_t a = __builtin_amdgcn_perm(r1, r0, 0x05010400u), b = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
-  const uint32_t d = __builtin_amdgcn_perm(r3, r2, 0x05010400u), e = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
-  c[0] = __builtin_amdgcn_perm(d, a, 0x05040100u);
-  c[1] = __builtin_amdgcn_perm(d, a, 0x07060302u);
-  c[2] = __builtin_amdgcn_perm(e, b, 0x05040100u);
-  c[3] = __builtin_amdgcn_perm(e, b, 0x07060302u);
+// Unit u (16 bytes) of row r of a slot's keys lies at u ^ key_swizzle(r): in a 16-byte read
+// the rows {0..3, 12..15} take unit u and {4..11} unit u ^ 1 at once (or the other way
+// round), which then fall on 16 distinct 16-byte groups of LDS's 256 bytes.
+template <int D> __device__ __forceinline__ int key_swizzle(int r) {
+  return D == 64 ? (-(r >> 2)) & 3 : D == 128 ? (r >> 1) & 7 : r & 15;
+}
+// The same for values: a half of a transposing read takes unit u of rows 0..7 (or 8..15)
+// and of the 16 rows further.
+template <int D> __device__ __forceinline__ int value_swizzle(int r) {
+  const int t = r >> 4;
+  return D == 64 ? ((r >> 2) & 1) | (t << 1) : D == 128 ? ((r >> 1) & 3) | (t << 2) : (r & 7) | (t << 3);
 }
 
-template <int DT, int CT, int D, int QT>
-__global__ __launch_bounds__(256, 2) void quantized_stream_kernel(QuantizedArgs a) {
+// Waits until at most n <= MOST slots' loads (PER each) are in flight.
+template <int PER, int MOST>
+__device__ __forceinline__ void wait_slots(int n) {
+  static_assert(PER * MOST < 64, "vmcnt holds 6 bits");
+  if constexpr (MOST > 0) {
+    if (n < MOST) {
+      wait_slots<PER, MOST - 1>(n);
+      return;
+    }
+  }
+  wait_vmcnt<PER * MOST>();
+}
+
+// STREAM: non-temporal loads, for requests of one tile each (nothing is read twice) over
+// caches too large to stay in the 256 MiB Infinity Cache, rows of whole 128-byte lines.
+template <int DT, int CT, int D, int QT, int HW, bool STREAM>
+__global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(QuantizedArgs a) {
   typedef typename B16<DT>::scalar scalar;
   typedef typename B16<DT>::x8 x8;
-  typedef StreamForm<QT> F;
-  typedef typename Bytes<D / 16>::type vbytes;
-  constexpr int ROWS = F::ROWS, KEYS = F::KEYS, KL = D / 64, VT = D / 16;
-  __shared__ f32x4 joined_o[4][VT][64];
-  __shared__ float2 joined_ml[4][16];
+  typedef typename B16<DT>::x4 x4;
+  typedef StreamForm<QT, HW> F;
+  constexpr int ROWS = F::ROWS, KEYS = F::KEYS, KW = 4 / HW, KL = D / 64, VT = D / 16;
+  constexpr int NS = q8_slots<D>(), V_AT = 32 * D, META_AT = 64 * D, SLOT = META_AT + 256;
+  constexpr int LOADS = 32 * D / 1024, LR = 1024 / D;  // of keys or values; rows of a load
+  constexpr int ALL_LOADS = 2 * LOADS + 1;
+  __shared__ __attribute__((aligned(256))) uint8_t ring[4][NS][SLOT];
+  __shared__ float2 joined_ml[4][QT][16];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int g = lane >> 4, i16 = lane & 15;
   const int H = a.H;
-  const int kv_head = uniform((int)(blockIdx.x % (uint32_t)a.HKV));
-  const uint32_t worker = (uint32_t)uniform((int)(blockIdx.x / (uint32_t)a.HKV));
+  // Heads of one worker side by side on one XCD: together they read whole rows.
+  const uint32_t index = xcd_contiguous(blockIdx.x, gridDim.x), groups = (uint32_t)a.HKV / HW;
+  const int kv_head = uniform((int)(index % groups) * HW + wave % HW);
+  const int part = wave / HW;  // this wave's run of a chunk's rows
+  const uint32_t worker = (uint32_t)uniform((int)(index / groups));
 
   TileShare share;
   if (!find_share<F>(a, worker, worker, share)) return;
@@ -165,9 +193,22 @@ __global__ __launch_bounds__(256, 2) void quantized_stream_kernel(QuantizedArgs 
   uint64_t left = share.end - share.begin;
   const float scale_log2 = a.scale * LOG2E;
   const uint32_t row_bytes = (uint32_t)a.HKV * D;
-  const uint32_t k_off = (uint32_t)i16 * row_bytes + 16u * g, v_off = (uint32_t)(4 * g) * row_bytes + (uint32_t)(VT * i16);
+  const uint32_t ring_base = lds_address(ring[0]) + (uint32_t)wave * (NS * SLOT);
 
-  for (;;) {
+  // Load p of a slot's keys or values brings rows LR p .. + LR - 1 of it, 16 bytes a lane.
+  const int ln_row = lane / (D / 16), ln_unit = lane % (D / 16);
+  auto load16 = [](uint32_t to, uint32_t off, const uint8_t* from) {
+    if constexpr (STREAM)
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" :: "s"(to), "v"(off), "s"(from) : "memory");
+    else
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(off), "s"(from) : "memory");
+  };
+  // Fragment addresses inside a slot; the XOR of a column group picks its unit.
+  const int rv = 16 * (i16 >> 3) + 4 * g + ((i16 >> 1) & 3);
+  const uint32_t k_at = (uint32_t)(i16 * D + ((g ^ key_swizzle<D>(i16)) << 4));
+  const uint32_t v_at = (uint32_t)(V_AT + rv * D + (value_swizzle<D>(rv) << 4) + (i16 & 1) * 8);
+
+  for (bool first_part = true;; first_part = false) {
     if (request >= a.B) return;  // never, unless cu_seqlens_q or seqused_kv change under the call
     const TileSpan<F, QuantizedArgs> span(a, request);
     if (place >= span.tiles) {  // on to the next request that has tokens (there is one: something is left)
@@ -200,7 +241,7 @@ __global__ __launch_bounds__(256, 2) void quantized_stream_kernel(QuantizedArgs 
     };
     const int begin = cut(offset), chunks = cut(stop);
     const bool whole = offset == 0 && stop == each;
-    if (!share.apart && offset == 0 && tid == 0 && kv_head == 0 && share.tiles_before + place < a.tiles) {
+    if (!share.apart && offset == 0 && tid == 0 && index % groups == 0 && share.tiles_before + place < a.tiles) {
       const uint64_t tile_end = share.end - left + each;  // in the sequence
       TileRecord r;
       r.start = start;
@@ -211,6 +252,52 @@ __global__ __launch_bounds__(256, 2) void quantized_stream_kernel(QuantizedArgs 
       a.records[share.tiles_before + place] = r;
     }
     left -= min(left, (uint64_t)(stop - offset));
+
+    // ---- cache rows to LDS: slot (chunk - begin) % NS holds this wave's 32 rows of a chunk ----
+    const int32_t* const table = a.table + (int64_t)request * a.W;
+    const int page_mask = (1 << a.page_shift) - 1;
+    // Chunks of which this wave has rows.
+    const int mine = min(chunks, (kv_end - part * 32 + KEYS - 1) / KEYS);
+    struct Pages { int id[2]; };  // of the two groups of 16 rows
+    auto key_of = [&](int chunk, int t) { return chunk * KEYS + part * 32 + 16 * t; };
+    auto holds = [&](const Pages& p, int chunk, int t) {
+      return key_of(chunk, t) < kv_end && (uint32_t)p.id[t] < (uint32_t)a.blocks;
+    };
+    auto slot_of = [&](int chunk) { return ring_base + (uint32_t)((chunk - begin) % NS) * SLOT; };
+    // Rows that are not there read the cache's first ones instead (hidden later).
+    auto cache_row = [&](const Pages& p, int chunk, int t) -> int64_t {
+      return holds(p, chunk, t) ? ((int64_t)p.id[t] << a.page_shift) + (key_of(chunk, t) & page_mask) : 0;
+    };
+    // A slot comes with 64 words: scales of its two groups' keys (words 0, 1) and values (2, 3), page numbers of the
+    // wave's rows NS chunks on (4, 5) and its own (6, 7). All that a step needs is in LDS before it: a scalar load
+    // that misses would hold up every LDS read behind it.
+    const int role = lane & 7;
+    auto fetch = [&](const Pages& p, int chunk) {
+      const uint32_t slot = slot_of(chunk);
+      const int64_t row[2] = {cache_row(p, chunk, 0), cache_row(p, chunk, 1)};
+      const int64_t block = ((role & 1 ? row[1] : row[0]) >> a.group_shift) * a.HKV + kv_head;
+      const int entry = key_of(chunk + (role < 6 ? NS : 0), role & 1) >> a.page_shift;
+      const void* from = role < 2 ? (const void*)(a.k_scale + block)
+                         : role < 4 ? (const void*)(a.v_scale + block) : (const void*)(table + min(entry, a.W - 1));
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                       :: "s"(opaque_uniform(slot + META_AT)), "v"(from) : "memory");
+#pragma unroll
+      for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l) {
+          const int t = l / (LOADS / 2), r = l * LR + ln_row;
+          const int unit = ln_unit ^ (which ? value_swizzle<D>(r) : key_swizzle<D>(r & 15));
+          load16(opaque_uniform(slot + (uint32_t)(which * V_AT + l * 1024)), (uint32_t)(r & 15) * row_bytes + ((uint32_t)unit << 4),
+                 (which ? a.v : a.k) + (row[t] * row_bytes + kv_head * D));
+        }
+    };
+
+    if (KW > 1 && !first_part) __syncthreads();  // the ring's other use is over
+    Pages first[NS];  // page numbers of the first chunks, before any load to LDS: one wait for all
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) first[i].id[t] = constant(table)[min(key_of(begin + i, t) >> a.page_shift, a.W - 1)];
 
     // Queries: columns 64 l + 16 g + 8 h .. + 7 of row i16 are operand 2 l + h.
     x8 qf[QT][2 * KL];
@@ -238,83 +325,86 @@ __global__ __launch_bounds__(256, 2) void quantized_stream_kernel(QuantizedArgs 
 #pragma unroll
       for (int c = 0; c < VT; ++c) o[qt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if (begin + i < mine) {
+        fetch(first[i], begin + i);
+      }
 
-    struct Part {  // a wave's 32 rows of a chunk
-      u32x4 k[2][KL];
-      vbytes v[8];
-      float ks[2], vs[2];
-      uint32_t good;  // bit t: the page of 16-row group t holds keys
-    };
-    const const_ints pages = constant(a.table + (int64_t)request * a.W);
-    const int page_mask = (1 << a.page_shift) - 1;
-    int page[2];  // of the next part to load, -1 past the end
-    auto look_up = [&](int chunk) {
+    // A step's keys and words are in registers before it, read while the step before multiplies its values.
+    u32x4 k[2][KL], meta[2];
+    auto read_keys = [&](int chunk) {
+      const uint32_t slot = slot_of(chunk), base = slot + k_at;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int key = chunk * KEYS + wave * 32 + 16 * t;
-        page[t] = chunk < chunks && key < kv_end ? pages[key >> a.page_shift] : -1;
+      for (int l = 0; l < KL; ++l)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) k[t][l] = *(const AFA_LDS u32x4*)(lds_at<uint8_t>(base ^ (uint32_t)(l << 6)) + t * 16 * D);
+      meta[0] = *lds_at<u32x4>(slot + META_AT);
+      meta[1] = *lds_at<u32x4>(slot + META_AT + 16);
+    };
+    if (begin < mine) {
+      wait_slots<ALL_LOADS, NS - 1>(min(NS - 1, mine - 1 - begin));
+      __asm__ volatile("" ::: "memory");
+      read_keys(begin);
+    }
+    for (int c = begin; c < mine; ++c) {
+      const int key0 = key_of(c, 0);
+      const uint32_t slot = slot_of(c);
+      const Pages own = {{uniform((int)meta[1][2]), uniform((int)meta[1][3])}}, next = {{uniform((int)meta[1][0]), uniform((int)meta[1][1])}};
+      const bool good[2] = {holds(own, c, 0), holds(own, c, 1)};
+      const bool edge = key0 + 32 > clean_end || !(good[0] && good[1]);  // uniform
+      if (edge) {
+        // Values that nobody sees may be codes of no number, which no weight of 0 would hide: half a row a lane.
+        const int r = lane >> 1;
+        if (!(key0 + r < kv_end && (r < 16 ? good[0] : good[1]))) {
+          const uint32_t at = slot + (uint32_t)(V_AT + r * D + (lane & 1) * (D / 2));
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) *(AFA_LDS u32x4*)(uintptr_t)(at + 16u * i) = u32x4{0u, 0u, 0u, 0u};
+        }
       }
-    };
-    typedef const __attribute__((address_space(4))) float* const_floats;
-    auto load = [&](int chunk, Part& p) {
-      p.good = 0;
+      typedef int i32x2 __attribute__((ext_vector_type(2)));
+      i32x2 v[VT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int key = chunk * KEYS + wave * 32 + 16 * t;
-        const bool inside = (uint32_t)page[t] < (uint32_t)a.blocks;
-        p.good |= inside ? 1u << t : 0u;
-        // Rows that are not there read the cache's first ones instead (hidden later).
-        const int64_t row = inside ? ((int64_t)page[t] << a.page_shift) + (key & page_mask) : 0;
-        const int64_t at = row * row_bytes + kv_head * D;
-        const uint8_t* k = a.k + at;
-        const uint8_t* v = a.v + at;
-        const int64_t block = (row >> a.group_shift) * a.HKV + kv_head;
-        p.ks[t] = ((const_floats)(uintptr_t)a.k_scale)[block];
-        p.vs[t] = ((const_floats)(uintptr_t)a.v_scale)[block];
-#pragma unroll
-        for (int l = 0; l < KL; ++l) p.k[t][l] = *(const u32x4*)(k + (k_off + 64u * l));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p.v[4 * t + r] = *(const vbytes*)(v + (v_off + (uint32_t)r * row_bytes));
-      }
-    };
-    auto attend = [&](int chunk, Part& p) {
-      const int key0 = chunk * KEYS + wave * 32;
-      if (key0 >= kv_end) return;
+      for (int c2 = 0; c2 < VT; ++c2)
+        v[c2] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((i32x2 AFA_LDS*)(uintptr_t)((slot + v_at) ^ (uint32_t)(c2 << 4)));
       f32x4 s[2][QT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) s[t][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int l = 0; l < KL; ++l)
+      for (int l = 0; l < KL; ++l)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const x8 kf = Codes<DT, CT>::decode(p.k[t][l][2 * h], p.k[t][l][2 * h + 1]);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const x8 kf = Codes<DT, CT>::decode(k[t][l][2 * h], k[t][l][2 * h + 1]);
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) s[t][qt] = B16<DT>::mfma(kf, qf[qt][2 * l + h], s[t][qt]);
           }
-      }
-      if (key0 + 32 > clean_end || p.good != 3u) {  // uniform
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key = 16 * t + 4 * g + r;
-            const bool page_holds = (p.good >> t) & 1u;
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) s[t][qt][r] = page_holds && key0 + key < limit[qt] ? s[t][qt][r] : -INFINITY;
-            // Values that nobody sees may be codes of no number, which no weight of 0 would hide.
-            if (!(page_holds && key0 + key < kv_end)) p.v[4 * t + r] = vbytes(0);
-          }
-      }
       float sk[2], lv[2], iv[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const bool page_holds = (p.good >> t) & 1u;  // else the scales are those of other rows
-        const float ks = page_holds ? p.ks[t] : 1.0f, vs = page_holds ? at_least(p.vs[t], Q8_LEAST_SCALE) : 1.0f;
+        // Without a page the scales are those of other rows.
+        const float ks = good[t] ? __uint_as_float(meta[0][t]) : 1.0f;
+        const float vs = good[t] ? at_least(__uint_as_float(meta[0][2 + t]), Q8_LEAST_SCALE) : 1.0f;
         sk[t] = at_least(ks * scale_log2, 1.17549435e-38f);  // not 0: times a hidden score
         lv[t] = __log2f(vs);
         iv[t] = 1.0f / vs;
+      }
+      if (c + NS < mine) {
+        __builtin_amdgcn_s_waitcnt(WAIT_LGKM0);  // the slot is read
+        __asm__ volatile("" ::: "memory");
+        fetch(next, c + NS);
+      }
+      if (edge) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+              s[t][qt][r] = good[t] && key0 + 16 * t + 4 * g + r < limit[qt] ? s[t][qt][r] : -INFINITY;
       }
       x8 pf[QT];
 #pragma unroll
@@ -322,15 +412,15 @@ __global__ __launch_bounds__(256, 2) void quantized_stream_kernel(QuantizedArgs 
         float top = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float mine = fmaxf(fmaxf(s[t][qt][0], s[t][qt][1]), fmaxf(s[t][qt][2], s[t][qt][3]));
-          top = fmaxf(top, __builtin_fmaf(mine, sk[t], lv[t]));
+          const float most = fmaxf(fmaxf(s[t][qt][0], s[t][qt][1]), fmaxf(s[t][qt][2], s[t][qt][3]));
+          top = fmaxf(top, __builtin_fmaf(most, sk[t], lv[t]));
         }
         const float m_new = fmaxf(m_run[qt], max_over_lane_groups(top));
         if (__ballot(m_new > m_run[qt] + q8_tau<DT>()) != 0ull) {
           const float alpha = fast_exp2(m_run[qt] - m_new);
           l_run[qt] *= alpha;
 #pragma unroll
-          for (int c = 0; c < VT; ++c) o[qt][c] *= alpha;
+          for (int c2 = 0; c2 < VT; ++c2) o[qt][c2] *= alpha;
           m_run[qt] = m_new;
         }
 #pragma unroll
@@ -346,80 +436,82 @@ __global__ __launch_bounds__(256, 2) void quantized_stream_kernel(QuantizedArgs 
           l_run[qt] = __builtin_fmaf(sum, iv[t], l_run[qt]);
         }
       }
-#pragma unroll
-      for (int w = 0; w < VT / 4; ++w) {
-        uint32_t lo[4], hi[4];
-        transpose4(p.v[0][w], p.v[1][w], p.v[2][w], p.v[3][w], lo);
-        transpose4(p.v[4][w], p.v[5][w], p.v[6][w], p.v[7][w], hi);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const x8 vf = Codes<DT, CT>::decode(lo[c], hi[c]);
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) o[qt][4 * w + c] = B16<DT>::mfma(vf, pf[qt], o[qt][4 * w + c]);
-        }
+      if (c + 1 < mine) {
+        wait_slots<ALL_LOADS, NS - 1>(min(NS - 1, mine - 2 - c));
+        __asm__ volatile("" ::: "memory");
+        read_keys(c + 1);
       }
-    };
-
-    Part even, odd;
-    look_up(begin);
-    if (begin < chunks) load(begin, even);
-    look_up(begin + 1);
-    for (int c = begin; c < chunks; c += 2) {
-      if (c + 1 < chunks) load(c + 1, odd);
-      look_up(c + 2);
-      attend(c, even);
-      if (c + 1 < chunks) {
-        if (c + 2 < chunks) load(c + 2, even);
-        look_up(c + 3);
-        attend(c + 1, odd);
+#pragma unroll
+      for (int c2 = 0; c2 < VT; ++c2) {
+        const x8 vf = Codes<DT, CT>::decode((uint32_t)v[c2][0], (uint32_t)v[c2][1]);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) o[qt][c2] = B16<DT>::mfma(vf, pf[qt], o[qt][c2]);
       }
     }
 
-    // The four waves' sums, 16 rows at a time. Lane (g, i) of column tile c, element r holds
-    // column VT (4 g + r) + c of row i; here a thread takes VT columns of a row.
-    const int row_of = tid & 15, unit = tid >> 4;
+    float total[QT];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      __syncthreads();  // the last round's are read
-      const float total = sum_over_lane_groups(l_run[qt]);
+    for (int qt = 0; qt < QT; ++qt) total[qt] = sum_over_lane_groups(l_run[qt]);
+    if constexpr (KW > 1) {
+      // The first of a head's waves sums up, through the others' rings, 16 rows at a time.
+      static_assert(VT * 1024 <= NS * SLOT, "a wave's output fits its ring");
 #pragma unroll
-      for (int c = 0; c < VT; ++c) joined_o[wave][c][lane] = o[qt][c];
-      if (g == 0) joined_ml[wave][i16] = make_float2(m_run[qt], total);
-      __syncthreads();
-      const int row = (int)tile * ROWS + qt * 16 + row_of;
-      if (row < rows) {
-        float2 ml[4];
-        float top = -1e30f, sum = 0.f, weight[4], acc[VT];
+      for (int qt = 0; qt < QT; ++qt) {
+        if (qt > 0) __syncthreads();  // the last rows are read
+        if (part > 0) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          ml[w] = joined_ml[w][row_of];
-          top = fmaxf(top, ml[w].x);
+          for (int c = 0; c < VT; ++c) *(AFA_LDS f32x4*)(uintptr_t)(ring_base + (uint32_t)(c * 1024 + lane * 16)) = o[qt][c];
+          if (g == 0) joined_ml[wave][qt][i16] = make_float2(m_run[qt], total[qt]);
         }
+        __syncthreads();
+        if (part == 0) {
+          float2 ml[KW];
+          ml[0] = make_float2(m_run[qt], total[qt]);
+          float top = ml[0].x;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          weight[w] = fast_exp2(ml[w].x - top);
-          sum = __builtin_fmaf(weight[w], ml[w].y, sum);
+          for (int w = 1; w < KW; ++w) {
+            ml[w] = joined_ml[wave + w * HW][qt][i16];
+            top = fmaxf(top, ml[w].x);
+          }
+          float weight = fast_exp2(ml[0].x - top);
+          total[qt] = weight * ml[0].y;
+          m_run[qt] = top;
+#pragma unroll
+          for (int c = 0; c < VT; ++c) o[qt][c] *= weight;
+#pragma unroll
+          for (int w = 1; w < KW; ++w) {
+            weight = fast_exp2(ml[w].x - top);
+            total[qt] = __builtin_fmaf(weight, ml[w].y, total[qt]);
+            const uint32_t from = ring_base + (uint32_t)(w * HW * NS * SLOT + lane * 16);
+#pragma unroll
+            for (int c = 0; c < VT; ++c) o[qt][c] += weight * *lds_at<f32x4>(from + c * 1024);
+          }
         }
+      }
+    }
+    if (part == 0) {
 #pragma unroll
-        for (int c = 0; c < VT; ++c) {
-          acc[c] = 0.f;
+      for (int qt = 0; qt < QT; ++qt) {
+        const int row = (int)tile * ROWS + qt * 16 + i16;
+        if (!whole) {
+          // As the registers hold it, [column tile][lane] of four columns: whole kilobytes per store.
+          const int64_t at = ((2 * (int64_t)worker + (offset == 0 ? 1 : 0)) * a.HKV + kv_head) * QT + qt;
+          float* po = a.partial_o + (at * VT * 64 + lane) * 4;
 #pragma unroll
-          for (int w = 0; w < 4; ++w)
-            acc[c] = __builtin_fmaf(weight[w], ((const float*)&joined_o[w][c][(unit >> 2) * 16 + row_of])[unit & 3], acc[c]);
-        }
-        if (whole) {
-          const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+          for (int c = 0; c < VT; ++c) *(f32x4*)(po + c * 256) = o[qt][c];
+          if (g == 0) *(float2*)(a.partial_ml + (at * 16 + i16) * 2) = make_float2(m_run[qt], total[qt]);
+        } else if (row < rows) {
+          const float inv = total[qt] > 0.f ? 1.0f / total[qt] : 0.f;
           const int token = row / H, head = kv_head * H + row - token * H;
-          scalar v[VT];
+          scalar* out = (scalar*)a.out + (int64_t)(start + token) * a.o_t + (int64_t)head * a.o_h + 4 * g;
 #pragma unroll
-          for (int c = 0; c < VT; ++c) v[c] = (scalar)(acc[c] * inv);
-          scalar* out = (scalar*)a.out + (int64_t)(start + token) * a.o_t + (int64_t)head * a.o_h + VT * unit;
-          __builtin_memcpy(__builtin_assume_aligned(out, 2 * VT < 16 ? 2 * VT : 16), v, sizeof(v));
-          if (a.lse && unit == 0) a.lse[(int64_t)(start + token) * (a.HKV * H) + head] = row_lse(top, sum);
-        } else {
-          const int64_t at = ((2 * (int64_t)worker + (offset == 0 ? 1 : 0)) * a.HKV + kv_head) * ROWS + qt * 16 + row_of;
-          __builtin_memcpy(__builtin_assume_aligned(a.partial_o + at * D + VT * unit, 16), acc, sizeof(acc));
-          if (unit == 0) *(float2*)(a.partial_ml + at * 2) = make_float2(top, sum);
+          for (int c = 0; c < VT; ++c) {
+            x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[qt][c][i] * inv);
+            *(x4*)(out + 16 * c) = v;
+          }
+          if (a.lse && g == 0) a.lse[(int64_t)(start + token) * (a.HKV * H) + head] = row_lse(m_run[qt], total[qt]);
         }
       }
     }
@@ -429,53 +521,483 @@ __global__ __launch_bounds__(256, 2) void quantized_stream_kernel(QuantizedArgs 
   }
 }
 
-// Combines the parts of the tiles that several workgroups share, in order:
-// out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p. 16 rows of a head a workgroup.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void quantized_merge_kernel(QuantizedArgs a, int tile_rows) {
+// ---- tile form -----------------------------------------------------------------
+//
+// For chunks of prompts: a tile is 16 QT rows for each of eight waves, whose queries and
+// outputs stay in registers; chunks of 64 cache rows go through LDS as 16-bit values, so
+// that a code is converted once a workgroup and not once a wave. A wave's codes come into
+// registers a step before they are converted and stored (keys two chunks ahead of their
+// use, values one; two slots each), page numbers a step before that. The scales' three
+// figures a 16-row group (of its keys, the values' exponent and reciprocal) go the same
+// way. QK of chunk c + 1 is issued ahead of the softmax of chunk c, whose exponentials
+// run in the shadow of the matrix instructions of QK (c + 1) and PV (c).
+template <int QT> struct TileForm {
+  static constexpr int ROWS = 128 * QT, KEYS = 64, THREADS = 512;
+  static constexpr uint32_t START = 5, LEAST = 4;
+  static constexpr float JOIN = 0.0f;
+};
+
+// Unit u (16 bytes) of key row r lies at u ^ this, units of value rows at u ^ twice value_rows<D>(r): the reads'
+// 16-byte (keys) and 32-byte (values, 16 columns of 4 rows a lane group) pieces then fall on distinct banks.
+template <int D> __device__ __forceinline__ int key_rows(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+template <int D> __device__ __forceinline__ int value_rows(int r) { return D == 64 ? (r >> 1) & 3 : r & 7; }
+
+template <int DT, int CT, int D, int QT>
+__global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a) {
   typedef typename B16<DT>::scalar scalar;
+  typedef typename B16<DT>::x8 x8;
+  typedef typename B16<DT>::x4 x4;
+  typedef TileForm<QT> F;
+  constexpr int ROWS = F::ROWS, KC = F::KEYS, KT = KC / 16, KSTEPS = D / 32, VT = D / 16, RB = 2 * D;
+  constexpr int CODES = KC * D / F::THREADS;                 // of a thread, of a chunk's keys or values
+  constexpr int PIECE = CODES < 16 ? 8 : 16, PIECES = CODES / PIECE;  // bytes of a load, loads
+  constexpr int TPR = D / PIECE;                            // threads of a row
+  typedef typename Bytes<PIECE>::type piece;
+  __shared__ __attribute__((aligned(256))) uint8_t keys[2][KC * RB], values[2][KC * RB];
+  __shared__ f32x4 figures[2][3];                           // of a chunk's four groups: sk, lv, iv
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int g = lane >> 4, i16 = lane & 15;
+  const int H = a.H;
+  // Heads first: with eight of them an XCD has a head's tiles, which read the same rows.
+  const int kv_head = uniform((int)(blockIdx.x % (uint32_t)a.HKV));
+  const uint32_t worker = (uint32_t)uniform((int)(blockIdx.x / (uint32_t)a.HKV));
+  TileShare share;
+  if (!find_share<F>(a, worker, worker, share)) return;
+  int request = share.request;
+  uint32_t place = share.place, offset = share.offset;
+  uint64_t left = share.end - share.begin;
+  const float scale_log2 = a.scale * LOG2E;
+  const uint32_t row_bytes = (uint32_t)a.HKV * D;
+
+  for (bool first_part = true;; first_part = false) {
+    if (request >= a.B) return;  // never, unless cu_seqlens_q or seqused_kv change under the call
+    const TileSpan<F, QuantizedArgs> span(a, request);
+    if (place >= span.tiles) {  // on to the next request that has tokens (there is one: something is left)
+      share.tiles_before += span.tiles;
+      place = 0;
+      ++request;
+      continue;
+    }
+    const uint32_t tile = (uint32_t)uniform((int)span.tile(place));
+    const uint32_t each = (uint32_t)uniform((int)span.counts(place));
+    if (share.apart && offset > 0) {  // an earlier workgroup's tile
+      if (left <= each - offset) return;
+      left -= each - offset;
+      offset = 0;
+      ++place;
+      continue;
+    }
+    int start, count;
+    request_tokens(constant(a.cu), request, a.T, start, count);
+    int used, ahead;
+    request_rows(a, request, start, used, ahead);
+    const int rows = count * H;
+    auto visible = [&](int t) { return a.causal ? min(max(ahead + t + 1, 0), used) : used; };
+    const int kv_end = visible((min((int)(tile + 1) * ROWS, rows) - 1) / H);
+    const int clean_chunks = visible((int)tile * ROWS / H) / KC;  // no row of the tile hides a key of these
+    const int all_chunks = (kv_end + KC - 1) / KC;
+    const uint32_t stop = share.apart ? each : (uint32_t)min((uint64_t)each, (uint64_t)offset + left);
+    auto cut = [&](uint32_t x) {
+      return x >= each ? all_chunks : (x <= F::START ? 0 : (int)((uint64_t)(x - F::START) * (uint32_t)all_chunks / (each - F::START)));
+    };
+    const int begin = cut(offset), chunks = cut(stop);
+    const bool whole = offset == 0 && stop == each;
+    if (!share.apart && offset == 0 && tid == 0 && kv_head == 0 && share.tiles_before + place < a.tiles) {
+      const uint64_t tile_end = share.end - left + each;  // in the sequence
+      TileRecord r;
+      r.start = start;
+      r.row = (int)tile * ROWS;
+      r.rows = min(ROWS, rows - (int)tile * ROWS);
+      r.first = (int)worker;
+      r.last = (int)((tile_end * (uint32_t)share.workers - 1) / share.total);
+      a.records[share.tiles_before + place] = r;
+    }
+    left -= min(left, (uint64_t)(stop - offset));
+
+    // ---- codes to registers, as values to LDS -----------------------------------
+    const int32_t* const table = a.table + (int64_t)request * a.W;
+    const int page_mask = (1 << a.page_shift) - 1;
+    // Page number of 16-row group lane & 3 of a chunk, -1 where it holds no keys.
+    auto look_up = [&](int chunk) {
+      const int key = chunk * KC + 16 * (lane & 3);
+      return key < kv_end ? table[min(key >> a.page_shift, a.W - 1)] : -1;
+    };
+    auto row_of_group = [&](int chunk, int id, int group) -> int64_t {  // -1 for none
+      return (uint32_t)id < (uint32_t)a.blocks ? ((int64_t)id << a.page_shift) + ((chunk * KC + 16 * group) & page_mask) : -1;
+    };
+    // Row of this thread's piece n, and its group, the same for all of a wave's (a wave's rows lie in one).
+    // Offsets are worked out anew each time: kept, they would be spilled.
+    auto piece_of = [&](int n, int& column) {
+      const int t = (int)opaque((uint32_t)tid);
+      column = t % TPR;
+      return n * (KC / PIECES) + t / TPR;
+    };
+    auto load_codes = [&](const uint8_t* cache, int chunk, int ids, piece (&to)[PIECES]) {
+#pragma unroll
+      for (int n = 0; n < PIECES; ++n) {
+        int column;
+        const int r = piece_of(n, column), group = (n * (KC / PIECES) + wave * (64 / TPR)) >> 4;
+        const int64_t row = row_of_group(chunk, __builtin_amdgcn_readlane(ids, group), group);
+        const uint8_t* from = cache + ((row < 0 ? 0 : row) * row_bytes + kv_head * D);
+        // Rows that are not there become zeros, which no weight can turn into anything else.
+        const uint32_t off = (uint32_t)(r & 15) * row_bytes + (uint32_t)(PIECE * column);
+        to[n] = piece(0);
+        if (row >= 0) {
+          if (chunk * KC + 16 * group + 16 <= kv_end)
+            to[n] = *(const piece*)(from + off);
+          else if (chunk * KC + r < kv_end)
+            to[n] = *(const piece*)(from + off);
+        }
+      }
+    };
+    auto store_values = [&](const piece (&codes)[PIECES], uint32_t slot, bool is_value) {
+#pragma unroll
+      for (int n = 0; n < PIECES; ++n) {
+        int column;
+        const int r = piece_of(n, column), turn = is_value ? 2 * value_rows<D>(r) : key_rows<D>(r);
+        const uint32_t at = slot + (uint32_t)(r * RB + (((column * (PIECE / 8)) ^ turn) << 4));
+#pragma unroll
+        for (int h = 0; h < PIECE / 8; ++h) {
+          uint32_t lo = codes[n][2 * h], hi = codes[n][2 * h + 1];
+          __asm__ volatile("" : "+v"(lo), "+v"(hi));  // converted here and not a step ahead, where the registers are taken
+          *(AFA_LDS x8*)(uintptr_t)(at ^ (uint32_t)(h << 4)) = Codes<DT, CT>::decode(lo, hi);
+        }
+      }
+    };
+    // Lanes 0 .. 3 of the first wave: key scales of a chunk's groups, 4 .. 7: value scales (0 where it holds no keys).
+    auto load_scale = [&](int chunk, int ids) {
+      const int64_t row = row_of_group(chunk, ids, lane & 3);
+      return wave == 0 && lane < 8 && row >= 0 ? (lane < 4 ? a.k_scale : a.v_scale)[(row >> a.group_shift) * a.HKV + kv_head] : 0.0f;
+    };
+    auto store_figures = [&](float scale, int ids, int chunk) {
+      if (wave != 0 || lane >= 8) return;
+      const bool there = (uint32_t)ids < (uint32_t)a.blocks;
+      float* const to = (float*)figures[chunk & 1];
+      if (lane < 4) {
+        to[lane] = at_least(scale * scale_log2, 1.17549435e-38f);  // not 0: times a hidden score
+      } else {
+        const float vs = at_least(scale, Q8_LEAST_SCALE);
+        to[lane] = there ? __log2f(vs) : -INFINITY;  // a group without keys weighs nothing
+        to[4 + lane] = there ? 1.0f / vs : 0.0f;
+      }
+    };
+
+    x8 qf[QT][KSTEPS];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int row = (int)tile * ROWS + (wave * QT + qt) * 16 + i16;
+      const bool valid = row < rows;
+      const int token = valid ? row / H : 0, head = kv_head * H + (valid ? row - token * H : 0);
+      const scalar* q = (const scalar*)a.q + (int64_t)(start + token) * a.q_t + (int64_t)head * a.q_h + 8 * g;
+#pragma unroll
+      for (int j = 0; j < KSTEPS; ++j)
+        qf[qt][j] = valid ? *(const x8*)(q + 32 * j) : __builtin_bit_cast(x8, u32x4{0u, 0u, 0u, 0u});
+    }
+    f32x4 o[QT][VT];
+    float m_run[QT], l_run[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      m_run[qt] = -1e30f;  // finite: a chunk that hides all its keys gives p = 0, never NaN
+      l_run[qt] = 0.f;
+#pragma unroll
+      for (int t = 0; t < VT; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // Fragment addresses (relative to a slot): rows 16 t + i16 of keys, 16 t + 4 g + (i16 >> 2) of values.
+    const int rv = 4 * g + (i16 >> 2);
+    const uint32_t qk_at = (uint32_t)(i16 * RB + ((g ^ key_rows<D>(i16)) << 4));
+    const uint32_t tr_at = (uint32_t)(rv * RB + (value_rows<D>(rv) << 5) + (i16 & 3) * 8);
+    constexpr int QK_FRAGS = KSTEPS * KT, LOOK = 5;
+    auto qk_chunk = [&](int chunk, f32x4 (&s)[KT][QT], auto&& between) {
+      const uint32_t base = opaque(lds_address(keys[chunk & 1]) + qk_at);
+      x8 kf[QK_FRAGS];
+      auto load = [&](int f) {  // (step j, key tile t)
+        const int j = f / KT, t = f % KT;
+        kf[f] = *(const AFA_LDS x8*)(lds_at<uint8_t>(base ^ (uint32_t)(j << 6)) + t * 16 * RB);
+      };
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) s[t][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int f = 0; f < LOOK; ++f) load(f);
+#pragma unroll
+      for (int f = 0; f < QK_FRAGS; ++f) {
+        if (f + LOOK < QK_FRAGS) load(f + LOOK);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) s[f % KT][qt] = B16<DT>::mfma(kf[f], qf[qt][f / KT], s[f % KT][qt]);
+        between(f);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    constexpr int PV_FRAGS = (KC / 32) * VT;
+    auto pv_chunk = [&](int chunk, x8 (&pf)[QT][KC / 32], auto&& between) {
+      const uint32_t base = opaque(lds_address(values[chunk & 1]) + tr_at);
+      constexpr int VLOOK = 3;
+      x4 lo[PV_FRAGS], hi[PV_FRAGS];
+      auto load = [&](int f) {  // (32 keys ks, column tile t)
+        const int ks = f / VT, t = f % VT;
+        const AFA_LDS uint8_t* p = lds_at<uint8_t>(base ^ (uint32_t)((t & 7) << 5)) + (t >> 3) * 256 + ks * 32 * RB;
+        lo[f] = B16<DT>::read_tr((const AFA_LDS void*)p);
+        hi[f] = B16<DT>::read_tr((const AFA_LDS void*)(p + 16 * RB));
+      };
+#pragma unroll
+      for (int f = 0; f < VLOOK; ++f) load(f);
+#pragma unroll
+      for (int f = 0; f < PV_FRAGS; ++f) {
+        if (f + VLOOK < PV_FRAGS) load(f + VLOOK);
+        const int ks = f / VT, t = f % VT;
+        const x8 vf = {lo[f][0], lo[f][1], lo[f][2], lo[f][3], hi[f][0], hi[f][1], hi[f][2], hi[f][3]};
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) o[qt][t] = B16<DT>::mfma(vf, pf[qt][ks], o[qt][t]);
+        between(f);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto mask = [&](int chunk, f32x4 (&s)[KT][QT]) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        const int row = (int)tile * ROWS + (wave * QT + qt) * 16 + (int)(opaque((uint32_t)tid) & 15u);
+        const int lim = visible(min(row, rows - 1) / H) - chunk * KC;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][qt][i] = 16 * t + 4 * g + i < lim ? s[t][qt][i] : -INFINITY;
+      }
+    };
+
+    auto keys_at = [&](int slot) { return lds_address(keys[0]) + (uint32_t)slot * (KC * RB); };
+    auto values_at = [&](int slot) { return lds_address(values[0]) + (uint32_t)slot * (KC * RB); };
+    if (!first_part) block_barrier();  // the slots are read
+    piece k_codes[PIECES], v_codes[PIECES];
+    f32x4 s_a[KT][QT], s_b[KT][QT];
+    int ids = -1, ids_ahead = -1, ids_v = -1;  // page numbers: of the chunk in k_codes' next load, ...
+    float scale = 0.f;
+    if (begin < chunks) {
+      const int ids0 = look_up(begin), ids1 = look_up(begin + 1);
+      ids = look_up(begin + 2);
+      ids_ahead = look_up(begin + 3);
+      piece first[PIECES];
+      load_codes(a.k, begin, ids0, first);
+      load_codes(a.v, begin, ids0, v_codes);
+      const float scale0 = load_scale(begin, ids0);
+      load_codes(a.k, begin + 1, ids1, k_codes);
+      store_values(first, keys_at(begin & 1), false);
+      store_values(v_codes, values_at(begin & 1), true);
+      store_figures(scale0, ids0, begin);
+      store_values(k_codes, keys_at((begin + 1) & 1), false);
+      load_codes(a.k, begin + 2, ids, k_codes);
+      load_codes(a.v, begin + 1, ids1, v_codes);
+      scale = load_scale(begin + 1, ids1);
+      ids_v = ids1;
+      block_barrier();
+      qk_chunk(begin, s_a, [](int) {});
+    }
+    constexpr int HALF = QT * 8, QK_EXP0 = QT + 2, PV_EXP_STEPS = PV_FRAGS / 2 - 1;
+    constexpr int STORE_V = QK_FRAGS / 2, STORE_K = 0;  // steps that the stores follow
+    auto iteration = [&](int c, f32x4 (&cur)[KT][QT], f32x4 (&nxt)[KT][QT]) {
+      // Keys of chunk c + 1, values and figures of c are stored, and every wave is past QK (c) and PV (c - 1),
+      // whose slots are free.
+      block_barrier();
+      const f32x4 lv = figures[c & 1][1];
+      float sk[KT], iv[KT];  // scalar registers
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        sk[t] = __int_as_float(uniform(__float_as_int(figures[c & 1][0][t])));
+        iv[t] = __int_as_float(uniform(__float_as_int(figures[c & 1][2][t])));
+      }
+      if (c >= clean_chunks) mask(c, cur);
+      x8 pf[QT][KC / 32];
+      float top[QT], m_new[QT], psum[QT];
+      f32x4 shift[QT];
+      auto exp_element = [&](int e) {  // (half, qt, key tile of the half, i)
+        const int h = e / HALF, qt = (e / 8) % QT, t = 2 * h + (e / 4) % 2, i = e % 4;
+        const float p = fast_exp2(__builtin_fmaf(cur[t][qt][i], sk[t], shift[qt][t]));
+        psum[qt] = __builtin_fmaf(p, iv[t], psum[qt]);
+        pf[qt][h][(t & 1) * 4 + i] = (scalar)p;
+      };
+      auto qk_between = [&](int f) {
+        if (f == QK_FRAGS / 2 - 1) __builtin_amdgcn_s_setprio(2);
+        if (f == STORE_V) {
+          store_values(v_codes, values_at((c + 1) & 1), true);  // of chunk c + 1
+          store_figures(scale, ids_v, c + 1);
+        }
+        if (f < QT) {
+          float m = -INFINITY;
+#pragma unroll
+          for (int t = 0; t < KT; ++t)
+            m = fmaxf(m, __builtin_fmaf(fmaxf(fmaxf(cur[t][f][0], cur[t][f][1]), fmaxf(cur[t][f][2], cur[t][f][3])), sk[t], lv[t]));
+          top[f] = m;
+        } else if (f == QT) {
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            m_new[qt] = fmaxf(m_run[qt], max_over_lane_groups(top[qt]));
+            psum[qt] = 0.f;
+          }
+        } else if (f == QT + 1) {
+          bool grow = false;
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) grow |= m_new[qt] > m_run[qt] + q8_tau<DT>();
+          if (__ballot(grow) != 0ull) {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+              const float alpha = fast_exp2(m_run[qt] - m_new[qt]);
+              l_run[qt] *= alpha;
+#pragma unroll
+              for (int t = 0; t < VT; ++t) o[qt][t] *= alpha;
+              m_run[qt] = m_new[qt];
+            }
+          }
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) shift[qt] = lv - m_run[qt];
+        } else {
+#pragma unroll
+          for (int e = 0; e < HALF; ++e)
+            if (QK_EXP0 + e * (QK_FRAGS - QK_EXP0) / HALF == f) exp_element(e);
+        }
+      };
+      auto pv_between = [&](int f) {
+        if (f == PV_FRAGS / 2 - 1) __builtin_amdgcn_s_setprio(0);
+        if (f == STORE_K) store_values(k_codes, keys_at(c & 1), false);  // of chunk c + 2
+        if (f == STORE_K + 1) {
+          load_codes(a.v, c + 2, ids, v_codes);
+          scale = load_scale(c + 2, ids);
+          load_codes(a.k, c + 3, ids_ahead, k_codes);
+          ids_v = ids;
+          ids = ids_ahead;
+          ids_ahead = look_up(c + 4);
+        }
+        if (f < PV_EXP_STEPS) {
+#pragma unroll
+          for (int e = 0; e < HALF; ++e)
+            if (e * PV_EXP_STEPS / HALF == f) exp_element(HALF + e);
+        } else if (f == PV_EXP_STEPS + 1) {
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) l_run[qt] += psum[qt];
+        }
+      };
+      // Wave priority steps down with the wave's progress through a chunk: of the
+      // two waves of a SIMD the one behind wins. The last chunk also runs a QK, over what its slot holds;
+      // nobody reads those scores.
+      __builtin_amdgcn_s_setprio(3);
+      qk_chunk(c + 1, nxt, qk_between);
+      __builtin_amdgcn_s_setprio(1);
+      pv_chunk(c, pf, pv_between);
+    };
+    for (int c = begin; c < chunks; c += 2) {
+      iteration(c, s_a, s_b);
+      if (c + 1 < chunks) iteration(c + 1, s_b, s_a);
+    }
+
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int group = wave * QT + qt, row = (int)tile * ROWS + group * 16 + i16;
+      const float total = sum_over_lane_groups(l_run[qt]);
+      if (!whole) {
+        const int64_t at = ((2 * (int64_t)worker + (offset == 0 ? 1 : 0)) * a.HKV + kv_head) * (ROWS / 16) + group;
+        float* po = a.partial_o + (at * VT * 64 + lane) * 4;
+        if ((int)tile * ROWS + group * 16 < rows) {
+#pragma unroll
+          for (int t = 0; t < VT; ++t) *(f32x4*)(po + t * 256) = o[qt][t];
+          if (g == 0) *(float2*)(a.partial_ml + (at * 16 + i16) * 2) = make_float2(m_run[qt], total);
+        }
+      } else if (row < rows) {
+        const float inv = total > 0.f ? 1.0f / total : 0.f;
+        const int token = row / H, head = kv_head * H + row - token * H;
+        scalar* out = (scalar*)a.out + (int64_t)(start + token) * a.o_t + (int64_t)head * a.o_h + 4 * g;
+#pragma unroll
+        for (int t = 0; t < VT; ++t) {
+          x4 v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[qt][t][i] * inv);
+          *(x4*)(out + 16 * t) = v;
+        }
+        if (a.lse && g == 0) a.lse[(int64_t)(start + token) * (a.HKV * H) + head] = row_lse(m_run[qt], total);
+      }
+    }
+    if (left == 0) return;
+    offset = 0;
+    ++place;
+  }
+}
+
+// Combines the parts of the tiles that several workgroups share, in a fixed order:
+// out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p. A workgroup takes 16 rows of a head.
+// Its waves take a column tile each, and with SPLIT > 1 every SPLIT-th part (few tiles, whose
+// parts are many), joined through LDS; AHEAD parts of loads are in flight.
+template <int DT, int D, int SPLIT>
+__global__ __launch_bounds__(64 * (D / 16) * SPLIT) void quantized_merge_kernel(QuantizedArgs a, int tile_groups) {
+  typedef typename B16<DT>::scalar scalar;
+  typedef typename B16<DT>::x4 x4;
   constexpr int VT = D / 16, AHEAD = 4;
-  const uint32_t groups = (uint32_t)tile_rows / 16;
-  const uint32_t tile = blockIdx.x / groups, group = blockIdx.x % groups;
-  const int kv_head = blockIdx.y;
+  __shared__ f32x4 joined_o[SPLIT > 1 ? SPLIT - 1 : 1][VT][64];
+  __shared__ float2 joined_ml[SPLIT > 1 ? SPLIT - 1 : 1][16];
+  const uint32_t tile = blockIdx.x / (uint32_t)tile_groups;
+  const int group = (int)(blockIdx.x % (uint32_t)tile_groups), kv_head = blockIdx.y;
   if (tile >= *constant((const int32_t*)a.tile_count)) return;
   const TileRecord record = a.records[tile];
-  const int row_of = (int)group * 16 + (threadIdx.x & 15), unit = threadIdx.x >> 4;
-  if (record.first == record.last || row_of >= record.rows) return;
-  const int parts = record.last - record.first + 1;
-  auto slot = [&](int p) {
-    return ((2 * (int64_t)(record.first + p) + (p == 0 ? 1 : 0)) * a.HKV + kv_head) * tile_rows + row_of;
+  if (record.first == record.last || group * 16 >= record.rows) return;
+  const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
+  const int c = wave % VT, sub = wave / VT;
+  const int parts = record.last - record.first + 1, mine = (parts - sub + SPLIT - 1) / SPLIT;  // sub, sub + SPLIT, ...
+  auto slot = [&](int k) {
+    const int p = sub + k * SPLIT;
+    return ((2 * (int64_t)(record.first + p) + (p == 0 ? 1 : 0)) * a.HKV + kv_head) * tile_groups + group;
   };
-  float top = -1e30f, total = 0.f, acc[VT];
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, a.partial_ml[slot(p) * 2]);
-#pragma unroll
-  for (int c = 0; c < VT; ++c) acc[c] = 0.f;
-  for (int p = 0; p < parts; p += AHEAD) {
+  auto sums = [&](int k) { return *(const float2*)(a.partial_ml + (slot(k) * 16 + i16) * 2); };
+  float top = -1e30f, total = 0.f;
+#pragma unroll 4
+  for (int k = g; k < mine; k += 4) top = fmaxf(top, sums(k).x);
+  top = max_over_lane_groups(top);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < mine; k += AHEAD) {
     float2 ml[AHEAD];
-    f32x4 v[AHEAD][VT / 4];
+    f32x4 v[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const int64_t at = slot(min(p + i, parts - 1));
-      ml[i] = *(const float2*)(a.partial_ml + at * 2);
-#pragma unroll
-      for (int j = 0; j < VT / 4; ++j) v[i][j] = *(const f32x4*)(a.partial_o + at * D + VT * unit + 4 * j);
+      const int q = min(k + i, mine - 1);
+      ml[i] = sums(q);
+      v[i] = *(const f32x4*)(a.partial_o + ((slot(q) * VT + c) * 64 + lane) * 4);
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const float weight = p + i < parts ? fast_exp2(ml[i].x - top) : 0.f;
+      const float weight = k + i < mine ? fast_exp2(ml[i].x - top) : 0.f;
       total = __builtin_fmaf(weight, ml[i].y, total);
-#pragma unroll
-      for (int c = 0; c < VT; ++c) acc[c] = __builtin_fmaf(weight, v[i][c / 4][c % 4], acc[c]);
+      o += weight * v[i];
     }
   }
-  const int packed = record.row + row_of, token = packed / a.H, head = kv_head * a.H + packed - token * a.H;
-  const float inv = total > 0.f ? 1.0f / total : 0.f;
-  scalar v[VT];
+  if constexpr (SPLIT > 1) {
+    if (sub > 0) {
+      joined_o[sub - 1][c][lane] = o;
+      if (c == 0 && g == 0) joined_ml[sub - 1][i16] = make_float2(top, total);
+    }
+    __syncthreads();
+    if (sub > 0) return;
+    const float own = top;
 #pragma unroll
-  for (int c = 0; c < VT; ++c) v[c] = (scalar)(acc[c] * inv);
-  scalar* out = (scalar*)a.out + (int64_t)(record.start + token) * a.o_t + (int64_t)head * a.o_h + VT * unit;
-  __builtin_memcpy(__builtin_assume_aligned(out, 2 * VT < 16 ? 2 * VT : 16), v, sizeof(v));
-  if (a.lse && unit == 0) a.lse[(int64_t)(record.start + token) * (a.HKV * a.H) + head] = row_lse(top, total);
+    for (int w = 0; w < SPLIT - 1; ++w) top = fmaxf(top, joined_ml[w][i16].x);
+    const float mine_weight = fast_exp2(own - top);
+    total *= mine_weight;
+    o *= mine_weight;
+#pragma unroll
+    for (int w = 0; w < SPLIT - 1; ++w) {
+      const float2 ml = joined_ml[w][i16];
+      const float weight = fast_exp2(ml.x - top);
+      total = __builtin_fmaf(weight, ml.y, total);
+      o += weight * joined_o[w][c][lane];
+    }
+  }
+  const int r = group * 16 + i16;
+  if (r >= record.rows) return;
+  const int packed = record.row + r, token = packed / a.H, head = kv_head * a.H + packed - token * a.H;
+  const float inv = total > 0.f ? 1.0f / total : 0.f;
+  x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[i] * inv);
+  *(x4*)((scalar*)a.out + (int64_t)(record.start + token) * a.o_t + (int64_t)head * a.o_h + 16 * c + 4 * g) = v;
+  if (a.lse && c == 0 && g == 0) a.lse[(int64_t)(record.start + token) * (a.HKV * a.H) + head] = row_lse(top, total);
 }
 
 namespace {
@@ -490,26 +1012,40 @@ int check_quantized(const QuantizedParams* p) {
   if (p->D != 64 && p->D != 128 && p->D != 256) return AFA_E_SHAPE;
   if (p->GROUP < 16 || (p->GROUP & (p->GROUP - 1)) || p->PAGE < p->GROUP || p->PAGE > (1 << 20) || (p->PAGE & (p->PAGE - 1)))
     return AFA_E_SHAPE;
-  // Packed rows, tiles, positions and the offsets of 64 cache rows are 32-bit numbers.
+  // Packed rows, tiles, positions and the offsets of 16 cache rows are 32-bit numbers.
   if ((int64_t)p->T * p->HQ > 0x7fffff00ll || (int64_t)p->W * p->PAGE > 0x7fffff00ll || p->B > 0x3fffffff) return AFA_E_SHAPE;
   if (p->HKV > 32768) return AFA_E_SHAPE;
   if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return AFA_E_SHAPE;
   return AFA_OK;
 }
 
-constexpr int Q8_SLOTS = 512;  // workgroups of four waves that the GPU holds
+constexpr int Q8_CUS = 256;
+constexpr int64_t Q8_STREAM_BYTES = 128ll << 20;
 
+// Form of a call. Tile form (256 rows; D = 256: 128) where a request has more than 256 rows on average and
+// its table room for 1536 (2000 tokens of 32 heads, 8 of them key/value heads, behind 18000: 675 us, 924 in the
+// stream form with 32 rows; 8 requests of 375 behind 1100 137 and 137; 1 of 1000 behind none 51 and 43, 16 of 48 behind
+// 2200 77 and 71). Below, tiles of 32 rows, or 16 where that holds a request. In the stream form a workgroup takes as
+// many neighbouring heads as leaves a tile at most 8 workgroups of its own (64 requests of 16K, 8 heads 286 us with 4, 298
+// with 2, 336 with 1; one of 16K 58, 39 and 29, since a part a workgroup has to be joined).
 struct QuantizedPlan {
-  int rows;       // of a tile
-  int workers;    // per key/value head
+  int rows;       // of a tile: 16 or 32 in the stream form, 128 or 256 in the tile form
+  int heads;      // key/value heads of a workgroup
+  int workers;    // workgroups of such heads
   int64_t tiles;  // the most that monotone cu_seqlens_q can give
+  bool stream;    // non-temporal loads
 };
 QuantizedPlan plan_quantized(const QuantizedParams* p) {
-  const int64_t H = p->HQ / p->HKV;
+  const int64_t H = p->HQ / p->HKV, each = ((int64_t)p->T + p->B - 1) / p->B * H;  // rows of a request
   QuantizedPlan plan;
-  plan.rows = ((int64_t)p->T + p->B - 1) / p->B * H > 16 ? 32 : 16;
-  plan.workers = std::max(1, Q8_SLOTS / p->HKV);
+  const bool tile_form = each > 256 && (int64_t)p->W * p->PAGE >= 1536;
+  plan.rows = tile_form ? (p->D == 256 ? 128 : 256) : each > 16 ? 32 : 16;
   plan.tiles = p->T * H / plan.rows + p->B;
+  plan.stream = p->D >= 128 && each <= 16 && 2ll * p->BLOCKS * p->PAGE * p->HKV * p->D >= Q8_STREAM_BYTES;
+  plan.heads = tile_form ? 1 : p->HKV % 4 == 0 ? 4 : p->HKV % 2 == 0 ? 2 : 1;
+  const int slots = tile_form || p->D == 256 ? Q8_CUS : 2 * Q8_CUS;
+  while (plan.heads > 1 && (int64_t)slots * plan.heads / p->HKV > 8 * plan.tiles) plan.heads /= 2;
+  plan.workers = std::max(1, slots / (p->HKV / plan.heads));
   return plan;
 }
 int64_t quantized_part_rows(const QuantizedPlan& plan, int HKV) { return 2ll * plan.workers * HKV * plan.rows; }
@@ -518,10 +1054,41 @@ uint64_t quantized_bytes(const QuantizedParams* p, const QuantizedPlan& plan) {
   return (uint64_t)(quantized_part_rows(plan, p->HKV) * (p->D + 2) * 4 + plan.tiles * (int64_t)sizeof(TileRecord) + 16);
 }
 
+template <int DT, int CT, int D, int QT, int HW>
+int launch_stream(const QuantizedArgs& a, const QuantizedPlan& plan, hipStream_t s) {
+  const dim3 grid((unsigned)(plan.workers * (a.HKV / HW))), block(256);
+  if constexpr (D >= 128 && QT == 1) {
+    if (plan.stream) {
+      hipLaunchKernelGGL((quantized_stream_kernel<DT, CT, D, QT, HW, true>), grid, block, 0, s, a);
+      return (int)hipGetLastError();
+    }
+  }
+  hipLaunchKernelGGL((quantized_stream_kernel<DT, CT, D, QT, HW, false>), grid, block, 0, s, a);
+  return (int)hipGetLastError();
+}
+template <int DT, int CT, int D, int QT>
+int launch_heads(const QuantizedArgs& a, const QuantizedPlan& plan, hipStream_t s) {
+  if (plan.heads == 4) return launch_stream<DT, CT, D, QT, 4>(a, plan, s);
+  if (plan.heads == 2) return launch_stream<DT, CT, D, QT, 2>(a, plan, s);
+  return launch_stream<DT, CT, D, QT, 1>(a, plan, s);
+}
+
+template <int DT, int CT, int D>
+int launch_form(const QuantizedArgs& a, const QuantizedPlan& plan, hipStream_t s) {
+  if (plan.rows == 16) return launch_heads<DT, CT, D, 1>(a, plan, s);
+  if (plan.rows == 32) return launch_heads<DT, CT, D, 2>(a, plan, s);
+  // Eight waves of 16 or 32 rows, of one head each.
+  hipLaunchKernelGGL((quantized_tile_kernel<DT, CT, D, D == 256 ? 1 : 2>), dim3((unsigned)(plan.workers * a.HKV)), dim3(512), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+// Merge workgroups up to here split their parts over 16 waves in all.
+constexpr int64_t Q8_FEW_JOBS = 512;
+
 template <int DT, int CT, int D>
 int launch_quantized(QuantizedArgs a, const QuantizedPlan& plan, void* workspace, hipStream_t s) {
   const int64_t groups = plan.tiles * (plan.rows / 16);
-  if (groups > 0xffffffffll / 256) return AFA_E_SHAPE;  // a launch counts its threads in 32 bits
+  if (groups > 0xffffffffll / 1024) return AFA_E_SHAPE;  // a launch counts its threads in 32 bits
   const int64_t part_rows = quantized_part_rows(plan, a.HKV);
   a.workers = plan.workers;
   a.partial_o = (float*)workspace;
@@ -529,14 +1096,13 @@ int launch_quantized(QuantizedArgs a, const QuantizedPlan& plan, void* workspace
   a.tile_count = (uint32_t*)(a.partial_ml + part_rows * 2);
   a.records = (TileRecord*)(a.tile_count + 4);
   a.tiles = (uint32_t)plan.tiles;
-  const dim3 grid((unsigned)(plan.workers * a.HKV));
-  if (plan.rows == 16)
-    hipLaunchKernelGGL((quantized_stream_kernel<DT, CT, D, 1>), grid, dim3(256), 0, s, a);
+  const int e = launch_form<DT, CT, D>(a, plan, s);
+  if (e) return e;
+  const dim3 grid((unsigned)groups, (unsigned)a.HKV);
+  if (groups * a.HKV <= Q8_FEW_JOBS && D < 256)
+    hipLaunchKernelGGL((quantized_merge_kernel<DT, D, D == 256 ? 1 : 256 / D>), grid, dim3(1024), 0, s, a, plan.rows / 16);
   else
-    hipLaunchKernelGGL((quantized_stream_kernel<DT, CT, D, 2>), grid, dim3(256), 0, s, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL((quantized_merge_kernel<DT, D>), dim3((unsigned)groups, (unsigned)a.HKV), dim3(256), 0, s, a, plan.rows);
+    hipLaunchKernelGGL((quantized_merge_kernel<DT, D, 1>), grid, dim3(4 * D), 0, s, a, plan.rows / 16);
   return (int)hipGetLastError();
 }
 
@@ -559,14 +1125,16 @@ extern "C" int workspace_size_quantized_attention(uint64_t* bytes, const Quantiz
   return AFA_OK;
 }
 
-extern "C" int form_quantized_attention(int64_t form[2], const QuantizedParams* p) {
+extern "C" int form_quantized_attention(int64_t form[4], const QuantizedParams* p) {
   using namespace afa;
   if (!form) return AFA_E_NULL;
   const int status = check_quantized(p);
   if (status) return status;
   const QuantizedPlan plan = plan_quantized(p);
   form[0] = plan.rows;
-  form[1] = plan.workers;
+  form[1] = plan.heads;
+  form[2] = plan.workers;
+  form[3] = plan.stream ? 1 : 0;
   return AFA_OK;
 }
 

@@ -487,10 +487,12 @@ int launch_quantized_attention(void* stream, const void* q, const void* k_cache,
                                void* workspace, uint64_t workspace_bytes, const QuantizedParams* params);
 
 /* Bytes of that workspace, on 16 bytes, and which form a call of these sizes
- * runs: form[0] packed (token, head) rows per tile, form[1] workgroups of a
- * key/value head that share the tiles. */
+ * runs: form[0] packed (token, head) rows per tile (16 or 32: waves on their own,
+ * 128 or 256: a workgroup of eight), form[1] key/value heads of a workgroup,
+ * form[2] workgroups of the same heads that share the tiles, form[3] 1 for cache
+ * loads that stay out of the caches. */
 int workspace_size_quantized_attention(uint64_t* bytes, const QuantizedParams* params);
-int form_quantized_attention(int64_t form[2], const QuantizedParams* params);
+int form_quantized_attention(int64_t form[4], const QuantizedParams* params);
 
 /* Copies page source[i] to page destination[i], i < pairs, in each of n_caches
  * tensors of BLOCKS pages (caches: device pointers, page_bytes: bytes of a page,

@@ -54,7 +54,7 @@ def test_append_pointers(lib, missing):
     ({"scale": 0.0}, -2), ({"scale": -1.0}, -2), ({"scale": math.nan}, -2), ({"scale": math.inf}, -2),
 ])
 def test_attention_rejections(lib, changes, status):
-    size, form = ct.c_uint64(), (ct.c_int64 * 2)()
+    size, form = ct.c_uint64(), (ct.c_int64 * 4)()
     params = ct.byref(attention(**changes))
     assert lib.launch_quantized_attention(None, *[p16] * 11, 1 << 30, params) == status
     assert lib.workspace_size_quantized_attention(ct.byref(size), params) == status
@@ -62,7 +62,7 @@ def test_attention_rejections(lib, changes, status):
 
 
 def test_attention_pointers_strides_and_workspace(lib):
-    size, form = ct.c_uint64(), (ct.c_int64 * 2)()
+    size, form = ct.c_uint64(), (ct.c_int64 * 4)()
     params = ct.byref(attention())
     launch = lambda pointers, workspace, nbytes, p=params: lib.launch_quantized_attention(None, *pointers, workspace, nbytes, p)
     pointers = [p16] * 9 + [None]
@@ -78,7 +78,25 @@ def test_attention_pointers_strides_and_workspace(lib):
     assert launch(pointers, P(8), size.value) == -4
     assert launch(pointers, None, 0, ct.byref(attention(T=0))) == 0
     assert lib.workspace_size_quantized_attention(None, params) == -1 and lib.form_quantized_attention(None, params) == -1
-    assert lib.form_quantized_attention(form, params) == 0 and form[0] >= 16 and form[1] >= 0
+    assert lib.form_quantized_attention(form, params) == 0 and list(form) == [16, 1, 256, 0]
+
+
+@pytest.mark.parametrize("changes,form", [
+    (dict(T=64, B=64, HQ=64, HKV=8, W=256, PAGE=64, BLOCKS=16384), [16, 4, 256, 1]),   # 64 requests of 16K
+    (dict(T=64, B=64, HQ=64, HKV=8, W=256, PAGE=64, BLOCKS=500), [16, 4, 256, 0]),     # 65 MB of cache
+    (dict(T=64, B=64, HQ=64, HKV=8, D=64, W=256, PAGE=64, BLOCKS=16384), [16, 4, 256, 0]),
+    (dict(T=64, B=64, HQ=64, HKV=8, D=256, W=256, PAGE=64, BLOCKS=16384), [16, 4, 128, 1]),
+    (dict(T=192, B=48, HQ=32, HKV=4, D=64), [32, 4, 512, 0]),
+    (dict(T=1, B=1, HQ=32, HKV=8), [16, 1, 64, 0]),
+    (dict(T=2000, B=1, HQ=32, HKV=8, PAGE=128, W=157, BLOCKS=157), [256, 1, 32, 0]),
+    (dict(T=2000, B=1, HQ=32, HKV=8, PAGE=128, W=11, BLOCKS=157), [32, 4, 256, 0]),    # no room for 1536 rows
+    (dict(T=2000, B=1, HQ=32, HKV=8, D=256, PAGE=128, W=157, BLOCKS=157), [128, 1, 32, 0]),
+    (dict(T=64, B=1, HQ=32, HKV=8, PAGE=128, W=157, BLOCKS=157), [32, 1, 64, 0]),
+    (dict(T=5, B=5, HQ=2000, HKV=2000, W=157), [16, 4, 1, 0]),
+])
+def test_forms(lib, changes, form):
+    got = (ct.c_int64 * 4)()
+    assert lib.form_quantized_attention(got, ct.byref(attention(**changes))) == 0 and list(got) == form
 
 
 def test_copy_rejections(lib):
