@@ -70,7 +70,8 @@ struct ForkArgs {
   int32_t* source;
   int32_t* destination;
   int32_t* missing;
-  int32_t* rows;      // workspace [B][W]: the table afterwards
+  int32_t* rows;      // workspace [B][W]: rows of other parents
+  int32_t* tails;     // workspace [B]
   int32_t* free_list; // workspace [BLOCKS]
   int32_t B, W, BLOCKS, page_shift, reserve;
 };
@@ -95,7 +96,8 @@ struct ForkRow {
   }
 };
 
-// Each row from its parent's, into the workspace, and the references that change with it.
+// Each row from its parent's, into the workspace (but for what a row keeps of its own), the references that change
+// with it, and the page that it will go on writing to, -1 where its next token starts a page.
 __global__ __launch_bounds__(256) void fork_rows_kernel(ForkArgs a) {
   const int b = (int)blockIdx.y;
   const ForkRow row(a, b);
@@ -103,8 +105,13 @@ __global__ __launch_bounds__(256) void fork_rows_kernel(ForkArgs a) {
   if (column >= a.W) return;
   const int64_t at = (int64_t)b * a.W + column;
   const int32_t old = a.table[at];
-  const int32_t now = row.parent >= 0 && column < row.held ? a.table[(int64_t)row.parent * a.W + column] : -1;
-  a.rows[at] = now;
+  int32_t now = -1;
+  if (row.parent >= 0 && column < row.held) now = row.parent == b ? old : a.table[(int64_t)row.parent * a.W + column];
+  if (column == min(row.held, (int64_t)a.W) - 1 || (row.held == 0 && column == 0)) {
+    const bool partial = row.parent >= 0 && (row.used & ((1 << a.page_shift) - 1)) && row.held <= a.W;
+    a.tails[b] = partial && names_page(now, a.BLOCKS) ? now : -1;
+  }
+  if (row.parent != b) a.rows[at] = now;
   if (old == now) return;
   if (names_page(old, a.BLOCKS)) atomicSub(a.counts + old, 1);
   if (names_page(now, a.BLOCKS)) atomicAdd(a.counts + now, 1);
@@ -128,22 +135,26 @@ __device__ __forceinline__ int block_scan(int v, int& total, int* words) {
   return before + upto - v;
 }
 
-// One workgroup: which rows need a page of their own, the free pages, and who gets which.
+// The first workgroup: which rows need a page of their own, the free pages, who gets which, and the columns of the table
+// that it decides: of a living row the last one that its tokens take and the reserved ones. The others bring the rest.
 __global__ __launch_bounds__(TABLE_THREADS) void fork_assign_kernel(ForkArgs a) {
   __shared__ int32_t tails[FORK_MAX_B];
   __shared__ int words[TABLE_THREADS / 64];
   __shared__ int64_t lacks[TABLE_THREADS / 64];
   const int tid = threadIdx.x;
-  // The page that a row will go on writing to, -1 where its next token starts a page.
-  for (int b = tid; b < a.B; b += TABLE_THREADS) {
+  if (blockIdx.x > 0) {
+    const int64_t at = (int64_t)(blockIdx.x - 1) * TABLE_THREADS + tid;
+    if (at >= (int64_t)a.B * a.W) return;
+    const int b = (int)(at / a.W), column = (int)(at - (int64_t)b * a.W);
     const ForkRow row(a, b);
-    int32_t tail = -1;
-    if (row.parent >= 0 && (row.used & ((1 << a.page_shift) - 1)) && row.held <= a.W) {
-      tail = a.rows[(int64_t)b * a.W + row.held - 1];
-      if (!names_page(tail, a.BLOCKS)) tail = -1;
-    }
-    tails[b] = tail;
+    if (row.parent >= 0 && column >= row.held - 1 && column < max(row.most, row.held)) return;
+    if (row.parent < 0 || column >= row.held)
+      a.table[at] = -1;
+    else if (row.parent != b)
+      a.table[at] = a.rows[at];
+    return;
   }
+  for (int b = tid; b < a.B; b += TABLE_THREADS) tails[b] = a.tails[b];
   __syncthreads();
   // All but the lowest of the rows that share such a page take a copy; all, where others hold it too.
   uint32_t copies = 0;  // bit i: row tid + i * TABLE_THREADS
@@ -155,6 +166,7 @@ __global__ __launch_bounds__(TABLE_THREADS) void fork_assign_kernel(ForkArgs a) 
     if (tail >= 0) {
       int same = 0;
       bool lowest = true;
+#pragma unroll 8
       for (int other = 0; other < a.B; ++other) {
         const bool equal = tails[other] == tail;
         same += equal;
@@ -225,7 +237,8 @@ __global__ __launch_bounds__(TABLE_THREADS) void fork_assign_kernel(ForkArgs a) 
     first += total;
     if (b < a.B) {
       int32_t from = -1, to = -1;
-      int32_t* const rows = a.rows + (int64_t)b * a.W;
+      int32_t* const rows = a.table + (int64_t)b * a.W;
+      const ForkRow row(a, b);
       auto take = [&](int64_t column) {
         const int32_t page = at < found ? a.free_list[at] : -1;
         ++at;
@@ -239,6 +252,8 @@ __global__ __launch_bounds__(TABLE_THREADS) void fork_assign_kernel(ForkArgs a) 
       if (copied) {
         to = take(held - 1);
         from = to >= 0 ? tails[b] : -1;
+      } else if (row.parent >= 0 && row.parent != b && held > 0 && held <= a.W) {
+        rows[held - 1] = a.rows[(int64_t)b * a.W + held - 1];
       }
       for (int64_t c = held; c < end; ++c) take(c);
       a.source[b] = from;
@@ -258,11 +273,6 @@ __global__ __launch_bounds__(TABLE_THREADS) void fork_assign_kernel(ForkArgs a) 
   }
 }
 
-__global__ __launch_bounds__(256) void fork_store_kernel(ForkArgs a) {
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x), n = (int64_t)a.B * a.W;
-  if (at < n) a.table[at] = a.rows[at];
-}
-
 // ---- compaction ----------------------------------------------------------------
 
 constexpr int SEGMENT = 256 * 16;  // pages of a workgroup
@@ -273,10 +283,12 @@ struct CompactArgs {
   int32_t* source;
   int32_t* destination;
   int32_t* segments;  // workspace: pages in use of each segment
-  int32_t* renamed;   // workspace [BLOCKS]: the new number of a page that moves, -1 of one that stays
+  int32_t* moves;     // workspace [BLOCKS]: of a page that moves, which move it is, else -1
   int64_t entries;    // of the table
   int32_t BLOCKS;
 };
+// Segments up to here are counted by every workgroup for itself, one launch less.
+constexpr int FEW_SEGMENTS = 4;
 
 __device__ __forceinline__ int sum_256(int v, int* words) {
   const int upto = wave_inclusive_scan(v);
@@ -289,6 +301,7 @@ __device__ __forceinline__ int sum_256(int v, int* words) {
 __global__ __launch_bounds__(256) void compact_count_kernel(CompactArgs a) {
   __shared__ int words[4];
   int mine = 0;
+#pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int64_t page = (int64_t)blockIdx.x * SEGMENT + i * 256 + threadIdx.x;
     mine += page < a.BLOCKS && a.counts[page] > 0;
@@ -299,47 +312,58 @@ __global__ __launch_bounds__(256) void compact_count_kernel(CompactArgs a) {
 
 // With n pages in use, the k-th of those from n on moves to the k-th free one below n.
 __global__ __launch_bounds__(256) void compact_moves_kernel(CompactArgs a, int segments) {
-  __shared__ int words[4], lane_sums[4];
+  __shared__ int words[4], round_sums[16][4];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  int before = 0, all = 0;
-  for (int i = tid; i < segments; i += 256) {
-    const int v = a.segments[i];
-    all += v;
-    if (i < (int)blockIdx.x) before += v;
+  const int64_t base = (int64_t)blockIdx.x * SEGMENT;
+  uint32_t bits = 0;  // bit i: page base + 256 i + tid is in use
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t page = base + i * 256 + tid;
+    bits |= page < a.BLOCKS && a.counts[page] > 0 ? 1u << i : 0u;
+  }
+  int before = 0, all = 0, stays = 0;
+  if (segments <= FEW_SEGMENTS) {
+    for (int64_t i = tid; i < a.BLOCKS; i += 256) {
+      const int v = a.counts[i] > 0;
+      all += v;
+      before += i < base ? v : 0;
+    }
+  } else {
+    for (int i = tid; i < segments; i += 256) {
+      const int v = a.segments[i];
+      all += v;
+      before += i < (int)blockIdx.x ? v : 0;
+    }
   }
   const int n = sum_256(all, words);
   before = sum_256(before, words);
-  // In use below n: the pages that stay. Those from n on are the moves.
-  const int64_t base = (int64_t)blockIdx.x * SEGMENT;
-  int stays = 0;  // counted by every workgroup: the segments before n's and its own part
-  {
-    const int whole = n / SEGMENT;
-    int v = 0;
-    for (int i = tid; i < whole; i += 256) v += a.segments[i];
-    for (int i = whole * SEGMENT + tid; i < n; i += 256) v += a.counts[i] > 0;
-    stays = sum_256(v, words);
+  // In use below n: the pages that stay.
+  const int whole = segments <= FEW_SEGMENTS ? 0 : n / SEGMENT;
+  for (int i = tid; i < whole; i += 256) stays += a.segments[i];
+  for (int i = whole * SEGMENT + tid; i < n; i += 256) stays += a.counts[i] > 0;
+  stays = sum_256(stays, words);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint64_t wave_bits = __ballot(bits >> i & 1u);
+    if (lane == 0) round_sums[i][wave] = __popcll(wave_bits);
   }
+  __syncthreads();
   int used = before;  // pages in use ahead of this round's
+#pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int64_t page = base + i * 256 + tid;
-    const bool here = page < a.BLOCKS;
-    const int in_use = here && a.counts[page] > 0;
-    const int upto = wave_inclusive_scan(in_use);
-    __syncthreads();
-    if (lane == 63) lane_sums[wave] = upto;
-    __syncthreads();
-    int ahead = used + upto - in_use;
+    const bool in_use = bits >> i & 1u;
+    int ahead = used + __popcll(__ballot(in_use) & ((1ull << lane) - 1));
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      if (w < wave) ahead += lane_sums[w];
-      used += lane_sums[w];
+      if (w < wave) ahead += round_sums[i][w];
+      used += round_sums[i][w];
     }
-    if (here) {
-      if (page < n) {
-        if (!in_use) a.destination[page - ahead] = (int)page;
-      } else if (in_use) {
-        a.source[ahead - stays] = (int)page;
-      }
+    if (page < a.BLOCKS) {
+      const int move = page >= n && in_use ? ahead - stays : -1;
+      a.moves[page] = move;
+      if (move >= 0) a.source[move] = (int)page;
+      if (page < n && !in_use) a.destination[page - ahead] = (int)page;
     }
   }
   const int moves = n - stays;
@@ -348,27 +372,23 @@ __global__ __launch_bounds__(256) void compact_moves_kernel(CompactArgs a, int s
       a.source[i] = -1;
       a.destination[i] = -1;
     }
-  for (int i = 0; i < 16; ++i)
-    if (base + i * 256 + tid < a.BLOCKS) a.renamed[base + i * 256 + tid] = -1;
 }
 
-__global__ __launch_bounds__(256) void compact_counts_kernel(CompactArgs a) {
+// The table's entries, and the counts of the pages that moved.
+__global__ __launch_bounds__(256) void compact_rename_kernel(CompactArgs a) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.BLOCKS / 2) return;
-  const int from = a.source[i], to = a.destination[i];
-  if (from < 0) return;
-  a.renamed[from] = to;
-  a.counts[to] = a.counts[from];
-  a.counts[from] = 0;
-}
-
-__global__ __launch_bounds__(256) void compact_table_kernel(CompactArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.entries) return;
-  const int32_t page = a.table[i];
-  if (!names_page(page, a.BLOCKS)) return;
-  const int32_t to = a.renamed[page];
-  if (to >= 0) a.table[i] = to;
+  if (i < a.entries) {
+    const int32_t page = a.table[i];
+    const int32_t move = names_page(page, a.BLOCKS) ? a.moves[page] : -1;
+    if (move >= 0) a.table[i] = a.destination[move];
+  }
+  if (i < a.BLOCKS / 2) {
+    const int from = a.source[i];
+    if (from >= 0) {
+      a.counts[a.destination[i]] = a.counts[from];
+      a.counts[from] = 0;
+    }
+  }
 }
 
 namespace {
@@ -382,7 +402,7 @@ int power_shift(int32_t power) {
 int check_fork(const ForkPagesParams* p) {
   if (!p) return AFA_E_NULL;
   if (p->B <= 0 || p->B > FORK_MAX_B || p->W <= 0 || p->BLOCKS <= 0 || p->reserve < 0) return AFA_E_SHAPE;
-  if (p->PAGE <= 0 || (p->PAGE & (p->PAGE - 1)) || p->W > 1 << 24) return AFA_E_SHAPE;
+  if (p->PAGE <= 0 || (p->PAGE & (p->PAGE - 1)) || p->W > 1 << 24 || (int64_t)p->B * p->W >= 1ll << 31) return AFA_E_SHAPE;
   return AFA_OK;
 }
 
@@ -435,7 +455,7 @@ extern "C" int workspace_size_fork_pages(uint64_t* bytes, const ForkPagesParams*
   if (!bytes) return AFA_E_NULL;
   const int status = check_fork(p);
   if (status) return status;
-  *bytes = rounded(4ull * p->B * p->W) + rounded(4ull * p->BLOCKS);
+  *bytes = rounded(4ull * p->B * p->W) + rounded(4ull * p->BLOCKS) + rounded(4ull * p->B);
   return AFA_OK;
 }
 
@@ -458,6 +478,7 @@ extern "C" int launch_fork_pages(void* stream, int32_t* block_table, int32_t* pa
   a.missing = missing;
   a.rows = (int32_t*)workspace;
   a.free_list = (int32_t*)((uint8_t*)workspace + rounded(4ull * p->B * p->W));
+  a.tails = (int32_t*)((uint8_t*)a.free_list + rounded(4ull * p->BLOCKS));
   a.B = p->B;
   a.W = p->W;
   a.BLOCKS = p->BLOCKS;
@@ -465,8 +486,8 @@ extern "C" int launch_fork_pages(void* stream, int32_t* block_table, int32_t* pa
   a.reserve = p->reserve;
   hipStream_t s = (hipStream_t)stream;
   hipLaunchKernelGGL(fork_rows_kernel, dim3((unsigned)((a.W + 255) / 256), (unsigned)a.B), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(fork_assign_kernel, dim3(1), dim3(TABLE_THREADS), 0, s, a);
-  hipLaunchKernelGGL(fork_store_kernel, dim3((unsigned)(((int64_t)a.B * a.W + 255) / 256)), dim3(256), 0, s, a);
+  const int64_t others = ((int64_t)a.B * a.W + TABLE_THREADS - 1) / TABLE_THREADS;
+  hipLaunchKernelGGL(fork_assign_kernel, dim3((unsigned)(1 + others)), dim3(TABLE_THREADS), 0, s, a);
   return (int)hipGetLastError();
 }
 
@@ -497,13 +518,13 @@ extern "C" int launch_compact_pages(void* stream, int32_t* block_table, int32_t*
   a.source = source;
   a.destination = destination;
   a.segments = (int32_t*)workspace;
-  a.renamed = (int32_t*)((uint8_t*)workspace + rounded(4ull * segments));
+  a.moves = (int32_t*)((uint8_t*)workspace + rounded(4ull * segments));
   a.entries = (int64_t)p->B * p->W;
   a.BLOCKS = p->BLOCKS;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(compact_count_kernel, dim3((unsigned)segments), dim3(256), 0, s, a);
+  if (segments > FEW_SEGMENTS) hipLaunchKernelGGL(compact_count_kernel, dim3((unsigned)segments), dim3(256), 0, s, a);
   hipLaunchKernelGGL(compact_moves_kernel, dim3((unsigned)segments), dim3(256), 0, s, a, segments);
-  hipLaunchKernelGGL(compact_counts_kernel, dim3((unsigned)((a.BLOCKS / 2 + 255) / 256)), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(compact_table_kernel, dim3((unsigned)((a.entries + 255) / 256)), dim3(256), 0, s, a);
+  const int64_t items = std::max<int64_t>(a.entries, a.BLOCKS / 2);
+  hipLaunchKernelGGL(compact_rename_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }

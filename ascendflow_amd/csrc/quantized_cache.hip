@@ -72,6 +72,21 @@ __device__ __forceinline__ uint32_t encode2(float a, float b) {
   }
 }
 
+// Four codes from values that round to codes. int8: next to 1.5 * 2^23 a float32 keeps whole numbers, in its low bits.
+template <int CT>
+__device__ __forceinline__ uint32_t encode4(const float* v) {
+#pragma clang fp contract(off)
+  if constexpr (CT == AFA_CODE_E4M3) {
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
+  } else {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(v[i] + 12582912.0f);
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), 0x05040100u);
+  }
+}
+
 template <int CT>
 __device__ __forceinline__ float decode1(uint32_t code) {
   if constexpr (CT == AFA_CODE_E4M3)
@@ -80,9 +95,13 @@ __device__ __forceinline__ float decode1(uint32_t code) {
     return (float)(int8_t)code;
 }
 
+template <int DT, int VEC> struct Piece16 { typedef typename B16<DT>::x8 type; };
+template <int DT> struct Piece16<DT, 1> { typedef typename B16<DT>::scalar type __attribute__((ext_vector_type(1))); };
+
 // VEC columns of a row: 8 (16 bytes of new values, 8 of codes) or 1.
 template <int DT, int CT, int VEC>
 __global__ __launch_bounds__(256) void append_quantized_kernel(AppendQuantizedArgs a) {
+#pragma clang fp contract(off)  // x / s is rounded before it becomes a code
   typedef typename B16<DT>::scalar scalar;
   typedef typename B16<DT>::x8 x8;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -130,27 +149,66 @@ __global__ __launch_bounds__(256) void append_quantized_kernel(AppendQuantizedAr
   const int at = block << a.group_shift;              // position of the block's first row
   const int low = max(first, at), high = min(limit, at + G);
   const int64_t token = (int64_t)count + (low - first);  // at position `low`
+  const int pieces = a.D / VEC, held = low - at, rows = high - low;
+  const scalar* const x = (const scalar*)a.x[which] + token * a.x_t[which] + head * a.x_h[which];
+  // The new rows, KEEP pieces of which stay in registers between the two passes: every one of 64 rows of 128 columns.
+  constexpr int KEEP = VEC == 8 ? 16 : 8;
+  typedef typename Piece16<DT, VEC>::type piece;
+  const uint32_t n = (uint32_t)(rows * pieces);
+  auto new_piece = [&](uint32_t i) {
+    const uint32_t r = q8_divide(i, a.pieces_m), c = i - r * (uint32_t)pieces;
+    return *(const piece*)(x + r * a.x_t[which] + c * VEC);
+  };
+  piece kept[KEEP];
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const uint32_t i = lane + 64u * k;
+    if (64u * k < n) kept[k] = new_piece(min(i, n - 1));  // a piece again where there is none: the same largest magnitude
+  }
+  // Under way before the page is known.
   const int page = a.table[(int64_t)request * a.W + (at >> a.page_shift)];
   if (page < 0 || page >= a.BLOCKS) return;
   const int64_t row0 = ((int64_t)page << a.page_shift) + (at & ((1 << a.page_shift) - 1));
   float* const scale_at = a.scale[which] + (row0 >> a.group_shift) * a.HKV + head;
-  const int pieces = a.D / VEC, held = low - at, rows = high - low;
   const int64_t row_stride = (int64_t)a.HKV * a.D;
   uint8_t* const codes = a.cache[which] + (row0 * a.HKV + head) * a.D;
-  const scalar* const x = (const scalar*)a.x[which] + token * a.x_t[which] + head * a.x_h[which];
   const float had = held > 0 ? *scale_at : 0.0f;
 
+  // The largest magnitude: of 16-bit values two at a time, where it is finite, else one by one.
   uint32_t top = 0;
-  for (uint32_t i = lane; i < (uint32_t)(rows * pieces); i += 64) {
-    const uint32_t r = q8_divide(i, a.pieces_m), c = i - r * (uint32_t)pieces;
-    const scalar* p = x + r * a.x_t[which] + c * VEC;
+  bool finite = false;
+  if constexpr (VEC == 8) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0};
+    auto largest2 = [&](const piece& p) {
+      const u32x4 w = __builtin_bit_cast(u32x4, p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+      if (64u * k < n) largest2(kept[k]);
+    for (uint32_t i = lane + 64u * KEEP; i < n; i += 64) largest2(new_piece(i));
+    const uint32_t bits = wave_max_bits(max((uint32_t)most[0], (uint32_t)most[1]));
+    finite = __builtin_amdgcn_readfirstlane((int)bits) < (DT == DT_BF16 ? 0x7f80 : 0x7c00);
+    top = __float_as_uint((float)__builtin_bit_cast(scalar, (uint16_t)bits));
+  }
+  if (!finite) top = 0;
+  auto largest = [&](const piece& p) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       const uint32_t bits = __float_as_uint((float)p[e]) & 0x7fffffffu;
       top = max(top, bits < 0x7f800000u ? bits : 0u);
     }
+  };
+  if (!finite) {
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+      if (64u * k < n) largest(kept[k]);
+    for (uint32_t i = lane + 64u * KEEP; i < n; i += 64) largest(new_piece(i));
+    top = wave_max_bits(top);
   }
-  float now = needed_scale<CT>(wave_max_bits(top));
+  float now = needed_scale<CT>(top);
   if (held > 0) now = now > had ? now : (had == had ? had : now);
   const float inverse = 1.0f / now;
 
@@ -170,19 +228,35 @@ __global__ __launch_bounds__(256) void append_quantized_kernel(AppendQuantizedAr
       const uint32_t r = q8_divide(i, a.pieces_m), c = i - r * (uint32_t)pieces;
       uint8_t* p = codes + r * row_stride + c * VEC;
       float v[VEC];
+      if constexpr (VEC == 8) {
+        const u32x2 w = *(const u32x2*)p;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = decode1<CT>(p[e]) * had * inverse;
+        for (int e = 0; e < VEC; ++e) v[e] = decode1<CT>((w[e / 4] >> (8 * (e % 4))) & 0xffu) * had * inverse;
+      } else {
+        v[0] = decode1<CT>(*p) * had * inverse;
+      }
       put(p, v);
     }
   }
-  for (uint32_t i = lane; i < (uint32_t)(rows * pieces); i += 64) {
+  auto put_new = [&](uint32_t i, const piece& p) {
     const uint32_t r = q8_divide(i, a.pieces_m), c = i - r * (uint32_t)pieces;
-    const scalar* p = x + r * a.x_t[which] + c * VEC;
+    uint8_t* const to = codes + (held + (int)r) * row_stride + c * VEC;
     float v[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = (float)p[e] * inverse;
-    put(codes + (held + (int)r) * row_stride + c * VEC, v);
-  }
+    if (VEC == 8 && finite) {  // nothing to hold inside the range: the scale holds the largest magnitude
+      u32x2 w;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w[h] = encode4<CT>(v + 4 * h);
+      *(u32x2*)to = w;
+    } else {
+      put(to, v);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k)
+    if (lane + 64u * k < n) put_new(lane + 64u * k, kept[k]);
+  for (uint32_t i = lane + 64u * KEEP; i < n; i += 64) put_new(i, new_piece(i));
   if (lane == 0) *scale_at = now;
 }
 
