@@ -554,7 +554,10 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
   constexpr int TPR = D / PIECE;                            // threads of a row
   typedef typename Bytes<PIECE>::type piece;
   __shared__ __attribute__((aligned(256))) uint8_t keys[2][KC * RB], values[2][KC * RB];
-  __shared__ f32x4 figures[2][3];                           // of a chunk's four groups: sk, lv, iv
+  constexpr int GROUPS = KC / 16, AHEAD = F::THREADS / 2 / GROUPS;  // chunks whose figures are brought together
+  // Of each group of rows: its page, -1 where it holds no keys; its keys' scale, the exponent of its values', one over that.
+  __shared__ int32_t page_ids[2][F::THREADS / 2];
+  __shared__ __attribute__((aligned(16))) float key_scale[2][F::THREADS / 2], value_exponent[2][F::THREADS / 2], value_inverse[2][F::THREADS / 2];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -570,6 +573,14 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
   uint64_t left = share.end - share.begin;
   const float scale_log2 = a.scale * LOG2E;
   const uint32_t row_bytes = (uint32_t)a.HKV * D;
+  const int64_t page_bytes = (int64_t)row_bytes << a.page_shift;
+  // This thread's pieces: bytes from their group's first row, and places in a slot of keys or values.
+  const int piece_row = tid / TPR, piece_column = tid % TPR;
+  const uint32_t piece_off = (uint32_t)(piece_row & 15) * row_bytes + (uint32_t)(PIECE * piece_column);
+  const bool odd_row = piece_row & 1;
+  const uint32_t key_to = (uint32_t)(piece_row * RB + (((piece_column * (PIECE / 8)) ^ key_rows<D>(piece_row)) << 4));
+  const uint32_t value_to = (uint32_t)(piece_row * RB + (((piece_column * (PIECE / 8)) ^ (2 * value_rows<D>(piece_row)) ^
+                                                          (PIECE == 16 && odd_row ? 1 : 0)) << 4));
 
   for (bool first_part = true;; first_part = false) {
     if (request >= a.B) return;  // never, unless cu_seqlens_q or seqused_kv change under the call
@@ -619,68 +630,73 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
     // ---- codes to registers, as values to LDS -----------------------------------
     const int32_t* const table = a.table + (int64_t)request * a.W;
     const int page_mask = (1 << a.page_shift) - 1;
-    // Page number of 16-row group lane & 3 of a chunk, -1 where it holds no keys.
-    auto look_up = [&](int chunk) {
-      const int key = chunk * KC + 16 * (lane & 3);
-      return key < kv_end ? table[min(key >> a.page_shift, a.W - 1)] : -1;
-    };
-    auto row_of_group = [&](int chunk, int id, int group) -> int64_t {  // -1 for none
-      return (uint32_t)id < (uint32_t)a.blocks ? ((int64_t)id << a.page_shift) + ((chunk * KC + 16 * group) & page_mask) : -1;
-    };
-    // Row of this thread's piece n, and its group, the same for all of a wave's (a wave's rows lie in one).
-    // Offsets are worked out anew each time: kept, they would be spilled.
-    auto piece_of = [&](int n, int& column) {
-      const int t = (int)opaque((uint32_t)tid);
-      column = t % TPR;
-      return n * (KC / PIECES) + t / TPR;
-    };
-    auto load_codes = [&](const uint8_t* cache, int chunk, int ids, piece (&to)[PIECES]) {
-#pragma unroll
-      for (int n = 0; n < PIECES; ++n) {
-        int column;
-        const int r = piece_of(n, column), group = (n * (KC / PIECES) + wave * (64 / TPR)) >> 4;
-        const int64_t row = row_of_group(chunk, __builtin_amdgcn_readlane(ids, group), group);
-        const uint8_t* from = cache + ((row < 0 ? 0 : row) * row_bytes + kv_head * D);
-        // Rows that are not there become zeros, which no weight can turn into anything else.
-        const uint32_t off = (uint32_t)(r & 15) * row_bytes + (uint32_t)(PIECE * column);
-        to[n] = piece(0);
-        if (row >= 0) {
-          if (chunk * KC + 16 * group + 16 <= kv_end)
-            to[n] = *(const piece*)(from + off);
-          else if (chunk * KC + r < kv_end)
-            to[n] = *(const piece*)(from + off);
-        }
+    // Pages and figures of AHEAD chunks from `chunk` on, a thread a group of keys or of values.
+    auto bring = [&](int chunk) {
+      const int t = (int)opaque((uint32_t)tid), at = t & (F::THREADS / 2 - 1), buffer = (chunk - begin) / AHEAD & 1;
+      const int key = chunk * KC + 16 * at;
+      const int id = key < kv_end ? table[min(key >> a.page_shift, a.W - 1)] : -1;
+      const bool there = (uint32_t)id < (uint32_t)a.blocks;
+      const bool is_value = t >= F::THREADS / 2;
+      float scale = 0.f;
+      if (there) {
+        const int64_t row = ((int64_t)id << a.page_shift) + (key & page_mask);
+        scale = (is_value ? a.v_scale : a.k_scale)[(row >> a.group_shift) * a.HKV + kv_head];
+      }
+      if (is_value) {
+        const float vs = at_least(scale, Q8_LEAST_SCALE);
+        value_exponent[buffer][at] = there ? __log2f(vs) : -INFINITY;  // a group without keys weighs nothing
+        value_inverse[buffer][at] = there ? 1.0f / vs : 0.0f;
+      } else {
+        page_ids[buffer][at] = there ? id : -1;
+        key_scale[buffer][at] = at_least(scale * scale_log2, 1.17549435e-38f);  // not 0: times a hidden score
       }
     };
-    auto store_values = [&](const piece (&codes)[PIECES], uint32_t slot, bool is_value) {
+    auto buffer_of = [&](int chunk) { return (chunk - begin) / AHEAD & 1; };
+    auto group_of = [&](int chunk) { return (chunk - begin) % AHEAD * GROUPS; };
+    // Piece n of this thread is of row n * (KC / PIECES) + tid / TPR of a chunk, and a wave's are of one group of 16 rows,
+    // whose page this is.
+    auto piece_group = [&](int n) { return (n * (KC / PIECES) + wave * (64 / TPR)) >> 4; };
+    struct Pages { int id[PIECES]; };
+    auto pages_of = [&](int chunk) {
+      Pages p;
+#pragma unroll
+      for (int n = 0; n < PIECES; ++n) p.id[n] = uniform(page_ids[buffer_of(chunk)][group_of(chunk) + piece_group(n)]);
+      return p;
+    };
+    typedef const __attribute__((address_space(1))) uint8_t* global_bytes;
+    typedef const __attribute__((address_space(1))) piece* global_piece;
+    // Every load is made, so that a wait for one counts those behind it: a group without keys reads the cache's first
+    // rows, and rows behind the last key are the page's own (hidden when they are stored).
+    auto load_codes = [&](const uint8_t* cache, int chunk, const Pages& p, piece (&to)[PIECES]) {
 #pragma unroll
       for (int n = 0; n < PIECES; ++n) {
-        int column;
-        const int r = piece_of(n, column), turn = is_value ? 2 * value_rows<D>(r) : key_rows<D>(r);
-        const uint32_t at = slot + (uint32_t)(r * RB + (((column * (PIECE / 8)) ^ turn) << 4));
+        const int id = p.id[n], key = chunk * KC + 16 * piece_group(n);
+        const int64_t at = id >= 0 ? (int64_t)id * page_bytes + (int64_t)(key & page_mask) * row_bytes : 0;
+        // In scalar registers, so that a thread's part of the address is one 32-bit register.
+        to[n] = *(global_piece)((global_bytes)(uintptr_t)uniform64((uintptr_t)cache + (uint64_t)(at + kv_head * D)) + piece_off);
+      }
+    };
+    auto store_values = [&](const piece (&codes)[PIECES], uint32_t to, bool is_value, int chunk, const Pages& p) {
+      to += is_value ? value_to : key_to;
+#pragma unroll
+      for (int n = 0; n < PIECES; ++n) {
+        piece mine = codes[n];
+        const int id = p.id[n];
+        if (id < 0 || chunk * KC + 16 * piece_group(n) + 16 > kv_end) {
+          // Rows that are not there become zeros, which no weight can turn into anything else.
+          const int key = chunk * KC + n * (KC / PIECES) + (int)(opaque((uint32_t)tid) / TPR);
+          if (id < 0 || key >= kv_end) mine = piece(0);
+        }
 #pragma unroll
         for (int h = 0; h < PIECE / 8; ++h) {
-          uint32_t lo = codes[n][2 * h], hi = codes[n][2 * h + 1];
+          uint32_t lo = mine[2 * h], hi = mine[2 * h + 1];
+          if (PIECE == 16 && is_value) {  // odd rows the other half first: its turn leaves rows' halves on one another's banks
+            lo = odd_row ? mine[2 - 2 * h] : lo;
+            hi = odd_row ? mine[3 - 2 * h] : hi;
+          }
           __asm__ volatile("" : "+v"(lo), "+v"(hi));  // converted here and not a step ahead, where the registers are taken
-          *(AFA_LDS x8*)(uintptr_t)(at ^ (uint32_t)(h << 4)) = Codes<DT, CT>::decode(lo, hi);
+          *(AFA_LDS x8*)(uintptr_t)((to ^ (uint32_t)(h << 4)) + (uint32_t)(n * (KC / PIECES) * RB)) = Codes<DT, CT>::decode(lo, hi);
         }
-      }
-    };
-    // Lanes 0 .. 3 of the first wave: key scales of a chunk's groups, 4 .. 7: value scales (0 where it holds no keys).
-    auto load_scale = [&](int chunk, int ids) {
-      const int64_t row = row_of_group(chunk, ids, lane & 3);
-      return wave == 0 && lane < 8 && row >= 0 ? (lane < 4 ? a.k_scale : a.v_scale)[(row >> a.group_shift) * a.HKV + kv_head] : 0.0f;
-    };
-    auto store_figures = [&](float scale, int ids, int chunk) {
-      if (wave != 0 || lane >= 8) return;
-      const bool there = (uint32_t)ids < (uint32_t)a.blocks;
-      float* const to = (float*)figures[chunk & 1];
-      if (lane < 4) {
-        to[lane] = at_least(scale * scale_log2, 1.17549435e-38f);  // not 0: times a hidden score
-      } else {
-        const float vs = at_least(scale, Q8_LEAST_SCALE);
-        to[lane] = there ? __log2f(vs) : -INFINITY;  // a group without keys weighs nothing
-        to[4 + lane] = there ? 1.0f / vs : 0.0f;
       }
     };
 
@@ -773,40 +789,42 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
     if (!first_part) block_barrier();  // the slots are read
     piece k_codes[PIECES], v_codes[PIECES];
     f32x4 s_a[KT][QT], s_b[KT][QT];
-    int ids = -1, ids_ahead = -1, ids_v = -1;  // page numbers: of the chunk in k_codes' next load, ...
-    float scale = 0.f;
+    Pages page1, page2;  // of chunks c + 1 and c + 2 ahead of step c
     if (begin < chunks) {
-      const int ids0 = look_up(begin), ids1 = look_up(begin + 1);
-      ids = look_up(begin + 2);
-      ids_ahead = look_up(begin + 3);
+      bring(begin);
+      block_barrier();
+      const Pages page0 = pages_of(begin);
+      page1 = pages_of(begin + 1);
+      page2 = pages_of(begin + 2);
       piece first[PIECES];
-      load_codes(a.k, begin, ids0, first);
-      load_codes(a.v, begin, ids0, v_codes);
-      const float scale0 = load_scale(begin, ids0);
-      load_codes(a.k, begin + 1, ids1, k_codes);
-      store_values(first, keys_at(begin & 1), false);
-      store_values(v_codes, values_at(begin & 1), true);
-      store_figures(scale0, ids0, begin);
-      store_values(k_codes, keys_at((begin + 1) & 1), false);
-      load_codes(a.k, begin + 2, ids, k_codes);
-      load_codes(a.v, begin + 1, ids1, v_codes);
-      scale = load_scale(begin + 1, ids1);
-      ids_v = ids1;
+      load_codes(a.k, begin, page0, first);
+      load_codes(a.v, begin, page0, v_codes);
+      load_codes(a.k, begin + 1, page1, k_codes);
+      store_values(first, keys_at(begin & 1), false, begin, page0);
+      store_values(v_codes, values_at(begin & 1), true, begin, page0);
+      load_codes(a.v, begin + 1, page1, v_codes);
+      store_values(k_codes, keys_at((begin + 1) & 1), false, begin + 1, page1);
+      load_codes(a.k, begin + 2, page2, k_codes);
       block_barrier();
       qk_chunk(begin, s_a, [](int) {});
     }
     constexpr int HALF = QT * 8, QK_EXP0 = QT + 2, PV_EXP_STEPS = PV_FRAGS / 2 - 1;
-    constexpr int STORE_V = QK_FRAGS / 2, STORE_K = 0;  // steps that the stores follow
+    constexpr int STORE_V = 0, STORE_K = QK_FRAGS / 2;  // steps that the stores follow
     auto iteration = [&](int c, f32x4 (&cur)[KT][QT], f32x4 (&nxt)[KT][QT]) {
-      // Keys of chunk c + 1, values and figures of c are stored, and every wave is past QK (c) and PV (c - 1),
+      // Keys of chunk c + 1 and values of c are stored, and every wave is past QK (c) and PV (c - 1),
       // whose slots are free.
       block_barrier();
-      const f32x4 lv = figures[c & 1][1];
+      const Pages page3 = pages_of(c + 3);
+      f32x4 lv;
       float sk[KT], iv[KT];  // scalar registers
+      {
+        const int buffer = buffer_of(c), at = group_of(c);
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        sk[t] = __int_as_float(uniform(__float_as_int(figures[c & 1][0][t])));
-        iv[t] = __int_as_float(uniform(__float_as_int(figures[c & 1][2][t])));
+        for (int t = 0; t < KT; ++t) {
+          lv[t] = value_exponent[buffer][at + t];
+          sk[t] = __int_as_float(uniform(__float_as_int(key_scale[buffer][at + t])));
+          iv[t] = __int_as_float(uniform(__float_as_int(value_inverse[buffer][at + t])));
+        }
       }
       if (c >= clean_chunks) mask(c, cur);
       x8 pf[QT][KC / 32];
@@ -821,8 +839,14 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
       auto qk_between = [&](int f) {
         if (f == QK_FRAGS / 2 - 1) __builtin_amdgcn_s_setprio(2);
         if (f == STORE_V) {
-          store_values(v_codes, values_at((c + 1) & 1), true);  // of chunk c + 1
-          store_figures(scale, ids_v, c + 1);
+          store_values(v_codes, values_at((c + 1) & 1), true, c + 1, page1);
+          load_codes(a.v, c + 2, page2, v_codes);
+        }
+        if (f == STORE_K) {
+          store_values(k_codes, keys_at(c & 1), false, c + 2, page2);
+          load_codes(a.k, c + 3, page3, k_codes);
+          page1 = page2;
+          page2 = page3;
         }
         if (f < QT) {
           float m = -INFINITY;
@@ -860,15 +884,6 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
       };
       auto pv_between = [&](int f) {
         if (f == PV_FRAGS / 2 - 1) __builtin_amdgcn_s_setprio(0);
-        if (f == STORE_K) store_values(k_codes, keys_at(c & 1), false);  // of chunk c + 2
-        if (f == STORE_K + 1) {
-          load_codes(a.v, c + 2, ids, v_codes);
-          scale = load_scale(c + 2, ids);
-          load_codes(a.k, c + 3, ids_ahead, k_codes);
-          ids_v = ids;
-          ids = ids_ahead;
-          ids_ahead = look_up(c + 4);
-        }
         if (f < PV_EXP_STEPS) {
 #pragma unroll
           for (int e = 0; e < HALF; ++e)
@@ -886,9 +901,14 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
       __builtin_amdgcn_s_setprio(1);
       pv_chunk(c, pf, pv_between);
     };
-    for (int c = begin; c < chunks; c += 2) {
-      iteration(c, s_a, s_b);
-      if (c + 1 < chunks) iteration(c + 1, s_b, s_a);
+    // Step c loads keys of chunk c + 3: the next AHEAD chunks' pages are brought four steps ahead of them (visible at the
+    // next step's barrier), outside of the steps, which then wait for none but their own loads.
+    for (int c = begin, until = begin + AHEAD - 4; c < chunks; until += AHEAD) {
+      for (; c < min(chunks, until); c += 2) {
+        iteration(c, s_a, s_b);
+        if (c + 1 < chunks) iteration(c + 1, s_b, s_a);
+      }
+      if (c < chunks) bring(until + 4);
     }
 
 #pragma unroll

@@ -88,8 +88,8 @@ def attention(q, k, v, table, cu, used, scale, causal=True):
             continue
         ids = table[b].tolist()
         there = [j for j in range(s) if 0 <= ids[j // page] < blocks]
-        block = torch.tensor([ids[j // page] for j in there], dtype=torch.long)
-        slot = torch.tensor([j % page for j in there], dtype=torch.long)
+        block = torch.tensor([ids[j // page] for j in there], dtype=torch.long, device=q.device)
+        slot = torch.tensor([j % page for j in there], dtype=torch.long, device=q.device)
         limit = [sum(1 for j in there if j < (length - n + i + 1 if causal else s)) for i in range(n)]
         keys, rows = (x[block, slot].repeat_interleave(HQ // HKV, dim=1) for x in (k, v))
         for whole, piece in zip(result, lr._attend(q[start:end].double(), keys, rows, scale, limit)):

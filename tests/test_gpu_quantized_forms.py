@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from ascendflow_amd import _native
-from tests.quantized_helpers import B16, call, check, paged
+from oracle import quantized_reference as qr
+from tests.quantized_helpers import B16, call, check, compare, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -219,3 +220,18 @@ def test_one_long_request_in_many_parts(device, D, n):
     assert form_of(t)[0] == (16 if n == 1 else 32 if n == 6 else 128 if D == 256 else 256)
     check(device, [n], [9000], tensors=t, scale=1e-3)
     assert B16["bf16"] is t["q"].dtype
+
+
+@pytest.mark.parametrize("page,group", [(16, 16), (128, 64)])
+def test_tiles_of_many_chunks(device, page, group):
+    """A workgroup goes over more chunks than it brings the pages and scales of at once: the definition on the device."""
+    n, length = 80, 33000
+    t = tiles(device, [n], [length], HQ=128, HKV=32, D=64, page=page, group=group, seed=11)
+    assert form_of(t)[1:3] == [1, 8]  # 8 workgroups a head share 2 tiles of 516 chunks
+    k, v = (qr.values(t[w + "_cache"], t[w + "_scale"].clamp(min=2.0 ** -80)) for w in ("k", "v"))
+    want = qr.attention(t["q"], k, v, t["block_table"], t["cu_seqlens_q"], t["seqused_kv"], 0.125)
+    used = t["v_scale"][torch.isfinite(t["v_scale"])]
+    lse = torch.empty((n, 128), device=device)
+    out = call(t, 0.125, lse=lse)
+    largest, exponents = used.max().item() * 448, used.log2().abs().max().item()
+    compare(out.cpu(), lse.cpu(), ([x.cpu() for x in want], largest, exponents), torch.bfloat16, length)
