@@ -4,8 +4,10 @@
 // A table row [W] names the pages of one request, -1 where it has none; `counts` holds
 // the number of references of each page, 0 for a free one. Everything is integers and
 // comparisons: what a call gives follows from its operands alone, whatever the order of
-// its atomics. Copies are bound by HBM; the others by launches and chains of dependent
-// loads over a table and a list of counts that fit the L2s.
+// its atomics. Copies are bound by HBM (500 pages of 64 KiB in 16 caches 180 us, 5.1 TB/s);
+// the others by launches and chains of dependent loads over a table and a list of counts
+// that fit the L2s: a fork of 32 rows 3.4 and 9.8 us, of 256 rows of 1024 pages 2.9 and 15,
+// a compaction of 2048 pages 5.8 and 2.1, of 300000 4.1, 8.5 and 3.2.
 #include <algorithm>
 
 #include "common.h"
@@ -138,7 +140,7 @@ __device__ __forceinline__ int block_scan(int v, int& total, int* words) {
 // The first workgroup: which rows need a page of their own, the free pages, who gets which, and the columns of the table
 // that it decides: of a living row the last one that its tokens take and the reserved ones. The others bring the rest.
 __global__ __launch_bounds__(TABLE_THREADS) void fork_assign_kernel(ForkArgs a) {
-  __shared__ int32_t tails[FORK_MAX_B];
+  __shared__ __attribute__((aligned(16))) int32_t tails[FORK_MAX_B];  // to a multiple of four, -1 behind the last
   __shared__ int words[TABLE_THREADS / 64];
   __shared__ int64_t lacks[TABLE_THREADS / 64];
   const int tid = threadIdx.x;
@@ -154,7 +156,8 @@ __global__ __launch_bounds__(TABLE_THREADS) void fork_assign_kernel(ForkArgs a) 
       a.table[at] = a.rows[at];
     return;
   }
-  for (int b = tid; b < a.B; b += TABLE_THREADS) tails[b] = a.tails[b];
+  const int quads = (a.B + 3) / 4;
+  for (int b = tid; b < 4 * quads; b += TABLE_THREADS) tails[b] = b < a.B ? a.tails[b] : -1;
   __syncthreads();
   // All but the lowest of the rows that share such a page take a copy; all, where others hold it too.
   uint32_t copies = 0;  // bit i: row tid + i * TABLE_THREADS
@@ -166,11 +169,12 @@ __global__ __launch_bounds__(TABLE_THREADS) void fork_assign_kernel(ForkArgs a) 
     if (tail >= 0) {
       int same = 0;
       bool lowest = true;
-#pragma unroll 8
-      for (int other = 0; other < a.B; ++other) {
-        const bool equal = tails[other] == tail;
-        same += equal;
-        lowest = lowest && !(equal && other < b);
+#pragma unroll 4
+      for (int q = 0; q < quads; ++q) {
+        const int4 others = ((const int4*)tails)[q];
+        const int equal = (others.x == tail ? 1 : 0) | (others.y == tail ? 2 : 0) | (others.z == tail ? 4 : 0) | (others.w == tail ? 8 : 0);
+        same += __popc(equal);
+        lowest = lowest && !(4 * q < b && (equal & ((1 << min(b - 4 * q, 4)) - 1)));
       }
       copied = !(lowest && load_count(a.counts + tail) == same);
     }

@@ -121,7 +121,9 @@ template <> struct Codes<DT_BF16, AFA_CODE_INT8> {
 // free, queries follow it). O^T[columns, rows] += V^T P^T: the accumulator layout of S^T
 // is the operand layout of P^T, and ds_read_b64_tr_b8 gives a lane a column's codes of the
 // eight keys whose weights it holds. Codes become 16-bit values between LDS and the
-// matrix instructions.
+// matrix instructions. Bound by HBM where requests are many or long (64 of 8K to 16K, 8
+// heads of 128 columns 279 us, 6.1 TB/s; 342 with rows kept in registers a chunk ahead and a
+// head a workgroup), by a cold start and the join where they are few (one of 4K 13 us).
 template <int QT, int HW> struct StreamForm {
   static constexpr int ROWS = 16 * QT, KEYS = 128 / HW, THREADS = 256;
   static constexpr uint32_t START = 1, LEAST = 2;
@@ -527,10 +529,14 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
 // outputs stay in registers; chunks of 64 cache rows go through LDS as 16-bit values, so
 // that a code is converted once a workgroup and not once a wave. A wave's codes come into
 // registers a step before they are converted and stored (keys two chunks ahead of their
-// use, values one; two slots each), page numbers a step before that. The scales' three
-// figures a 16-row group (of its keys, the values' exponent and reciprocal) go the same
-// way. QK of chunk c + 1 is issued ahead of the softmax of chunk c, whose exponentials
-// run in the shadow of the matrix instructions of QK (c + 1) and PV (c).
+// use, values one; two slots each). Page numbers and the scales' three figures a 16-row
+// group (of its keys, the values' exponent and reciprocal) are brought for 64 chunks at
+// once, so that a step's loads are its codes' alone and each is waited for by count. QK of
+// chunk c + 1 is issued ahead of the softmax of chunk c, whose exponentials run in the
+// shadow of the matrix instructions of QK (c + 1) and PV (c). 2000 tokens of 32 heads, 8 of
+// them key/value heads, behind 18000: 614 us, 1.01 PFLOP/s; bound by the matrix pipes (41%
+// busy), every wave's LDS reads of every row and the exponentials; 506 without loading,
+// converting and storing codes.
 template <int QT> struct TileForm {
   static constexpr int ROWS = 128 * QT, KEYS = 64, THREADS = 512;
   static constexpr uint32_t START = 5, LEAST = 4;
@@ -1043,8 +1049,8 @@ constexpr int Q8_CUS = 256;
 constexpr int64_t Q8_STREAM_BYTES = 128ll << 20;
 
 // Form of a call. Tile form (256 rows; D = 256: 128) where a request has more than 256 rows on average and
-// its table room for 1536 (2000 tokens of 32 heads, 8 of them key/value heads, behind 18000: 675 us, 924 in the
-// stream form with 32 rows; 8 requests of 375 behind 1100 137 and 137; 1 of 1000 behind none 51 and 43, 16 of 48 behind
+// its table room for 1536 (2000 tokens of 32 heads, 8 of them key/value heads, behind 18000: 614 us, 924 in the
+// stream form with 32 rows; 8 requests of 375 behind 1100 130 and 137; 1 of 1000 behind none 51 and 43, 16 of 48 behind
 // 2200 77 and 71). Below, tiles of 32 rows, or 16 where that holds a request. In the stream form a workgroup takes as
 // many neighbouring heads as leaves a tile at most 8 workgroups of its own (64 requests of 16K, 8 heads 286 us with 4, 298
 // with 2, 336 with 1; one of 16K 58, 39 and 29, since a part a workgroup has to be joined).
