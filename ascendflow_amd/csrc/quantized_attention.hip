@@ -1038,8 +1038,8 @@ int check_quantized(const QuantizedParams* p) {
   if (p->D != 64 && p->D != 128 && p->D != 256) return AFA_E_SHAPE;
   if (p->GROUP < 16 || (p->GROUP & (p->GROUP - 1)) || p->PAGE < p->GROUP || p->PAGE > (1 << 20) || (p->PAGE & (p->PAGE - 1)))
     return AFA_E_SHAPE;
-  // Packed rows, tiles, positions and the offsets of 16 cache rows are 32-bit numbers.
-  if ((int64_t)p->T * p->HQ > 0x7fffff00ll || (int64_t)p->W * p->PAGE > 0x7fffff00ll || p->B > 0x3fffffff) return AFA_E_SHAPE;
+  // Packed rows, tiles, positions (some chunks past the last too) and the offsets of 16 cache rows are 32-bit numbers.
+  if ((int64_t)p->T * p->HQ > 0x7fffff00ll || (int64_t)p->W * p->PAGE > 1ll << 30 || p->B > 0x3fffffff) return AFA_E_SHAPE;
   if (p->HKV > 32768) return AFA_E_SHAPE;
   if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return AFA_E_SHAPE;
   return AFA_OK;

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void append_quantized_kernel(AppendQuantizedAr
         n = max(min(stop, a.T) - start, 0);
         // Token t lies at used - cu[b + 1] + t; positions below 0 or past the table are not there.
         const int64_t place = (int64_t)a.used[b] - stop + start;
-        const int64_t held = min((int64_t)a.W << a.page_shift, (int64_t)1 << 30);
+        const int64_t held = (int64_t)a.W << a.page_shift;
         low = (int)min(max(place, (int64_t)0), held);
         high = (int)min(max(place + n, (int64_t)0), held);
         if (high > low) mine = (uint32_t)(((high - 1) >> a.group_shift) - (low >> a.group_shift) + 1);
@@ -298,6 +298,7 @@ extern "C" int launch_append_quantized_kv(void* stream, const void* k, const voi
   if (p->T < 0 || p->B <= 0 || p->W <= 0 || p->BLOCKS <= 0 || p->HKV <= 0 || p->D <= 0) return AFA_E_SHAPE;
   if (p->D > Q8_MAX_D || p->HKV > Q8_MAX_HKV || p->GROUP > Q8_MAX_GROUP || p->T >= 1 << 23 || p->B >= 1 << 23) return AFA_E_SHAPE;
   if (p->GROUP < 16 || (p->GROUP & (p->GROUP - 1)) || p->PAGE < p->GROUP || (p->PAGE & (p->PAGE - 1))) return AFA_E_SHAPE;
+  if ((int64_t)p->W * p->PAGE > 1ll << 30) return AFA_E_SHAPE;  // positions are 32-bit numbers
   if (!k || !v || !block_table || !cu_seqlens_q || !seqused_kv || !k_cache || !v_cache || !k_scale || !v_scale)
     return AFA_E_NULL;
   if (p->T == 0) return AFA_OK;

@@ -55,6 +55,7 @@ def _check(lib, q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens_q
     if softmax_lse is not None:
         check_tensor("softmax_lse", softmax_lse, (T, HQ), torch.float32, device)
     require(B > 0 and W > 0, "requests and pages must not be empty")
+    require(W * PAGE <= 1 << 30 and B < 1 << 30, "a table of at most 2^30 rows, and fewer requests")
     require(D in (64, 128, 256), "the columns of a head must be 64, 128 or 256")
     require(0 < SCALE < math.inf, "positive, finite attention scale")
     qt, qh = live_strides(q)[:2]

@@ -70,6 +70,7 @@ def _check(lib, k, v, block_table, cu_seqlens_q, seqused_kv, k_cache, v_cache, k
     require(B > 0 and W > 0, "requests and pages must not be empty")
     require(D <= 1024 and HKV <= 32768 and T < 1 << 23 and B < 1 << 23,
             "at most 1024 columns, 32768 heads, and 2^23 - 1 tokens and requests")
+    require(W * PAGE <= 1 << 30, "a table of at most 2^30 rows")
     kt, kh = live_strides(k)[:2]
     vt, vh = live_strides(v)[:2]
     call = _Call()

@@ -447,7 +447,7 @@ int form_latent_attention_expanded(int64_t form[2], const LatentExpandedParams* 
  * behind the new ones are left as they are. No two new tokens may name the same
  * row, and no two requests append to the same block. PAGE and GROUP are powers
  * of two, 16 <= GROUP <= PAGE, GROUP up to 1024, D up to 1024, HKV up to 32768,
- * T below 2^23. */
+ * T below 2^23, W * PAGE up to 2^30. */
 typedef struct AppendQuantizedKvParams {
   int32_t dtype;
   int32_t code;            /* AFA_CODE_* */
@@ -468,8 +468,8 @@ int launch_append_quantized_kv(void* stream, const void* k, const void* v, const
  * NULL. Empty rows, pages outside the cache, tokens of no request and scores
  * that are not finite as there; scales of rows that a token of the request sees
  * have to be finite and positive, and value scales below 2^-80 count as that.
- * The workspace holds partial results; calls that may run at the same time need
- * workspaces of their own. */
+ * W * PAGE up to 2^30. The workspace holds partial results; calls that may run at
+ * the same time need workspaces of their own. */
 typedef struct QuantizedParams {
   int32_t dtype;
   int32_t code;            /* AFA_CODE_* */

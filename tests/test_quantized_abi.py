@@ -36,6 +36,7 @@ def attention(**changes):
     ({"dtype": 2}, -3), ({"code": 2}, -3), ({"code": -1}, -3), ({"T": -1}, -2), ({"T": 1 << 23}, -2), ({"B": 0}, -2), ({"W": 0}, -2),
     ({"BLOCKS": 0}, -2), ({"HKV": 0}, -2), ({"HKV": 32769}, -2), ({"D": 0}, -2), ({"D": 1025}, -2), ({"GROUP": 8}, -2),
     ({"GROUP": 24}, -2), ({"GROUP": 64}, -2), ({"PAGE": 48}, -2), ({"GROUP": 2048, "PAGE": 2048}, -2), ({"PAGE": 0}, -2), ({"T": 0}, 0),
+    ({"W": (1 << 25) + 1}, -2), ({"W": 1 << 25, "T": 0}, 0),
 ])
 def test_append_rejections(lib, changes, status):
     assert lib.launch_append_quantized_kv(None, *[p16] * 9, ct.byref(append(**changes))) == status
@@ -50,7 +51,7 @@ def test_append_pointers(lib, missing):
 @pytest.mark.parametrize("changes,status", [
     ({"dtype": 2}, -3), ({"code": 3}, -3), ({"T": -1}, -2), ({"B": 0}, -2), ({"HQ": 0}, -2), ({"HKV": 0}, -2), ({"HQ": 7}, -2),
     ({"D": 96}, -2), ({"D": 512}, -2), ({"PAGE": 8}, -2), ({"PAGE": 48}, -2), ({"GROUP": 64}, -2), ({"GROUP": 8}, -2), ({"GROUP": 0}, -2),
-    ({"W": 0}, -2), ({"BLOCKS": 0}, -2), ({"W": 1 << 27}, -2), ({"T": 1 << 29}, -2), ({"HKV": 65536, "HQ": 65536}, -2),
+    ({"W": 0}, -2), ({"BLOCKS": 0}, -2), ({"W": (1 << 25) + 1}, -2), ({"T": 1 << 29}, -2), ({"HKV": 65536, "HQ": 65536}, -2),
     ({"scale": 0.0}, -2), ({"scale": -1.0}, -2), ({"scale": math.nan}, -2), ({"scale": math.inf}, -2),
 ])
 def test_attention_rejections(lib, changes, status):
