@@ -134,7 +134,7 @@ def quantized_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_s
             _native.check(status, "launch_quantized_attention")
         if not new or softmax_lse is not None:
             mark_written([t for t in (None if new else out, softmax_lse) if t is not None])
-    return ForwardOnly.apply("quantized_attention", out, q, k_scale, v_scale) if graph else out
+    return ForwardOnly.apply("quantized_attention", out, q, k_cache, v_cache, k_scale, v_scale) if graph else out
 
 
 @torch.library.custom_op("ascendflow_amd::quantized_attention", mutates_args=())

@@ -217,6 +217,16 @@ def test_no_tokens(device):
     assert call(paged(device, [0], [10]), 0.1).shape == (0, 8, 128)
 
 
+@pytest.mark.parametrize("name", ["k_cache", "v_cache", "k_scale", "v_scale"])
+def test_a_gradient_of_the_cache_alone_is_refused_in_backward(device, name):
+    t = paged(device, [1, 2], [40, 70])
+    t[name].requires_grad_(True)
+    out = call(t, 0.1)
+    assert out.requires_grad
+    with pytest.raises(RuntimeError, match="forward only"):
+        out.sum().backward()
+
+
 def test_forward_only(device):
     t = paged(device, [1, 2], [40, 70])
     t["q"].requires_grad_(True)
