@@ -405,7 +405,7 @@ int power_shift(int32_t power) {
 
 int check_fork(const ForkPagesParams* p) {
   if (!p) return AFA_E_NULL;
-  if (p->B <= 0 || p->B > FORK_MAX_B || p->W <= 0 || p->BLOCKS <= 0 || p->reserve < 0) return AFA_E_SHAPE;
+  if (p->B <= 0 || p->B > FORK_MAX_B || p->W <= 0 || p->BLOCKS <= 0 || p->BLOCKS > 1 << 28 || p->reserve < 0) return AFA_E_SHAPE;
   if (p->PAGE <= 0 || (p->PAGE & (p->PAGE - 1)) || p->W > 1 << 24 || (int64_t)p->B * p->W >= 1ll << 31) return AFA_E_SHAPE;
   return AFA_OK;
 }

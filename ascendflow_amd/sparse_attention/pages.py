@@ -34,6 +34,7 @@ def _check_copies(lib, source, destination, caches):
     first = caches[0]
     require(first.dim() >= 2 and first.numel() > 0, "a cache must be [BLOCKS, ...], not empty")
     BLOCKS, device = first.shape[0], first.device
+    require(BLOCKS < 1 << 31 and source.numel() < 1 << 31, "at most 2^31 - 1 pages and pairs")
     for i, cache in enumerate(caches):
         require(cache.dim() >= 2 and cache.numel() > 0, "a cache must be [BLOCKS, ...], not empty")
         check_tensor(f"caches[{i}]", cache, (BLOCKS, *cache.shape[1:]), cache.dtype, device)
@@ -100,7 +101,8 @@ def _check_fork(lib, block_table, page_counts, parents, seqused_kv, PAGE, reserv
     check_tensor("seqused_kv", seqused_kv, (B,), torch.int32, block_table.device)
     require(PAGE > 0 and PAGE & (PAGE - 1) == 0 and PAGE <= 1 << 20, "PAGE must be a power of two up to 2^20")
     require(0 <= reserve <= 1 << 20, "reserve must be 0 to 2^20 tokens")
-    require(B <= 8192 and B * W < 1 << 31, "at most 8192 requests and 2^31 - 1 entries of a table")
+    require(B <= 8192 and B * W < 1 << 31 and BLOCKS <= 1 << 28,
+            "at most 8192 requests, 2^31 - 1 entries of a table and 2^28 pages")
     params = _native.ForkPagesParams(B=B, W=W, PAGE=PAGE, BLOCKS=BLOCKS, reserve=reserve)
     nbytes = ct.c_uint64(0)
     _native.check(lib.workspace_size_fork_pages(ct.byref(nbytes), ct.byref(params)), "workspace_size_fork_pages")

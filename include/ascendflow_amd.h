@@ -512,7 +512,8 @@ int launch_copy_pages(void* stream, const void* const* caches, const uint64_t* p
  * [BLOCKS], the references of each page, follows all of it; free pages (count 0)
  * are handed out from the lowest up, row by row, the copy first. missing[0]
  * counts the pages that were wanted beyond the free ones or beyond the table's
- * width (2^31 - 1 at most); their entries are -1. B up to 8192, PAGE a power of two. */
+ * width (2^31 - 1 at most); their entries are -1. B up to 8192, BLOCKS up to 2^28,
+ * PAGE a power of two. */
 typedef struct ForkPagesParams {
   int32_t B, W, PAGE, BLOCKS, reserve;
 } ForkPagesParams;

@@ -109,9 +109,16 @@ def test_copy_rejections(lib):
     assert call(n=0) == call(pairs=0) == 0
 
 
+def test_pages_and_pairs_past_32_bits_are_refused():
+    many, few, number = torch.empty(1 << 32, 1, dtype=torch.int8), torch.empty(2, 1, dtype=torch.int8), torch.zeros(1, dtype=torch.int32)
+    for operands in ((many, number, number), (few, number.expand(1 << 31), number)):
+        with pytest.raises(ValueError, match="at most 2\\^31 - 1 pages"):
+            copy_pages(*operands)
+
+
 @pytest.mark.parametrize("changes,status", [
     ({"B": 0}, -2), ({"B": 8193}, -2), ({"W": 0}, -2), ({"W": 1 << 25}, -2), ({"PAGE": 0}, -2), ({"PAGE": 24}, -2), ({"BLOCKS": 0}, -2),
-    ({"reserve": -1}, -2),
+    ({"reserve": -1}, -2), ({"BLOCKS": (1 << 28) + 1}, -2),
 ])
 def test_fork_rejections(lib, changes, status):
     params = ct.byref(_native.ForkPagesParams(**{**dict(B=2, W=4, PAGE=16, BLOCKS=9, reserve=1), **changes}))
