@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void append_quantized_kernel(AppendQuantizedAr
   if (head >= a.HKV) return;
 
   // The block: each request's new tokens touch a run of blocks; this wave's is number blockIdx.x of them all.
-  int request = -1, first = 0, count = 0, limit = 0, end = 0, block = 0;
+  int request = -1, first = 0, count = 0, limit = 0, block = 0;
   {
     uint32_t before = 0;
     const uint32_t index = blockIdx.x;

@@ -89,6 +89,20 @@ def test_copy_refusals(device, change):
         copy_pages(*change(cache, s, d))
 
 
+def test_copy_op(device):
+    caches = [torch.arange(4 * 16, device=device, dtype=torch.int32).view(4, 16).to(dt) for dt in (torch.int8, torch.float32)]
+    want = [c.clone() for c in caches]
+    for w in want:
+        w[3] = w[1]
+    leaf = caches[1].clone().requires_grad_(True)
+    pairs = i32(device, [1, -1]), i32(device, [3, 0])
+    torch.ops.ascendflow_amd.copy_pages(caches, *pairs)
+    assert all(torch.equal(c, w) for c, w in zip(caches, want)) and all(c._version > 0 for c in caches)
+    with torch.no_grad():
+        torch.ops.ascendflow_amd.copy_pages([leaf], *pairs)
+    assert torch.equal(leaf, want[1])
+
+
 # ---- forks -----------------------------------------------------------------------
 
 
