@@ -34,6 +34,17 @@ __device__ __forceinline__ float at_least(float v, float bound) {
   return __int_as_float(max(__float_as_int(v), __float_as_int(bound)));
 }
 
+// A row's running maximum before its first key. Finite, and below every score of a key.
+constexpr float Q8_NO_MAXIMUM = -3.402823466e+38f;
+
+// Weights are 2^(s sk + (lv - m)) with one rounding, of a maximum m = s sk + lv that was rounded: what that rounding
+// took is a factor of every weight of a row, at most 2 up to |m| = 2^24. From there on it could leave the range: s sk + lv
+// takes the place of s then, rounded as m is, with 1 for sk and 0 for lv.
+constexpr float Q8_FAR = 16777216.0f;  // 2^24
+__device__ __forceinline__ bool q8_far(float m) {  // there is a maximum, finite and far from zero
+  return (__float_as_uint(m) & 0x7fffffffu) - __float_as_uint(Q8_FAR) < __float_as_uint(-Q8_NO_MAXIMUM) - __float_as_uint(Q8_FAR);
+}
+
 struct QuantizedArgs {
   const void* q;
   const uint8_t* k;
@@ -322,7 +333,7 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
     float m_run[QT], l_run[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      m_run[qt] = -1e30f;  // finite: a chunk that hides all its keys gives p = 0, never NaN
+      m_run[qt] = Q8_NO_MAXIMUM;  // finite: a chunk that hides all its keys gives p = 0, never NaN
       l_run[qt] = 0.f;
 #pragma unroll
       for (int c = 0; c < VT; ++c) o[qt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -425,13 +436,22 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
           for (int c2 = 0; c2 < VT; ++c2) o[qt][c2] *= alpha;
           m_run[qt] = m_new;
         }
+        float factor[2] = {sk[0], sk[1]}, shift[2] = {lv[0] - m_run[qt], lv[1] - m_run[qt]};
+        if (__ballot(q8_far(m_new)) != 0ull) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][qt][r] = __builtin_fmaf(s[t][qt][r], sk[t], lv[t]);
+            factor[t] = 1.0f;
+            shift[t] = -m_run[qt];
+          }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float shift = lv[t] - m_run[qt];
           float sum = 0.f;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float w = fast_exp2(__builtin_fmaf(s[t][qt][r], sk[t], shift));
+            const float w = fast_exp2(__builtin_fmaf(s[t][qt][r], factor[t], shift[t]));
             sum += w;
             pf[qt][4 * t + r] = (scalar)w;
           }
@@ -564,6 +584,7 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
   // Of each group of rows: its page, -1 where it holds no keys; its keys' scale, the exponent of its values', one over that.
   __shared__ int32_t page_ids[2][F::THREADS / 2];
   __shared__ __attribute__((aligned(16))) float key_scale[2][F::THREADS / 2], value_exponent[2][F::THREADS / 2], value_inverse[2][F::THREADS / 2];
+  __shared__ __attribute__((aligned(16))) float most_scale[2][4];  // the largest of the keys' scales, of each wave that brings them
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -654,7 +675,11 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
         value_inverse[buffer][at] = there ? 1.0f / vs : 0.0f;
       } else {
         page_ids[buffer][at] = there ? id : -1;
-        key_scale[buffer][at] = at_least(scale * scale_log2, 1.17549435e-38f);  // not 0: times a hidden score
+        float most = at_least(scale * scale_log2, 1.17549435e-38f);  // not 0: times a hidden score
+        key_scale[buffer][at] = most;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+        if (lane == 0) most_scale[buffer][wave] = most;
       }
     };
     auto buffer_of = [&](int chunk) { return (chunk - begin) / AHEAD & 1; };
@@ -717,11 +742,25 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
       for (int j = 0; j < KSTEPS; ++j)
         qf[qt][j] = valid ? *(const x8*)(q + 32 * j) : __builtin_bit_cast(x8, u32x4{0u, 0u, 0u, 0u});
     }
+    // Up to this scale of its keys no score of this wave is far from zero (half of it for lv).
+    float far_scale = 0.f;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += fabsf((float)qf[qt][j][e]);
+      far_scale = fmaxf(far_scale, sum_over_lane_groups(sum));
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) far_scale = fmaxf(far_scale, __shfl_xor(far_scale, d));
+    far_scale = __int_as_float(uniform(__float_as_int(0.5f * Q8_FAR / (far_scale * (CT == AFA_CODE_E4M3 ? 448.0f : 128.0f)))));
     f32x4 o[QT][VT];
     float m_run[QT], l_run[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      m_run[qt] = -1e30f;  // finite: a chunk that hides all its keys gives p = 0, never NaN
+      m_run[qt] = Q8_NO_MAXIMUM;  // finite: a chunk that hides all its keys gives p = 0, never NaN
       l_run[qt] = 0.f;
 #pragma unroll
       for (int t = 0; t < VT; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -816,6 +855,7 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
     }
     constexpr int HALF = QT * 8, QK_EXP0 = QT + 2, PV_EXP_STEPS = PV_FRAGS / 2 - 1;
     constexpr int STORE_V = 0, STORE_K = QK_FRAGS / 2;  // steps that the stores follow
+    int far = 0;  // scores of these chunks may be far from zero
     auto iteration = [&](int c, f32x4 (&cur)[KT][QT], f32x4 (&nxt)[KT][QT]) {
       // Keys of chunk c + 1 and values of c are stored, and every wave is past QK (c) and PV (c - 1),
       // whose slots are free.
@@ -832,7 +872,20 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
           iv[t] = __int_as_float(uniform(__float_as_int(value_inverse[buffer][at + t])));
         }
       }
-      if (c >= clean_chunks) mask(c, cur);
+      if (c >= clean_chunks || far) {
+        mask(c, cur);
+        if (far) {
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) cur[t][qt][i] = __builtin_fmaf(cur[t][qt][i], sk[t], lv[t]);
+            sk[t] = 1.0f;
+            lv[t] = 0.0f;
+          }
+        }
+      }
       x8 pf[QT][KC / 32];
       float top[QT], m_new[QT], psum[QT];
       f32x4 shift[QT];
@@ -907,14 +960,21 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
       __builtin_amdgcn_s_setprio(1);
       pv_chunk(c, pf, pv_between);
     };
-    // Step c loads keys of chunk c + 3: the next AHEAD chunks' pages are brought four steps ahead of them (visible at the
-    // next step's barrier), outside of the steps, which then wait for none but their own loads.
+    // Step c loads keys of chunk c + 3: the next AHEAD chunks' pages are brought four steps ahead of them, outside of the
+    // steps, which then wait for none but their own loads.
     for (int c = begin, until = begin + AHEAD - 4; c < chunks; until += AHEAD) {
+      float most = 0.f;
+      for (int buffer = 0; buffer < (c == begin ? 1 : 2); ++buffer)
+        for (int w = 0; w < 4; ++w) most = fmaxf(most, most_scale[buffer][w]);
+      far = uniform(most > far_scale ? 1 : 0);
       for (; c < min(chunks, until); c += 2) {
         iteration(c, s_a, s_b);
         if (c + 1 < chunks) iteration(c + 1, s_b, s_a);
       }
-      if (c < chunks) bring(until + 4);
+      if (c < chunks) {
+        bring(until + 4);
+        block_barrier();
+      }
     }
 
 #pragma unroll
@@ -973,7 +1033,7 @@ __global__ __launch_bounds__(64 * (D / 16) * SPLIT) void quantized_merge_kernel(
     return ((2 * (int64_t)(record.first + p) + (p == 0 ? 1 : 0)) * a.HKV + kv_head) * tile_groups + group;
   };
   auto sums = [&](int k) { return *(const float2*)(a.partial_ml + (slot(k) * 16 + i16) * 2); };
-  float top = -1e30f, total = 0.f;
+  float top = Q8_NO_MAXIMUM, total = 0.f;
 #pragma unroll 4
   for (int k = g; k < mine; k += 4) top = fmaxf(top, sums(k).x);
   top = max_over_lane_groups(top);

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from oracle import quantized_reference as qr
 from tests.quantized_helpers import call, check, paged
 
 pytestmark = pytest.mark.gpu
@@ -215,6 +216,60 @@ def test_custom_op(device):
 
 def test_no_tokens(device):
     assert call(paged(device, [0], [10]), 0.1).shape == (0, 8, 128)
+
+
+@pytest.mark.parametrize("counts,lengths", [([1, 1], [300, 37]), ([40], [200]), ([450], [1700])])
+@pytest.mark.parametrize("dtype,codes", [("bf16", "e4m3"), ("f16", "int8")])
+@pytest.mark.parametrize("negative", [False, True])
+@pytest.mark.parametrize("exponent", [16, 24, 30, 60, 110])
+def test_scores_far_from_zero(device, counts, lengths, dtype, codes, negative, exponent):
+    far_scores(device, counts, lengths, dtype, codes, negative, exponent)
+
+
+@pytest.mark.parametrize("counts,lengths", [([1, 1], [9000, 3000]), ([40], [5000]), ([450], [5000]), ([300, 400], [900, 9000])])
+@pytest.mark.parametrize("exponent", [24, 60])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scores_far_from_zero_in_some_pages(device, counts, lengths, exponent, D):
+    far_scores(device, counts, lengths, "bf16", "int8", False, exponent, D, some=True)
+
+
+def far_scores(device, counts, lengths, dtype, codes, negative, exponent, D=128, some=False):
+    """Scores whose float32 steps are many units (`some`: of each request's last twentieth of the pages that all its
+    tokens see): a row is its best key's where the next is clearly behind."""
+    t = paged(device, counts, lengths, HQ=4, HKV=2, D=D, page=32, codes=codes, dtype=dtype, seed=exponent)
+    factor = torch.full((t["k_scale"].shape[0], 1, 1), 1.0 if some else 2.0 ** exponent)
+    if some:
+        for b, (n, s) in enumerate(zip(counts, lengths)):
+            pages = (s - n) // 32
+            factor[t["block_table"][b, pages - pages // 20 - 1:pages].long().cpu()] = 2.0 ** exponent
+    t["k_scale"] = t["k_scale"] * factor.to(device)
+    if negative:
+        t["q"] = -t["q"].abs()
+        t["k_cache"] = (t["k_cache"].view(torch.uint8) & 0x7f).view(t["k_cache"].dtype)
+    T, HQ, D = t["q"].shape
+    lse = torch.empty((T, HQ), device=device)
+    out = call(t, D ** -0.5, lse=lse).cpu().double()
+    lse = lse.cpu().double()
+    cpu = {n: x.cpu() for n, x in t.items()}
+    caches = [qr.values(cpu[w + "_cache"], cpu[w + "_scale"]).double() for w in "kv"]
+    eps, told, at = torch.finfo(t["q"].dtype).eps / 2, 0, 0
+    for b, (n, s) in enumerate(zip(counts, lengths)):
+        pages = cpu["block_table"][b, :-(-s // 32)].long()
+        k, v = [c[pages].reshape(-1, 2, D)[:s].repeat_interleave(2, 1).transpose(0, 1) for c in caches]
+        q = cpu["q"][at:at + n].double().transpose(0, 1)
+        scores, reach = q @ k.transpose(1, 2) * D ** -0.5, (q.abs() @ k.abs().transpose(1, 2)).amax(-1) * D ** -0.5
+        hidden = torch.arange(s) > s - n + torch.arange(n)[:, None]
+        top = scores.masked_fill(hidden, -torch.inf).topk(min(s, 2), dim=-1)
+        # A product of D terms in float32 is off by D 2^-24 of their magnitudes; 60 are what no weight is seen behind.
+        clear = top.values[..., 0] - top.values[..., -1] > 60 + 4 * D * 2.0 ** -24 * reach
+        want = v.gather(1, top.indices[..., :1].expand(-1, -1, D))
+        # The weight is rounded where it meets the value but not in the sum, and then the result is.
+        off = (out[at:at + n].transpose(0, 1) - want).abs() - want.abs() * (2 * eps + 2.0 ** -16)
+        assert off[clear].max() <= 1e-30
+        assert ((lse[at:at + n].T - top.values[..., 0]).abs() <= 60 + (D + 8) * 2.0 ** -24 * reach)[clear].all()
+        told += clear.sum().item()
+        at += n
+    assert told > 0.8 * T * HQ
 
 
 @pytest.mark.parametrize("name", ["k_cache", "v_cache", "k_scale", "v_scale"])
