@@ -554,7 +554,7 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
 // once, so that a step's loads are its codes' alone and each is waited for by count. QK of
 // chunk c + 1 is issued ahead of the softmax of chunk c, whose exponentials run in the
 // shadow of the matrix instructions of QK (c + 1) and PV (c). 2000 tokens of 32 heads, 8 of
-// them key/value heads, behind 18000: 614 us, 1.01 PFLOP/s; bound by the matrix pipes (41%
+// them key/value heads, behind 18000: 617 us, 1.01 PFLOP/s; bound by the matrix pipes (41%
 // busy), every wave's LDS reads of every row and the exponentials; 506 without loading,
 // converting and storing codes.
 template <int QT> struct TileForm {
@@ -1109,7 +1109,7 @@ constexpr int Q8_CUS = 256;
 constexpr int64_t Q8_STREAM_BYTES = 128ll << 20;
 
 // Form of a call. Tile form (256 rows; D = 256: 128) where a request has more than 256 rows on average and
-// its table room for 1536 (2000 tokens of 32 heads, 8 of them key/value heads, behind 18000: 614 us, 924 in the
+// its table room for 1536 (2000 tokens of 32 heads, 8 of them key/value heads, behind 18000: 617 us, 924 in the
 // stream form with 32 rows; 8 requests of 375 behind 1100 130 and 137; 1 of 1000 behind none 51 and 43, 16 of 48 behind
 // 2200 77 and 71). Below, tiles of 32 rows, or 16 where that holds a request. In the stream form a workgroup takes as
 // many neighbouring heads as leaves a tile at most 8 workgroups of its own (64 requests of 16K, 8 heads 286 us with 4, 298

@@ -85,7 +85,7 @@ def quantized_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_s
     ``k_cache`` and ``v_cache`` [BLOCKS, PAGE, HKV, D]: contiguous, float8_e4m3fn or
     int8, PAGE a power of two from 16 on; ``k_scale`` and ``v_scale`` float32
     [BLOCKS, PAGE / GROUP, HKV], GROUP a power of two, 16 to 1024.
-    ``block_table`` int32 [B, W], ``cu_seqlens_q`` int32 [B + 1], ``seqused_kv`` int32
+    ``block_table`` int32 [B, W] (at most 2^30 rows), ``cu_seqlens_q`` int32 [B + 1], ``seqused_kv`` int32
     [B]: rows of each request, the new tokens' included (``append_quantized_kv``
     writes them). With ``CAUSAL`` token j of a request's n sees rows up to
     ``seqused_kv[b] - n + j``, without all of them. Rows past the table are not

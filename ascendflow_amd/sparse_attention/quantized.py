@@ -90,7 +90,7 @@ def append_quantized_kv(k, v, k_cache, v_cache, k_scale, v_scale, block_table, c
     contiguous, float8_e4m3fn or int8, PAGE a power of two from 16 on. ``k_scale``
     and ``v_scale`` float32 [BLOCKS, PAGE / GROUP, HKV]: a scale for each block of
     GROUP tokens (a power of two, 16 to 1024) and head. ``block_table`` int32
-    [B, W], ``cu_seqlens_q`` int32 [B + 1], ``seqused_kv`` int32 [B]. Token j of the
+    [B, W] (at most 2^30 rows), ``cu_seqlens_q`` int32 [B + 1], ``seqused_kv`` int32 [B]. Token j of the
     n new ones of request b goes to position ``seqused_kv[b] - n + j``.
 
     The scale of a block is the least power of two (from 2^-80 on) that holds its
