@@ -316,7 +316,7 @@ __global__ __launch_bounds__(256) void compact_count_kernel(CompactArgs a) {
 
 // With n pages in use, the k-th of those from n on moves to the k-th free one below n.
 __global__ __launch_bounds__(256) void compact_moves_kernel(CompactArgs a, int segments) {
-  __shared__ int words[4], round_sums[16][4];
+  __shared__ int words[4], step_sums[16][4];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t base = (int64_t)blockIdx.x * SEGMENT;
   uint32_t bits = 0;  // bit i: page base + 256 i + tid is in use
@@ -349,10 +349,10 @@ __global__ __launch_bounds__(256) void compact_moves_kernel(CompactArgs a, int s
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const uint64_t wave_bits = __ballot(bits >> i & 1u);
-    if (lane == 0) round_sums[i][wave] = __popcll(wave_bits);
+    if (lane == 0) step_sums[i][wave] = __popcll(wave_bits);
   }
   __syncthreads();
-  int used = before;  // pages in use ahead of this round's
+  int used = before;  // pages in use ahead of these 256
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int64_t page = base + i * 256 + tid;
@@ -360,8 +360,8 @@ __global__ __launch_bounds__(256) void compact_moves_kernel(CompactArgs a, int s
     int ahead = used + __popcll(__ballot(in_use) & ((1ull << lane) - 1));
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      if (w < wave) ahead += round_sums[i][w];
-      used += round_sums[i][w];
+      if (w < wave) ahead += step_sums[i][w];
+      used += step_sums[i][w];
     }
     if (page < a.BLOCKS) {
       const int move = page >= n && in_use ? ahead - stays : -1;
