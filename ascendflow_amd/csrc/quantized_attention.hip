@@ -9,7 +9,10 @@
 //   p_j = 2^(x_j - m),  out = sum_j p_j v_j / sum_j p_j / b_j,  m the running maximum of x.
 // So the scales cost one multiply-add per 16 keys instead of one per element, and the
 // weight that contributes most is 1, which no type rounds. Scales count as at least 2^-80
-// (append writes none below), which keeps every ratio of them inside float32.
+// (append writes none below), so that 1 / b is a number. Their ratios are not bounded by
+// that (append writes up to 2^122): a p_j of 0 may stand for a key that counts in the
+// denominator. Where the value scales of a tile's keys lie that far apart, the wave sums
+// its denominators anew (sum_weights).
 //
 // The sums, the maximum and the output are float32; p is rounded to the query's type (a
 // matrix operand has to be), at most half a step of each weight, while the denominator
@@ -43,6 +46,39 @@ constexpr float Q8_NO_MAXIMUM = -3.402823466e+38f;
 constexpr float Q8_FAR = 16777216.0f;  // 2^24
 __device__ __forceinline__ bool q8_far(float m) {  // there is a maximum, finite and far from zero
   return (__float_as_uint(m) & 0x7fffffffu) - __float_as_uint(Q8_FAR) < __float_as_uint(-Q8_NO_MAXIMUM) - __float_as_uint(Q8_FAR);
+}
+
+// Whether sums of p_j / b_j over that many keys may lack some that count, given the least and the most of their value scales.
+// p is 0 below 2^-126, rescaling drops no more than that, and m is at most the largest weight's exponent + log2 of the largest b
+// (bfloat16; float16's may be 2^8 less than it will be): what is dropped of a key is under 2^(spread - 126) of the largest
+// weight, of all keys under 2^-26.
+template <int DT>
+__device__ __forceinline__ bool far_apart(float least, float most, int keys) {
+  return (uniform(__float_as_int(most)) >> 23) - (uniform(__float_as_int(least)) >> 23) + 1 + (32 - __clz(keys)) > 100 - (int)q8_tau<DT>();
+}
+
+// v 2^e for a result inside float32's range, subnormal ones included.
+__device__ __forceinline__ float times_exp2(float v, float e) {
+  const bool low = e < 0.f;
+  return v * fast_exp2(e + (low ? 64.f : -64.f)) * (low ? 5.42101086e-20f : 1.84467441e+19f);
+}
+
+// Denominators total_p of parts whose maxima are m_p, as of one part whose maximum is `top`: sum_p 2^(m_p - top) total_p.
+// The weights may be 0 where the products are not, so a part's exponent goes into the weight's, in units of 2^unit, the
+// largest of the products' exponents.
+__device__ __forceinline__ float part_exponent(float m, float total, float top) {
+  return (m - top) + (float)__builtin_amdgcn_frexp_expf(total);
+}
+__device__ __forceinline__ float part_weight(float m, float total, float top, float unit) {
+  return __builtin_amdgcn_frexp_mantf(total) * fast_exp2(part_exponent(m, total, top) - unit);
+}
+// Whether the plain sum lacks a product: a weight that is 0 next to a total that is not.
+__device__ __forceinline__ bool weight_lost(float m, float total, float top) { return m - top < -126.f && total > 0.f; }
+
+// ln(sum of e^scores), also of a denominator below float32's normal numbers.
+__device__ __forceinline__ float q8_lse(float m, float total) {
+  const bool low = __float_as_uint(total) - 1u < 0x007fffffu;
+  return row_lse(low ? m - 64.f : m, low ? total * 1.84467441e+19f : total);
 }
 
 struct QuantizedArgs {
@@ -119,6 +155,71 @@ template <> struct Codes<DT_BF16, AFA_CODE_INT8> {
     return __builtin_bit_cast(bf16x8, w);
   }
 };
+
+// ---- denominators anew ---------------------------------------------------------
+
+// total = sum_j 2^(x_j - m - log2 b_j) over a wave's keys, each weight an exponential of its own next to a maximum of
+// their own, so that none is lost however far the value scales lie apart; x_j and m as the numerators have them. It reads
+// the keys once more, straight from the cache: the price of scales that far apart.
+// Operand f of lane group g's queries holds columns column(f, g) .. + 7; group i is the 16 keys from first_key(i) on.
+template <int DT, int CT, int D, int QT, typename X8, typename Column, typename Key>
+__device__ __forceinline__ void sum_weights(const QuantizedArgs& a, const int32_t* table, int kv_head, int kv_end,
+                                            float scale_log2, int groups, Key&& first_key, Column&& column,
+                                            const X8 (&qf)[QT][D / 32], const int (&limit)[QT], const float (&m)[QT],
+                                            float (&total)[QT]) {
+  const int lane = (int)opaque(threadIdx.x) & 63, g = lane >> 4, i16 = lane & 15;  // worked out here, not ahead of the loops
+  float top[QT], sum[QT];
+  bool far[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    top[qt] = Q8_NO_MAXIMUM;
+    sum[qt] = 0.f;
+    far[qt] = q8_far(m[qt]);
+  }
+#pragma unroll 1
+  for (int i = 0; i < groups; ++i) {
+    const int key = uniform(first_key(i));
+    if (key >= kv_end) continue;
+    const int id = uniform(table[min(key >> a.page_shift, a.W - 1)]);
+    if ((uint32_t)id >= (uint32_t)a.blocks) continue;
+    const int64_t row = ((int64_t)id << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+    const int64_t block = (row >> a.group_shift) * a.HKV + kv_head;
+    const float sk = at_least(a.k_scale[block] * scale_log2, 1.17549435e-38f);
+    const float lv = __log2f(at_least(a.v_scale[block], Q8_LEAST_SCALE));
+    const uint8_t* const codes = a.k + ((row + i16) * a.HKV + kv_head) * D;
+    f32x4 s[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) s[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int f = 0; f < D / 32; ++f) {
+      const u32x2 w = *(const u32x2*)(codes + column(f, g));
+      const X8 kf = Codes<DT, CT>::decode(w[0], w[1]);
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) s[qt] = B16<DT>::mfma(kf, qf[qt][f], s[qt]);
+    }
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      float e[4], most = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float near = __builtin_fmaf(s[qt][r], sk, lv - m[qt]), away = __builtin_fmaf(s[qt][r], sk, lv) - m[qt];
+        e[r] = key + 4 * g + r < limit[qt] ? (far[qt] ? away : near) - lv : -INFINITY;
+        most = fmaxf(most, e[r]);
+      }
+      const float now = fmaxf(top[qt], max_over_lane_groups(most));
+      sum[qt] *= fast_exp2(top[qt] - now);
+      top[qt] = now;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[qt] += fast_exp2(e[r] - now);
+    }
+  }
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const float all = times_exp2(sum_over_lane_groups(sum[qt]), fmaxf(top[qt], -200.f));
+    // A sum that is not a number stays so.
+    total[qt] = (__float_as_uint(total[qt]) & 0x7fffffffu) > 0x7f800000u ? total[qt] : all;
+  }
+}
 
 // ---- stream form ---------------------------------------------------------------
 //
@@ -331,6 +432,7 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
 
     f32x4 o[QT][VT];
     float m_run[QT], l_run[QT];
+    float least_scale = INFINITY, most_scale = 0.f;  // of this wave's values (1 where a group has no page)
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       m_run[qt] = Q8_NO_MAXIMUM;  // finite: a chunk that hides all its keys gives p = 0, never NaN
@@ -404,6 +506,8 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
         sk[t] = at_least(ks * scale_log2, 1.17549435e-38f);  // not 0: times a hidden score
         lv[t] = __log2f(vs);
         iv[t] = 1.0f / vs;
+        least_scale = fminf(least_scale, vs);
+        most_scale = fmaxf(most_scale, vs);
       }
       if (c + NS < mine) {
         __builtin_amdgcn_s_waitcnt(WAIT_LGKM0);  // the slot is read
@@ -474,6 +578,10 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
     float total[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) total[qt] = sum_over_lane_groups(l_run[qt]);
+    if (__builtin_expect(far_apart<DT>(least_scale, most_scale, kv_end), 0))
+      sum_weights<DT, CT, D, QT>(a, table, kv_head, kv_end, scale_log2, 2 * (mine - begin),
+                                 [&](int i) { return key_of(begin + (i >> 1), i & 1); },
+                                 [](int f, int g) { return 64 * (f >> 1) + 16 * g + 8 * (f & 1); }, qf, limit, m_run, total);
     if constexpr (KW > 1) {
       // The first of a head's waves sums up, through the others' rings, 16 rows at a time.
       static_assert(VT * 1024 <= NS * SLOT, "a wave's output fits its ring");
@@ -495,18 +603,31 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
             ml[w] = joined_ml[wave + w * HW][qt][i16];
             top = fmaxf(top, ml[w].x);
           }
-          float weight = fast_exp2(ml[0].x - top);
-          total[qt] = weight * ml[0].y;
           m_run[qt] = top;
+          float weight[KW];
+          bool lost = false;
+          total[qt] = 0.f;
 #pragma unroll
-          for (int c = 0; c < VT; ++c) o[qt][c] *= weight;
+          for (int w = 0; w < KW; ++w) {
+            weight[w] = fast_exp2(ml[w].x - top);
+            total[qt] = __builtin_fmaf(weight[w], ml[w].y, total[qt]);
+            lost |= weight_lost(ml[w].x, ml[w].y, top);
+          }
+          if (__builtin_expect(__ballot(lost) != 0ull, 0)) {
+            float unit = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < KW; ++w) unit = fmaxf(unit, part_exponent(ml[w].x, ml[w].y, top));
+#pragma unroll
+            for (int w = 0; w < KW; ++w) sum += part_weight(ml[w].x, ml[w].y, top, unit);
+            total[qt] = times_exp2(sum, unit);
+          }
+#pragma unroll
+          for (int c = 0; c < VT; ++c) o[qt][c] *= weight[0];
 #pragma unroll
           for (int w = 1; w < KW; ++w) {
-            weight = fast_exp2(ml[w].x - top);
-            total[qt] = __builtin_fmaf(weight, ml[w].y, total[qt]);
             const uint32_t from = ring_base + (uint32_t)(w * HW * NS * SLOT + lane * 16);
 #pragma unroll
-            for (int c = 0; c < VT; ++c) o[qt][c] += weight * *lds_at<f32x4>(from + c * 1024);
+            for (int c = 0; c < VT; ++c) o[qt][c] += weight[w] * *lds_at<f32x4>(from + c * 1024);
           }
         }
       }
@@ -533,7 +654,7 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
             for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[qt][c][i] * inv);
             *(x4*)(out + 16 * c) = v;
           }
-          if (a.lse && g == 0) a.lse[(int64_t)(start + token) * (a.HKV * H) + head] = row_lse(m_run[qt], total[qt]);
+          if (a.lse && g == 0) a.lse[(int64_t)(start + token) * (a.HKV * H) + head] = q8_lse(m_run[qt], total[qt]);
         }
       }
     }
@@ -585,6 +706,8 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
   __shared__ int32_t page_ids[2][F::THREADS / 2];
   __shared__ __attribute__((aligned(16))) float key_scale[2][F::THREADS / 2], value_exponent[2][F::THREADS / 2], value_inverse[2][F::THREADS / 2];
   __shared__ __attribute__((aligned(16))) float most_scale[2][4];  // the largest of the keys' scales, of each wave that brings them
+  // The range of the values' scales that a thread brought: the bits of the largest, and infinity's less those of the least.
+  __shared__ uint32_t value_most[F::THREADS / 2], value_rest[F::THREADS / 2];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -673,6 +796,14 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
         const float vs = at_least(scale, Q8_LEAST_SCALE);
         value_exponent[buffer][at] = there ? __log2f(vs) : -INFINITY;  // a group without keys weighs nothing
         value_inverse[buffer][at] = there ? 1.0f / vs : 0.0f;
+        const uint32_t bits = there ? __float_as_uint(vs) : 0u, rest = there ? 0x7f800000u - bits : 0u;
+        if (chunk == begin) {
+          value_most[at] = bits;
+          value_rest[at] = rest;
+        } else {  // in place, without a register more: the loop around has none
+          __hip_atomic_fetch_max(&value_most[at], bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          __hip_atomic_fetch_max(&value_rest[at], rest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
       } else {
         page_ids[buffer][at] = there ? id : -1;
         float most = at_least(scale * scale_log2, 1.17549435e-38f);  // not 0: times a hidden score
@@ -977,10 +1108,31 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
       }
     }
 
+    float totals[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) totals[qt] = sum_over_lane_groups(l_run[qt]);
+    uint32_t most = 0u, rest = 0u;
+    if (begin < chunks) {
+#pragma unroll
+      for (int i = 0; i < F::THREADS / 2; i += 64) {
+        most = max(most, value_most[i + lane]);
+        rest = max(rest, value_rest[i + lane]);
+      }
+    }
+    most = (uint32_t)__builtin_amdgcn_readlane((int)wave_max(most), 63);
+    rest = (uint32_t)__builtin_amdgcn_readlane((int)wave_max(rest), 63);
+    if (__builtin_expect(far_apart<DT>(__uint_as_float(0x7f800000u - rest), __uint_as_float(most), kv_end), 0)) {
+      int limit[QT];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) limit[qt] = visible(min((int)tile * ROWS + (wave * QT + qt) * 16 + i16, rows - 1) / H);
+      sum_weights<DT, CT, D, QT>(a, table, kv_head, kv_end, scale_log2, (chunks - begin) * GROUPS,
+                                 [&](int i) { return begin * KC + 16 * i; }, [](int f, int g) { return 32 * f + 8 * g; }, qf, limit,
+                                 m_run, totals);
+    }
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int group = wave * QT + qt, row = (int)tile * ROWS + group * 16 + i16;
-      const float total = sum_over_lane_groups(l_run[qt]);
+      const float total = totals[qt];
       if (!whole) {
         const int64_t at = ((2 * (int64_t)worker + (offset == 0 ? 1 : 0)) * a.HKV + kv_head) * (ROWS / 16) + group;
         float* po = a.partial_o + (at * VT * 64 + lane) * 4;
@@ -1000,7 +1152,7 @@ __global__ __launch_bounds__(512, 1) void quantized_tile_kernel(QuantizedArgs a)
           for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[qt][t][i] * inv);
           *(x4*)(out + 16 * t) = v;
         }
-        if (a.lse && g == 0) a.lse[(int64_t)(start + token) * (a.HKV * H) + head] = row_lse(m_run[qt], total);
+        if (a.lse && g == 0) a.lse[(int64_t)(start + token) * (a.HKV * H) + head] = q8_lse(m_run[qt], total);
       }
     }
     if (left == 0) return;
@@ -1037,6 +1189,7 @@ __global__ __launch_bounds__(64 * (D / 16) * SPLIT) void quantized_merge_kernel(
 #pragma unroll 4
   for (int k = g; k < mine; k += 4) top = fmaxf(top, sums(k).x);
   top = max_over_lane_groups(top);
+  bool lost = false;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int k = 0; k < mine; k += AHEAD) {
     float2 ml[AHEAD];
@@ -1051,8 +1204,22 @@ __global__ __launch_bounds__(64 * (D / 16) * SPLIT) void quantized_merge_kernel(
     for (int i = 0; i < AHEAD; ++i) {
       const float weight = k + i < mine ? fast_exp2(ml[i].x - top) : 0.f;
       total = __builtin_fmaf(weight, ml[i].y, total);
+      lost |= weight_lost(ml[i].x, ml[i].y, top);
       o += weight * v[i];
     }
+  }
+  if (__builtin_expect(__ballot(lost) != 0ull, 0)) {
+    float unit = -INFINITY, sum = 0.f;
+    for (int k = g; k < mine; k += 4) {
+      const float2 ml = sums(k);
+      unit = fmaxf(unit, part_exponent(ml.x, ml.y, top));
+    }
+    unit = max_over_lane_groups(unit);
+    for (int k = g; k < mine; k += 4) {
+      const float2 ml = sums(k);
+      sum += part_weight(ml.x, ml.y, top, unit);
+    }
+    total = times_exp2(sum_over_lane_groups(sum), unit);
   }
   if constexpr (SPLIT > 1) {
     if (sub > 0) {
@@ -1061,10 +1228,11 @@ __global__ __launch_bounds__(64 * (D / 16) * SPLIT) void quantized_merge_kernel(
     }
     __syncthreads();
     if (sub > 0) return;
-    const float own = top;
+    const float2 own = make_float2(top, total);
 #pragma unroll
     for (int w = 0; w < SPLIT - 1; ++w) top = fmaxf(top, joined_ml[w][i16].x);
-    const float mine_weight = fast_exp2(own - top);
+    lost = weight_lost(own.x, own.y, top);
+    const float mine_weight = fast_exp2(own.x - top);
     total *= mine_weight;
     o *= mine_weight;
 #pragma unroll
@@ -1072,7 +1240,17 @@ __global__ __launch_bounds__(64 * (D / 16) * SPLIT) void quantized_merge_kernel(
       const float2 ml = joined_ml[w][i16];
       const float weight = fast_exp2(ml.x - top);
       total = __builtin_fmaf(weight, ml.y, total);
+      lost |= weight_lost(ml.x, ml.y, top);
       o += weight * joined_o[w][c][lane];
+    }
+    if (__builtin_expect(__ballot(lost) != 0ull, 0)) {
+      float unit = part_exponent(own.x, own.y, top);
+#pragma unroll
+      for (int w = 0; w < SPLIT - 1; ++w) unit = fmaxf(unit, part_exponent(joined_ml[w][i16].x, joined_ml[w][i16].y, top));
+      float sum = part_weight(own.x, own.y, top, unit);
+#pragma unroll
+      for (int w = 0; w < SPLIT - 1; ++w) sum += part_weight(joined_ml[w][i16].x, joined_ml[w][i16].y, top, unit);
+      total = times_exp2(sum, unit);
     }
   }
   const int r = group * 16 + i16;
@@ -1083,7 +1261,7 @@ __global__ __launch_bounds__(64 * (D / 16) * SPLIT) void quantized_merge_kernel(
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = (scalar)(o[i] * inv);
   *(x4*)((scalar*)a.out + (int64_t)(record.start + token) * a.o_t + (int64_t)head * a.o_h + 16 * c + 4 * g) = v;
-  if (a.lse && c == 0 && g == 0) a.lse[(int64_t)(record.start + token) * (a.HKV * a.H) + head] = row_lse(top, total);
+  if (a.lse && c == 0 && g == 0) a.lse[(int64_t)(record.start + token) * (a.HKV * a.H) + head] = q8_lse(top, total);
 }
 
 namespace {

@@ -98,6 +98,9 @@ def quantized_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_s
     Rows behind ``seqused_kv`` have no effect and pages outside the cache hold no
     keys, but the rows that some token of a request sees have to be finite, and
     their scales finite and positive (value scales below 2^-80 count as 2^-80).
+    However far the value scales lie apart, every key has its weight in the sum;
+    in ``out``, values whose weight times scale is below 2^-126 of a row's largest
+    are lost. Value scales more than about 2^85 apart cost a second pass over keys.
 
     Forward only: a backward pass that reaches the result raises; with ``out`` or
     ``softmax_lse`` the call is refused where a gradient would be recorded.

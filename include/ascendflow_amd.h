@@ -468,6 +468,9 @@ int launch_append_quantized_kv(void* stream, const void* k, const void* v, const
  * NULL. Empty rows, pages outside the cache, tokens of no request and scores
  * that are not finite as there; scales of rows that a token of the request sees
  * have to be finite and positive, and value scales below 2^-80 count as that.
+ * Every key has its weight in the denominator however far the value scales lie
+ * apart; values whose weight times scale is below 2^-126 of a row's largest are
+ * lost from out.
  * W * PAGE up to 2^30. The workspace holds partial results; calls that may run at
  * the same time need workspaces of their own. */
 typedef struct QuantizedParams {
