@@ -427,9 +427,11 @@ extern "C" int launch_copy_pages(void* stream, const void* const* caches, const 
   if (n_caches < 0 || pairs < 0 || BLOCKS <= 0) return AFA_E_SHAPE;
   if (n_caches == 0 || pairs == 0) return AFA_OK;
   if (!caches || !page_bytes || !source || !destination) return AFA_E_NULL;
-  for (int32_t i = 0; i < n_caches; ++i) {
+  for (int32_t i = 0; i < n_caches; ++i) {  // of all caches before the first is written
     if (!caches[i]) return AFA_E_NULL;
     if (page_bytes[i] == 0 || page_bytes[i] > 1ull << 36) return AFA_E_SHAPE;
+    // A launch counts its threads in 32 bits.
+    if ((page_bytes[i] + COPY_BYTES - 1) / COPY_BYTES * (uint64_t)pairs > 0xffffffffull / 256) return AFA_E_SHAPE;
   }
   hipStream_t s = (hipStream_t)stream;
   for (int32_t first = 0; first < n_caches; first += COPY_CACHES) {
@@ -445,7 +447,6 @@ extern "C" int launch_copy_pages(void* stream, const void* const* caches, const 
       most = std::max(most, a.bytes[i]);
     }
     const uint64_t parts = (most + COPY_BYTES - 1) / COPY_BYTES;
-    if (parts * (uint64_t)pairs > 0xffffffffull / 256) return AFA_E_SHAPE;  // a launch counts its threads in 32 bits
     a.parts = (int32_t)parts;
     hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(parts * pairs), (unsigned)n), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
