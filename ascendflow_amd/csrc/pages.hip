@@ -430,15 +430,13 @@ extern "C" int launch_copy_pages(void* stream, const void* const* caches, const 
   for (int32_t i = 0; i < n_caches; ++i) {  // of all caches before the first is written
     if (!caches[i]) return AFA_E_NULL;
     if (page_bytes[i] == 0 || page_bytes[i] > 1ull << 36) return AFA_E_SHAPE;
-    // A launch counts its threads in 32 bits.
-    if ((page_bytes[i] + COPY_BYTES - 1) / COPY_BYTES * (uint64_t)pairs > 0xffffffffull / 256) return AFA_E_SHAPE;
+    // Far more than the list of a compaction takes: half as many pairs as a cache has pages.
+    if ((page_bytes[i] + COPY_BYTES - 1) / COPY_BYTES * (uint64_t)pairs > 1ull << 32) return AFA_E_SHAPE;
   }
   hipStream_t s = (hipStream_t)stream;
   for (int32_t first = 0; first < n_caches; first += COPY_CACHES) {
     const int n = std::min(n_caches - first, COPY_CACHES);
     CopyArgs a;
-    a.source = source;
-    a.destination = destination;
     a.blocks = BLOCKS;
     uint64_t most = 0;
     for (int i = 0; i < n; ++i) {
@@ -448,9 +446,15 @@ extern "C" int launch_copy_pages(void* stream, const void* const* caches, const 
     }
     const uint64_t parts = (most + COPY_BYTES - 1) / COPY_BYTES;
     a.parts = (int32_t)parts;
-    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(parts * pairs), (unsigned)n), dim3(256), 0, s, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
+    const int64_t each = (int64_t)(0xffffffffull / 256 / parts);  // pairs of a launch, which counts its threads in 32 bits
+    for (int64_t at = 0; at < pairs; at += each) {
+      a.source = source + at;
+      a.destination = destination + at;
+      const uint64_t groups = parts * (uint64_t)std::min<int64_t>(each, pairs - at);
+      hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)groups, (unsigned)n), dim3(256), 0, s, a);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return (int)e;
+    }
   }
   return AFA_OK;
 }

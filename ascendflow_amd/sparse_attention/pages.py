@@ -59,6 +59,8 @@ def copy_pages(caches, source, destination):
     ``source`` and ``destination`` int32 [pairs], as ``fork_pages`` and
     ``compact_pages`` give them: a pair with a number outside the cache (-1) copies
     nothing. No page may be a destination twice, or a destination and a source.
+    A list that ``compact_pages`` returns is taken whatever its length; a call that
+    is refused has copied nothing.
     Refused where a gradient would be recorded; can be captured in a graph.
     """
     lib = _native.library()

@@ -500,7 +500,9 @@ int form_quantized_attention(int64_t form[4], const QuantizedParams* params);
 /* Copies page source[i] to page destination[i], i < pairs, in each of n_caches
  * tensors of BLOCKS pages (caches: device pointers, page_bytes: bytes of a page,
  * both arrays on the host). Pairs with a number outside [0, BLOCKS) copy
- * nothing. No destination may be named twice or be a source as well. */
+ * nothing. No destination may be named twice or be a source as well. Pairs times
+ * the 16 KiB pieces of the largest page, up to 2^32 (what compact_pages lists is
+ * far below); a call that is refused has copied nothing. */
 int launch_copy_pages(void* stream, const void* const* caches, const uint64_t* page_bytes, int32_t n_caches,
                       const int32_t* source, const int32_t* destination, int32_t pairs, int32_t BLOCKS);
 
