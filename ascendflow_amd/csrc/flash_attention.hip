@@ -784,7 +784,6 @@ __global__ __launch_bounds__(256) void fa_merge_kernel(FaSplitArgs args) {
   for (int d = 16; d > 0; d >>= 1) L += __shfl_xor(L, d, 32);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   const float* src = args.partial_o + row * 128 + 4 * u;
-#pragma unroll 8
   for (int s = 0; s < args.splits; ++s) {
     const float ws = __shfl(s < 32 ? w[0] : w[1], s & 31, 32);
     acc += *(const f32x4*)(src + (int64_t)s * total * 128) * ws;
