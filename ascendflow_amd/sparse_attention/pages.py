@@ -134,6 +134,14 @@ def fork_pages(block_table, page_counts, parents, seqused_kv, *, PAGE, reserve=0
     were wanted beyond the free ones or the table's width, whose entries are -1:
     the attentions find no keys there and the appends write nothing.
 
+    A call that lacks pages loses state: a row whose partly filled page had to be
+    copied and could not be has -1 in its place, its tokens there are gone for
+    that row (whoever else holds the page keeps it), and no later call wants that
+    entry again or counts it in ``missing``. Where pages may run out, keep
+    copies of ``block_table`` and ``page_counts`` from before the call and read
+    ``missing`` before ``copy_pages``, appends or new lengths: the call writes no cache,
+    so putting both back undoes it, and it can be made again once rows have ended.
+
     Can be captured in a graph.
     """
     lib = _native.library()

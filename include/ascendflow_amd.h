@@ -517,8 +517,11 @@ int launch_copy_pages(void* stream, const void* const* caches, const uint64_t* p
  * [BLOCKS], the references of each page, follows all of it; free pages (count 0)
  * are handed out from the lowest up, row by row, the copy first. missing[0]
  * counts the pages that were wanted beyond the free ones or beyond the table's
- * width (2^31 - 1 at most); their entries are -1. B up to 8192, BLOCKS up to 2^28,
- * PAGE a power of two. */
+ * width (2^31 - 1 at most); their entries are -1. That includes a page to be
+ * copied: its row's tokens on it are lost to that row, and an entry of -1 below a
+ * row's length is not wanted again by later calls. No cache is written, so that
+ * block_table and page_counts saved before the call undo it. B up to 8192, BLOCKS
+ * up to 2^28, PAGE a power of two. */
 typedef struct ForkPagesParams {
   int32_t B, W, PAGE, BLOCKS, reserve;
 } ForkPagesParams;
