@@ -8,8 +8,8 @@
 // and rows that the block held before are rounded anew where s grew. A power of two
 // wastes at most one bit of int8's range and none of e4m3's precision, and makes the
 // rounding anew exact (e4m3, but for codes that fall among its subnormals) or a shift
-// (int8): codes depend little on the order in which a block was filled. The exponent
-// comes from the bits of A, so nothing is rounded but x / s itself.
+// with a rounding (int8), which leaves a code within one step of the last scale however the
+// block was filled. The exponent comes from the bits of A, so nothing is rounded but x / s.
 //
 // One wave takes the new rows of one block, of one head's keys or values: a pass for A,
 // the rows held before where the scale grows, a pass for the codes, the rows in registers

@@ -97,7 +97,8 @@ def append_quantized_kv(k, v, k_cache, v_cache, k_scale, v_scale, block_table, c
     rows' largest finite magnitude with the largest code (448 or 127). A block
     that held rows before the new ones keeps its scale while that is enough;
     where it grows, those rows are rounded anew (in e4m3 exactly, but for codes
-    that become subnormal). Values are rounded to nearest, ties to even;
+    that become subnormal; int8 codes stay within one step of the last scale, but
+    depend on how the block was filled). Values are rounded to nearest, ties to even;
     infinities become the largest code, NaN e4m3's NaN or, in int8, 0.
 
     Tokens of no request, negative positions, positions beyond the table and pages
