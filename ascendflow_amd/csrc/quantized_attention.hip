@@ -161,7 +161,9 @@ template <> struct Codes<DT_BF16, AFA_CODE_INT8> {
 
 // total = sum_j 2^(x_j - m - log2 b_j) over a wave's keys, each weight an exponential of its own next to a maximum of
 // their own, so that none is lost however far the value scales lie apart; x_j and m as the numerators have them. It reads
-// the keys once more, straight from the cache: the price of scales that far apart.
+// the keys once more, straight from the cache: the price of scales that far apart (64 requests of 16K 283 -> 564 us, 2000
+// tokens behind 18K 618 -> 2134). The range of the scales and the joins that tell cost other calls up to 2% (one request of
+// 4K 20.6 -> 20.9 us, 48 x 4 tokens 38.5 -> 39.2 in a graph).
 // Operand f of lane group g's queries holds columns column(f, g) .. + 7; group i is the 16 keys from first_key(i) on.
 template <int DT, int CT, int D, int QT, typename X8, typename Column, typename Key>
 __device__ __forceinline__ void sum_weights(const QuantizedArgs& a, const int32_t* table, int kv_head, int kv_end,
@@ -235,8 +237,9 @@ __device__ __forceinline__ void sum_weights(const QuantizedArgs& a, const int32_
 // is the operand layout of P^T, and ds_read_b64_tr_b8 gives a lane a column's codes of the
 // eight keys whose weights it holds. Codes become 16-bit values between LDS and the
 // matrix instructions. Bound by HBM where requests are many or long (64 of 8K to 16K, 8
-// heads of 128 columns 279 us, 6.1 TB/s; 342 with rows kept in registers a chunk ahead and a
-// head a workgroup), by a cold start and the join where they are few (one of 4K 13 us).
+// heads of 128 columns 280 us, 6.1 TB/s; 342 with rows kept in registers a chunk ahead and a
+// head a workgroup), by a cold start and the join where they are few (one of 4K 13 us). 32
+// rows of 256 columns, or of one head of 128, spill 10 to 38 registers, around the chunk loop.
 template <int QT, int HW> struct StreamForm {
   static constexpr int ROWS = 16 * QT, KEYS = 128 / HW, THREADS = 256;
   static constexpr uint32_t START = 1, LEAST = 2;
@@ -276,8 +279,9 @@ __device__ __forceinline__ void wait_slots(int n) {
   wait_vmcnt<PER * MOST>();
 }
 
-// STREAM: non-temporal loads, for requests of one tile each (nothing is read twice) over
-// caches too large to stay in the 256 MiB Infinity Cache, rows of whole 128-byte lines.
+// STREAM: non-temporal loads, for requests of one tile each (nothing is read twice but
+// pages that requests share, a case not measured) over caches too large to stay in the
+// 256 MiB Infinity Cache, rows of whole 128-byte lines.
 template <int DT, int CT, int D, int QT, int HW, bool STREAM>
 __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(QuantizedArgs a) {
   typedef typename B16<DT>::scalar scalar;
@@ -683,9 +687,11 @@ __global__ __launch_bounds__(256, q8_groups<D>()) void quantized_stream_kernel(Q
 // once, so that a step's loads are its codes' alone and each is waited for by count. QK of
 // chunk c + 1 is issued ahead of the softmax of chunk c, whose exponentials run in the
 // shadow of the matrix instructions of QK (c + 1) and PV (c). 2000 tokens of 32 heads, 8 of
-// them key/value heads, behind 18000: 617 us, 1.01 PFLOP/s; bound by the matrix pipes (41%
+// them key/value heads, behind 18000: 618 us, 1.01 PFLOP/s; bound by the matrix pipes (41%
 // busy), every wave's LDS reads of every row and the exponentials; 506 without loading,
-// converting and storing codes.
+// converting and storing codes. 128 columns spill 63 to 95 registers, 256 columns 19 to 26, all
+// outside the chunk loop. 8 x 500 tokens of 16 heads, 4 of them key/value heads of 256 columns,
+// behind 3500: 297 to 311 us in each pair of types, 0.8 PFLOP/s.
 template <int QT> struct TileForm {
   static constexpr int ROWS = 128 * QT, KEYS = 64, THREADS = 512;
   static constexpr uint32_t START = 5, LEAST = 4;
@@ -1308,7 +1314,7 @@ constexpr int Q8_CUS = 256;
 constexpr int64_t Q8_STREAM_BYTES = 128ll << 20;
 
 // Form of a call. Tile form (256 rows; D = 256: 128) where a request has more than 256 rows on average and
-// its table room for 1536 (2000 tokens of 32 heads, 8 of them key/value heads, behind 18000: 617 us, 924 in the
+// its table room for 1536 (2000 tokens of 32 heads, 8 of them key/value heads, behind 18000: 618 us, 924 in the
 // stream form with 32 rows; 8 requests of 375 behind 1100 130 and 137; 1 of 1000 behind none 51 and 43, 16 of 48 behind
 // 2200 77 and 71). Below, tiles of 32 rows, or 16 where that holds a request. In the stream form a workgroup takes as
 // many neighbouring heads as leaves a tile at most 8 workgroups of its own (64 requests of 16K, 8 heads 286 us with 4, 298
