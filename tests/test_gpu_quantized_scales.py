@@ -170,3 +170,55 @@ def test_scores_far_from_zero(device, n, order, exponent):
     assert off[clear].max() <= 1e-30
     assert ((lse.cpu().double().T - top.values[..., 0]).abs() <= 60 + (D + 8) * 2.0 ** -24 * reach)[clear].all()
     assert clear.sum().item() > 0.5 * n * 4
+
+
+@pytest.mark.parametrize("n", [1, 6, 300])
+def test_past_32_bit_offsets(device, n):
+    """The second reading of the keys too: pages past 2^32 bytes of each cache."""
+    page, HKV, D = 128, 8, 128
+    blocks = 2**32 // (page * HKV * D) + 40
+    small = spread_scales(paged(device, [n], [1600], HQ=16, HKV=HKV, D=D, page=page, group=32, spare_pages=0), -80, 60, "mixed")
+    far = blocks - 1 - torch.arange(small["k_cache"].shape[0], device=device)
+    moved = dict(small)
+    for w in ("k", "v"):
+        cache = torch.empty((blocks, page, HKV, D), dtype=torch.uint8, device=device)
+        cache[far] = small[w + "_cache"].view(torch.uint8)
+        moved[w + "_cache"] = cache.view(torch.float8_e4m3fn)
+        scale = torch.empty((blocks, 4, HKV), device=device)
+        scale[far] = small[w + "_scale"]
+        moved[w + "_scale"] = scale
+    moved["block_table"] = far[small["block_table"].long()].to(torch.int32)
+    check(device, [n], [1600], small)
+    assert torch.equal(call(small, 0.05), call(moved, 0.05))
+
+
+@pytest.mark.parametrize("page,group", [(16, 16), (128, 16), (1024, 1024)])
+@pytest.mark.parametrize("HQ,HKV", [(5, 5), (24, 8), (13, 1)])
+def test_pages_and_heads(device, page, group, HQ, HKV):
+    counts, lengths = [3, 1, 280], [2 * page + 5, 1500, 1700]
+    t = paged(device, counts, lengths, HQ=HQ, HKV=HKV, D=64, page=page, group=group, codes="int8", seed=HQ)
+    check(device, counts, lengths, spread_scales(t, -80, 55, "mixed"))
+
+
+def test_in_a_graph_and_on_another_stream(device):
+    calls = [spread_scales(paged(device, c, s, HQ=8, page=64, seed=2), -80, 70, "falling") for c, s in (([1, 2], [900, 120]), ([400], [1700]))]
+    for t in calls:
+        first = call(t, 0.06)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            second = call(t, 0.06)
+        torch.cuda.current_stream().wait_stream(stream)
+        assert torch.equal(first, second) and torch.equal(first, call(t, 0.06))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        outs = [call(t, 0.06) for t in calls]
+    for step in range(3):
+        for t in calls:
+            t["q"].normal_()
+            t["seqused_kv"] -= step
+            t["v_scale"] *= 2.0 ** step
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, call(t, 0.06)) for out, t in zip(outs, calls)), step
