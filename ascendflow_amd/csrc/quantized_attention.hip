@@ -55,7 +55,8 @@ __device__ __forceinline__ bool q8_far(float m) {  // there is a maximum, finite
 // weight, of all keys under 2^-26.
 template <int DT>
 __device__ __forceinline__ bool far_apart(float least, float most, int keys) {
-  return (uniform(__float_as_int(most)) >> 23) - (uniform(__float_as_int(least)) >> 23) + 1 + (32 - __clz(keys)) > 100 - (int)q8_tau<DT>();
+  const int spread = (uniform(__float_as_int(most)) >> 23) - (uniform(__float_as_int(least)) >> 23) + 1;
+  return spread + (32 - __clz(keys)) > 100 - (int)q8_tau<DT>();
 }
 
 // v 2^e for a result inside float32's range, subnormal ones included.
